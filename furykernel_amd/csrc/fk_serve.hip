@@ -1,0 +1,314 @@
+// fk_serve.hip — the operators of a served batch as one C call each
+// (include/fkrocm_serve.h), their kernels compiled into the C ABI's library.
+//
+// Each entry checks its arguments against what its kernels take, on the host
+// and before anything is queued, then launches on the caller's stream.
+
+#include "../../include/fkrocm_serve.h"
+
+#include <hip/hip_runtime.h>
+
+#include <cstdarg>
+#include <cstdio>
+#include <cstring>
+
+#include "fk_internal.h"
+#include "kernels/fk_page_plan.h"
+#include "kernels/fk_paged_attend.h"
+#include "kernels/fk_paged_store.h"
+
+namespace {
+
+__global__ void __launch_bounds__(FK_PLAN_THREADS) op_page_plan(fk_page_plan_args a) { fk::page_plan(a); }
+
+template <int T, bool BF16>
+__global__ void __launch_bounds__(FK_STORE_THREADS) op_paged_store(fk_paged_store_args a) {
+  fk::paged_store<T, BF16>(a);
+}
+
+template <uint32_t DP, bool FULL, bool BF16>
+__global__ void __launch_bounds__(FK_PAGED_THREADS, DP == 256 ? 1 : 2)
+    op_paged_attend(fk_paged_attend_args a, fk::PagedPlan pl) {
+  fk::paged_attend<DP, FULL, BF16>(a, pl);
+}
+
+template <bool BF16>
+__global__ void __launch_bounds__(64 * FK_JOIN_WAVES)
+    op_paged_attend_join(fk_paged_attend_args a, fk::PagedPlan pl, uint32_t groups) {
+  fk::paged_attend_join<BF16>(a, pl, groups);
+}
+
+int use_device(fk_ctx *ctx) {
+  const hipError_t e = hipSetDevice(ctx->device);
+  return e == hipSuccess ? FK_OK : fk_fail(ctx, FK_ERR_HIP, "hipSetDevice: %s", hipGetErrorString(e));
+}
+
+int launched(fk_ctx *ctx, const char *what) {
+  const hipError_t e = hipGetLastError();
+  return e == hipSuccess ? FK_OK : fk_fail(ctx, FK_ERR_HIP, "%s: %s", what, hipGetErrorString(e));
+}
+
+hipStream_t stream_of(fk_ctx *ctx, fk_stream *s) { return s ? s->stream : ctx->stream; }
+
+// What a check of a call's arguments finds: FK_OK, or a status and the reason.
+struct Refusal {
+  char text[512] = "";
+  __attribute__((format(printf, 3, 4))) int operator()(int status, const char *fmt, ...) {
+    va_list ap;
+    va_start(ap, fmt);
+    vsnprintf(text, sizeof text, fmt, ap);
+    va_end(ap);
+    return status;
+  }
+};
+
+// A span of device memory a call reads or writes.
+struct Span {
+  const char *name;
+  uint64_t addr, bytes;
+};
+
+bool meets(const Span &a, const Span &b) {
+  return a.bytes && b.bytes && a.addr < b.addr + b.bytes && b.addr < a.addr + a.bytes;
+}
+
+// Every span there and aligned; no output over another span.
+int check_spans(Refusal &no, const Span *reads, size_t n_reads, const Span *writes, size_t n_writes, uint32_t align) {
+  for (size_t i = 0; i < n_reads + n_writes; i++) {
+    const Span &s = i < n_reads ? reads[i] : writes[i - n_reads];
+    if (s.bytes && (s.addr == 0 || s.addr % align))
+      return no(FK_ERR_ARG, "%s is null or not %u-byte aligned", s.name, align);
+  }
+  for (size_t i = 0; i < n_writes; i++) {
+    for (size_t j = 0; j < n_reads; j++)
+      if (meets(writes[i], reads[j])) return no(FK_ERR_ARG, "%s overlaps %s", writes[i].name, reads[j].name);
+    for (size_t j = 0; j < i; j++)
+      if (meets(writes[i], writes[j])) return no(FK_ERR_ARG, "%s overlaps %s", writes[i].name, writes[j].name);
+  }
+  return FK_OK;
+}
+
+// The attention's launch for these sizes: head_dim's tile width, its
+// threadgroups and what the kernels take; 0 threadgroups and the reason if
+// the kernels do not take them.
+struct AttendLaunch {
+  uint32_t width = 0, groups = 0;
+  fk::PagedPlan plan{};
+  const char *why = "";
+};
+
+AttendLaunch attend_launch(const fk_paged_attend_args &a) {
+  AttendLaunch l;
+  const uint64_t length = (uint64_t)a.table_len * a.block_size;
+  if (a.requests == 0 || a.kv_heads == 0 || a.heads == 0 || a.heads % a.kv_heads) {
+    l.why = "requests and heads that kv_heads divides";
+  } else if (a.head_dim == 0 || a.head_dim % 8 || a.head_dim > 256) {
+    l.why = "head_dim a multiple of 8, at most 256";
+  } else if (a.block_size == 0 || a.blocks == 0 || a.table_len == 0) {
+    l.why = "blocks, their size and a table";
+  } else if (length >= 1ull << 31 || (uint64_t)a.blocks * a.block_size >= 1ull << 32) {
+    l.why = "a table of fewer than 2^31 positions, a pool of fewer than 2^32";
+  } else if ((uint64_t)a.heads * a.head_dim >= 1ull << 31 || a.requests >= 1u << 24) {
+    l.why = "rows of fewer than 2^31 elements, fewer than 2^24 requests";
+  } else {
+    l.width = a.head_dim <= 64 ? 64 : (a.head_dim <= 128 ? 128 : 256);
+    l.plan.group = a.heads / a.kv_heads;
+    l.plan.head_tiles = (l.plan.group + 15) / 16;
+    l.plan.rows = l.plan.group < 16 ? l.plan.group : 16;
+    l.plan.length = (uint32_t)length;
+    const uint64_t unit = (l.width == 64 ? 64 : 32) * FK_PAGED_WAVES;
+    const uint64_t seen = a.window && a.window < length ? a.window + unit : length;
+    // the kernels count units in 32 bits
+    const __uint128_t units = (__uint128_t)a.requests * a.kv_heads * l.plan.head_tiles * ((seen + unit - 1) / unit);
+    if (units >= 1ull << 32) {
+      l.why = "fewer than 2^32 units of keys";
+      return l;
+    }
+    // as many as the chip's 256 compute units hold at once
+    const uint64_t most = l.width == 256 ? 256 : 512;
+    l.groups = (uint32_t)(units < most ? (uint64_t)units : most);
+  }
+  return l;
+}
+
+size_t attend_bytes(const fk_paged_attend_args &a, const AttendLaunch &l) {
+  return l.groups * (sizeof(fk::PagedJoin) + 2 * (size_t)l.plan.rows * (a.head_dim + 2) * sizeof(float));
+}
+
+template <uint32_t DP, bool BF16>
+void queue_attend(const fk_paged_attend_args &a, const AttendLaunch &l, hipStream_t s) {
+  if (a.head_dim == DP)
+    hipLaunchKernelGGL((op_paged_attend<DP, true, BF16>), dim3(l.groups), dim3(FK_PAGED_THREADS), 0, s, a, l.plan);
+  else
+    hipLaunchKernelGGL((op_paged_attend<DP, false, BF16>), dim3(l.groups), dim3(FK_PAGED_THREADS), 0, s, a, l.plan);
+}
+
+int check(const fk_page_plan_args &a, Refusal &no) {
+  if (a.requests == 0 || a.requests >= 1u << 24 || a.table_len == 0 || a.block_size == 0)
+    return no(FK_ERR_ARG, "%u requests (1 to 2^24 - 1), tables of %u blocks of %u", a.requests, a.table_len,
+              a.block_size);
+  if ((uint64_t)a.table_len * a.block_size >= 1ull << 32 || a.tokens == 0xFFFFFFFFu)
+    return no(FK_ERR_RANGE, "tables of %u blocks of %u, %u tokens: past 32 bits", a.table_len, a.block_size, a.tokens);
+  const uint64_t n = a.requests, t = a.tokens;
+  const Span reads[] = {{"cached", a.cached, 4 * n},
+                        {"fresh", a.fresh, 4 * n},
+                        {"free_blocks", a.free_blocks, 4ull * a.free_len},
+                        {"head", a.head, 4}};
+  const Span writes[] = {{"table", a.table, 4 * n * a.table_len}, {"lengths", a.lengths, 4 * n},
+                         {"starts", a.starts, 4 * (n + 1)},       {"slots", a.slots, 4 * t},
+                         {"positions", a.positions, 4 * t},       {"owner", a.owner, 4 * t},
+                         {"counts", a.counts, 16}};
+  return check_spans(no, reads, 4, writes, 7, 4);
+}
+
+// Units of 16 elements that a token's rows have: one thread's work.
+uint64_t store_units(const fk_paged_store_args &a) {
+  return ((a.q ? (uint64_t)a.heads : 0) + 2ull * a.kv_heads) * (a.head_dim / 16);
+}
+
+int check(const fk_paged_store_args &a, Refusal &no) {
+  if (a.kv_heads == 0 || a.head_dim == 0 || a.head_dim % 16 || a.head_dim > 256 || (a.q && a.heads == 0))
+    return no(FK_ERR_ARG, "%u heads over %u of width %u (a multiple of 16, at most 256)", a.heads, a.kv_heads,
+              a.head_dim);
+  if (a.block_size == 0 || a.blocks == 0 || (uint64_t)a.blocks * a.block_size >= 1ull << 32)
+    return no(FK_ERR_RANGE, "%u blocks of %u", a.blocks, a.block_size);
+  if (a.rows_type > FK_T_BF16) return no(FK_ERR_ARG, "rows of type %u", a.rows_type);
+  if (2ull * a.rotated > a.head_dim || (a.rotated && a.rope_rows == 0))
+    return no(FK_ERR_ARG, "RoPE of %u pairs of a head of %u from a table of %u rows", a.rotated, a.head_dim,
+              a.rope_rows);
+  const uint64_t T = a.tokens, wide = a.rows_type == FK_T_F32 ? 4 : 2, row16 = 16 / wide;
+  const uint64_t qw = a.q ? (uint64_t)a.heads * a.head_dim : 0, kw = (uint64_t)a.kv_heads * a.head_dim;
+  const uint64_t most = 1ull << 40;
+  if ((a.q && (a.q_stride % row16 || a.q_stride < qw || a.q_stride >= most)) || a.k_stride % row16 ||
+      a.k_stride < kw || a.k_stride >= most || a.v_stride % row16 || a.v_stride < kw || a.v_stride >= most)
+    return no(FK_ERR_ARG, "row strides %llu, %llu, %llu: at least a row, multiples of 16 bytes",
+              (unsigned long long)a.q_stride, (unsigned long long)a.k_stride, (unsigned long long)a.v_stride);
+  if ((__uint128_t)store_units(a) * T >= (1ull << 32) - FK_STORE_THREADS)
+    return no(FK_ERR_RANGE, "%u tokens of %llu units of 16 elements: past 32 bits", a.tokens,
+              (unsigned long long)store_units(a));
+  auto rows = [&](uint64_t stride, uint64_t width) { return T ? ((T - 1) * stride + width) * wide : 0; };
+  const __uint128_t pool = (__uint128_t)a.blocks * a.block_size * kw * 2;
+  if (pool >= 1ull << 48) return no(FK_ERR_RANGE, "a pool of 2^48 bytes and more");
+  const Span reads[] = {{"q", a.q, a.q ? rows(a.q_stride, qw) : 0},
+                        {"k", a.k, rows(a.k_stride, kw)},
+                        {"v", a.v, rows(a.v_stride, kw)},
+                        {"slots", a.slots, 4 * T},
+                        {"positions", a.positions, a.rotated ? 4 * T : 0},
+                        {"rope", a.rope, a.rotated ? 8ull * a.rope_rows * a.rotated : 0}};
+  const Span writes[] = {{"qr", a.qr, T * qw * 2}, {"kpool", a.kpool, (uint64_t)pool}, {"vpool", a.vpool, (uint64_t)pool}};
+  return check_spans(no, reads, 6, writes, 3, 16);
+}
+
+int check(const fk_paged_attend_args &a, const AttendLaunch &l, Refusal &no) {
+  if (l.groups == 0)
+    return no(FK_ERR_ARG, "%u requests, %u heads over %u of width %u, %u blocks of %u, tables of %u: it takes %s",
+              a.requests, a.heads, a.kv_heads, a.head_dim, a.blocks, a.block_size, a.table_len, l.why);
+  const uint64_t n = a.requests, w = (uint64_t)a.heads * a.head_dim, most = 1ull << 38;
+  if (a.q_stride < w || a.q_stride % 8 || a.q_stride >= most || a.out_stride < w || a.out_stride >= most)
+    return no(FK_ERR_ARG, "row strides %llu and %llu: at least %llu, q's a multiple of 8",
+              (unsigned long long)a.q_stride, (unsigned long long)a.out_stride, (unsigned long long)w);
+  const size_t bytes = attend_bytes(a, l);
+  if (a.workspace_bytes < bytes)
+    return no(FK_ERR_RANGE, "a workspace of %llu bytes, %zu needed", (unsigned long long)a.workspace_bytes, bytes);
+  const __uint128_t pool = (__uint128_t)a.blocks * a.block_size * a.kv_heads * a.head_dim * 2;
+  if (pool >= 1ull << 48) return no(FK_ERR_RANGE, "a pool of 2^48 bytes and more");
+  if (a.starts && a.q_rows == 0) return no(FK_ERR_ARG, "starts of no rows of q");
+  const uint64_t q_rows = a.starts ? a.q_rows : n;
+  const Span reads[] = {{"q", a.q, ((q_rows - 1) * a.q_stride + w) * 2},
+                        {"kpool", a.kpool, (uint64_t)pool},
+                        {"vpool", a.vpool, (uint64_t)pool},
+                        {"table", a.table, 4 * n * a.table_len},
+                        {"lengths", a.lengths, 4 * n},
+                        {"starts", a.starts, a.starts ? 4 * (n + 1) : 0}};
+  const Span writes[] = {{"out", a.out, ((n - 1) * a.out_stride + w) * (a.out_f32 ? 4 : 2)},
+                         {"workspace", a.workspace, bytes}};
+  return check_spans(no, reads, 6, writes, 2, 16);
+}
+
+// A call's arguments as its entry takes them, or the refusal on the context.
+template <typename Args, typename... More>
+int admit(fk_ctx *ctx, const char *what, const Args *a, const More &...more) {
+  if (!ctx || !a) return fk_fail(ctx, FK_ERR_ARG, "%s: null argument", what);
+  Refusal no;
+  if (int st = check(*a, more..., no)) return fk_fail(ctx, st, "%s: %s", what, no.text);
+  return use_device(ctx);
+}
+
+}  // namespace
+
+extern "C" int fk_serve_check(const char *entry, const void *args, size_t args_bytes, char *err, size_t err_cap) {
+  Refusal no;
+  int st = FK_OK;
+  auto is = [&](const char *name, size_t bytes) {
+    if (!entry || std::strcmp(entry, name)) return false;
+    if (!args || args_bytes != bytes) {
+      st = no(FK_ERR_ARG, "%s: %zu bytes of arguments, it takes %zu", name, args_bytes, bytes);
+      return false;
+    }
+    return true;
+  };
+  if (is("fk_page_plan", sizeof(fk_page_plan_args))) {
+    st = check(*static_cast<const fk_page_plan_args *>(args), no);
+  } else if (is("fk_paged_store", sizeof(fk_paged_store_args))) {
+    st = check(*static_cast<const fk_paged_store_args *>(args), no);
+  } else if (is("fk_paged_attend", sizeof(fk_paged_attend_args))) {
+    const fk_paged_attend_args &a = *static_cast<const fk_paged_attend_args *>(args);
+    st = check(a, attend_launch(a), no);
+  } else if (st == FK_OK) {
+    st = no(FK_ERR_NOT_FOUND, "no operator %s", entry ? entry : "(null)");
+  }
+  if (err && err_cap) snprintf(err, err_cap, "%s", no.text);
+  return st;
+}
+
+extern "C" int fk_page_plan(fk_ctx *ctx, const fk_page_plan_args *a, fk_stream *stream) {
+  if (int st = admit(ctx, "fk_page_plan", a)) return st;
+  const uint64_t groups = ((uint64_t)a->tokens + FK_PLAN_THREADS - 1) / FK_PLAN_THREADS;
+  const uint32_t g = (uint32_t)(groups < 1 ? 1 : (groups > 256 ? 256 : groups));
+  hipLaunchKernelGGL(op_page_plan, dim3(g), dim3(FK_PLAN_THREADS), 0, stream_of(ctx, stream), *a);
+  return launched(ctx, "fk_page_plan");
+}
+
+extern "C" int fk_paged_store(fk_ctx *ctx, const fk_paged_store_args *a, fk_stream *stream) {
+  if (int st = admit(ctx, "fk_paged_store", a)) return st;
+  if (a->tokens == 0) return FK_OK;
+  const uint64_t units = store_units(*a) * a->tokens;
+  const dim3 grid((uint32_t)((units + FK_STORE_THREADS - 1) / FK_STORE_THREADS)), block(FK_STORE_THREADS);
+  const hipStream_t s = stream_of(ctx, stream);
+#define FK_STORE_CASE(T_)                                                                                 \
+  case T_:                                                                                                \
+    if (a->cache_bf16) hipLaunchKernelGGL((op_paged_store<T_, true>), grid, block, 0, s, *a);             \
+    else hipLaunchKernelGGL((op_paged_store<T_, false>), grid, block, 0, s, *a);                          \
+    break
+  switch (a->rows_type) {
+    FK_STORE_CASE(FK_T_F32);
+    FK_STORE_CASE(FK_T_F16);
+    FK_STORE_CASE(FK_T_BF16);
+  }
+#undef FK_STORE_CASE
+  return launched(ctx, "fk_paged_store");
+}
+
+extern "C" size_t fk_paged_attend_workspace(const fk_paged_attend_args *a) {
+  return a ? attend_bytes(*a, attend_launch(*a)) : 0;
+}
+
+extern "C" int fk_paged_attend(fk_ctx *ctx, const fk_paged_attend_args *a, fk_stream *stream) {
+  const AttendLaunch l = a ? attend_launch(*a) : AttendLaunch{};
+  if (int st = admit(ctx, "fk_paged_attend", a, l)) return st;
+  const hipStream_t s = stream_of(ctx, stream);
+  if (a->cache_bf16) {
+    if (l.width == 64) queue_attend<64, true>(*a, l, s);
+    else if (l.width == 128) queue_attend<128, true>(*a, l, s);
+    else queue_attend<256, true>(*a, l, s);
+  } else {
+    if (l.width == 64) queue_attend<64, false>(*a, l, s);
+    else if (l.width == 128) queue_attend<128, false>(*a, l, s);
+    else queue_attend<256, false>(*a, l, s);
+  }
+  if (int st = launched(ctx, "fk_paged_attend")) return st;
+  const dim3 grid(l.groups * l.plan.rows), block(64 * FK_JOIN_WAVES);
+  if (a->cache_bf16) hipLaunchKernelGGL((op_paged_attend_join<true>), grid, block, 0, s, *a, l.plan, l.groups);
+  else hipLaunchKernelGGL((op_paged_attend_join<false>), grid, block, 0, s, *a, l.plan, l.groups);
+  return launched(ctx, "fk_paged_attend (join)");
+}

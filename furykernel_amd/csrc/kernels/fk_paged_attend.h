@@ -1,0 +1,554 @@
+// fk_paged_attend.h — attention of one new token a request over paged caches
+// (include/fkrocm_serve.h: fk_paged_attend).
+//
+// out = softmax(scale q Kᵀ) V, one pass over the keys with a running maximum m,
+// sum l and weighted values o: a tile's scores s give m' = max(m, max s),
+// o' = o e^(m - m') + e^(s - m') V, l' likewise, and two such states of one
+// row join the same way.  The K and V rows' stream bounds it: 4 bytes an
+// element pair against 4 flops a query head.
+//
+// How the work is split.  A pair is a request, a kv head and up to 16 of its
+// query heads (the columns of the matrix operations); its keys are cut into
+// units of 4 tiles.  The units of all pairs, in order, are shared out evenly
+// over the launch's threadgroups (two a CU), each a run of units: a long
+// request goes to as many threadgroups as its share of the batch's keys, a
+// run of short ones to one, whatever the mix, and no length is needed on the
+// host.  Every threadgroup finds its run by a prefix sum of the lengths of its
+// own.  A run's pair that ends in another threadgroup leaves its state in the
+// workspace, at most two a threadgroup, and paged_attend_join adds them in
+// order, so the same lengths give the same bits.
+//
+// In a threadgroup each of the 4 wavefronts takes a quarter of a pair's tiles
+// with a state of its own; nothing is shared until they meet at the pair's
+// end.  A tile's K and V rows (KT keys) go straight into the wavefront's LDS;
+// the next tile's K is loaded as soon as the scores are made and its V after
+// the values, so loads are in flight all the time without a second buffer.
+// Pages may end anywhere in a tile: each lane finds its key's block, from 64
+// table entries that the wavefront holds a lane each.
+//
+// Matrix operations (v_mfma_f32_16x16x32): S = K Qᵀ, then Oᵀ = Vᵀ Pᵀ with the
+// probabilities in the registers that made them, V transposed by the LDS's
+// transposing reads.  The probabilities go in as two 16-bit parts, p cut off
+// and what that leaves, which keeps 16 bits of them in bf16 and 21 in f16: the
+// operation has matrix cycles to spare and the result nearly the precision of
+// binary32 products.  Both parts of a p above 0 are above 0 (the second is
+// taken from p (1 + 2^-20), which the sum counts too), so that a value of
+// infinity gives infinity and not the difference of two.  A reference 15
+// below the running maximum keeps f16's smallest step at 2^-39 of the largest
+// probability.
+#pragma once
+
+#include "fk_common.h"
+#include "fk_mfma.h"
+
+#include "../../../include/fkrocm_serve.h"
+
+#define FK_PAGED_WAVES 4
+#define FK_PAGED_THREADS (64 * FK_PAGED_WAVES)
+#define FK_PAGED_LDS __attribute__((address_space(3)))
+#define FK_PAGED_GLOBAL __attribute__((address_space(1)))
+// s_waitcnt vmcnt(n), the other counters untouched (vmcnt's low four bits at
+// 3:0, its high two at 15:14).
+#define FK_PAGED_VMCNT(N) (((N) & 15) | (((N) >> 4) << 14) | (0x7 << 4) | (0xf << 8))
+
+typedef short fk_paged_short4 __attribute__((ext_vector_type(4)));
+typedef __bf16 fk_paged_bf16x8 __attribute__((ext_vector_type(8)));
+
+namespace fk {
+
+// What the kernels take beside the call's arguments.
+struct PagedPlan {
+  uint32_t group;      // query heads a kv head
+  uint32_t head_tiles; // groups of up to 16 of them
+  uint32_t rows;       // query heads a pair's state holds: min(group, 16)
+  uint32_t length;     // positions a table row covers
+};
+
+// A run's pair left unfinished: its first and last threadgroup, what it is.
+struct PagedJoin {
+  uint32_t last;       // the last threadgroup with a part of it; 0: none
+  uint32_t request, head, rows;
+};
+
+// A pair's state in the workspace: `rows` rows of head_dim values, then the
+// maximum and the sum of each.
+__device__ __forceinline__ uint64_t paged_state(uint32_t group, uint32_t side, uint32_t rows, uint32_t d) {
+  return ((uint64_t)group * 2 + side) * rows * (d + 2);
+}
+
+// The keys of a request that its token sees, in tiles of KT aligned to KT.
+struct PagedKeys {
+  uint32_t first, last;   // positions first .. last - 1
+  uint32_t tile0, tiles;
+};
+
+template <uint32_t KT>
+__device__ __forceinline__ PagedKeys paged_keys(uint32_t length, uint32_t window, uint32_t most) {
+  PagedKeys k;
+  k.last = min(length, most);
+  k.first = window && k.last > window ? k.last - window : 0u;
+  k.tile0 = k.first / KT;
+  k.tiles = (k.last + KT - 1) / KT - k.tile0;
+  return k;
+}
+
+// A request's positions, 0 if it has no query, and its query's row.
+__device__ __forceinline__ uint32_t paged_length(const fk_paged_attend_args &a, uint32_t r) {
+  const uint32_t length = reinterpret_cast<const uint32_t *>(a.lengths)[r];
+  if (!a.starts) return length;
+  const uint32_t *const s = reinterpret_cast<const uint32_t *>(a.starts) + r;
+  return s[1] > s[0] && s[1] <= a.q_rows ? length : 0u;
+}
+__device__ __forceinline__ uint64_t paged_query(const fk_paged_attend_args &a, uint32_t r) {
+  return a.starts ? reinterpret_cast<const uint32_t *>(a.starts)[r + 1] - 1u : r;
+}
+
+// Over lanes l, l ^ 16, l ^ 32 and l ^ 48.
+__device__ __forceinline__ float paged_max(float x) {
+  auto s = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  x = __builtin_fmaxf(__uint_as_float(s[0]), __uint_as_float(s[1]));
+  s = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return __builtin_fmaxf(__uint_as_float(s[0]), __uint_as_float(s[1]));
+}
+__device__ __forceinline__ float paged_sum(float x) {
+  auto s = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  x = __uint_as_float(s[0]) + __uint_as_float(s[1]);
+  s = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return __uint_as_float(s[0]) + __uint_as_float(s[1]);
+}
+
+// A reference to take exponentials from: 0 in place of that of a row that has
+// seen no score.
+__device__ __forceinline__ float paged_ref(float m) { return m == -__builtin_inff() ? 0.0f : m; }
+
+// Eight 16-bit operands of a matrix operation.
+template <bool BF16>
+struct PagedOperand;
+template <>
+struct PagedOperand<false> {
+  typedef _Float16 elem;
+  typedef fk_half8 vec;
+  static __device__ __forceinline__ fk_float4v mfma(vec a, vec b, fk_float4v c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
+  }
+  // p0 and p1 cut off to 16 bits, as elements i and i + 1 and as they were.
+  static __device__ __forceinline__ void cut(float p0, float p1, vec &to, int i, float *c0, float *c1) {
+    const auto h = __builtin_amdgcn_cvt_pkrtz(p0, p1);
+    to[i] = (elem)h[0];
+    to[i + 1] = (elem)h[1];
+    *c0 = (float)h[0];
+    *c1 = (float)h[1];
+  }
+};
+template <>
+struct PagedOperand<true> {
+  typedef __bf16 elem;
+  typedef fk_paged_bf16x8 vec;
+  static __device__ __forceinline__ fk_float4v mfma(vec a, vec b, fk_float4v c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
+  }
+  static __device__ __forceinline__ void cut(float p0, float p1, vec &to, int i, float *c0, float *c1) {
+    const uint32_t u0 = __float_as_uint(p0) & 0xFFFF0000u, u1 = __float_as_uint(p1) & 0xFFFF0000u;
+    to[i] = __builtin_bit_cast(elem, (uint16_t)(u0 >> 16));
+    to[i + 1] = __builtin_bit_cast(elem, (uint16_t)(u1 >> 16));
+    *c0 = __uint_as_float(u0);
+    *c1 = __uint_as_float(u1);
+  }
+};
+
+template <bool BF16>
+__device__ __forceinline__ uint16_t paged_round(float x) {
+  return __builtin_bit_cast(uint16_t, (typename PagedOperand<BF16>::elem)x);
+}
+
+// DP: the head's width in the tiles (64, 128 or 256; head_dim at most that);
+// FULL: head_dim is DP.
+template <uint32_t DP, bool FULL, bool BF16>
+__device__ __forceinline__ void paged_attend(const fk_paged_attend_args &a, const PagedPlan &pl) {
+  using Op = PagedOperand<BF16>;
+  using vec = typename Op::vec;
+  using elem = typename Op::elem;
+  constexpr uint32_t KT = DP == 64 ? 64 : 32;    // keys a tile: 8 KB of K at 64 and 128, 16 KB at 256
+  constexpr uint32_t UNITS = DP / 8;             // 16-byte pieces of a row
+  constexpr uint32_t KPL = 64 / UNITS;           // rows a load of the wavefront covers
+  constexpr uint32_t LOADS = KT / KPL;           // loads a tile's K or V takes
+  constexpr uint32_t UK = KT * FK_PAGED_WAVES;   // keys a unit
+  __shared__ __attribute__((aligned(16))) uint16_t kv[FK_PAGED_WAVES][2][KT * DP];
+  __shared__ float sm[FK_PAGED_WAVES][16], sl[FK_PAGED_WAVES][16];
+  __shared__ uint32_t chunk_units[FK_PAGED_THREADS], wave_units[FK_PAGED_WAVES];
+  const uint32_t lane = threadIdx.x & (FK_WAVE - 1);
+  const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x / FK_WAVE);
+  const uint32_t n = a.requests, D = FULL ? DP : a.head_dim;
+  const uint32_t per_request = a.kv_heads * pl.head_tiles;
+  auto length_of = [&](uint32_t r) { return paged_length(a, r); };
+  const uint32_t width = a.heads * D;
+  PagedJoin *const joins = reinterpret_cast<PagedJoin *>(a.workspace);
+  float *const states = reinterpret_cast<float *>(a.workspace + gridDim.x * sizeof(PagedJoin));
+
+  // The units of each thread's requests, and before them.
+  const uint32_t chunk = (n + FK_PAGED_THREADS - 1) / FK_PAGED_THREADS;
+  const uint32_t r0 = min(threadIdx.x * chunk, n), r1 = min(r0 + chunk, n);
+  auto units_of = [&](uint32_t r) {
+    return (paged_keys<KT>(length_of(r), a.window, pl.length).tiles + FK_PAGED_WAVES - 1) / FK_PAGED_WAVES * per_request;
+  };
+  uint32_t mine = 0;
+  for (uint32_t r = r0; r < r1; r++) mine += units_of(r);
+  uint32_t upto = mine;
+#pragma unroll
+  for (int d = 1; d < 64; d *= 2) {
+    const uint32_t o = __shfl_up(upto, d, 64);
+    if (lane >= (uint32_t)d) upto += o;
+  }
+  if (lane == 63) wave_units[wave] = upto;
+  // (rows of pieces past head_dim are zeros in K, which no load writes)
+  if (!FULL)
+    for (uint32_t i = threadIdx.x; i < FK_PAGED_WAVES * KT * UNITS; i += FK_PAGED_THREADS)
+      reinterpret_cast<uint4 *>(kv[i / (KT * UNITS)][0])[i % (KT * UNITS)] = make_uint4(0, 0, 0, 0);
+  __syncthreads();
+  uint32_t before = upto - mine, total = 0;
+#pragma unroll
+  for (uint32_t w = 0; w < FK_PAGED_WAVES; w++) {
+    before += w < wave ? wave_units[w] : 0u;
+    total += wave_units[w];
+  }
+  chunk_units[threadIdx.x] = before;
+  __syncthreads();
+
+  // Requests that see nothing: rows of zeros.
+  for (uint32_t r = blockIdx.x; r < n; r += gridDim.x)
+    if (length_of(r) == 0)
+      for (uint32_t e = threadIdx.x; e < width; e += FK_PAGED_THREADS) {
+        if (a.out_f32) reinterpret_cast<float *>(a.out)[r * a.out_stride + e] = 0.0f;
+        else reinterpret_cast<uint16_t *>(a.out)[r * a.out_stride + e] = 0;
+      }
+
+  // This threadgroup's run of units.
+  const uint32_t groups = min(gridDim.x, total);
+  if (blockIdx.x >= groups) {
+    if (threadIdx.x == 0) joins[blockIdx.x].last = 0;
+    return;
+  }
+  const uint32_t begin = (uint32_t)((uint64_t)blockIdx.x * total / groups);
+  const uint32_t end = (uint32_t)((uint64_t)(blockIdx.x + 1) * total / groups);
+  uint32_t lo = 0;
+#pragma unroll
+  for (uint32_t step = FK_PAGED_THREADS / 2; step > 0; step /= 2)
+    if (chunk_units[lo + step] <= begin) lo += step;
+  uint32_t at = __builtin_amdgcn_readfirstlane(chunk_units[lo]);  // the units before request r
+  uint32_t r = __builtin_amdgcn_readfirstlane(lo * chunk);
+  uint32_t here = units_of(r);
+  while (at + here <= begin) {
+    at += here;
+    here = units_of(++r);
+  }
+
+  uint16_t *const kbuf = kv[wave][0], *const vbuf = kv[wave][1];
+  const char *const kpool = reinterpret_cast<const char *>(a.kpool);
+  const char *const vpool = reinterpret_cast<const char *>(a.vpool);
+  const float c = a.scale * 1.4426950408889634f;  // scores to log2 units
+  const uint32_t piece = lane % UNITS, krow = lane / UNITS;
+  PagedJoin join = {0, 0, 0, 0};
+
+  for (uint32_t pos = begin; pos < end;) {
+    while (pos >= at + here) {
+      at += here;
+      here = units_of(++r);
+    }
+    const PagedKeys ks = paged_keys<KT>(length_of(r), a.window, pl.length);
+    const uint32_t per_pair = here / per_request;
+    const uint32_t pair = (pos - at) / per_pair;
+    const uint32_t pair0 = at + pair * per_pair;
+    const uint32_t g = pair / pl.head_tiles, h0 = g * pl.group + pair % pl.head_tiles * 16;
+    const uint32_t G = min(pl.group - pair % pl.head_tiles * 16, 16u);
+    const uint32_t seg1 = min(end, pair0 + per_pair);
+    // the segment's tiles, a quarter to each wavefront
+    const uint32_t s0 = (pos - pair0) * FK_PAGED_WAVES, s1 = min((seg1 - pair0) * FK_PAGED_WAVES, ks.tiles);
+    const uint32_t t0 = ks.tile0 + s0 + wave * (s1 - s0) / FK_PAGED_WAVES;
+    const uint32_t t1 = ks.tile0 + s0 + (wave + 1) * (s1 - s0) / FK_PAGED_WAVES;
+
+    // Q (B of S = K Qᵀ): lane l holds head l mod 16 (past the group: its
+    // last), d 32 h + 8 (l div 16) .. + 7, zeros past the head.
+    vec qf[DP / 32];
+    const uint64_t q_row = paged_query(a, r);
+#pragma unroll
+    for (uint32_t h = 0; h < DP / 32; h++) {
+      const uint32_t d = 32 * h + 8 * (lane / 16);
+      uint4 w = make_uint4(0, 0, 0, 0);
+      if (d < D)
+        w = *reinterpret_cast<const uint4 *>(reinterpret_cast<const uint16_t *>(a.q) + q_row * a.q_stride +
+                                             (uint64_t)(h0 + min(lane % 16, G - 1)) * D + d);
+      qf[h] = __builtin_bit_cast(vec, w);
+    }
+
+    const uint32_t *const row = reinterpret_cast<const uint32_t *>(a.table) + (uint64_t)r * a.table_len;
+    const uint32_t last_entry = (ks.last - 1) / a.block_size;
+    uint32_t entry0 = 0, entries = 0;   // the table entries entry0 + lane, none yet
+    bool held = false;
+    uint64_t off[LOADS];                // the tile's rows in the pools, in bytes
+    // K's piece u at place u ^ (key's) of its row, V's 32-byte pairs of pieces
+    // likewise, so that the reads below meet different banks.
+    auto rows_of = [&](uint32_t tile) {
+      const uint32_t key0 = max(tile * KT, ks.first), key1 = min(tile * KT + KT, ks.last) - 1;
+      const uint32_t need0 = key0 / a.block_size, need1 = key1 / a.block_size;
+      if (!held || need1 > entry0 + 63) {
+        entry0 = need0;
+        entries = min(row[min(entry0 + lane, last_entry)], a.blocks - 1);
+        held = true;
+        // landed here, so that no tile without this load waits for one
+        __builtin_amdgcn_s_waitcnt(FK_PAGED_VMCNT(0));
+        asm volatile("" : "+v"(entries));
+      }
+#pragma unroll
+      for (uint32_t q = 0; q < LOADS; q++) {
+        // keys outside the request's own are its own all the same (masked)
+        const uint32_t key = min(max(tile * KT + q * KPL + krow, ks.first), ks.last - 1);
+        const uint32_t entry = key / a.block_size;
+        const uint32_t block = __shfl(entries, entry - entry0, 64);
+        off[q] = (((uint64_t)block * a.kv_heads + g) * a.block_size + (key - entry * a.block_size)) * (2 * D);
+      }
+    };
+    auto load = [&](const char *pool, uint16_t *buf, bool keys) {
+#pragma unroll
+      for (uint32_t q = 0; q < LOADS; q++) {
+        const uint32_t key = q * KPL + krow;
+        const uint32_t turn = keys ? (DP == 64 ? (key >> 1) & 7u : key & 15u)
+                                   : (DP == 64 ? ((key >> 1) & 3u) << 1 : (key & 7u) << 1);
+        const uint32_t u = piece ^ turn;
+        if (FULL || u * 8 < D)
+          __builtin_amdgcn_global_load_lds((const FK_PAGED_GLOBAL void *)(pool + off[q] + u * 16),
+                                           (FK_PAGED_LDS void *)(buf + q * 512), 16, 0, 2);
+      }
+    };
+
+    fk_float4v o[DP / 16];
+#pragma unroll
+    for (uint32_t d = 0; d < DP / 16; d++) o[d] = fk_float4v{0.0f, 0.0f, 0.0f, 0.0f};
+    float m = -__builtin_inff(), l = 0.0f;
+
+    if (t0 < t1) {
+      rows_of(t0);
+      load(kpool, kbuf, true);
+      load(vpool, vbuf, false);
+    }
+    for (uint32_t t = t0; t < t1; t++) {
+      const bool more = t + 1 < t1;
+      __builtin_amdgcn_s_waitcnt(FK_PAGED_VMCNT(LOADS));  // K landed, V's loads in flight
+      asm volatile("" ::: "memory");
+      // S: groups of 16 keys; register i of group s is key 16 s + 4 (l div 16)
+      // + i of the tile, head l mod 16.
+      fk_float4v sc[KT / 16];
+#pragma unroll
+      for (uint32_t s = 0; s < KT / 16; s++) {
+        sc[s] = fk_float4v{0.0f, 0.0f, 0.0f, 0.0f};
+        const uint32_t key = 16 * s + lane % 16, turn = DP == 64 ? (key >> 1) & 7u : key & 15u;
+#pragma unroll
+        for (uint32_t h = 0; h < DP / 32; h++) {
+          const uint4 w = *reinterpret_cast<const uint4 *>(&kbuf[key * DP + ((4 * h + lane / 16) ^ turn) * 8]);
+          sc[s] = Op::mfma(__builtin_bit_cast(vec, w), qf[h], sc[s]);
+        }
+      }
+      // The reads are done before the next tile's loads land on them.
+#pragma unroll
+      for (uint32_t s = 0; s < KT / 16; s++) asm volatile("" : "+v"(sc[s])::"memory");
+      if (more) {
+        rows_of(t + 1);
+        load(kpool, kbuf, true);
+      }
+      float mt = -__builtin_inff();
+#pragma unroll
+      for (uint32_t s = 0; s < KT / 16; s++)
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+          const uint32_t k = t * KT + 16 * s + 4 * (lane / 16) + i;
+          sc[s][i] = k < ks.last && k >= ks.first ? sc[s][i] * c : -__builtin_inff();
+          mt = __builtin_fmaxf(mt, sc[s][i]);
+        }
+      const float mn = __builtin_fmaxf(m, paged_max(mt) - 15.0f);
+      const float mc = paged_ref(mn);
+      const float alpha = __builtin_amdgcn_exp2f(m - mc);
+      m = mn;
+      vec ph[KT / 32], pr[KT / 32];
+      float sum = 0.0f;
+#pragma unroll
+      for (uint32_t s = 0; s < KT / 16; s++)
+#pragma unroll
+        for (int i = 0; i < 4; i += 2) {
+          const float p0 = __builtin_amdgcn_exp2f(sc[s][i] - mc), p1 = __builtin_amdgcn_exp2f(sc[s][i + 1] - mc);
+          const float w0 = p0 * 1.00000095367431640625f, w1 = p1 * 1.00000095367431640625f;
+          sum += w0 + w1;
+          float c0, c1;
+          Op::cut(p0, p1, ph[s / 2], s % 2 * 4 + i, &c0, &c1);
+          pr[s / 2][s % 2 * 4 + i] = (elem)(w0 - c0);
+          pr[s / 2][s % 2 * 4 + i + 1] = (elem)(w1 - c1);
+        }
+      l = l * alpha + paged_sum(sum);
+#pragma unroll
+      for (uint32_t d = 0; d < DP / 16; d++) o[d] *= alpha;
+      if (more) __builtin_amdgcn_s_waitcnt(FK_PAGED_VMCNT(LOADS));  // V landed, the next K in flight
+      else __builtin_amdgcn_s_waitcnt(FK_PAGED_VMCNT(0));
+      asm volatile("" ::: "memory");
+      if (t * KT < ks.first || t * KT + KT > ks.last) {
+        // Rows outside the request's keys hold other values: zeros, so that
+        // an infinity there is nothing to a probability of 0.
+#pragma unroll
+        for (uint32_t q = 0; q < LOADS; q++) {
+          const uint32_t k = t * KT + q * KPL + krow;
+          if (k < ks.first || k >= ks.last)
+            reinterpret_cast<uint4 *>(vbuf)[q * 64 + lane] = make_uint4(0, 0, 0, 0);
+        }
+        asm volatile("" ::: "memory");
+      }
+      // Oᵀ += Vᵀ Pᵀ.  Transposed reads: within 16 lanes, lane 4 k + q reads key
+      // K0 + k, d D0 + 4 q .. + 3 and receives keys K0 .. K0 + 3 of d D0 + (its
+      // index): keys 32 h + 4 (l div 16) .. + 3 and 16 further, ph[h]'s order.
+      const uint32_t tk = 4 * (lane / 16) + lane % 16 / 4, td = 4 * (lane & 3);
+#pragma unroll
+      for (uint32_t d = 0; d < DP / 16; d++)
+#pragma unroll
+        for (uint32_t h = 0; h < KT / 32; h++) {
+          fk_paged_short4 w[2];
+#pragma unroll
+          for (uint32_t q = 0; q < 2; q++) {
+            const uint32_t key = 32 * h + 16 * q + tk;
+            const uint32_t turn = DP == 64 ? (key >> 1) & 3u : key & 7u;
+            w[q] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                (FK_PAGED_LDS fk_paged_short4 *)&vbuf[key * DP + ((16 * d + td) ^ (turn << 4))]);
+          }
+          const uint2 w0 = __builtin_bit_cast(uint2, w[0]), w1 = __builtin_bit_cast(uint2, w[1]);
+          const vec vf = __builtin_bit_cast(vec, make_uint4(w0.x, w0.y, w1.x, w1.y));
+          o[d] = Op::mfma(vf, ph[h], o[d]);
+          o[d] = Op::mfma(vf, pr[h], o[d]);
+        }
+#pragma unroll
+      for (uint32_t d = 0; d < DP / 16; d++) asm volatile("" : "+v"(o[d])::"memory");
+      if (more) load(vpool, vbuf, false);
+    }
+
+    // The wavefronts' states meet, each in the place of its V rows: head l
+    // mod 16, d 16 dt + 4 (l div 16) + i.
+    float *const so = reinterpret_cast<float *>(vbuf);
+    if (lane % 16 < G) {
+#pragma unroll
+      for (uint32_t d = 0; d < DP / 16; d++)
+        *reinterpret_cast<fk_float4v *>(&so[lane % 16 * DP + 16 * d + 4 * (lane / 16)]) = o[d];
+      if (lane < 16) {
+        sm[wave][lane] = m;
+        sl[wave][lane] = l;
+      }
+    }
+    __syncthreads();
+    const bool whole = pos == pair0 && seg1 == pair0 + per_pair;
+    const uint32_t side = pair0 < begin ? 0u : 1u;
+    float *const to = states + paged_state(blockIdx.x, side, pl.rows, D);
+    for (uint32_t e = threadIdx.x; e < G * D; e += FK_PAGED_THREADS) {
+      const uint32_t q = e / D, d = e - q * D;
+      float mm = sm[0][q];
+#pragma unroll
+      for (uint32_t w = 1; w < FK_PAGED_WAVES; w++) mm = __builtin_fmaxf(mm, sm[w][q]);
+      const float mc = paged_ref(mm);
+      float ll = 0.0f, oo = 0.0f;
+#pragma unroll
+      for (uint32_t w = 0; w < FK_PAGED_WAVES; w++) {
+        const float f = __builtin_amdgcn_exp2f(sm[w][q] - mc);
+        ll += sl[w][q] * f;
+        oo += reinterpret_cast<const float *>(kv[w][1])[q * DP + d] * f;
+      }
+      if (whole) {
+        const uint64_t where = r * a.out_stride + (uint64_t)(h0 + q) * D + d;
+        if (a.out_f32) reinterpret_cast<float *>(a.out)[where] = oo / ll;
+        else reinterpret_cast<uint16_t *>(a.out)[where] = paged_round<BF16>(oo / ll);
+      } else {
+        to[q * D + d] = oo;
+        if (d == 0) {
+          to[pl.rows * D + 2 * q] = mm;
+          to[pl.rows * D + 2 * q + 1] = ll;
+        }
+      }
+    }
+    if (!whole && side == 1) {
+      // the pair starts here and ends in a later threadgroup: that of its
+      // last unit
+      join.last = (uint32_t)(((uint64_t)(pair0 + per_pair) * groups + total - 1) / total) - 1;
+      join.request = r;
+      join.head = h0;
+      join.rows = G;
+    }
+    __syncthreads();  // before the next pair's rows land on the states
+    pos = seg1;
+  }
+  if (threadIdx.x == 0) joins[blockIdx.x] = join;
+}
+
+// The states of a pair that several threadgroups made, joined in their order:
+// threadgroup (first threadgroup of the pair, query head), its wavefronts
+// every 8th state each.
+#define FK_JOIN_WAVES 8
+template <bool BF16>
+__device__ __forceinline__ void paged_attend_join(const fk_paged_attend_args &a, const PagedPlan &pl,
+                                                  uint32_t groups) {
+  __shared__ float so[FK_JOIN_WAVES][256], sm[FK_JOIN_WAVES], sl[FK_JOIN_WAVES];
+  const uint32_t first = blockIdx.x / pl.rows, q = blockIdx.x % pl.rows;
+  const PagedJoin j = reinterpret_cast<const PagedJoin *>(a.workspace)[first];
+  if (j.last == 0 || q >= j.rows) return;
+  const float *const states = reinterpret_cast<const float *>(a.workspace + groups * sizeof(PagedJoin));
+  const uint32_t D = a.head_dim;
+  const uint32_t lane = threadIdx.x & (FK_WAVE - 1), wave = threadIdx.x / FK_WAVE;
+  float mm = -__builtin_inff(), ll = 0.0f, oo[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+  constexpr uint32_t U = 4;  // states at once
+  for (uint32_t w0 = first + wave; w0 <= j.last; w0 += U * FK_JOIN_WAVES) {
+    float m[U], l[U], o[U][4];
+#pragma unroll
+    for (uint32_t s = 0; s < U; s++) {
+      const uint32_t w = min(w0 + s * FK_JOIN_WAVES, j.last);
+      const float *const from = states + paged_state(w, w == first ? 1u : 0u, pl.rows, D);
+      const bool there = w0 + s * FK_JOIN_WAVES <= j.last;
+      m[s] = there ? from[pl.rows * D + 2 * q] : -__builtin_inff();
+      l[s] = there ? from[pl.rows * D + 2 * q + 1] : 0.0f;
+#pragma unroll
+      for (uint32_t i = 0; i < 4; i++) {
+        const uint32_t d = lane + 64 * i;
+        o[s][i] = there && d < D ? from[q * D + d] : 0.0f;
+      }
+    }
+    float mn = mm;
+#pragma unroll
+    for (uint32_t s = 0; s < U; s++) mn = __builtin_fmaxf(mn, m[s]);
+    const float mc = paged_ref(mn);
+    const float f0 = __builtin_amdgcn_exp2f(mm - mc);
+    ll *= f0;
+#pragma unroll
+    for (uint32_t i = 0; i < 4; i++) oo[i] *= f0;
+#pragma unroll
+    for (uint32_t s = 0; s < U; s++) {
+      const float f = __builtin_amdgcn_exp2f(m[s] - mc);
+      ll += l[s] * f;
+#pragma unroll
+      for (uint32_t i = 0; i < 4; i++) oo[i] += o[s][i] * f;
+    }
+    mm = mn;
+  }
+#pragma unroll
+  for (uint32_t i = 0; i < 4; i++) so[wave][lane + 64 * i] = oo[i];
+  if (lane == 0) {
+    sm[wave] = mm;
+    sl[wave] = ll;
+  }
+  __syncthreads();
+  if (threadIdx.x >= D) return;
+  mm = sm[0];
+#pragma unroll
+  for (uint32_t w = 1; w < FK_JOIN_WAVES; w++) mm = __builtin_fmaxf(mm, sm[w]);
+  const float mc = paged_ref(mm);
+  float l = 0.0f, o = 0.0f;
+#pragma unroll
+  for (uint32_t w = 0; w < FK_JOIN_WAVES; w++) {
+    const float f = __builtin_amdgcn_exp2f(sm[w] - mc);
+    l += sl[w] * f;
+    o += so[w][threadIdx.x] * f;
+  }
+  const uint64_t where = j.request * a.out_stride + (uint64_t)(j.head + q) * D + threadIdx.x;
+  if (a.out_f32) reinterpret_cast<float *>(a.out)[where] = o / l;
+  else reinterpret_cast<uint16_t *>(a.out)[where] = paged_round<BF16>(o / l);
+}
+
+}  // namespace fk

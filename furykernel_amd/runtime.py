@@ -137,6 +137,11 @@ ENTRY_POINTS: list[tuple[str, object, list]] = [
     ("fk_table_enqueue", _int, [_vp, _u32, _u32, _vp]),
     ("fk_attend_decode", _int, [_vp, _vp, _vp]),
     ("fk_attend_decode_noalloc", _int, [_vp, _vp, _vp]),
+    ("fk_page_plan", _int, [_vp, _vp, _vp]),
+    ("fk_paged_store", _int, [_vp, _vp, _vp]),
+    ("fk_paged_attend_workspace", _sz, [_vp]),
+    ("fk_paged_attend", _int, [_vp, _vp, _vp]),
+    ("fk_serve_check", _int, [ctypes.c_char_p, _vp, _sz, ctypes.c_char_p, _sz]),
     ("fk_rtc_compile", _int, [ctypes.c_char_p, ctypes.c_char_p, ctypes.POINTER(ctypes.c_char_p), _int, _PP,
                               ctypes.POINTER(_sz), ctypes.POINTER(ctypes.c_char_p)]),
     ("fk_rtc_free", None, [_vp]),
@@ -402,6 +407,31 @@ def attend_decode(device: "Device", args: ctypes.Structure, stream: "Stream | No
     """One decode attention step through the library's operation
     (include/fkrocm_ops.h); `args` is a ``kernels.AttendArgs``."""
     _check(device.ctx, getattr(library(), entry)(device.ctx, ctypes.byref(args), _sh(stream)))
+
+
+def serve_check(entry: str, args: ctypes.Structure) -> None:
+    """The checks an operator of a served batch makes of its arguments, on the
+    host (raises ``FkError`` with the reason)."""
+    err = ctypes.create_string_buffer(512)
+    st = library().fk_serve_check(entry.encode(), ctypes.byref(args), ctypes.sizeof(args), err, 512)
+    if st != FK_OK:
+        raise FkError(st, f"{entry}: {err.value.decode()}")
+
+
+class Operation:
+    """An operation of the library bound to its arguments (a C struct, filled
+    once): each ``enqueue`` is one call.  `held` are the buffers whose
+    addresses the arguments carry, kept as long as the operation."""
+
+    def __init__(self, device: "Device", entry: str, args: ctypes.Structure, held: tuple = ()):
+        self.device, self.entry, self.args, self.held = device, entry, args, held
+        self._call = getattr(library(), entry)
+        self._args = ctypes.byref(args)
+
+    def enqueue(self, stream: "Stream | None" = None) -> None:
+        status = self._call(self.device.ctx, self._args, None if stream is None else stream.handle)
+        if status != FK_OK:
+            _check(self.device.ctx, status)
 
 
 class Device:

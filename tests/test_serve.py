@@ -1,0 +1,209 @@
+"""The operators of a served batch without a GPU: the C structs' layouts, the
+checks that their entries make of the arguments, and the bindings' checks of
+their buffers (no launch is made of what they refuse)."""
+
+import ctypes
+import re
+from pathlib import Path
+
+import pytest
+
+from furykernel_amd import paged, runtime
+from furykernel_amd.kernels import LaunchError
+
+HEADER = (Path(__file__).resolve().parents[1] / "include" / "fkrocm_serve.h").read_text()
+STRUCTS = {"fk_page_plan_args": paged.PagePlanArgs, "fk_paged_store_args": paged.PagedStoreArgs,
+           "fk_paged_attend_args": paged.PagedAttendArgs}
+
+
+class FakeDevice:
+    ctx = None
+
+
+DEVICE = FakeDevice()
+
+
+class FakeBuffer:
+    """A buffer of this size at an address of its own, with nothing behind it."""
+    at = 1 << 40
+
+    def __init__(self, size, device=DEVICE, ptr=None):
+        self.size, self.device = size, device
+        self.ptr = FakeBuffer.at if ptr is None else ptr
+        FakeBuffer.at += (size + 511) // 256 * 256
+
+
+@pytest.mark.parametrize("name", sorted(STRUCTS))
+def test_the_structs_fields_are_the_headers(name):
+    body = re.search(r"typedef struct %s \{(.*?)\} %s;" % (name, name), HEADER, re.S).group(1)
+    body = re.sub(r"/\*.*?\*/", "", body, flags=re.S)
+    fields = []
+    for decl in filter(None, (d.strip() for d in body.split(";"))):
+        kind, names = decl.split(None, 1)
+        fields += [(n.strip(), {"uint64_t": ctypes.c_uint64, "uint32_t": ctypes.c_uint32,
+                                "float": ctypes.c_float}[kind]) for n in names.split(",")]
+    assert STRUCTS[name]._fields_ == fields
+
+
+def attend_sizes(**over):
+    return {**dict(requests=3, heads=8, kv_heads=2, head_dim=64, block_size=16, blocks=20, table_len=5), **over}
+
+
+def attend(over=(), sizes=(), **kw):
+    z = attend_sizes(**dict(sizes))
+    n, w = z["requests"], z["heads"] * z["head_dim"]
+    pool = z["blocks"] * z["block_size"] * z["kv_heads"] * z["head_dim"] * 2
+    bufs = dict(q=FakeBuffer(n * w * 2), kpool=FakeBuffer(pool), vpool=FakeBuffer(pool),
+                table=FakeBuffer(4 * n * z["table_len"]), lengths=FakeBuffer(4 * n), out=FakeBuffer(n * w * 2),
+                workspace=FakeBuffer(1 << 26))
+    bufs.update(dict(over))
+    return paged.PagedAttend(DEVICE, **bufs, **z, scale=0.125, **kw)
+
+
+def test_attend_takes_what_it_says():
+    attend()
+    attend(out_type="f32", over={"out": FakeBuffer(3 * 512 * 4)})
+    attend(q_stride=520, over={"q": FakeBuffer((2 * 520 + 512) * 2)})
+    for d in (8, 72, 128, 200, 256):
+        attend(sizes={"head_dim": d})
+    attend(sizes={"heads": 34, "window": 7})
+
+
+@pytest.mark.parametrize("sizes", [
+    {"requests": 0}, {"heads": 0}, {"kv_heads": 0}, {"heads": 7}, {"head_dim": 0}, {"head_dim": 12},
+    {"head_dim": 264}, {"block_size": 0}, {"blocks": 0}, {"table_len": 0}, {"table_len": 1 << 28},
+    {"blocks": 1 << 28}, {"requests": 1 << 24}, {"requests": 1 << 23, "table_len": 1 << 20}, {"requests": -1},
+    {"window": 1 << 32}])
+def test_attend_refuses_sizes(sizes):
+    with pytest.raises(LaunchError):
+        attend(sizes=sizes)
+
+
+@pytest.mark.parametrize("name", ["q", "kpool", "vpool", "table", "lengths", "out", "workspace"])
+def test_attend_refuses_buffers(name):
+    sizes = attend_sizes()
+    full = {"q": 3072, "kpool": 81920, "vpool": 81920, "table": 60, "lengths": 12, "out": 3072,
+            "workspace": paged.attend_workspace(**sizes)}[name]
+    attend({name: FakeBuffer(full)})
+    for bad in (FakeBuffer(full - 1), FakeBuffer(full, FakeDevice()), FakeBuffer(full, ptr=FakeBuffer.at + 8)):
+        with pytest.raises(LaunchError):
+            attend({name: bad})
+
+
+def test_attend_refuses_overlaps_strides_and_types():
+    q = FakeBuffer(3 * 512 * 4)
+    for over, kw in (({"q": q, "out": q}, {}), ({"lengths": q, "workspace": q}, {}), ({}, {"q_stride": 504}),
+                     ({"q": q}, {"q_stride": 516}), ({}, {"out_stride": 511}), ({}, {"cache": "f32"}),
+                     ({}, {"cache": "bf16", "out_type": "f16"}), ({}, {"out_stride": 513})):
+        with pytest.raises(LaunchError):
+            attend(over, **kw)
+
+
+def test_attend_refuses_starts_without_rows():
+    starts, q = FakeBuffer(16), FakeBuffer(7 * 512 * 2)
+    attend({"starts": starts, "q": q}, q_rows=7)
+    for over, rows in (({"starts": starts, "q": q}, 0), ({"starts": starts, "q": q}, 8), ({"starts": starts, "q": q}, -1),
+                       ({"starts": FakeBuffer(12), "q": q}, 7)):
+        with pytest.raises(LaunchError):
+            attend(over, q_rows=rows)
+
+
+def plan(over=(), **sizes):
+    z = {**dict(requests=4, tokens=9, table_len=3, block_size=16, free_len=5), **sizes}
+    n, t = z["requests"], z["tokens"]
+    words = dict(cached=n, fresh=n, free=z["free_len"], head=1, table=n * z["table_len"], lengths=n, starts=n + 1,
+                 slots=t, positions=t, owner=t, counts=4)
+    bufs = {k: FakeBuffer(4 * max(v, 0)) for k, v in words.items()}
+    bufs.update(dict(over))
+    return paged.PagePlan(DEVICE, **bufs, **z)
+
+
+def test_plan_takes_what_it_says():
+    plan()
+    plan(tokens=0)
+    plan(free_len=0)
+    plan(requests=100000, tokens=1 << 20)
+
+
+@pytest.mark.parametrize("sizes", [{"requests": 0}, {"requests": 1 << 24}, {"table_len": 0}, {"block_size": 0},
+                                   {"block_size": 1 << 31, "table_len": 2}, {"tokens": -1}, {"tokens": 0xFFFFFFFF}])
+def test_plan_refuses_sizes(sizes):
+    with pytest.raises(LaunchError):
+        plan(**sizes)
+
+
+def test_plan_refuses_buffers_and_overlaps():
+    words = dict(cached=4, fresh=4, free=5, head=1, table=12, lengths=4, starts=5, slots=9, positions=9, owner=9,
+                 counts=4)
+    for name, count in words.items():
+        for bad in (FakeBuffer(4 * count - 1), FakeBuffer(4 * count, FakeDevice()),
+                    FakeBuffer(4 * count, ptr=FakeBuffer.at + 2)):
+            with pytest.raises(LaunchError):
+                plan({name: bad})
+    one = FakeBuffer(4096)
+    for a, b in (("cached", "lengths"), ("head", "counts"), ("free", "table"), ("slots", "owner")):
+        with pytest.raises(LaunchError, match="overlaps"):
+            plan({a: one, b: one})
+    counts = FakeBuffer(16)
+    with pytest.raises(LaunchError, match="overlaps"):   # the next head is not this step's
+        plan({"counts": counts, "head": FakeBuffer(4, ptr=counts.ptr + 12)})
+
+
+def store(over=(), sizes=(), **kw):
+    z = {**dict(tokens=5, heads=4, kv_heads=2, head_dim=64, block_size=16, blocks=3, rotated=32, rope_rows=100),
+         **dict(sizes)}
+    T, d = z["tokens"], z["head_dim"]
+    pool = z["blocks"] * z["block_size"] * z["kv_heads"] * d * 2
+    bufs = dict(q=FakeBuffer(4 * T * z["heads"] * d), k=FakeBuffer(4 * T * z["kv_heads"] * d),
+                v=FakeBuffer(4 * T * z["kv_heads"] * d), slots=FakeBuffer(4 * T), positions=FakeBuffer(4 * T),
+                rope=FakeBuffer(8 * z["rope_rows"] * max(z["rotated"], 0)), qr=FakeBuffer(2 * T * z["heads"] * d),
+                kpool=FakeBuffer(pool), vpool=FakeBuffer(pool))
+    bufs.update(dict(over))
+    return paged.PagedStore(DEVICE, **bufs, **z, **kw)
+
+
+def test_store_takes_what_it_says():
+    store()
+    store(sizes={"rotated": 0}, over={"rope": None, "positions": None})
+    store(sizes={"heads": 0}, over={"q": None, "qr": None})
+    store(sizes={"tokens": 0})
+    store(sizes={"head_dim": 16, "rotated": 8})
+    store(sizes={"head_dim": 256}, rows_type="bf16", cache="bf16")
+    fused = FakeBuffer(4 * 5 * 520)
+    store({"q": fused, "k": fused, "v": fused}, q_stride=520, k_stride=520, v_stride=520, k_offset=256, v_offset=384)
+
+
+@pytest.mark.parametrize("sizes", [
+    {"kv_heads": 0}, {"head_dim": 8}, {"head_dim": 40}, {"head_dim": 272}, {"block_size": 0}, {"blocks": 0},
+    {"blocks": 1 << 31}, {"rotated": 33}, {"rope_rows": 0}, {"tokens": 1 << 28}, {"tokens": -3}])
+def test_store_refuses_sizes(sizes):
+    with pytest.raises(LaunchError):
+        store(sizes=sizes)
+
+
+def test_store_refuses_buffers_strides_and_types():
+    for name in ("q", "k", "v", "slots", "positions", "rope", "qr", "kpool", "vpool"):
+        good = store().held[("q", "k", "v", "slots", "positions", "rope", "qr", "kpool", "vpool").index(name)]
+        for bad in (FakeBuffer(good.size - 1), FakeBuffer(good.size, FakeDevice()),
+                    FakeBuffer(good.size, ptr=FakeBuffer.at + 4)):
+            with pytest.raises(LaunchError):
+                store({name: bad})
+    big = FakeBuffer(1 << 20)
+    for over, kw in (({"q": None}, {}), ({"qr": None}, {}), ({"rope": None}, {}), ({"positions": None}, {}),
+                     ({"k": big}, {"k_stride": 130}), ({"k": big}, {"k_stride": 64}), ({"v": big}, {"v_offset": 2}),
+                     ({"v": big}, {"v_offset": -4}), ({}, {"rows_type": "i8"}), ({}, {"cache": "f32"}),
+                     ({"kpool": big, "vpool": big}, {}), ({"q": big, "kpool": big}, {}), ({"q": big}, {"q_offset": 1})):
+        with pytest.raises(LaunchError):
+            store(over, **kw)
+
+
+def test_the_check_refuses_unknown_entries_and_sizes_of_arguments():
+    lib = runtime.library()
+    err = ctypes.create_string_buffer(200)
+    args = paged.PagePlanArgs()
+    for entry, n, status in ((b"fk_nothing", 8, -4), (b"fk_page_plan", 8, -2), (None, 8, -4)):
+        assert lib.fk_serve_check(entry, ctypes.byref(args), n, err, 200) == status and err.value
+    assert lib.fk_serve_check(b"fk_page_plan", None, ctypes.sizeof(args), err, 200) == -2
+    for entry in (lib.fk_page_plan, lib.fk_paged_store, lib.fk_paged_attend):
+        assert entry(None, ctypes.byref(args), None) == -2
+    assert lib.fk_paged_attend_workspace(None) == 0
