@@ -132,7 +132,7 @@ AttendLaunch attend_launch(const fk_paged_attend_args &a) {
 }
 
 size_t attend_bytes(const fk_paged_attend_args &a, const AttendLaunch &l) {
-  return l.groups * (sizeof(fk::PagedJoin) + 2 * (size_t)l.plan.rows * (a.head_dim + 2) * sizeof(float));
+  return l.groups * (sizeof(fk::u32x4) + 2 * (size_t)l.plan.rows * (a.head_dim + 2) * sizeof(float));
 }
 
 template <uint32_t DP, bool BF16>

@@ -17,6 +17,8 @@
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
+#include "fk_address.h"
+
 #include "../../../include/fkrocm_serve.h"
 
 #define FK_PLAN_THREADS 1024
@@ -38,8 +40,8 @@ __device__ __forceinline__ uint32_t plan_pages(uint64_t positions, uint32_t bloc
 // Request r whose tokens start at `start` (64 bits: no sum of lengths wraps).
 __device__ __forceinline__ PlanRequest plan_request(const fk_page_plan_args &a, uint32_t r, uint64_t start) {
   PlanRequest q;
-  q.cached = reinterpret_cast<const uint32_t *>(a.cached)[r];
-  q.fresh = reinterpret_cast<const uint32_t *>(a.fresh)[r];
+  q.cached = global_at<const uint32_t>(a.cached)[r];
+  q.fresh = global_at<const uint32_t>(a.fresh)[r];
   const uint64_t total = (uint64_t)q.cached + q.fresh;
   q.fits = total <= (uint64_t)a.table_len * a.block_size && start + q.fresh <= a.tokens;
   q.held = q.fits ? plan_pages(q.cached, a.block_size) : 0u;
@@ -94,8 +96,8 @@ __device__ __forceinline__ void page_plan(const fk_page_plan_args &a) {
   const uint32_t chunk = (uint32_t)(((uint64_t)n + FK_PLAN_THREADS - 1) / FK_PLAN_THREADS);
   const uint32_t r0 = (uint32_t)min((uint64_t)tid * chunk, (uint64_t)n);
   const uint32_t r1 = (uint32_t)min((uint64_t)r0 + chunk, (uint64_t)n);
-  const uint32_t *fresh = reinterpret_cast<const uint32_t *>(a.fresh);
-  const uint32_t head = *reinterpret_cast<const uint32_t *>(a.head);
+  const auto fresh = global_at<const uint32_t>(a.fresh);
+  const uint32_t head = *global_at<const uint32_t>(a.head);
   const uint32_t avail = a.free_len > head ? a.free_len - head : 0u;
   if (tid == 0) refused = taken = 0;
 
@@ -129,8 +131,8 @@ __device__ __forceinline__ void page_plan(const fk_page_plan_args &a) {
       if (fits && q.need) most = (uint32_t)after;
       out += !fits;
       if (writes) {
-        reinterpret_cast<uint32_t *>(a.lengths)[r] = fits ? q.cached + q.fresh : q.cached;
-        reinterpret_cast<uint32_t *>(a.starts)[r] = plan_u32(at);
+        global_at<uint32_t>(a.lengths)[r] = fits ? q.cached + q.fresh : q.cached;
+        global_at<uint32_t>(a.starts)[r] = plan_u32(at);
       }
       at += q.fresh;
     }
@@ -142,8 +144,8 @@ __device__ __forceinline__ void page_plan(const fk_page_plan_args &a) {
   if (counts) {
     __syncthreads();
     if (tid == 0) {
-      reinterpret_cast<uint32_t *>(a.starts)[n] = plan_u32(total);
-      uint32_t *c = reinterpret_cast<uint32_t *>(a.counts);
+      global_at<uint32_t>(a.starts)[n] = plan_u32(total);
+      const auto c = global_at<uint32_t>(a.counts);
       c[0] = plan_u32(total);
       c[1] = taken;
       c[2] = refused;
@@ -151,8 +153,8 @@ __device__ __forceinline__ void page_plan(const fk_page_plan_args &a) {
     }
   }
 
-  const uint32_t *table = reinterpret_cast<const uint32_t *>(a.table);
-  const uint32_t *free_blocks = reinterpret_cast<const uint32_t *>(a.free_blocks);
+  const auto table = global_at<const uint32_t>(a.table);
+  const auto free_blocks = global_at<const uint32_t>(a.free_blocks);
   for (uint64_t t64 = (uint64_t)blockIdx.x * FK_PLAN_THREADS + tid; t64 < a.tokens;
        t64 += (uint64_t)gridDim.x * FK_PLAN_THREADS) {
     const uint32_t t = (uint32_t)t64;
@@ -181,14 +183,14 @@ __device__ __forceinline__ void page_plan(const fk_page_plan_args &a) {
           block = table[(uint64_t)r * a.table_len + page];
         } else {
           block = free_blocks[head + (uint32_t)blocks + (page - q.held)];
-          if (within == 0) reinterpret_cast<uint32_t *>(a.table)[(uint64_t)r * a.table_len + page] = block;
+          if (within == 0) global_at<uint32_t>(a.table)[(uint64_t)r * a.table_len + page] = block;
         }
         slot = plan_u32((uint64_t)block * a.block_size + within);
       }
     }
-    reinterpret_cast<uint32_t *>(a.slots)[t] = slot;
-    reinterpret_cast<uint32_t *>(a.positions)[t] = pos;
-    reinterpret_cast<uint32_t *>(a.owner)[t] = owner;
+    global_at<uint32_t>(a.slots)[t] = slot;
+    global_at<uint32_t>(a.positions)[t] = pos;
+    global_at<uint32_t>(a.owner)[t] = owner;
   }
 }
 

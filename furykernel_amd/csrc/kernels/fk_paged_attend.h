@@ -38,6 +38,7 @@
 // probability.
 #pragma once
 
+#include "fk_address.h"
 #include "fk_common.h"
 #include "fk_mfma.h"
 
@@ -46,7 +47,6 @@
 #define FK_PAGED_WAVES 4
 #define FK_PAGED_THREADS (64 * FK_PAGED_WAVES)
 #define FK_PAGED_LDS __attribute__((address_space(3)))
-#define FK_PAGED_GLOBAL __attribute__((address_space(1)))
 // s_waitcnt vmcnt(n), the other counters untouched (vmcnt's low four bits at
 // 3:0, its high two at 15:14).
 #define FK_PAGED_VMCNT(N) (((N) & 15) | (((N) >> 4) << 14) | (0x7 << 4) | (0xf << 8))
@@ -64,11 +64,10 @@ struct PagedPlan {
   uint32_t length;     // positions a table row covers
 };
 
-// A run's pair left unfinished: its first and last threadgroup, what it is.
-struct PagedJoin {
-  uint32_t last;       // the last threadgroup with a part of it; 0: none
-  uint32_t request, head, rows;
-};
+// A run's pair that ends in another threadgroup, in the workspace: the last
+// threadgroup with a part of it (0: there is no such pair), its request, its
+// first query head and how many it has.
+enum { FK_JOIN_LAST, FK_JOIN_REQUEST, FK_JOIN_HEAD, FK_JOIN_ROWS };
 
 // A pair's state in the workspace: `rows` rows of head_dim values, then the
 // maximum and the sum of each.
@@ -94,13 +93,13 @@ __device__ __forceinline__ PagedKeys paged_keys(uint32_t length, uint32_t window
 
 // A request's positions, 0 if it has no query, and its query's row.
 __device__ __forceinline__ uint32_t paged_length(const fk_paged_attend_args &a, uint32_t r) {
-  const uint32_t length = reinterpret_cast<const uint32_t *>(a.lengths)[r];
+  const uint32_t length = global_at<const uint32_t>(a.lengths)[r];
   if (!a.starts) return length;
-  const uint32_t *const s = reinterpret_cast<const uint32_t *>(a.starts) + r;
+  const auto s = global_at<const uint32_t>(a.starts) + r;
   return s[1] > s[0] && s[1] <= a.q_rows ? length : 0u;
 }
 __device__ __forceinline__ uint64_t paged_query(const fk_paged_attend_args &a, uint32_t r) {
-  return a.starts ? reinterpret_cast<const uint32_t *>(a.starts)[r + 1] - 1u : r;
+  return a.starts ? global_at<const uint32_t>(a.starts)[r + 1] - 1u : r;
 }
 
 // Over lanes l, l ^ 16, l ^ 32 and l ^ 48.
@@ -182,8 +181,8 @@ __device__ __forceinline__ void paged_attend(const fk_paged_attend_args &a, cons
   const uint32_t per_request = a.kv_heads * pl.head_tiles;
   auto length_of = [&](uint32_t r) { return paged_length(a, r); };
   const uint32_t width = a.heads * D;
-  PagedJoin *const joins = reinterpret_cast<PagedJoin *>(a.workspace);
-  float *const states = reinterpret_cast<float *>(a.workspace + gridDim.x * sizeof(PagedJoin));
+  const auto joins = global_at<u32x4>(a.workspace);
+  const auto states = global_at<float>(a.workspace + gridDim.x * sizeof(u32x4));
 
   // The units of each thread's requests, and before them.
   const uint32_t chunk = (n + FK_PAGED_THREADS - 1) / FK_PAGED_THREADS;
@@ -218,14 +217,14 @@ __device__ __forceinline__ void paged_attend(const fk_paged_attend_args &a, cons
   for (uint32_t r = blockIdx.x; r < n; r += gridDim.x)
     if (length_of(r) == 0)
       for (uint32_t e = threadIdx.x; e < width; e += FK_PAGED_THREADS) {
-        if (a.out_f32) reinterpret_cast<float *>(a.out)[r * a.out_stride + e] = 0.0f;
-        else reinterpret_cast<uint16_t *>(a.out)[r * a.out_stride + e] = 0;
+        if (a.out_f32) global_at<float>(a.out)[r * a.out_stride + e] = 0.0f;
+        else global_at<uint16_t>(a.out)[r * a.out_stride + e] = 0;
       }
 
   // This threadgroup's run of units.
   const uint32_t groups = min(gridDim.x, total);
   if (blockIdx.x >= groups) {
-    if (threadIdx.x == 0) joins[blockIdx.x].last = 0;
+    if (threadIdx.x == 0) joins[blockIdx.x] = u32x4{0, 0, 0, 0};
     return;
   }
   const uint32_t begin = (uint32_t)((uint64_t)blockIdx.x * total / groups);
@@ -243,11 +242,11 @@ __device__ __forceinline__ void paged_attend(const fk_paged_attend_args &a, cons
   }
 
   uint16_t *const kbuf = kv[wave][0], *const vbuf = kv[wave][1];
-  const char *const kpool = reinterpret_cast<const char *>(a.kpool);
-  const char *const vpool = reinterpret_cast<const char *>(a.vpool);
+  const auto kpool = global_at<const char>(a.kpool);
+  const auto vpool = global_at<const char>(a.vpool);
   const float c = a.scale * 1.4426950408889634f;  // scores to log2 units
   const uint32_t piece = lane % UNITS, krow = lane / UNITS;
-  PagedJoin join = {0, 0, 0, 0};
+  u32x4 join = {0, 0, 0, 0};
 
   for (uint32_t pos = begin; pos < end;) {
     while (pos >= at + here) {
@@ -273,14 +272,13 @@ __device__ __forceinline__ void paged_attend(const fk_paged_attend_args &a, cons
 #pragma unroll
     for (uint32_t h = 0; h < DP / 32; h++) {
       const uint32_t d = 32 * h + 8 * (lane / 16);
-      uint4 w = make_uint4(0, 0, 0, 0);
-      if (d < D)
-        w = *reinterpret_cast<const uint4 *>(reinterpret_cast<const uint16_t *>(a.q) + q_row * a.q_stride +
-                                             (uint64_t)(h0 + min(lane % 16, G - 1)) * D + d);
+      u32x4 w = {0, 0, 0, 0};
+      if (FULL || d < D)
+        w = *global_at<const u32x4>(a.q + 2 * (q_row * a.q_stride + (uint64_t)(h0 + min(lane % 16, G - 1)) * D + d));
       qf[h] = __builtin_bit_cast(vec, w);
     }
 
-    const uint32_t *const row = reinterpret_cast<const uint32_t *>(a.table) + (uint64_t)r * a.table_len;
+    const auto row = global_at<const uint32_t>(a.table) + (uint64_t)r * a.table_len;
     const uint32_t last_entry = (ks.last - 1) / a.block_size;
     uint32_t entry0 = 0, entries = 0;   // the table entries entry0 + lane, none yet
     bool held = false;
@@ -307,7 +305,7 @@ __device__ __forceinline__ void paged_attend(const fk_paged_attend_args &a, cons
         off[q] = (((uint64_t)block * a.kv_heads + g) * a.block_size + (key - entry * a.block_size)) * (2 * D);
       }
     };
-    auto load = [&](const char *pool, uint16_t *buf, bool keys) {
+    auto load = [&](global_ptr<const char> pool, uint16_t *buf, bool keys) {
 #pragma unroll
       for (uint32_t q = 0; q < LOADS; q++) {
         const uint32_t key = q * KPL + krow;
@@ -315,7 +313,7 @@ __device__ __forceinline__ void paged_attend(const fk_paged_attend_args &a, cons
                                    : (DP == 64 ? ((key >> 1) & 3u) << 1 : (key & 7u) << 1);
         const uint32_t u = piece ^ turn;
         if (FULL || u * 8 < D)
-          __builtin_amdgcn_global_load_lds((const FK_PAGED_GLOBAL void *)(pool + off[q] + u * 16),
+          __builtin_amdgcn_global_load_lds((global_ptr<const void>)(pool + off[q] + u * 16),
                                            (FK_PAGED_LDS void *)(buf + q * 512), 16, 0, 2);
       }
     };
@@ -439,7 +437,7 @@ __device__ __forceinline__ void paged_attend(const fk_paged_attend_args &a, cons
     __syncthreads();
     const bool whole = pos == pair0 && seg1 == pair0 + per_pair;
     const uint32_t side = pair0 < begin ? 0u : 1u;
-    float *const to = states + paged_state(blockIdx.x, side, pl.rows, D);
+    const auto to = states + paged_state(blockIdx.x, side, pl.rows, D);
     for (uint32_t e = threadIdx.x; e < G * D; e += FK_PAGED_THREADS) {
       const uint32_t q = e / D, d = e - q * D;
       float mm = sm[0][q];
@@ -455,8 +453,8 @@ __device__ __forceinline__ void paged_attend(const fk_paged_attend_args &a, cons
       }
       if (whole) {
         const uint64_t where = r * a.out_stride + (uint64_t)(h0 + q) * D + d;
-        if (a.out_f32) reinterpret_cast<float *>(a.out)[where] = oo / ll;
-        else reinterpret_cast<uint16_t *>(a.out)[where] = paged_round<BF16>(oo / ll);
+        if (a.out_f32) global_at<float>(a.out)[where] = oo / ll;
+        else global_at<uint16_t>(a.out)[where] = paged_round<BF16>(oo / ll);
       } else {
         to[q * D + d] = oo;
         if (d == 0) {
@@ -468,10 +466,10 @@ __device__ __forceinline__ void paged_attend(const fk_paged_attend_args &a, cons
     if (!whole && side == 1) {
       // the pair starts here and ends in a later threadgroup: that of its
       // last unit
-      join.last = (uint32_t)(((uint64_t)(pair0 + per_pair) * groups + total - 1) / total) - 1;
-      join.request = r;
-      join.head = h0;
-      join.rows = G;
+      join[FK_JOIN_LAST] = (uint32_t)(((uint64_t)(pair0 + per_pair) * groups + total - 1) / total) - 1;
+      join[FK_JOIN_REQUEST] = r;
+      join[FK_JOIN_HEAD] = h0;
+      join[FK_JOIN_ROWS] = G;
     }
     __syncthreads();  // before the next pair's rows land on the states
     pos = seg1;
@@ -488,20 +486,20 @@ __device__ __forceinline__ void paged_attend_join(const fk_paged_attend_args &a,
                                                   uint32_t groups) {
   __shared__ float so[FK_JOIN_WAVES][256], sm[FK_JOIN_WAVES], sl[FK_JOIN_WAVES];
   const uint32_t first = blockIdx.x / pl.rows, q = blockIdx.x % pl.rows;
-  const PagedJoin j = reinterpret_cast<const PagedJoin *>(a.workspace)[first];
-  if (j.last == 0 || q >= j.rows) return;
-  const float *const states = reinterpret_cast<const float *>(a.workspace + groups * sizeof(PagedJoin));
+  const u32x4 j = global_at<const u32x4>(a.workspace)[first];
+  if (j[FK_JOIN_LAST] == 0 || q >= j[FK_JOIN_ROWS]) return;
+  const auto states = global_at<const float>(a.workspace + groups * sizeof(u32x4));
   const uint32_t D = a.head_dim;
   const uint32_t lane = threadIdx.x & (FK_WAVE - 1), wave = threadIdx.x / FK_WAVE;
   float mm = -__builtin_inff(), ll = 0.0f, oo[4] = {0.0f, 0.0f, 0.0f, 0.0f};
   constexpr uint32_t U = 4;  // states at once
-  for (uint32_t w0 = first + wave; w0 <= j.last; w0 += U * FK_JOIN_WAVES) {
+  for (uint32_t w0 = first + wave; w0 <= j[FK_JOIN_LAST]; w0 += U * FK_JOIN_WAVES) {
     float m[U], l[U], o[U][4];
 #pragma unroll
     for (uint32_t s = 0; s < U; s++) {
-      const uint32_t w = min(w0 + s * FK_JOIN_WAVES, j.last);
-      const float *const from = states + paged_state(w, w == first ? 1u : 0u, pl.rows, D);
-      const bool there = w0 + s * FK_JOIN_WAVES <= j.last;
+      const uint32_t w = min(w0 + s * FK_JOIN_WAVES, j[FK_JOIN_LAST]);
+      const auto from = states + paged_state(w, w == first ? 1u : 0u, pl.rows, D);
+      const bool there = w0 + s * FK_JOIN_WAVES <= j[FK_JOIN_LAST];
       m[s] = there ? from[pl.rows * D + 2 * q] : -__builtin_inff();
       l[s] = there ? from[pl.rows * D + 2 * q + 1] : 0.0f;
 #pragma unroll
@@ -546,9 +544,9 @@ __device__ __forceinline__ void paged_attend_join(const fk_paged_attend_args &a,
     l += sl[w] * f;
     o += so[w][threadIdx.x] * f;
   }
-  const uint64_t where = j.request * a.out_stride + (uint64_t)(j.head + q) * D + threadIdx.x;
-  if (a.out_f32) reinterpret_cast<float *>(a.out)[where] = o / l;
-  else reinterpret_cast<uint16_t *>(a.out)[where] = paged_round<BF16>(o / l);
+  const uint64_t where = j[FK_JOIN_REQUEST] * a.out_stride + (uint64_t)(j[FK_JOIN_HEAD] + q) * D + threadIdx.x;
+  if (a.out_f32) global_at<float>(a.out)[where] = o / l;
+  else global_at<uint16_t>(a.out)[where] = paged_round<BF16>(o / l);
 }
 
 }  // namespace fk
