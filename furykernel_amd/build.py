@@ -50,8 +50,8 @@ def _run(cmd: list[str]) -> None:
 
 def build_runtime() -> Path:
     """The C ABI's library: the runtime and manifest (host code) and the
-    operations (fk_ops.hip, fk_serve.hip, whose kernels are built with the
-    kernels' flags)."""
+    operations (fk_ops.hip, fk_serve.hip, fk_mx4.hip, whose kernels are built
+    with the kernels' flags)."""
     tmp = RUNTIME_SO.with_suffix(".so.tmp")
     objs = []
     for src in (CSRC / "fk_runtime.cpp", CSRC / "fk_manifest.cpp"):
@@ -59,7 +59,7 @@ def build_runtime() -> Path:
         _run([HIPCC, "-c", "-fPIC", "-O2", "-std=c++17", "-Wno-unused-value", "-Wno-unused-result",
               f"-I{ROOT / 'include'}", str(src), "-o", str(obj)])
         objs.append(obj)
-    for src in (CSRC / "fk_ops.hip", CSRC / "fk_serve.hip"):
+    for src in (CSRC / "fk_ops.hip", CSRC / "fk_serve.hip", CSRC / "fk_mx4.hip"):
         obj = PACKAGE / f".{src.stem}.o"
         _run([HIPCC, "-c", "-fPIC", *KERNEL_FLAGS, f"-I{ROOT / 'include'}", str(src), "-o", str(obj)])
         objs.append(obj)

@@ -4,18 +4,25 @@
 // Each entry checks its arguments against what its kernels take, on the host
 // and before anything is queued, then launches on the caller's stream.
 
+#include "../../include/fkrocm_mx4.h"
 #include "../../include/fkrocm_serve.h"
 
 #include <hip/hip_runtime.h>
 
-#include <cstdarg>
 #include <cstdio>
 #include <cstring>
 
-#include "fk_internal.h"
+#include "fk_admit.h"
 #include "kernels/fk_page_plan.h"
 #include "kernels/fk_paged_attend.h"
 #include "kernels/fk_paged_store.h"
+
+using fk::admit;
+using fk::check_spans;
+using fk::launched;
+using fk::Refusal;
+using fk::Span;
+using fk::stream_of;
 
 namespace {
 
@@ -36,56 +43,6 @@ template <bool BF16>
 __global__ void __launch_bounds__(64 * FK_JOIN_WAVES)
     op_paged_attend_join(fk_paged_attend_args a, fk::PagedPlan pl, uint32_t groups) {
   fk::paged_attend_join<BF16>(a, pl, groups);
-}
-
-int use_device(fk_ctx *ctx) {
-  const hipError_t e = hipSetDevice(ctx->device);
-  return e == hipSuccess ? FK_OK : fk_fail(ctx, FK_ERR_HIP, "hipSetDevice: %s", hipGetErrorString(e));
-}
-
-int launched(fk_ctx *ctx, const char *what) {
-  const hipError_t e = hipGetLastError();
-  return e == hipSuccess ? FK_OK : fk_fail(ctx, FK_ERR_HIP, "%s: %s", what, hipGetErrorString(e));
-}
-
-hipStream_t stream_of(fk_ctx *ctx, fk_stream *s) { return s ? s->stream : ctx->stream; }
-
-// What a check of a call's arguments finds: FK_OK, or a status and the reason.
-struct Refusal {
-  char text[512] = "";
-  __attribute__((format(printf, 3, 4))) int operator()(int status, const char *fmt, ...) {
-    va_list ap;
-    va_start(ap, fmt);
-    vsnprintf(text, sizeof text, fmt, ap);
-    va_end(ap);
-    return status;
-  }
-};
-
-// A span of device memory a call reads or writes.
-struct Span {
-  const char *name;
-  uint64_t addr, bytes;
-};
-
-bool meets(const Span &a, const Span &b) {
-  return a.bytes && b.bytes && a.addr < b.addr + b.bytes && b.addr < a.addr + a.bytes;
-}
-
-// Every span there and aligned; no output over another span.
-int check_spans(Refusal &no, const Span *reads, size_t n_reads, const Span *writes, size_t n_writes, uint32_t align) {
-  for (size_t i = 0; i < n_reads + n_writes; i++) {
-    const Span &s = i < n_reads ? reads[i] : writes[i - n_reads];
-    if (s.bytes && (s.addr == 0 || s.addr % align))
-      return no(FK_ERR_ARG, "%s is null or not %u-byte aligned", s.name, align);
-  }
-  for (size_t i = 0; i < n_writes; i++) {
-    for (size_t j = 0; j < n_reads; j++)
-      if (meets(writes[i], reads[j])) return no(FK_ERR_ARG, "%s overlaps %s", writes[i].name, reads[j].name);
-    for (size_t j = 0; j < i; j++)
-      if (meets(writes[i], writes[j])) return no(FK_ERR_ARG, "%s overlaps %s", writes[i].name, writes[j].name);
-  }
-  return FK_OK;
 }
 
 // The attention's launch for these sizes: head_dim's tile width, its
@@ -143,7 +100,11 @@ void queue_attend(const fk_paged_attend_args &a, const AttendLaunch &l, hipStrea
     hipLaunchKernelGGL((op_paged_attend<DP, false, BF16>), dim3(l.groups), dim3(FK_PAGED_THREADS), 0, s, a, l.plan);
 }
 
-int check(const fk_page_plan_args &a, Refusal &no) {
+}  // namespace
+
+namespace fk {
+
+static int check(const fk_page_plan_args &a, Refusal &no) {
   if (a.requests == 0 || a.requests >= 1u << 24 || a.table_len == 0 || a.block_size == 0)
     return no(FK_ERR_ARG, "%u requests (1 to 2^24 - 1), tables of %u blocks of %u", a.requests, a.table_len,
               a.block_size);
@@ -162,11 +123,11 @@ int check(const fk_page_plan_args &a, Refusal &no) {
 }
 
 // Units of 16 elements that a token's rows have: one thread's work.
-uint64_t store_units(const fk_paged_store_args &a) {
+static uint64_t store_units(const fk_paged_store_args &a) {
   return ((a.q ? (uint64_t)a.heads : 0) + 2ull * a.kv_heads) * (a.head_dim / 16);
 }
 
-int check(const fk_paged_store_args &a, Refusal &no) {
+static int check(const fk_paged_store_args &a, Refusal &no) {
   if (a.kv_heads == 0 || a.head_dim == 0 || a.head_dim % 16 || a.head_dim > 256 || (a.q && a.heads == 0))
     return no(FK_ERR_ARG, "%u heads over %u of width %u (a multiple of 16, at most 256)", a.heads, a.kv_heads,
               a.head_dim);
@@ -199,7 +160,7 @@ int check(const fk_paged_store_args &a, Refusal &no) {
   return check_spans(no, reads, 6, writes, 3, 16);
 }
 
-int check(const fk_paged_attend_args &a, const AttendLaunch &l, Refusal &no) {
+static int check(const fk_paged_attend_args &a, const AttendLaunch &l, Refusal &no) {
   if (l.groups == 0)
     return no(FK_ERR_ARG, "%u requests, %u heads over %u of width %u, %u blocks of %u, tables of %u: it takes %s",
               a.requests, a.heads, a.kv_heads, a.head_dim, a.blocks, a.block_size, a.table_len, l.why);
@@ -225,16 +186,10 @@ int check(const fk_paged_attend_args &a, const AttendLaunch &l, Refusal &no) {
   return check_spans(no, reads, 6, writes, 2, 16);
 }
 
-// A call's arguments as its entry takes them, or the refusal on the context.
-template <typename Args, typename... More>
-int admit(fk_ctx *ctx, const char *what, const Args *a, const More &...more) {
-  if (!ctx || !a) return fk_fail(ctx, FK_ERR_ARG, "%s: null argument", what);
-  Refusal no;
-  if (int st = check(*a, more..., no)) return fk_fail(ctx, st, "%s: %s", what, no.text);
-  return use_device(ctx);
-}
+}  // namespace fk
 
-}  // namespace
+using fk::check;
+using fk::store_units;
 
 extern "C" int fk_serve_check(const char *entry, const void *args, size_t args_bytes, char *err, size_t err_cap) {
   Refusal no;
@@ -254,6 +209,12 @@ extern "C" int fk_serve_check(const char *entry, const void *args, size_t args_b
   } else if (is("fk_paged_attend", sizeof(fk_paged_attend_args))) {
     const fk_paged_attend_args &a = *static_cast<const fk_paged_attend_args *>(args);
     st = check(a, attend_launch(a), no);
+  } else if (is("fk_mx4_quantize", sizeof(fk_mx4_quantize_args))) {
+    st = check(*static_cast<const fk_mx4_quantize_args *>(args), no);
+  } else if (is("fk_mx4_dequantize", sizeof(fk_mx4_dequantize_args))) {
+    st = check(*static_cast<const fk_mx4_dequantize_args *>(args), no);
+  } else if (is("fk_mx4_gemm", sizeof(fk_mx4_gemm_args))) {
+    st = check(*static_cast<const fk_mx4_gemm_args *>(args), no);
   } else if (st == FK_OK) {
     st = no(FK_ERR_NOT_FOUND, "no operator %s", entry ? entry : "(null)");
   }

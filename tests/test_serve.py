@@ -8,11 +8,13 @@ from pathlib import Path
 
 import pytest
 
-from furykernel_amd import paged, runtime
+from furykernel_amd import mx4, paged, runtime
 from furykernel_amd.kernels import LaunchError
 
-HEADER = (Path(__file__).resolve().parents[1] / "include" / "fkrocm_serve.h").read_text()
-STRUCTS = {"fk_page_plan_args": paged.PagePlanArgs, "fk_paged_store_args": paged.PagedStoreArgs,
+INCLUDE = Path(__file__).resolve().parents[1] / "include"
+HEADER = (INCLUDE / "fkrocm_serve.h").read_text() + (INCLUDE / "fkrocm_mx4.h").read_text()
+STRUCTS = {"fk_mx4_quantize_args": mx4.QuantizeArgs, "fk_mx4_dequantize_args": mx4.DequantizeArgs,
+           "fk_mx4_gemm_args": mx4.GemmArgs, "fk_page_plan_args": paged.PagePlanArgs, "fk_paged_store_args": paged.PagedStoreArgs,
            "fk_paged_attend_args": paged.PagedAttendArgs}
 
 
@@ -207,3 +209,56 @@ def test_the_check_refuses_unknown_entries_and_sizes_of_arguments():
     for entry in (lib.fk_page_plan, lib.fk_paged_store, lib.fk_paged_attend):
         assert entry(None, ctypes.byref(args), None) == -2
     assert lib.fk_paged_attend_workspace(None) == 0
+
+
+# 4-bit microscaled matrices ----------------------------------------------------
+
+
+def matrix(rows, k):
+    m = mx4.Mx4Matrix.__new__(mx4.Mx4Matrix)
+    lib = runtime.library()
+    m.device, m.rows, m.k = DEVICE, rows, k
+    m.codes, m.scales = FakeBuffer(lib.fk_mx4_codes_bytes(rows, k)), FakeBuffer(lib.fk_mx4_scales_bytes(rows, k))
+    return m
+
+
+def test_mx4_matrices_hold_whole_tiles():
+    lib = runtime.library()
+    for rows, k, tiles in ((1, 1, 1), (16, 256, 1), (17, 256, 2), (16, 257, 2), (100, 3080, 7 * 13)):
+        assert lib.fk_mx4_codes_bytes(rows, k) == tiles * 2048 and lib.fk_mx4_scales_bytes(rows, k) == tiles * 128
+    for rows, k in ((0, 5), (5, 0), (0xFFFFFFFF, 32), (1 << 30, 1 << 30)):
+        assert lib.fk_mx4_codes_bytes(rows, k) == 0 == lib.fk_mx4_scales_bytes(rows, k)
+
+
+def test_mx4_operations_refuse_what_does_not_fit():
+    a, b = matrix(20, 100), matrix(33, 100)
+    mx4.Quantize(DEVICE, FakeBuffer(4 * 2000), a)
+    mx4.Quantize(DEVICE, FakeBuffer(2 * (19 * 101 + 100 + 3)), a, "bf16", x_stride=101, x_offset=3)
+    mx4.Dequantize(DEVICE, a, FakeBuffer(4 * 2000), scales=FakeBuffer(4 * 20 * 4))
+    mx4.Gemm(DEVICE, a, b, FakeBuffer(4 * 20 * 33))
+    big = FakeBuffer(1 << 20)
+    short = matrix(20, 100)
+    short.codes = FakeBuffer(short.codes.size - 1)
+    bad = [lambda: mx4.Quantize(DEVICE, FakeBuffer(4 * 2000 - 1), a),
+           lambda: mx4.Quantize(DEVICE, big, a, "i8"), lambda: mx4.Quantize(DEVICE, big, a, x_stride=99),
+           lambda: mx4.Quantize(DEVICE, big, a, x_offset=-1), lambda: mx4.Quantize(DEVICE, big, short),
+           lambda: mx4.Quantize(DEVICE, FakeBuffer(8000, ptr=FakeBuffer.at + 2), a),
+           lambda: mx4.Quantize(DEVICE, FakeBuffer(8000, FakeDevice()), a),
+           lambda: mx4.Quantize(DEVICE, FakeBuffer(8000, ptr=a.codes.ptr), a),
+           lambda: mx4.Dequantize(DEVICE, a, FakeBuffer(4 * 2000 - 1)),
+           lambda: mx4.Dequantize(DEVICE, a, big, y_stride=99),
+           lambda: mx4.Dequantize(DEVICE, a, big, scales=FakeBuffer(4 * 20 * 4 - 1)),
+           lambda: mx4.Dequantize(DEVICE, a, big, scales=big),
+           lambda: mx4.Dequantize(DEVICE, a, FakeBuffer(8000, ptr=a.scales.ptr)),
+           lambda: mx4.Gemm(DEVICE, a, b, FakeBuffer(4 * 20 * 33 - 1)),
+           lambda: mx4.Gemm(DEVICE, a, matrix(33, 101), big), lambda: mx4.Gemm(DEVICE, a, b, big, "i8"),
+           lambda: mx4.Gemm(DEVICE, a, b, big, c_stride=32), lambda: mx4.Gemm(DEVICE, short, b, big),
+           lambda: mx4.Gemm(DEVICE, a, b, FakeBuffer(1 << 13, ptr=b.codes.ptr)), lambda: mx4.Mx4Matrix(DEVICE, 0, 5),
+           lambda: mx4.Mx4Matrix(DEVICE, -1, 5)]
+    for i, call in enumerate(bad):
+        with pytest.raises(LaunchError):
+            call()
+            print(f"call {i} was taken")
+    lib = runtime.library()
+    for entry in (lib.fk_mx4_quantize, lib.fk_mx4_dequantize, lib.fk_mx4_gemm):
+        assert entry(None, None, None) == -2
