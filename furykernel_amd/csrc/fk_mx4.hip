@@ -4,6 +4,7 @@
 #include "../../include/fkrocm_mx4.h"
 
 #include <hip/hip_runtime.h>
+#include <cstdlib>
 
 #include "fk_admit.h"
 #include "kernels/fk_mx4.h"
@@ -30,6 +31,11 @@ __global__ void __launch_bounds__(FK_MX4_THREADS) op_mx4_dequantize(fk_mx4_dequa
 template <uint32_t MB, uint32_t NB, uint32_t W, int T>
 __global__ void __launch_bounds__(64 * W) op_mx4_gemm_few(fk_mx4_gemm_args a) {
   fk::mx4_gemm_few<MB, NB, W, T>(a);
+}
+
+template <uint32_t GB, int T>
+__global__ void __launch_bounds__(256, GB == 4 ? 1 : 2) op_mx4_gemm_many(fk_mx4_gemm_args a) {
+  fk::mx4_gemm_many<GB, T>(a);
 }
 
 uint64_t codes_bytes(uint32_t rows, uint32_t k) { return (uint64_t)fk::mx4_row_tiles(rows) * fk::mx4_pairs(k) * 2048; }
@@ -75,6 +81,14 @@ template <uint32_t MB, uint32_t NB, uint32_t W, int T>
 void queue_few(const fk_mx4_gemm_args &a, hipStream_t s) {
   const uint32_t tm = (fk::mx4_row_tiles(a.m) + MB - 1) / MB, tn = (fk::mx4_row_tiles(a.n) + NB - 1) / NB;
   hipLaunchKernelGGL((op_mx4_gemm_few<MB, NB, W, T>), dim3(tm * tn), dim3(64 * W), 0, s, a);
+}
+
+template <uint32_t GB, int T>
+void queue_many(const fk_mx4_gemm_args &a, hipStream_t s) {
+  constexpr uint32_t side = fk::mx4_many_tiles<GB>();
+  const uint32_t tm = (fk::mx4_row_tiles(a.m) + side - 1) / side, tn = (fk::mx4_row_tiles(a.n) + side - 1) / side;
+  const uint32_t most = GB == 4 ? 256 : 512;  // as many as the chip holds at once
+  hipLaunchKernelGGL((op_mx4_gemm_many<GB, T>), dim3(tm * tn < most ? tm * tn : most), dim3(256), fk::mx4_many_lds<GB>(), s, a);
 }
 
 }  // namespace
@@ -156,8 +170,20 @@ extern "C" int fk_mx4_gemm(fk_ctx *ctx, const fk_mx4_gemm_args *a, fk_stream *st
   const hipStream_t s = stream_of(ctx, stream);
   of_type(a->c_type, [&](auto t) {
     constexpr int T = decltype(t)::value;
-    if (a->m <= 16) queue_few<1, 1, 8, T>(*a, s);
-    else queue_few<4, 4, 4, T>(*a, s);
+    const char *f = getenv("FK_MX4_FORM");
+    const int form = f ? atoi(f) : (a->m <= 16 ? 0 : a->m <= 128 ? 3 : 5);
+    switch (form) {
+      case 0: queue_few<1, 1, 8, T>(*a, s); break;
+      case 1: queue_few<1, 2, 8, T>(*a, s); break;
+      case 2: queue_few<2, 2, 8, T>(*a, s); break;
+      case 3: queue_few<4, 4, 4, T>(*a, s); break;
+      case 4: queue_many<2, T>(*a, s); break;
+      case 6: queue_few<4, 2, 8, T>(*a, s); break;
+      case 7: queue_few<4, 1, 8, T>(*a, s); break;
+      case 8: queue_few<2, 1, 8, T>(*a, s); break;
+      case 9: queue_few<8, 2, 4, T>(*a, s); break;
+      default: queue_many<4, T>(*a, s);
+    }
   });
   return launched(ctx, "fk_mx4_gemm");
 }

@@ -127,4 +127,294 @@ __device__ __forceinline__ void mx4_gemm_few(const fk_mx4_gemm_args &a) {
   }
 }
 
+// Many rows: v_mfma_scale_f32_32x32x64_f8f6f4, twice the rate of the 16 × 16
+// form on this chip (36 cycles for twice its work, against 29): lane l holds a
+// block of row l mod 32, k 32 (l div 32) .. + 31, and D[8 (r div 4) + 4 (l div
+// 32) + r mod 4][l mod 32] as register r.
+//
+// A threadgroup of 4 wavefronts takes a tile of 2 GB × 2 GB blocks of 32 × 32
+// (256 × 256 at GB 4), each wavefront GB × GB of them, accumulated in AGPRs.
+// A step is one tile of k (128): the operands' 1 KB blocks go straight into a
+// ring of 4 LDS stages, two steps ahead of the one being read, and are read
+// back 16 bytes a lane, 16 lanes 256 consecutive bytes; a step's loads, reads
+// and matrix operations are interleaved, one barrier a step.  The scales come
+// to registers, two steps' in one load of two bytes a lane, a pair of steps
+// ahead.
+#define FK_MX4_STAGES 4
+#define FK_MX4_LDS __attribute__((address_space(3)))
+template <uint32_t GB>
+__host__ __device__ constexpr uint32_t mx4_many_lds() {
+  return FK_MX4_STAGES * 2 * 4 * GB * 1024;
+}
+// Row tiles of a tile's side.
+template <uint32_t GB>
+__host__ __device__ constexpr uint32_t mx4_many_tiles() {
+  return 4 * GB;
+}
+
+template <int TILE>
+__device__ __forceinline__ fk_float16v mx4_mfma32(u32x4 b, uint32_t bs, u32x4 a, uint32_t as, fk_float16v c) {
+  return __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(mx4_operand(b), mx4_operand(a), c, 4, 4, TILE, (int)bs, TILE,
+                                                         (int)as);
+}
+
+// A wavefront's 32 GB rows of 32 GB columns into C, through its own share of
+// an LDS stage: of 32 rows at a time RB bytes each are written as the
+// operation left them, a lane 4 columns of a row, and read back a row's
+// consecutive 16 bytes a lane, so that stores are RB whole bytes of a row.
+// wide: C's rows are 16-byte aligned.
+template <uint32_t GB, int T>
+__device__ __forceinline__ void mx4_store_many(const fk_mx4_gemm_args &a, bool wide, uint32_t m0, uint32_t n0,
+                                               fk_float16v (&acc)[GB][GB], char *stage) {
+  constexpr uint32_t RB = GB * 64, BYTES = mx4_bytes_of(T), COLS = RB / BYTES, UNITS = RB / 16, EACH = 16 / BYTES;
+  const uint32_t lane = threadIdx.x % FK_WAVE;
+  // 16-byte unit u of row m at place u ^ turn(m): no bank twice in 16 lanes
+  auto place = [](uint32_t m, uint32_t u) { return m * RB + (u ^ (UNITS == 16 ? m & 15u : (m >> 1) & 7u)) * 16; };
+#pragma unroll
+  for (uint32_t i = 0; i < GB; i++)
+#pragma unroll
+    for (uint32_t c = 0; c < 32 * GB / COLS; c++) {
+      const uint32_t row = lane % 32;
+      // (taken here: rounded further ahead, they would not fit the registers)
+#pragma unroll
+      for (uint32_t j = 0; j < COLS / 32; j++) asm volatile("" : "+a"(acc[i][c * (COLS / 32) + j]));
+#pragma unroll
+      for (uint32_t j = 0; j < COLS / 32; j++)
+#pragma unroll
+        for (uint32_t q = 0; q < 4; q++) {
+          const fk_float16v &v = acc[i][c * (COLS / 32) + j];
+          const uint32_t col = 32 * j + 8 * q + 4 * (lane / 32);
+          char *const to = stage + place(row, col / EACH) + col % EACH * BYTES;
+          if constexpr (T == FK_T_F32) {
+            *reinterpret_cast<fk_float4v *>(to) = fk_float4v{v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]};
+          } else if constexpr (T == FK_T_F16) {
+            typedef _Float16 half4 __attribute__((ext_vector_type(4)));
+            *reinterpret_cast<half4 *>(to) =
+                half4{(_Float16)v[4 * q], (_Float16)v[4 * q + 1], (_Float16)v[4 * q + 2], (_Float16)v[4 * q + 3]};
+          } else {
+            typedef __bf16 bf4 __attribute__((ext_vector_type(4)));
+            *reinterpret_cast<bf4 *>(to) =
+                bf4{(__bf16)v[4 * q], (__bf16)v[4 * q + 1], (__bf16)v[4 * q + 2], (__bf16)v[4 * q + 3]};
+          }
+        }
+      asm volatile("" ::: "memory");
+#pragma unroll
+      for (uint32_t t = 0; t < 32 * UNITS / FK_WAVE; t++) {
+        const uint32_t r = t * (FK_WAVE / UNITS) + lane / UNITS, u = lane % UNITS;
+        const u32x4 w = *reinterpret_cast<const u32x4 *>(stage + place(r, u));
+        const uint32_t m = m0 + 32 * i + r, n = n0 + c * COLS + u * EACH;
+        const uint64_t at = a.c + ((uint64_t)m * a.c_stride + n) * BYTES;
+        if (m < a.m && n < a.n) {
+          if (wide && n + EACH <= a.n) {
+            *global_at<u32x4>(at) = w;
+          } else {
+#pragma unroll
+            for (uint32_t e = 0; e < EACH; e++)
+              if (n + e < a.n) {
+                if constexpr (BYTES == 4) global_at<uint32_t>(at)[e] = w[e];
+                else global_at<uint16_t>(at)[e] = (uint16_t)(w[e / 2] >> (16 * (e % 2)));
+              }
+          }
+        }
+      }
+      asm volatile("" ::: "memory");  // read before the next rows are written
+    }
+}
+
+template <uint32_t GB, int T>
+__device__ __forceinline__ void mx4_gemm_many(const fk_mx4_gemm_args &a) {
+  extern __shared__ u32x4 mx4_lds[];
+  constexpr uint32_t ROWS = mx4_many_tiles<GB>();  // row tiles of an operand's slab
+  constexpr uint32_t SLAB = ROWS * 1024;           // its bytes a step
+  constexpr uint32_t STAGE = 2 * SLAB;             // A's, then B's
+  constexpr uint32_t Q = ROWS / 4;                 // loads of an operand a wavefront makes a step
+  constexpr uint32_t H = GB / 2;                   // A's blocks of half a step
+  const uint32_t lane = threadIdx.x % FK_WAVE;
+  const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x / FK_WAVE);
+  const uint32_t wm = wave & 1, wn = wave >> 1;
+  const uint32_t pairs = mx4_pairs(a.k), rows_a = mx4_row_tiles(a.m), rows_b = mx4_row_tiles(a.n);
+  const uint32_t tiles_m = (rows_a + ROWS - 1) / ROWS, tiles = tiles_m * ((rows_b + ROWS - 1) / ROWS);
+
+  // A tile's sources.  A wavefront's loads: row tiles Q wave + q of each slab
+  // (past the last: the last again, whose blocks are not stored), a lane's 16
+  // bytes in their place; the scales of its blocks: of row l mod 32, block 2 h
+  // + l div 32.
+  const uint32_t half = lane % 32 / 16, place = lane / 32 * 16 + lane % 16;
+  uint32_t tm, tn;
+  __amdgpu_buffer_rsrc_t a_src, b_src, as_src, bs_src;
+  uint32_t a_at[Q], b_at[Q], as_at[GB], bs_at[GB];
+  auto sources = [&](uint32_t tile) {
+    tm = tile % tiles_m * ROWS;
+    tn = tile / tiles_m * ROWS;
+    const uint32_t have_a = min(rows_a - tm, ROWS), have_b = min(rows_b - tn, ROWS);
+    a_src = buffer((const void *)(a.a_codes + (uint64_t)tm * pairs * 2048), (size_t)have_a * pairs * 2048);
+    b_src = buffer((const void *)(a.b_codes + (uint64_t)tn * pairs * 2048), (size_t)have_b * pairs * 2048);
+    as_src = buffer((const void *)(a.a_scales + (uint64_t)tm * pairs * 128), (size_t)have_a * pairs * 128);
+    bs_src = buffer((const void *)(a.b_scales + (uint64_t)tn * pairs * 128), (size_t)have_b * pairs * 128);
+#pragma unroll
+    for (uint32_t q = 0; q < Q; q++) {
+      a_at[q] = min(wave * Q + q, have_a - 1) * pairs * 2048 + lane * 16;
+      b_at[q] = min(wave * Q + q, have_b - 1) * pairs * 2048 + lane * 16;
+    }
+#pragma unroll
+    for (uint32_t i = 0; i < GB; i++) {
+      as_at[i] = min(2 * (wm * GB + i) + half, have_a - 1) * pairs * 128 + place * 2;
+      bs_at[i] = min(2 * (wn * GB + i) + half, have_b - 1) * pairs * 128 + place * 2;
+    }
+  };
+  FK_MX4_LDS char *const stage0 = (FK_MX4_LDS char *)mx4_lds + wave * Q * 1024;
+  const uint32_t ra = (2 * wm * GB + half) * 64 + place, rb = SLAB / 16 + (2 * wn * GB + half) * 64 + place;
+
+  fk_float16v acc[GB][GB];
+  u32x4 fa0[GB][2], fb0[GB][2], fa1[GB][2], fb1[GB][2];
+  uint32_t sa0[GB][2], sb0[GB][2], sa1[GB][2], sb1[GB][2];
+#define FK_MX4_PIN(X) asm volatile("" : "+v"(X))
+#define FK_MX4_PIN_ACC()                                                    \
+  _Pragma("unroll") for (uint32_t i_ = 0; i_ < GB; i_++)                    \
+  _Pragma("unroll") for (uint32_t j_ = 0; j_ < GB; j_++) asm volatile("" : "+a"(acc[i_][j_]))
+#define FK_MX4_VMCNT(N) __builtin_amdgcn_s_waitcnt(((N) & 15) | (((N) >> 4) << 14) | (0x7 << 4) | (0xf << 8))
+#define FK_MX4_BARRIER()                  \
+  do {                                    \
+    asm volatile("" ::: "memory");        \
+    __builtin_amdgcn_s_barrier();         \
+    asm volatile("" ::: "memory");        \
+  } while (0)
+#define FK_MX4_SCALES(SA, SB, P)                                                                              \
+  _Pragma("unroll") for (uint32_t i_ = 0; i_ < GB; i_++)                                                      \
+  _Pragma("unroll") for (uint32_t h_ = 0; h_ < 2; h_++) {                                                     \
+    SA[i_][h_] = __builtin_amdgcn_raw_buffer_load_b16(as_src, as_at[i_] + 64 * h_, (P) * 128, 0);             \
+    SB[i_][h_] = __builtin_amdgcn_raw_buffer_load_b16(bs_src, bs_at[i_] + 64 * h_, (P) * 128, 0);             \
+  }
+#define FK_MX4_MFMAS(TILE, FA, FB, SA, SB, I0)                                                                \
+  _Pragma("unroll") for (uint32_t h = 0; h < 2; h++)                                                          \
+  _Pragma("unroll") for (uint32_t i = (I0); i < (I0) + H; i++)                                                \
+  _Pragma("unroll") for (uint32_t j = 0; j < GB; j++)                                                         \
+      acc[i][j] = mx4_mfma32<TILE>(FB[j][h], SB[j][h], FA[i][h], SA[i][h], acc[i][j])
+  // One step in two halves, A's blocks 0 .. H - 1 then the rest against all
+  // of B's.  The first half issues the loads of A's part of step LOAD (and,
+  // where TILE is 0, those of the next pair's scales before them), and reads
+  // the next step's B blocks and A blocks 0 .. H - 1; the second B's loads and
+  // the next step's other A blocks.  WAIT: the loads that may still be in
+  // flight when the step begins.
+#define FK_MX4_STEP(TILE, FA, FB, NA, NB, SA, SB, NSA, NSB, WAIT, NEXT_PAIR, LOAD, ST_LOAD, ST_READ)          \
+  do {                                                                                                        \
+    FK_MX4_VMCNT(WAIT);                                                                                       \
+    FK_MX4_BARRIER();                                                                                         \
+    __builtin_amdgcn_sched_barrier(0);                                                                        \
+    const uint32_t so_ = (LOAD) * 1024;                                                                       \
+    FK_MX4_LDS char *d_ = stage0 + (ST_LOAD) * STAGE;                                                         \
+    const u32x4 *s_ = mx4_lds + (ST_READ) * (STAGE / 16);                                                     \
+    if (TILE == 0) FK_MX4_SCALES(NSA, NSB, NEXT_PAIR)                                                         \
+    _Pragma("unroll") for (uint32_t q = 0; q < Q; q++)                                                        \
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(a_src, d_ + q * 1024, 16, a_at[q], so_, 0, 0);               \
+    _Pragma("unroll") for (uint32_t j = 0; j < GB; j++)                                                       \
+    _Pragma("unroll") for (uint32_t h = 0; h < 2; h++) NB[j][h] = s_[rb + 128 * j + 32 * h];                  \
+    _Pragma("unroll") for (uint32_t i = 0; i < H; i++)                                                        \
+    _Pragma("unroll") for (uint32_t h = 0; h < 2; h++) NA[i][h] = s_[ra + 128 * i + 32 * h];                  \
+    FK_MX4_MFMAS(TILE, FA, FB, SA, SB, 0);                                                                    \
+    _Pragma("unroll") for (uint32_t g_ = 0; g_ < 2 * H * GB; g_++) {                                          \
+      __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);                                                      \
+      __builtin_amdgcn_sched_group_barrier(0x020, TILE == 0 ? 2 : 1, 0);                                      \
+      __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);                                                      \
+    }                                                                                                         \
+    __builtin_amdgcn_sched_barrier(0);                                                                        \
+    _Pragma("unroll") for (uint32_t i = H; i < GB; i++)                                                       \
+    _Pragma("unroll") for (uint32_t h = 0; h < 2; h++) FK_MX4_PIN(FA[i][h]);                                  \
+    _Pragma("unroll") for (uint32_t q = 0; q < Q; q++)                                                        \
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(b_src, d_ + SLAB + q * 1024, 16, b_at[q], so_, 0, 0);        \
+    _Pragma("unroll") for (uint32_t i = H; i < GB; i++)                                                       \
+    _Pragma("unroll") for (uint32_t h = 0; h < 2; h++) NA[i][h] = s_[ra + 128 * i + 32 * h];                  \
+    FK_MX4_MFMAS(TILE, FA, FB, SA, SB, H);                                                                    \
+    _Pragma("unroll") for (uint32_t g_ = 0; g_ < H * GB; g_++) {                                              \
+      __builtin_amdgcn_sched_group_barrier(0x008, 2, 0);                                                      \
+      __builtin_amdgcn_sched_group_barrier(0x020, 1, 0);                                                      \
+      __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);                                                      \
+    }                                                                                                         \
+    __builtin_amdgcn_sched_barrier(0);                                                                        \
+    _Pragma("unroll") for (uint32_t j = 0; j < GB; j++)                                                       \
+    _Pragma("unroll") for (uint32_t h = 0; h < 2; h++) FK_MX4_PIN(NB[j][h]);                                  \
+    _Pragma("unroll") for (uint32_t i = 0; i < H; i++)                                                        \
+    _Pragma("unroll") for (uint32_t h = 0; h < 2; h++) FK_MX4_PIN(NA[i][h]);                                  \
+    FK_MX4_PIN_ACC();                                                                                         \
+  } while (0)
+
+  // At step s (after its barrier) step s's blocks are in registers but for
+  // A's second half, on its way from stage s mod 4, and steps s + 1 and s + 2
+  // are in their stages or on their way there.  Loads past the last step
+  // repeat it into stages that no step reads, so every wait counts the same
+  // loads.
+  const uint32_t steps = 2 * pairs, last = steps - 1;
+#define FK_MX4_T(X) ((X) < last ? (X) : last)
+  // The first three steps of a tile, and its first scales, on their way.
+#define FK_MX4_FIRST()                                                                                        \
+  do {                                                                                                        \
+    FK_MX4_SCALES(sa0, sb0, 0)                                                                                \
+    _Pragma("unroll") for (uint32_t t_ = 0; t_ + 1 < FK_MX4_STAGES; t_++) {                                   \
+      const uint32_t so_ = FK_MX4_T(t_) * 1024;                                                               \
+      FK_MX4_LDS char *d_ = stage0 + t_ * STAGE;                                                              \
+      _Pragma("unroll") for (uint32_t q = 0; q < Q; q++) {                                                    \
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(a_src, d_ + q * 1024, 16, a_at[q], so_, 0, 0);               \
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(b_src, d_ + SLAB + q * 1024, 16, b_at[q], so_, 0, 0);        \
+      }                                                                                                       \
+    }                                                                                                         \
+  } while (0)
+  // Tile after tile, the next one's first loads under this one's stores: the
+  // stores go by way of the fourth stage, which step 0 loads.
+  const bool wide = a.c_stride * mx4_bytes_of(T) % 16 == 0 && a.c % 16 == 0;
+  sources(blockIdx.x);
+  FK_MX4_FIRST();
+  for (uint32_t tile = blockIdx.x; tile < tiles; tile += gridDim.x) {
+#pragma unroll
+  for (uint32_t i = 0; i < GB; i++)
+#pragma unroll
+    for (uint32_t j = 0; j < GB; j++)
+#pragma unroll
+      for (int r = 0; r < 16; r++) acc[i][j][r] = 0.0f;
+  // step 0 landed (what was stored since is waited for with it)
+  FK_MX4_VMCNT(2 * Q * (FK_MX4_STAGES - 2));
+  FK_MX4_BARRIER();
+#pragma unroll
+  for (uint32_t i = 0; i < GB; i++)
+#pragma unroll
+    for (uint32_t h = 0; h < 2; h++) {
+      fb0[i][h] = mx4_lds[rb + 128 * i + 32 * h];
+      fa0[i][h] = mx4_lds[ra + 128 * i + 32 * h];
+    }
+#pragma unroll
+  for (uint32_t i = 0; i < GB; i++)
+#pragma unroll
+    for (uint32_t h = 0; h < 2; h++) {
+      FK_MX4_PIN(fb0[i][h]);
+      if (i < H) FK_MX4_PIN(fa0[i][h]);
+    }
+  for (uint32_t p = 0; p < pairs; p++) {
+    const uint32_t s = 2 * p, next = p + 1 < pairs ? p + 1 : p;
+    FK_MX4_STEP(0, fa0, fb0, fa1, fb1, sa0, sb0, sa1, sb1, 2 * Q, next, FK_MX4_T(s + 3), (s + 3) % 4, (s + 1) % 4);
+    FK_MX4_STEP(1, fa1, fb1, fa0, fb0, sa0, sb0, sa1, sb1, 2 * Q + 4 * GB, next, FK_MX4_T(s + 4), s % 4, (s + 2) % 4);
+#pragma unroll
+    for (uint32_t i = 0; i < GB; i++)
+#pragma unroll
+      for (uint32_t h = 0; h < 2; h++) sa0[i][h] = sa1[i][h], sb0[i][h] = sb1[i][h];
+  }
+  // Nothing lands in LDS any more, and no wavefront reads it.
+  __builtin_amdgcn_s_waitcnt(0);
+  FK_MX4_BARRIER();
+  const uint32_t m = 16 * tm + 32 * wm * GB, n = 16 * tn + 32 * wn * GB;
+  if (tile + gridDim.x < tiles) {
+    sources(tile + gridDim.x);
+    FK_MX4_FIRST();
+  }
+  mx4_store_many<GB, T>(a, wide, m, n, acc, reinterpret_cast<char *>(mx4_lds) + 3 * STAGE + wave * (STAGE / 4));
+  }
+#undef FK_MX4_PIN
+#undef FK_MX4_PIN_ACC
+#undef FK_MX4_VMCNT
+#undef FK_MX4_BARRIER
+#undef FK_MX4_SCALES
+#undef FK_MX4_MFMAS
+#undef FK_MX4_STEP
+#undef FK_MX4_FIRST
+#undef FK_MX4_T
+}
+
 }  // namespace fk
