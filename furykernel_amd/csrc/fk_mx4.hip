@@ -4,7 +4,10 @@
 #include "../../include/fkrocm_mx4.h"
 
 #include <hip/hip_runtime.h>
-#include <cstdlib>
+
+#include <cmath>
+#include <iterator>
+#include <utility>
 
 #include "fk_admit.h"
 #include "kernels/fk_mx4.h"
@@ -33,9 +36,14 @@ __global__ void __launch_bounds__(64 * W) op_mx4_gemm_few(fk_mx4_gemm_args a) {
   fk::mx4_gemm_few<MB, NB, W, T>(a);
 }
 
-template <uint32_t GB, int T>
-__global__ void __launch_bounds__(256, GB == 4 ? 1 : 2) op_mx4_gemm_many(fk_mx4_gemm_args a) {
-  fk::mx4_gemm_many<GB, T>(a);
+template <int T>
+__global__ void __launch_bounds__(256, 1) op_mx4_gemm_many(fk_mx4_gemm_args a) {
+  fk::mx4_gemm_many<T>(a);
+}
+
+template <uint32_t GM, uint32_t GN, int T>
+__global__ void __launch_bounds__(256, GM * GN == 8 ? 2 : 3) op_mx4_gemm_mid(fk_mx4_gemm_args a) {
+  fk::mx4_gemm_mid<GM, GN, T>(a);
 }
 
 uint64_t codes_bytes(uint32_t rows, uint32_t k) { return (uint64_t)fk::mx4_row_tiles(rows) * fk::mx4_pairs(k) * 2048; }
@@ -77,18 +85,67 @@ void of_type(uint32_t type, F &&f) {
   else f(std::integral_constant<int, FK_T_BF16>{});
 }
 
-template <uint32_t MB, uint32_t NB, uint32_t W, int T>
-void queue_few(const fk_mx4_gemm_args &a, hipStream_t s) {
-  const uint32_t tm = (fk::mx4_row_tiles(a.m) + MB - 1) / MB, tn = (fk::mx4_row_tiles(a.n) + NB - 1) / NB;
-  hipLaunchKernelGGL((op_mx4_gemm_few<MB, NB, W, T>), dim3(tm * tn), dim3(64 * W), 0, s, a);
+// The forms of the product: blocks of 16 of a threadgroup's tile, the
+// wavefronts that share a tile's k (few) or the threadgroups the chip holds at
+// once (mid, many).
+enum Kind { FEW, MID, MANY };
+struct Form {
+  const char *name;
+  Kind kind;
+  uint32_t mb, nb, by;
+  double base, step, work;
+};
+// What each costs, in µs, fitted to its times on 105 products (1 to 8192 rows
+// by 512 to 16384, k of 2048 to 8192):
+//   few         base, `step` for each pair of tiles of k a wavefront takes, and
+//               `work` for a thousand KB that all threadgroups read (mb + nb
+//               blocks a pair each: what a tile reads again, others read too)
+//   mid, many   `step` a pair, `work` for 10^5 blocks times pairs, and `base`
+//               for every time the tiles fill the chip
+// The form of the least cost is 1.03 times the fastest one's time on average
+// over them, at most 1.43 (100 rows by 2048, k 8192: 9.5 µs, 64 × 16 blocks
+// would take 7.1).
+constexpr Form forms[] = {{"few 1x1", FEW, 1, 1, 8, 2.29, 0.05, 0.107},    {"few 2x2", FEW, 2, 2, 8, 1.70, 0.81, 0.135},
+                          {"few 4x2", FEW, 4, 2, 8, 1.94, 0.79, 0.122},    {"few 8x2", FEW, 8, 2, 4, 2.07, 0.80, 0.107},
+                          {"mid 8x8", MID, 8, 8, 768, 3.35, 0.45, 2.84},   {"mid 16x8", MID, 16, 8, 512, 5.16, 0.65, 2.39},
+                          {"many 16x16", MANY, 16, 16, 256, 10.0, 0.85, 1.77}};
+
+uint64_t tiles_of(const Form &f, uint32_t m, uint32_t n) {
+  return (uint64_t)((fk::mx4_row_tiles(m) + f.mb - 1) / f.mb) * ((fk::mx4_row_tiles(n) + f.nb - 1) / f.nb);
 }
 
-template <uint32_t GB, int T>
-void queue_many(const fk_mx4_gemm_args &a, hipStream_t s) {
-  constexpr uint32_t side = fk::mx4_many_tiles<GB>();
-  const uint32_t tm = (fk::mx4_row_tiles(a.m) + side - 1) / side, tn = (fk::mx4_row_tiles(a.n) + side - 1) / side;
-  const uint32_t most = GB == 4 ? 256 : 512;  // as many as the chip holds at once
-  hipLaunchKernelGGL((op_mx4_gemm_many<GB, T>), dim3(tm * tn < most ? tm * tn : most), dim3(256), fk::mx4_many_lds<GB>(), s, a);
+double cost(const Form &f, uint32_t m, uint32_t n, uint32_t k) {
+  const double t = (double)tiles_of(f, m, n), pairs = fk::mx4_pairs(k);
+  if (f.kind == FEW) return f.base + f.step * std::ceil(pairs / f.by) + f.work * 1e-3 * t * pairs * (f.mb + f.nb);
+  return f.base * std::ceil(t / f.by) + f.step * pairs + f.work * 1e-5 * t * f.mb * f.nb * pairs;
+}
+
+// mid and many address a tile's slab with 32 bits.
+bool takes(const Form &f, uint32_t k) { return f.kind == FEW || fk::mx4_pairs(k) < 1u << 16; }
+
+uint32_t pick(uint32_t m, uint32_t n, uint32_t k) {
+  uint32_t best = 0;
+  for (uint32_t i = 1; i < std::size(forms); i++)
+    if (takes(forms[i], k) && cost(forms[i], m, n, k) < cost(forms[best], m, n, k)) best = i;
+  return best;
+}
+
+template <uint32_t I, int T>
+void queue_form(const fk_mx4_gemm_args &a, hipStream_t s) {
+  constexpr Form f = forms[I];
+  const uint32_t tiles = (uint32_t)tiles_of(f, a.m, a.n);
+  if constexpr (f.kind == FEW)
+    hipLaunchKernelGGL((op_mx4_gemm_few<f.mb, f.nb, f.by, T>), dim3(tiles), dim3(64 * f.by), 0, s, a);
+  else if constexpr (f.kind == MID)
+    hipLaunchKernelGGL((op_mx4_gemm_mid<f.mb / 4, f.nb / 4, T>), dim3(tiles), dim3(256),
+                       (fk::mx4_mid_lds<f.mb / 4, f.nb / 4>()), s, a);
+  else
+    hipLaunchKernelGGL((op_mx4_gemm_many<T>), dim3(tiles < f.by ? tiles : f.by), dim3(256), fk::mx4_many_lds, s, a);
+}
+
+template <int T, size_t... I>
+void queue_picked(uint32_t form, const fk_mx4_gemm_args &a, hipStream_t s, std::index_sequence<I...>) {
+  ((form == I ? queue_form<I, T>(a, s) : void()), ...);
 }
 
 }  // namespace
@@ -123,6 +180,9 @@ int check(const fk_mx4_gemm_args &a, Refusal &no) {
   if (!matrix(a.m, a.k) || !matrix(a.n, a.k)) return no(FK_ERR_RANGE, "no product of %u and %u rows of %u", a.m, a.n, a.k);
   if ((uint64_t)mx4_row_tiles(a.m) * mx4_row_tiles(a.n) >= 1ull << 31)
     return no(FK_ERR_RANGE, "a product of %u by %u: 2^31 tiles and more", a.m, a.n);
+  const Form &f = forms[pick(a.m, a.n, a.k)];
+  if (f.kind != MANY && tiles_of(f, a.m, a.n) >= 1ull << 23)  // a launch of 2^32 threads
+    return no(FK_ERR_RANGE, "a product of %u by %u, k %u: 2^23 threadgroups and more", a.m, a.n, a.k);
   if (int st = check_rows(no, "c", a.c, a.c_stride, a.n, a.c_type)) return st;
   const Span reads[] = {{"a_codes", a.a_codes, codes_bytes(a.m, a.k)},
                         {"a_scales", a.a_scales, scales_bytes(a.m, a.k)},
@@ -165,25 +225,15 @@ extern "C" int fk_mx4_dequantize(fk_ctx *ctx, const fk_mx4_dequantize_args *a, f
   return launched(ctx, "fk_mx4_dequantize");
 }
 
+extern "C" const char *fk_mx4_gemm_form(uint32_t m, uint32_t n, uint32_t k) {
+  return matrix(m, k) && matrix(n, k) ? forms[pick(m, n, k)].name : "";
+}
+
 extern "C" int fk_mx4_gemm(fk_ctx *ctx, const fk_mx4_gemm_args *a, fk_stream *stream) {
   if (int st = admit(ctx, "fk_mx4_gemm", a)) return st;
   const hipStream_t s = stream_of(ctx, stream);
   of_type(a->c_type, [&](auto t) {
-    constexpr int T = decltype(t)::value;
-    const char *f = getenv("FK_MX4_FORM");
-    const int form = f ? atoi(f) : (a->m <= 16 ? 0 : a->m <= 128 ? 3 : 5);
-    switch (form) {
-      case 0: queue_few<1, 1, 8, T>(*a, s); break;
-      case 1: queue_few<1, 2, 8, T>(*a, s); break;
-      case 2: queue_few<2, 2, 8, T>(*a, s); break;
-      case 3: queue_few<4, 4, 4, T>(*a, s); break;
-      case 4: queue_many<2, T>(*a, s); break;
-      case 6: queue_few<4, 2, 8, T>(*a, s); break;
-      case 7: queue_few<4, 1, 8, T>(*a, s); break;
-      case 8: queue_few<2, 1, 8, T>(*a, s); break;
-      case 9: queue_few<8, 2, 4, T>(*a, s); break;
-      default: queue_many<4, T>(*a, s);
-    }
+    queue_picked<decltype(t)::value>(pick(a->m, a->n, a->k), *a, s, std::make_index_sequence<std::size(forms)>{});
   });
   return launched(ctx, "fk_mx4_gemm");
 }

@@ -127,30 +127,45 @@ __device__ __forceinline__ void mx4_gemm_few(const fk_mx4_gemm_args &a) {
   }
 }
 
-// Many rows: v_mfma_scale_f32_32x32x64_f8f6f4, twice the rate of the 16 × 16
-// form on this chip (36 cycles for twice its work, against 29): lane l holds a
-// block of row l mod 32, k 32 (l div 32) .. + 31, and D[8 (r div 4) + 4 (l div
-// 32) + r mod 4][l mod 32] as register r.
+// More rows: v_mfma_scale_f32_32x32x64_f8f6f4, 1.2 times the rate of the 16 ×
+// 16 form here on random operands (6.5 and 5.4 PFLOP/s in registers alone,
+// where the chip's power holds its clock down; 9.6 and 5.9 on zeros): lane l
+// holds a block of row l mod 32, k 32 (l div 32) .. + 31, and D[8 (r div 4) + 4
+// (l div 32) + r mod 4][l mod 32] as register r.
 //
-// A threadgroup of 4 wavefronts takes a tile of 2 GB × 2 GB blocks of 32 × 32
-// (256 × 256 at GB 4), each wavefront GB × GB of them, accumulated in AGPRs.
-// A step is one tile of k (128): the operands' 1 KB blocks go straight into a
-// ring of 4 LDS stages, two steps ahead of the one being read, and are read
-// back 16 bytes a lane, 16 lanes 256 consecutive bytes; a step's loads, reads
-// and matrix operations are interleaved, one barrier a step.  The scales come
-// to registers, two steps' in one load of two bytes a lane, a pair of steps
-// ahead.
+// A threadgroup of 4 wavefronts, two by two, takes a tile of 64 GM rows and 64
+// GN columns, each wavefront GM × GN blocks of 32 × 32.  A step is one tile of
+// k (128): the operands' 1 KB blocks go straight into a ring of LDS stages and
+// are read back 16 bytes a lane, 16 lanes 256 consecutive bytes, no bank
+// twice.  The scales come to registers, two steps' in one load of two bytes a
+// lane, a pair of steps ahead.  Two kernels, by what hides what:
+//
+// - mx4_gemm_mid: three stages, the operands read as they are needed, and two
+//   or three threadgroups a CU, one's loads, reads and stores under another's
+//   matrix operations.
+// - mx4_gemm_many: 256 × 256 tiles whose sums take half the register file, so
+//   one threadgroup a CU: four stages, the next step's operands read and a
+//   later step's loaded between a step's matrix operations, and tile after
+//   tile with the next one's first loads under the stores.  Half the traffic
+//   for each product, which pays where k is long: 8192 x 8192, k 8192 248 µs
+//   (4.4 PFLOP/s, mid 265), k 2048 91 (mid 81).
 #define FK_MX4_STAGES 4
 #define FK_MX4_LDS __attribute__((address_space(3)))
-template <uint32_t GB>
-__host__ __device__ constexpr uint32_t mx4_many_lds() {
-  return FK_MX4_STAGES * 2 * 4 * GB * 1024;
+constexpr uint32_t mx4_many_side = 16;  // row tiles of a tile's side
+constexpr uint32_t mx4_many_lds = FK_MX4_STAGES * 2 * mx4_many_side * 1024;
+template <uint32_t GM, uint32_t GN>
+constexpr uint32_t mx4_mid_lds() {
+  return 3 * 4 * (GM + GN) * 1024;
 }
-// Row tiles of a tile's side.
-template <uint32_t GB>
-__host__ __device__ constexpr uint32_t mx4_many_tiles() {
-  return 4 * GB;
-}
+// s_waitcnt vmcnt(n), the other counters untouched.
+#define FK_MX4_VMCNT(N) __builtin_amdgcn_s_waitcnt(((N) & 15) | (((N) >> 4) << 14) | (0x7 << 4) | (0xf << 8))
+// The barrier without __syncthreads' wait for every load in flight.
+#define FK_MX4_BARRIER()                  \
+  do {                                    \
+    asm volatile("" ::: "memory");        \
+    __builtin_amdgcn_s_barrier();         \
+    asm volatile("" ::: "memory");        \
+  } while (0)
 
 template <int TILE>
 __device__ __forceinline__ fk_float16v mx4_mfma32(u32x4 b, uint32_t bs, u32x4 a, uint32_t as, fk_float16v c) {
@@ -158,26 +173,32 @@ __device__ __forceinline__ fk_float16v mx4_mfma32(u32x4 b, uint32_t bs, u32x4 a,
                                                          (int)as);
 }
 
-// A wavefront's 32 GB rows of 32 GB columns into C, through its own share of
+// A wavefront's 32 GM rows of 32 GN columns into C, through its own share of
 // an LDS stage: of 32 rows at a time RB bytes each are written as the
 // operation left them, a lane 4 columns of a row, and read back a row's
 // consecutive 16 bytes a lane, so that stores are RB whole bytes of a row.
 // wide: C's rows are 16-byte aligned.
-template <uint32_t GB, int T>
+template <uint32_t GM, uint32_t GN, bool AGPR, int T>
 __device__ __forceinline__ void mx4_store_many(const fk_mx4_gemm_args &a, bool wide, uint32_t m0, uint32_t n0,
-                                               fk_float16v (&acc)[GB][GB], char *stage) {
-  constexpr uint32_t RB = GB * 64, BYTES = mx4_bytes_of(T), COLS = RB / BYTES, UNITS = RB / 16, EACH = 16 / BYTES;
+                                               fk_float16v (&acc)[GM][GN], char *stage) {
+  constexpr uint32_t RB = GN * 64, BYTES = mx4_bytes_of(T), COLS = RB / BYTES, UNITS = RB / 16, EACH = 16 / BYTES;
   const uint32_t lane = threadIdx.x % FK_WAVE;
+  // a C that the L2s would not hold goes past them (8192 x 8192 of f16, k
+  // 2048: 89.0 µs, so 82.1)
+  const bool stream = (uint64_t)a.m * a.n * BYTES >= 32u << 20;
   // 16-byte unit u of row m at place u ^ turn(m): no bank twice in 16 lanes
   auto place = [](uint32_t m, uint32_t u) { return m * RB + (u ^ (UNITS == 16 ? m & 15u : (m >> 1) & 7u)) * 16; };
 #pragma unroll
-  for (uint32_t i = 0; i < GB; i++)
+  for (uint32_t i = 0; i < GM; i++)
 #pragma unroll
-    for (uint32_t c = 0; c < 32 * GB / COLS; c++) {
+    for (uint32_t c = 0; c < 32 * GN / COLS; c++) {
       const uint32_t row = lane % 32;
       // (taken here: rounded further ahead, they would not fit the registers)
 #pragma unroll
-      for (uint32_t j = 0; j < COLS / 32; j++) asm volatile("" : "+a"(acc[i][c * (COLS / 32) + j]));
+      for (uint32_t j = 0; j < COLS / 32; j++) {
+        if constexpr (AGPR) asm volatile("" : "+a"(acc[i][c * (COLS / 32) + j]));
+        else asm volatile("" : "+v"(acc[i][c * (COLS / 32) + j]));
+      }
 #pragma unroll
       for (uint32_t j = 0; j < COLS / 32; j++)
 #pragma unroll
@@ -206,7 +227,8 @@ __device__ __forceinline__ void mx4_store_many(const fk_mx4_gemm_args &a, bool w
         const uint64_t at = a.c + ((uint64_t)m * a.c_stride + n) * BYTES;
         if (m < a.m && n < a.n) {
           if (wide && n + EACH <= a.n) {
-            *global_at<u32x4>(at) = w;
+            if (stream) __builtin_nontemporal_store(w, global_at<u32x4>(at));
+            else *global_at<u32x4>(at) = w;
           } else {
 #pragma unroll
             for (uint32_t e = 0; e < EACH; e++)
@@ -221,10 +243,113 @@ __device__ __forceinline__ void mx4_store_many(const fk_mx4_gemm_args &a, bool w
     }
 }
 
-template <uint32_t GB, int T>
+template <uint32_t GM, uint32_t GN, int T>
+__device__ __forceinline__ void mx4_gemm_mid(const fk_mx4_gemm_args &a) {
+  extern __shared__ u32x4 mx4_lds[];
+  constexpr uint32_t RA = 4 * GM, RN = 4 * GN;     // row tiles of the slabs
+  constexpr uint32_t SLAB = RA * 1024, STAGE = (RA + RN) * 1024;
+  const uint32_t lane = threadIdx.x % FK_WAVE;
+  const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x / FK_WAVE);
+  const uint32_t wm = wave & 1, wn = wave >> 1;
+  const uint32_t pairs = mx4_pairs(a.k), rows_a = mx4_row_tiles(a.m), rows_b = mx4_row_tiles(a.n);
+  const uint32_t tiles_m = (rows_a + RA - 1) / RA;
+  const uint32_t tm = blockIdx.x % tiles_m * RA, tn = blockIdx.x / tiles_m * RN;
+  const uint32_t half = lane % 32 / 16, place = lane / 32 * 16 + lane % 16;
+  const uint32_t have_a = min(rows_a - tm, RA), have_b = min(rows_b - tn, RN);
+  const auto a_src = buffer((const void *)(a.a_codes + (uint64_t)tm * pairs * 2048), (size_t)have_a * pairs * 2048);
+  const auto b_src = buffer((const void *)(a.b_codes + (uint64_t)tn * pairs * 2048), (size_t)have_b * pairs * 2048);
+  const auto as_src = buffer((const void *)(a.a_scales + (uint64_t)tm * pairs * 128), (size_t)have_a * pairs * 128);
+  const auto bs_src = buffer((const void *)(a.b_scales + (uint64_t)tn * pairs * 128), (size_t)have_b * pairs * 128);
+  uint32_t a_at[GM], b_at[GN], as_at[GM], bs_at[GN];
+#pragma unroll
+  for (uint32_t i = 0; i < GM; i++) {
+    a_at[i] = min(wave * GM + i, have_a - 1) * pairs * 2048 + lane * 16;
+    as_at[i] = min(2 * (wm * GM + i) + half, have_a - 1) * pairs * 128 + place * 2;
+  }
+#pragma unroll
+  for (uint32_t i = 0; i < GN; i++) {
+    b_at[i] = min(wave * GN + i, have_b - 1) * pairs * 2048 + lane * 16;
+    bs_at[i] = min(2 * (wn * GN + i) + half, have_b - 1) * pairs * 128 + place * 2;
+  }
+  FK_MX4_LDS char *const a_to = (FK_MX4_LDS char *)mx4_lds + wave * GM * 1024;
+  FK_MX4_LDS char *const b_to = (FK_MX4_LDS char *)mx4_lds + SLAB + wave * GN * 1024;
+  const uint32_t ra = (2 * wm * GM + half) * 64 + place, rb = SLAB / 16 + (2 * wn * GN + half) * 64 + place;
+  fk_float16v acc[GM][GN];
+#pragma unroll
+  for (uint32_t i = 0; i < GM; i++)
+#pragma unroll
+    for (uint32_t j = 0; j < GN; j++)
+#pragma unroll
+      for (int r = 0; r < 16; r++) acc[i][j][r] = 0.0f;
+  uint32_t sa[2][GM][2], sb[2][GN][2];
+  const uint32_t steps = 2 * pairs, last = steps - 1;
+  auto codes = [&](uint32_t step, uint32_t stage) {
+    const uint32_t so = min(step, last) * 1024;
+#pragma unroll
+    for (uint32_t q = 0; q < GM; q++)
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(a_src, a_to + stage * STAGE + q * 1024, 16, a_at[q], so, 0, 0);
+#pragma unroll
+    for (uint32_t q = 0; q < GN; q++)
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(b_src, b_to + stage * STAGE + q * 1024, 16, b_at[q], so, 0, 0);
+  };
+  auto scales = [&](uint32_t (&s)[GM][2], uint32_t (&t)[GN][2], uint32_t pair) {
+#pragma unroll
+    for (uint32_t h = 0; h < 2; h++) {
+#pragma unroll
+      for (uint32_t i = 0; i < GM; i++) s[i][h] = __builtin_amdgcn_raw_buffer_load_b16(as_src, as_at[i] + 64 * h, pair * 128, 0);
+#pragma unroll
+      for (uint32_t i = 0; i < GN; i++) t[i][h] = __builtin_amdgcn_raw_buffer_load_b16(bs_src, bs_at[i] + 64 * h, pair * 128, 0);
+    }
+  };
+  scales(sa[0], sb[0], 0);
+  codes(0, 0);
+  codes(1, 1);
+  uint32_t at = 0, to = 2;   // the stage a step reads, and the one it loads
+#define FK_MX4_MID(TILE, WAIT, S)                                                                             \
+  do {                                                                                                        \
+    FK_MX4_VMCNT(WAIT);                                                                                       \
+    FK_MX4_BARRIER();                                                                                         \
+    __builtin_amdgcn_sched_barrier(0);                                                                        \
+    if (TILE == 0) scales(sa[1], sb[1], min(p + 1, pairs - 1));                                               \
+    codes((S) + 2, to);                                                                                       \
+    const u32x4 *s_ = mx4_lds + at * (STAGE / 16);                                                            \
+    u32x4 fa[GM][2], fb[GN][2];                                                                               \
+    _Pragma("unroll") for (uint32_t h = 0; h < 2; h++) {                                                      \
+      _Pragma("unroll") for (uint32_t j = 0; j < GN; j++) fb[j][h] = s_[rb + 128 * j + 32 * h];               \
+      _Pragma("unroll") for (uint32_t i = 0; i < GM; i++) fa[i][h] = s_[ra + 128 * i + 32 * h];               \
+    }                                                                                                         \
+    _Pragma("unroll") for (uint32_t h = 0; h < 2; h++)                                                        \
+    _Pragma("unroll") for (uint32_t i = 0; i < GM; i++)                                                       \
+    _Pragma("unroll") for (uint32_t j = 0; j < GN; j++)                                                       \
+        acc[i][j] = mx4_mfma32<TILE>(fb[j][h], sb[0][j][h], fa[i][h], sa[0][i][h], acc[i][j]);                \
+    at = at == 2 ? 0 : at + 1;                                                                                \
+    to = to == 2 ? 0 : to + 1;                                                                                \
+  } while (0)
+  for (uint32_t p = 0; p < pairs; p++) {
+    FK_MX4_MID(0, GM + GN, 2 * p);
+    FK_MX4_MID(1, 3 * (GM + GN), 2 * p + 1);
+#pragma unroll
+    for (uint32_t h = 0; h < 2; h++) {
+#pragma unroll
+      for (uint32_t i = 0; i < GM; i++) sa[0][i][h] = sa[1][i][h];
+#pragma unroll
+      for (uint32_t i = 0; i < GN; i++) sb[0][i][h] = sb[1][i][h];
+    }
+  }
+  __builtin_amdgcn_s_waitcnt(0);
+  FK_MX4_BARRIER();
+#undef FK_MX4_MID
+  const bool wide = a.c_stride * mx4_bytes_of(T) % 16 == 0 && a.c % 16 == 0;
+  mx4_store_many<GM, GN, false, T>(a, wide, 16 * tm + 32 * wm * GM, 16 * tn + 32 * wn * GN, acc,
+                                   reinterpret_cast<char *>(mx4_lds) + wave * GN * 2048);
+}
+
+
+template <int T>
 __device__ __forceinline__ void mx4_gemm_many(const fk_mx4_gemm_args &a) {
   extern __shared__ u32x4 mx4_lds[];
-  constexpr uint32_t ROWS = mx4_many_tiles<GB>();  // row tiles of an operand's slab
+  constexpr uint32_t GB = mx4_many_side / 4;       // a wavefront's blocks of 32, each way
+  constexpr uint32_t ROWS = mx4_many_side;         // row tiles of an operand's slab
   constexpr uint32_t SLAB = ROWS * 1024;           // its bytes a step
   constexpr uint32_t STAGE = 2 * SLAB;             // A's, then B's
   constexpr uint32_t Q = ROWS / 4;                 // loads of an operand a wavefront makes a step
@@ -272,13 +397,6 @@ __device__ __forceinline__ void mx4_gemm_many(const fk_mx4_gemm_args &a) {
 #define FK_MX4_PIN_ACC()                                                    \
   _Pragma("unroll") for (uint32_t i_ = 0; i_ < GB; i_++)                    \
   _Pragma("unroll") for (uint32_t j_ = 0; j_ < GB; j_++) asm volatile("" : "+a"(acc[i_][j_]))
-#define FK_MX4_VMCNT(N) __builtin_amdgcn_s_waitcnt(((N) & 15) | (((N) >> 4) << 14) | (0x7 << 4) | (0xf << 8))
-#define FK_MX4_BARRIER()                  \
-  do {                                    \
-    asm volatile("" ::: "memory");        \
-    __builtin_amdgcn_s_barrier();         \
-    asm volatile("" ::: "memory");        \
-  } while (0)
 #define FK_MX4_SCALES(SA, SB, P)                                                                              \
   _Pragma("unroll") for (uint32_t i_ = 0; i_ < GB; i_++)                                                      \
   _Pragma("unroll") for (uint32_t h_ = 0; h_ < 2; h_++) {                                                     \
@@ -365,51 +483,49 @@ __device__ __forceinline__ void mx4_gemm_many(const fk_mx4_gemm_args &a) {
   FK_MX4_FIRST();
   for (uint32_t tile = blockIdx.x; tile < tiles; tile += gridDim.x) {
 #pragma unroll
-  for (uint32_t i = 0; i < GB; i++)
+    for (uint32_t i = 0; i < GB; i++)
 #pragma unroll
-    for (uint32_t j = 0; j < GB; j++)
+      for (uint32_t j = 0; j < GB; j++)
 #pragma unroll
-      for (int r = 0; r < 16; r++) acc[i][j][r] = 0.0f;
-  // step 0 landed (what was stored since is waited for with it)
-  FK_MX4_VMCNT(2 * Q * (FK_MX4_STAGES - 2));
-  FK_MX4_BARRIER();
-#pragma unroll
-  for (uint32_t i = 0; i < GB; i++)
-#pragma unroll
-    for (uint32_t h = 0; h < 2; h++) {
-      fb0[i][h] = mx4_lds[rb + 128 * i + 32 * h];
-      fa0[i][h] = mx4_lds[ra + 128 * i + 32 * h];
-    }
-#pragma unroll
-  for (uint32_t i = 0; i < GB; i++)
-#pragma unroll
-    for (uint32_t h = 0; h < 2; h++) {
-      FK_MX4_PIN(fb0[i][h]);
-      if (i < H) FK_MX4_PIN(fa0[i][h]);
-    }
-  for (uint32_t p = 0; p < pairs; p++) {
-    const uint32_t s = 2 * p, next = p + 1 < pairs ? p + 1 : p;
-    FK_MX4_STEP(0, fa0, fb0, fa1, fb1, sa0, sb0, sa1, sb1, 2 * Q, next, FK_MX4_T(s + 3), (s + 3) % 4, (s + 1) % 4);
-    FK_MX4_STEP(1, fa1, fb1, fa0, fb0, sa0, sb0, sa1, sb1, 2 * Q + 4 * GB, next, FK_MX4_T(s + 4), s % 4, (s + 2) % 4);
+        for (int r = 0; r < 16; r++) acc[i][j][r] = 0.0f;
+    // step 0 landed (what was stored since is waited for with it)
+    FK_MX4_VMCNT(2 * Q * (FK_MX4_STAGES - 2));
+    FK_MX4_BARRIER();
 #pragma unroll
     for (uint32_t i = 0; i < GB; i++)
 #pragma unroll
-      for (uint32_t h = 0; h < 2; h++) sa0[i][h] = sa1[i][h], sb0[i][h] = sb1[i][h];
-  }
-  // Nothing lands in LDS any more, and no wavefront reads it.
-  __builtin_amdgcn_s_waitcnt(0);
-  FK_MX4_BARRIER();
-  const uint32_t m = 16 * tm + 32 * wm * GB, n = 16 * tn + 32 * wn * GB;
-  if (tile + gridDim.x < tiles) {
-    sources(tile + gridDim.x);
-    FK_MX4_FIRST();
-  }
-  mx4_store_many<GB, T>(a, wide, m, n, acc, reinterpret_cast<char *>(mx4_lds) + 3 * STAGE + wave * (STAGE / 4));
+      for (uint32_t h = 0; h < 2; h++) {
+        fb0[i][h] = mx4_lds[rb + 128 * i + 32 * h];
+        fa0[i][h] = mx4_lds[ra + 128 * i + 32 * h];
+      }
+#pragma unroll
+    for (uint32_t i = 0; i < GB; i++)
+#pragma unroll
+      for (uint32_t h = 0; h < 2; h++) {
+        FK_MX4_PIN(fb0[i][h]);
+        if (i < H) FK_MX4_PIN(fa0[i][h]);
+      }
+    for (uint32_t p = 0; p < pairs; p++) {
+      const uint32_t s = 2 * p, next = p + 1 < pairs ? p + 1 : p;
+      FK_MX4_STEP(0, fa0, fb0, fa1, fb1, sa0, sb0, sa1, sb1, 2 * Q, next, FK_MX4_T(s + 3), (s + 3) % 4, (s + 1) % 4);
+      FK_MX4_STEP(1, fa1, fb1, fa0, fb0, sa0, sb0, sa1, sb1, 2 * Q + 4 * GB, next, FK_MX4_T(s + 4), s % 4, (s + 2) % 4);
+#pragma unroll
+      for (uint32_t i = 0; i < GB; i++)
+#pragma unroll
+        for (uint32_t h = 0; h < 2; h++) sa0[i][h] = sa1[i][h], sb0[i][h] = sb1[i][h];
+    }
+    // Nothing lands in LDS any more, and no wavefront reads it.
+    __builtin_amdgcn_s_waitcnt(0);
+    FK_MX4_BARRIER();
+    const uint32_t m = 16 * tm + 32 * wm * GB, n = 16 * tn + 32 * wn * GB;
+    if (tile + gridDim.x < tiles) {
+      sources(tile + gridDim.x);
+      FK_MX4_FIRST();
+    }
+    mx4_store_many<GB, GB, true, T>(a, wide, m, n, acc, reinterpret_cast<char *>(mx4_lds) + 3 * STAGE + wave * (STAGE / 4));
   }
 #undef FK_MX4_PIN
 #undef FK_MX4_PIN_ACC
-#undef FK_MX4_VMCNT
-#undef FK_MX4_BARRIER
 #undef FK_MX4_SCALES
 #undef FK_MX4_MFMAS
 #undef FK_MX4_STEP

@@ -146,6 +146,7 @@ ENTRY_POINTS: list[tuple[str, object, list]] = [
     ("fk_mx4_quantize", _int, [_vp, _vp, _vp]),
     ("fk_mx4_dequantize", _int, [_vp, _vp, _vp]),
     ("fk_mx4_gemm", _int, [_vp, _vp, _vp]),
+    ("fk_mx4_gemm_form", ctypes.c_char_p, [_u32, _u32, _u32]),
     ("fk_serve_check", _int, [ctypes.c_char_p, _vp, _sz, ctypes.c_char_p, _sz]),
     ("fk_rtc_compile", _int, [ctypes.c_char_p, ctypes.c_char_p, ctypes.POINTER(ctypes.c_char_p), _int, _PP,
                               ctypes.POINTER(_sz), ctypes.POINTER(ctypes.c_char_p)]),

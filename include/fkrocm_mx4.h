@@ -86,6 +86,10 @@ typedef struct fk_mx4_gemm_args {
 
 int fk_mx4_gemm(fk_ctx *ctx, const fk_mx4_gemm_args *args, fk_stream *stream);
 
+/* The name of the kernel form that a product of these sizes takes ("" for one
+ * that is refused); for profiles and tests. */
+const char *fk_mx4_gemm_form(uint32_t m, uint32_t n, uint32_t k);
+
 #ifdef __cplusplus
 }
 #endif
