@@ -21,14 +21,14 @@ using fk::stream_of;
 
 namespace {
 
-template <int T, bool WIDE>
+template <int T>
 __global__ void __launch_bounds__(FK_MX4_THREADS) op_mx4_quantize(fk_mx4_quantize_args a) {
-  fk::mx4_quantize<T, WIDE>(a);
+  fk::mx4_quantize<T>(a);
 }
 
-template <int T, bool WIDE>
+template <int T>
 __global__ void __launch_bounds__(FK_MX4_THREADS) op_mx4_dequantize(fk_mx4_dequantize_args a) {
-  fk::mx4_dequantize<T, WIDE>(a);
+  fk::mx4_dequantize<T>(a);
 }
 
 template <uint32_t MB, uint32_t NB, uint32_t W, int T>
@@ -42,7 +42,7 @@ __global__ void __launch_bounds__(256, 1) op_mx4_gemm_many(fk_mx4_gemm_args a) {
 }
 
 template <uint32_t GM, uint32_t GN, int T>
-__global__ void __launch_bounds__(256, GM * GN == 8 ? 2 : 3) op_mx4_gemm_mid(fk_mx4_gemm_args a) {
+__global__ void __launch_bounds__(256, 3) op_mx4_gemm_mid(fk_mx4_gemm_args a) {
   fk::mx4_gemm_mid<GM, GN, T>(a);
 }
 
@@ -55,8 +55,8 @@ bool matrix(uint32_t rows, uint32_t k) {
          (uint64_t)fk::mx4_row_tiles(rows) * fk::mx4_pairs(k) < 1ull << 31;
 }
 
-// Rows of `type` from `addr` on, `stride` elements apart: aligned to their
-// elements, and to 16 bytes if whole eights go at a time.
+// Rows of `type` from `addr` on, `stride` elements apart, aligned to their
+// elements.
 int check_rows(Refusal &no, const char *name, uint64_t addr, uint64_t stride, uint64_t width, uint32_t type) {
   if (type > FK_T_BF16) return no(FK_ERR_ARG, "%s of type %u", name, type);
   if (stride < width || stride >= 1ull << 40)
@@ -64,9 +64,6 @@ int check_rows(Refusal &no, const char *name, uint64_t addr, uint64_t stride, ui
   if (addr == 0 || addr % fk::mx4_bytes_of((int)type))
     return no(FK_ERR_ARG, "%s is null or not aligned to its elements", name);
   return FK_OK;
-}
-bool wide_rows(uint64_t addr, uint64_t stride, uint64_t k, uint32_t type) {
-  return addr % 16 == 0 && k % 8 == 0 && stride * fk::mx4_bytes_of((int)type) % 16 == 0;
 }
 uint64_t rows_bytes(uint64_t rows, uint64_t stride, uint64_t width, uint32_t type) {
   return ((rows - 1) * stride + width) * fk::mx4_bytes_of((int)type);
@@ -95,20 +92,19 @@ struct Form {
   uint32_t mb, nb, by;
   double base, step, work;
 };
-// What each costs, in µs, fitted to its times on 105 products (1 to 8192 rows
-// by 512 to 16384, k of 2048 to 8192):
+// What each costs, in µs, fitted to its times on 98 products (1 to 8192 rows
+// by 512 to 16384, k of 2048 to 8192, the operands from memory each time):
 //   few         base, `step` for each pair of tiles of k a wavefront takes, and
 //               `work` for a thousand KB that all threadgroups read (mb + nb
 //               blocks a pair each: what a tile reads again, others read too)
 //   mid, many   `step` a pair, `work` for 10^5 blocks times pairs, and `base`
 //               for every time the tiles fill the chip
-// The form of the least cost is 1.03 times the fastest one's time on average
-// over them, at most 1.43 (100 rows by 2048, k 8192: 9.5 µs, 64 × 16 blocks
-// would take 7.1).
-constexpr Form forms[] = {{"few 1x1", FEW, 1, 1, 8, 2.29, 0.05, 0.107},    {"few 2x2", FEW, 2, 2, 8, 1.70, 0.81, 0.135},
-                          {"few 4x2", FEW, 4, 2, 8, 1.94, 0.79, 0.122},    {"few 8x2", FEW, 8, 2, 4, 2.07, 0.80, 0.107},
-                          {"mid 8x8", MID, 8, 8, 768, 3.35, 0.45, 2.84},   {"mid 16x8", MID, 16, 8, 512, 5.16, 0.65, 2.39},
-                          {"many 16x16", MANY, 16, 16, 256, 10.0, 0.85, 1.77}};
+// The form of the least cost takes 1.02 times the fastest one's time on
+// average over them, at most 1.26 (32 rows by 8192, k 2048: 5.4 µs, 64 x 16
+// blocks 4.3).
+constexpr Form forms[] = {{"few 1x1", FEW, 1, 1, 8, 2.54, 0.25, 0.169}, {"few 4x1", FEW, 4, 1, 8, 2.71, 0.34, 0.127},
+                          {"few 4x2", FEW, 4, 2, 8, 3.34, 0.43, 0.153}, {"few 8x2", FEW, 8, 2, 4, 3.73, 0.65, 0.120},
+                          {"mid 8x8", MID, 8, 8, 768, 3.86, 0.57, 3.10}, {"many 16x16", MANY, 16, 16, 256, 10.3, 0.83, 1.61}};
 
 uint64_t tiles_of(const Form &f, uint32_t m, uint32_t n) {
   return (uint64_t)((fk::mx4_row_tiles(m) + f.mb - 1) / f.mb) * ((fk::mx4_row_tiles(n) + f.nb - 1) / f.nb);
@@ -204,10 +200,7 @@ extern "C" int fk_mx4_quantize(fk_ctx *ctx, const fk_mx4_quantize_args *a, fk_st
   const dim3 grid(pair_groups(a->rows, a->k)), block(FK_MX4_THREADS);
   const hipStream_t s = stream_of(ctx, stream);
   of_type(a->x_type, [&](auto t) {
-    if (wide_rows(a->x, a->x_stride, a->k, a->x_type))
-      hipLaunchKernelGGL((op_mx4_quantize<decltype(t)::value, true>), grid, block, 0, s, *a);
-    else
-      hipLaunchKernelGGL((op_mx4_quantize<decltype(t)::value, false>), grid, block, 0, s, *a);
+    hipLaunchKernelGGL((op_mx4_quantize<decltype(t)::value>), grid, block, 0, s, *a);
   });
   return launched(ctx, "fk_mx4_quantize");
 }
@@ -217,10 +210,7 @@ extern "C" int fk_mx4_dequantize(fk_ctx *ctx, const fk_mx4_dequantize_args *a, f
   const dim3 grid(pair_groups(a->rows, a->k)), block(FK_MX4_THREADS);
   const hipStream_t s = stream_of(ctx, stream);
   of_type(a->y_type, [&](auto t) {
-    if (wide_rows(a->y, a->y_stride, a->k, a->y_type))
-      hipLaunchKernelGGL((op_mx4_dequantize<decltype(t)::value, true>), grid, block, 0, s, *a);
-    else
-      hipLaunchKernelGGL((op_mx4_dequantize<decltype(t)::value, false>), grid, block, 0, s, *a);
+    hipLaunchKernelGGL((op_mx4_dequantize<decltype(t)::value>), grid, block, 0, s, *a);
   });
   return launched(ctx, "fk_mx4_dequantize");
 }

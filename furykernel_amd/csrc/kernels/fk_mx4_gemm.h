@@ -27,30 +27,26 @@ __device__ __forceinline__ fk_float4v mx4_mfma(u32x4 b, uint32_t bs, u32x4 a, ui
                                                           (int)as);
 }
 
-// Four consecutive columns n .. n + 3 of row m of C; WIDE: n and the stride
-// are multiples of 4 and c is aligned.
+// Four consecutive columns n .. n + 3 of row m of C.
 template <int T>
-__device__ __forceinline__ void mx4_store_c(const fk_mx4_gemm_args &a, bool wide, uint32_t m, uint32_t n, fk_float4v v) {
+__device__ __forceinline__ void mx4_store_c(const fk_mx4_gemm_args &a, uint32_t m, uint32_t n, fk_float4v v) {
   if (m >= a.m || n >= a.n) return;
   const uint64_t at = a.c + ((uint64_t)m * a.c_stride + n) * mx4_bytes_of(T);
-  if (wide) {
+  if (n + 4 <= a.n) {
     if constexpr (T == FK_T_F32) {
-      *global_at<fk_float4v>(at) = v;
+      *global_at<mx4_float4>(at) = v;
     } else if constexpr (T == FK_T_F16) {
-      typedef _Float16 half4 __attribute__((ext_vector_type(4)));
+      typedef _Float16 half4 __attribute__((ext_vector_type(4), aligned(2)));
       *global_at<half4>(at) = half4{(_Float16)v[0], (_Float16)v[1], (_Float16)v[2], (_Float16)v[3]};
     } else {
-      typedef __bf16 bf4 __attribute__((ext_vector_type(4)));
+      typedef __bf16 bf4 __attribute__((ext_vector_type(4), aligned(2)));
       *global_at<bf4>(at) = bf4{(__bf16)v[0], (__bf16)v[1], (__bf16)v[2], (__bf16)v[3]};
     }
   } else {
 #pragma unroll
-    for (uint32_t r = 0; r < 4; r++)
+    for (uint32_t r = 0; r < 3; r++)
       if (n + r < a.n) mx4_store<T>(at, r, v[r]);
   }
-}
-__device__ __forceinline__ bool mx4_wide_c(const fk_mx4_gemm_args &a) {
-  return a.n % 4 == 0 && a.c_stride % 4 == 0 && a.c % 16 == 0;
 }
 
 // Few rows: a threadgroup takes MB × NB blocks of 16 × 16, its W wavefronts
@@ -118,12 +114,11 @@ __device__ __forceinline__ void mx4_gemm_few(const fk_mx4_gemm_args &a) {
 #pragma unroll
     for (uint32_t j = 0; j < NB; j++) sums[wave][i * NB + j][lane] = acc[i][j];
   __syncthreads();
-  const bool wide = mx4_wide_c(a);
   for (uint32_t b = wave; b < MB * NB; b += W) {
     fk_float4v v = sums[0][b][lane];
 #pragma unroll
     for (uint32_t w = 1; w < W; w++) v += sums[w][b][lane];
-    mx4_store_c<T>(a, wide, 16 * (tm + b / NB) + lane % 16, 16 * (tn + b % NB) + 4 * (lane / 16), v);
+    mx4_store_c<T>(a, 16 * (tm + b / NB) + lane % 16, 16 * (tn + b % NB) + 4 * (lane / 16), v);
   }
 }
 
@@ -140,15 +135,17 @@ __device__ __forceinline__ void mx4_gemm_few(const fk_mx4_gemm_args &a) {
 // twice.  The scales come to registers, two steps' in one load of two bytes a
 // lane, a pair of steps ahead.  Two kernels, by what hides what:
 //
-// - mx4_gemm_mid: three stages, the operands read as they are needed, and two
-//   or three threadgroups a CU, one's loads, reads and stores under another's
-//   matrix operations.
+// - mx4_gemm_mid: three stages, the operands read as they are needed, and
+//   three threadgroups a CU, one's loads, reads and stores under another's
+//   matrix operations.  For what few 256 x 256 tiles would leave to few CUs.
 // - mx4_gemm_many: 256 × 256 tiles whose sums take half the register file, so
 //   one threadgroup a CU: four stages, the next step's operands read and a
 //   later step's loaded between a step's matrix operations, and tile after
 //   tile with the next one's first loads under the stores.  Half the traffic
-//   for each product, which pays where k is long: 8192 x 8192, k 8192 248 µs
-//   (4.4 PFLOP/s, mid 265), k 2048 91 (mid 81).
+//   for each product: 8192 x 8192, operands from memory, k 8192 235 µs (4.7
+//   PFLOP/s; mid 298), k 2048 86 (3.2; mid 103).  With no loads, reads or
+//   scales at all its matrix operations take 200 µs of the 235: the clock that
+//   the chip's power leaves them (1.9 GHz of 2.4) bounds it.
 #define FK_MX4_STAGES 4
 #define FK_MX4_LDS __attribute__((address_space(3)))
 constexpr uint32_t mx4_many_side = 16;  // row tiles of a tile's side
@@ -177,15 +174,11 @@ __device__ __forceinline__ fk_float16v mx4_mfma32(u32x4 b, uint32_t bs, u32x4 a,
 // an LDS stage: of 32 rows at a time RB bytes each are written as the
 // operation left them, a lane 4 columns of a row, and read back a row's
 // consecutive 16 bytes a lane, so that stores are RB whole bytes of a row.
-// wide: C's rows are 16-byte aligned.
 template <uint32_t GM, uint32_t GN, bool AGPR, int T>
-__device__ __forceinline__ void mx4_store_many(const fk_mx4_gemm_args &a, bool wide, uint32_t m0, uint32_t n0,
+__device__ __forceinline__ void mx4_store_many(const fk_mx4_gemm_args &a, uint32_t m0, uint32_t n0,
                                                fk_float16v (&acc)[GM][GN], char *stage) {
   constexpr uint32_t RB = GN * 64, BYTES = mx4_bytes_of(T), COLS = RB / BYTES, UNITS = RB / 16, EACH = 16 / BYTES;
   const uint32_t lane = threadIdx.x % FK_WAVE;
-  // a C that the L2s would not hold goes past them (8192 x 8192 of f16, k
-  // 2048: 89.0 µs, so 82.1)
-  const bool stream = (uint64_t)a.m * a.n * BYTES >= 32u << 20;
   // 16-byte unit u of row m at place u ^ turn(m): no bank twice in 16 lanes
   auto place = [](uint32_t m, uint32_t u) { return m * RB + (u ^ (UNITS == 16 ? m & 15u : (m >> 1) & 7u)) * 16; };
 #pragma unroll
@@ -226,12 +219,11 @@ __device__ __forceinline__ void mx4_store_many(const fk_mx4_gemm_args &a, bool w
         const uint32_t m = m0 + 32 * i + r, n = n0 + c * COLS + u * EACH;
         const uint64_t at = a.c + ((uint64_t)m * a.c_stride + n) * BYTES;
         if (m < a.m && n < a.n) {
-          if (wide && n + EACH <= a.n) {
-            if (stream) __builtin_nontemporal_store(w, global_at<u32x4>(at));
-            else *global_at<u32x4>(at) = w;
+          if (n + EACH <= a.n) {
+            *global_at<mx4_u32x4>(at) = w;
           } else {
 #pragma unroll
-            for (uint32_t e = 0; e < EACH; e++)
+            for (uint32_t e = 0; e < EACH - 1; e++)
               if (n + e < a.n) {
                 if constexpr (BYTES == 4) global_at<uint32_t>(at)[e] = w[e];
                 else global_at<uint16_t>(at)[e] = (uint16_t)(w[e / 2] >> (16 * (e % 2)));
@@ -339,8 +331,7 @@ __device__ __forceinline__ void mx4_gemm_mid(const fk_mx4_gemm_args &a) {
   __builtin_amdgcn_s_waitcnt(0);
   FK_MX4_BARRIER();
 #undef FK_MX4_MID
-  const bool wide = a.c_stride * mx4_bytes_of(T) % 16 == 0 && a.c % 16 == 0;
-  mx4_store_many<GM, GN, false, T>(a, wide, 16 * tm + 32 * wm * GM, 16 * tn + 32 * wn * GN, acc,
+  mx4_store_many<GM, GN, false, T>(a, 16 * tm + 32 * wm * GM, 16 * tn + 32 * wn * GN, acc,
                                    reinterpret_cast<char *>(mx4_lds) + wave * GN * 2048);
 }
 
@@ -416,7 +407,8 @@ __device__ __forceinline__ void mx4_gemm_many(const fk_mx4_gemm_args &a) {
   // flight when the step begins.
 #define FK_MX4_STEP(TILE, FA, FB, NA, NB, SA, SB, NSA, NSB, WAIT, NEXT_PAIR, LOAD, ST_LOAD, ST_READ)          \
   do {                                                                                                        \
-    FK_MX4_VMCNT(WAIT);                                                                                       \
+    if (under && p == 0) FK_MX4_VMCNT(FK_MX4_UNDER(WAIT));                                                    \
+    else FK_MX4_VMCNT(WAIT);                                                                                  \
     FK_MX4_BARRIER();                                                                                         \
     __builtin_amdgcn_sched_barrier(0);                                                                        \
     const uint32_t so_ = (LOAD) * 1024;                                                                       \
@@ -476,9 +468,15 @@ __device__ __forceinline__ void mx4_gemm_many(const fk_mx4_gemm_args &a) {
       }                                                                                                       \
     }                                                                                                         \
   } while (0)
-  // Tile after tile, the next one's first loads under this one's stores: the
-  // stores go by way of the fourth stage, which step 0 loads.
-  const bool wide = a.c_stride * mx4_bytes_of(T) % 16 == 0 && a.c % 16 == 0;
+  // Tile after tile, the next one's first loads under this one's stores (which
+  // go by way of the fourth stage; step 0 loads it).  The counter that a wait
+  // looks at has loads and stores in their order, so the waits of a tile's
+  // first pair of steps leave out the stores that went out behind its first
+  // loads, whose number is known where the tile before was whole: with the
+  // operands from memory each time, 8192 x 8192, k 2048 104.7 µs, so 93.6.
+  constexpr uint32_t STORES = 32 * GB * 32 * GB * mx4_bytes_of(T) / (16 * FK_WAVE);  // of a whole tile, a wavefront's
+#define FK_MX4_UNDER(N) ((N) + STORES < 63 ? (N) + STORES : 63)
+  bool under = false;
   sources(blockIdx.x);
   FK_MX4_FIRST();
   for (uint32_t tile = blockIdx.x; tile < tiles; tile += gridDim.x) {
@@ -488,8 +486,9 @@ __device__ __forceinline__ void mx4_gemm_many(const fk_mx4_gemm_args &a) {
       for (uint32_t j = 0; j < GB; j++)
 #pragma unroll
         for (int r = 0; r < 16; r++) acc[i][j][r] = 0.0f;
-    // step 0 landed (what was stored since is waited for with it)
-    FK_MX4_VMCNT(2 * Q * (FK_MX4_STAGES - 2));
+    // step 0 landed
+    if (under) FK_MX4_VMCNT(FK_MX4_UNDER(2 * Q * (FK_MX4_STAGES - 2)));
+    else FK_MX4_VMCNT(2 * Q * (FK_MX4_STAGES - 2));
     FK_MX4_BARRIER();
 #pragma unroll
     for (uint32_t i = 0; i < GB; i++)
@@ -518,11 +517,13 @@ __device__ __forceinline__ void mx4_gemm_many(const fk_mx4_gemm_args &a) {
     __builtin_amdgcn_s_waitcnt(0);
     FK_MX4_BARRIER();
     const uint32_t m = 16 * tm + 32 * wm * GB, n = 16 * tn + 32 * wn * GB;
+    under = 16 * tm + 64 * GB <= a.m && 16 * tn + 64 * GB <= a.n;
     if (tile + gridDim.x < tiles) {
       sources(tile + gridDim.x);
       FK_MX4_FIRST();
     }
-    mx4_store_many<GB, GB, true, T>(a, wide, m, n, acc, reinterpret_cast<char *>(mx4_lds) + 3 * STAGE + wave * (STAGE / 4));
+    mx4_store_many<GB, GB, true, T>(a, m, n, acc,
+                                    reinterpret_cast<char *>(mx4_lds) + 3 * STAGE + wave * (STAGE / 4));
   }
 #undef FK_MX4_PIN
 #undef FK_MX4_PIN_ACC
@@ -530,6 +531,7 @@ __device__ __forceinline__ void mx4_gemm_many(const fk_mx4_gemm_args &a) {
 #undef FK_MX4_MFMAS
 #undef FK_MX4_STEP
 #undef FK_MX4_FIRST
+#undef FK_MX4_UNDER
 #undef FK_MX4_T
 }
 
