@@ -26,6 +26,7 @@ using fk::stream_of;
 
 namespace {
 
+__global__ void __launch_bounds__(FK_PLAN_THREADS) op_page_plan_held(fk_page_plan_args a) { fk::page_plan_held(a); }
 __global__ void __launch_bounds__(FK_PLAN_THREADS) op_page_plan(fk_page_plan_args a) { fk::page_plan(a); }
 
 template <int T, bool BF16>
@@ -39,17 +40,17 @@ __global__ void __launch_bounds__(FK_PAGED_THREADS, DP == 256 ? 1 : 2)
   fk::paged_attend<DP, FULL, BF16>(a, pl);
 }
 
-template <bool BF16>
-__global__ void __launch_bounds__(64 * FK_JOIN_WAVES)
+template <uint32_t W, bool BF16>
+__global__ void __launch_bounds__(64 * W)
     op_paged_attend_join(fk_paged_attend_args a, fk::PagedPlan pl, uint32_t groups) {
-  fk::paged_attend_join<BF16>(a, pl, groups);
+  fk::paged_attend_join<W, BF16>(a, pl, groups);
 }
 
 // The attention's launch for these sizes: head_dim's tile width, its
-// threadgroups and what the kernels take; 0 threadgroups and the reason if
+// threadgroups, the joins' entries and what the kernels take; 0 threadgroups and the reason if
 // the kernels do not take them.
 struct AttendLaunch {
-  uint32_t width = 0, groups = 0;
+  uint32_t width = 0, groups = 0, joins = 0;
   fk::PagedPlan plan{};
   const char *why = "";
 };
@@ -77,13 +78,29 @@ AttendLaunch attend_launch(const fk_paged_attend_args &a) {
     const uint64_t seen = a.window && a.window < length ? a.window + unit : length;
     // the kernels count units in 32 bits
     const __uint128_t units = (__uint128_t)a.requests * a.kv_heads * l.plan.head_tiles * ((seen + unit - 1) / unit);
-    if (units >= 1ull << 32) {
-      l.why = "fewer than 2^32 units of keys";
+    if (units >= 1ull << 31) {
+      l.why = "fewer than 2^31 units of keys";
       return l;
     }
     // as many as the chip's 256 compute units hold at once
     const uint64_t most = l.width == 256 ? 256 : 512;
     l.groups = (uint32_t)(units < most ? (uint64_t)units : most);
+    const uint64_t pairs = (uint64_t)a.requests * a.kv_heads * l.plan.head_tiles;
+    l.plan.by_pair = pairs <= l.groups;
+    l.joins = l.plan.by_pair ? (uint32_t)pairs : l.groups;
+    // Few units a pair at most: a threadgroup takes pairs whole, which saves the
+    // prefix sum and the join and costs a unit's time each where the pairs are
+    // few.  Requests of u units (256 keys of 64, 128 of 128 and 256), split and
+    // whole, µs, 8 kv heads (256: 2):
+    //           u = 1          2            3            4           8
+    //   1 of 64   7.4   5.0   9.4   6.8    9.4   9.5   10.0  11.7   10.8  19.9
+    //   1 of 128  8.3   6.0  10.3   7.9   10.6   9.8   10.9  11.3   11.4  19.1
+    //   1 of 256 12.4   9.7  14.5  13.5   14.3  16.5   14.0  19.5   14.3  31.3
+    //   41 of 128 11.6  9.8  15.7  14.3   21.6  17.4   25.2  21.2   38.2  35.5
+    // (many requests of one length gain from it at any length, ragged ones
+    // wait for their longest: the bound is what the host knows).
+    l.plan.whole = (seen + unit - 1) / unit <= (l.width == 256 ? 2 : 3);
+    if (l.plan.whole) l.groups = (uint32_t)(pairs < most ? pairs : most);
   }
   return l;
 }
@@ -98,6 +115,13 @@ void queue_attend(const fk_paged_attend_args &a, const AttendLaunch &l, hipStrea
     hipLaunchKernelGGL((op_paged_attend<DP, true, BF16>), dim3(l.groups), dim3(FK_PAGED_THREADS), 0, s, a, l.plan);
   else
     hipLaunchKernelGGL((op_paged_attend<DP, false, BF16>), dim3(l.groups), dim3(FK_PAGED_THREADS), 0, s, a, l.plan);
+}
+
+template <uint32_t W>
+void queue_join(const fk_paged_attend_args &a, const AttendLaunch &l, hipStream_t s) {
+  const dim3 grid(l.joins * l.plan.rows), block(64 * W);
+  if (a.cache_bf16) hipLaunchKernelGGL((op_paged_attend_join<W, true>), grid, block, 0, s, a, l.plan, l.groups);
+  else hipLaunchKernelGGL((op_paged_attend_join<W, false>), grid, block, 0, s, a, l.plan, l.groups);
 }
 
 }  // namespace
@@ -226,7 +250,8 @@ extern "C" int fk_page_plan(fk_ctx *ctx, const fk_page_plan_args *a, fk_stream *
   if (int st = admit(ctx, "fk_page_plan", a)) return st;
   const uint64_t groups = ((uint64_t)a->tokens + FK_PLAN_THREADS - 1) / FK_PLAN_THREADS;
   const uint32_t g = (uint32_t)(groups < 1 ? 1 : (groups > 256 ? 256 : groups));
-  hipLaunchKernelGGL(op_page_plan, dim3(g), dim3(FK_PLAN_THREADS), 0, stream_of(ctx, stream), *a);
+  hipLaunchKernelGGL(a->requests <= FK_PLAN_HELD ? op_page_plan_held : op_page_plan, dim3(g), dim3(FK_PLAN_THREADS), 0,
+                     stream_of(ctx, stream), *a);
   return launched(ctx, "fk_page_plan");
 }
 
@@ -268,8 +293,10 @@ extern "C" int fk_paged_attend(fk_ctx *ctx, const fk_paged_attend_args *a, fk_st
     else queue_attend<256, false>(*a, l, s);
   }
   if (int st = launched(ctx, "fk_paged_attend")) return st;
-  const dim3 grid(l.groups * l.plan.rows), block(64 * FK_JOIN_WAVES);
-  if (a->cache_bf16) hipLaunchKernelGGL((op_paged_attend_join<true>), grid, block, 0, s, *a, l.plan, l.groups);
-  else hipLaunchKernelGGL((op_paged_attend_join<false>), grid, block, 0, s, *a, l.plan, l.groups);
+  if (l.plan.whole) return FK_OK;
+  const uint32_t states = l.groups / l.joins;  // of a pair, about
+  if (states >= 8) queue_join<8>(*a, l, s);
+  else if (states >= 4) queue_join<4>(*a, l, s);
+  else queue_join<2>(*a, l, s);
   return launched(ctx, "fk_paged_attend (join)");
 }

@@ -7,11 +7,13 @@
 // prefix sums for itself (no threadgroup waits for another, nothing is kept
 // in memory between) and then takes its own tokens.
 //
-// The 1024 threads hold the sums of n / 1024 consecutive requests each; a
-// token finds its thread's chunk by bisection in LDS and its request by
-// walking the chunk.  A block is the free list's next, so its number follows
-// from the sums alone: no token waits for a table entry that this launch
-// writes.  A request's new page is written by the token that opens it.
+// Up to 2048 requests stay in LDS, two a thread: their lengths are read once,
+// and a token finds its request by bisection there.  Of more, each of the 1024
+// threads holds the sums of n / 1024 consecutive ones; a token finds its
+// thread's chunk by bisection and its request by walking the chunk.  A block is
+// the free list's next, so its number follows from the sums alone: no token
+// waits for a table entry that this launch writes.  A request's new page is
+// written by the token that opens it.
 #pragma once
 
 #include <hip/hip_runtime.h>
@@ -33,63 +35,176 @@ struct PlanRequest {
   bool fits;            // its table row and the step's tokens hold it
 };
 
-__device__ __forceinline__ uint32_t plan_pages(uint64_t positions, uint32_t block) {
-  return (uint32_t)((positions + block - 1) / block);
+__device__ __forceinline__ uint32_t plan_pages(uint32_t positions, uint32_t block) {
+  return positions ? (positions - 1) / block + 1 : 0u;
 }
 
-// Request r whose tokens start at `start` (64 bits: no sum of lengths wraps).
-__device__ __forceinline__ PlanRequest plan_request(const fk_page_plan_args &a, uint32_t r, uint64_t start) {
+// Sums of tokens stop at 2^32 - 1, which no step has: what is past it is past
+// every step's end.
+__device__ __forceinline__ uint32_t plan_add(uint32_t x, uint32_t y) { return __builtin_elementwise_add_sat(x, y); }
+
+// A request whose tokens start at `start`.
+__device__ __forceinline__ PlanRequest plan_request(const fk_page_plan_args &a, uint32_t cached, uint32_t fresh,
+                                                    uint32_t start) {
   PlanRequest q;
-  q.cached = global_at<const uint32_t>(a.cached)[r];
-  q.fresh = global_at<const uint32_t>(a.fresh)[r];
+  q.cached = cached;
+  q.fresh = fresh;
   const uint64_t total = (uint64_t)q.cached + q.fresh;
-  q.fits = total <= (uint64_t)a.table_len * a.block_size && start + q.fresh <= a.tokens;
+  q.fits = total <= (uint64_t)a.table_len * a.block_size && plan_add(start, fresh) <= a.tokens;
   q.held = q.fits ? plan_pages(q.cached, a.block_size) : 0u;
-  q.need = q.fits ? plan_pages(total, a.block_size) - q.held : 0u;
+  q.need = q.fits ? plan_pages((uint32_t)total, a.block_size) - q.held : 0u;
   return q;
 }
 
-// The sum of the lanes before this one, and the wavefront's.
-template <typename T>
-__device__ __forceinline__ T wave_before(T v, T *total) {
-  const int lane = threadIdx.x & 63;
-  T s = v;
-#pragma unroll
-  for (int d = 1; d < 64; d *= 2) {
-    const T o = __shfl_up(s, d, 64);
-    if (lane >= d) s += o;
-  }
-  *total = __shfl(s, 63, 64);
-  return s - v;
+__device__ __forceinline__ PlanRequest plan_request(const fk_page_plan_args &a, uint32_t r, uint32_t start) {
+  return plan_request(a, global_at<const uint32_t>(a.cached)[r], global_at<const uint32_t>(a.fresh)[r], start);
+}
+
+// A lane's value from DPP control CTRL's lane, 0 where there is none or the
+// row is none of ROWS.
+template <int CTRL, int ROWS>
+__device__ __forceinline__ uint32_t plan_dpp(uint32_t v) {
+  return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, ROWS, 0xF, false);
+}
+
+// The sum of the lanes up to this one.
+__device__ __forceinline__ uint32_t wave_upto(uint32_t v) {
+  v = plan_add(v, plan_dpp<0x111, 0xF>(v));  // row_shr 1, 2, 4, 8
+  v = plan_add(v, plan_dpp<0x112, 0xF>(v));
+  v = plan_add(v, plan_dpp<0x114, 0xF>(v));
+  v = plan_add(v, plan_dpp<0x118, 0xF>(v));
+  v = plan_add(v, plan_dpp<0x142, 0xA>(v));  // row_bcast 15: rows 0 and 2 onto 1 and 3
+  return plan_add(v, plan_dpp<0x143, 0xC>(v));  // row_bcast 31: the lower half onto the upper
 }
 
 // The sum of the threads before this one, and the threadgroup's; `slots`
-// holds a value a wavefront and is free again when every thread is past its
-// next barrier.
-template <typename T>
-__device__ __forceinline__ T group_before(T v, T *slots, T *total) {
-  T mine;
-  const T within = wave_before(v, &mine);
-  const uint32_t wave = threadIdx.x / 64;
-  if ((threadIdx.x & 63) == 0) slots[wave] = mine;
+// holds a value a wavefront and is used once.
+__device__ __forceinline__ uint32_t group_before(uint32_t v, uint32_t *slots, uint32_t *total) {
+  const uint32_t upto = wave_upto(v), wave = threadIdx.x / 64, lane = threadIdx.x & 63;
+  // (before this lane: the lane below's sum, which a difference would lose
+  // where the sum has stopped)
+  const uint32_t below = __shfl_up(upto, 1, 64);
+  if (lane == 63) slots[wave] = upto;
   __syncthreads();
-  T before = 0, all = 0;
+  uint32_t before = 0, all = 0;
 #pragma unroll
   for (uint32_t w = 0; w < FK_PLAN_WAVES; w++) {
-    const T s = slots[w];
-    before += w < wave ? s : (T)0;
-    all += s;
+    before = plan_add(before, w < wave ? slots[w] : 0u);
+    all = plan_add(all, slots[w]);
   }
   *total = all;
-  return before + within;
+  return plan_add(before, lane ? below : 0u);
 }
 
+// x, or the largest count for what is past it.
 __device__ __forceinline__ uint32_t plan_u32(uint64_t x) { return x < 0xFFFFFFFFull ? (uint32_t)x : 0xFFFFFFFFu; }
 
+// Token t of a request whose position is pos: its slot.  `held` blocks are in
+// the table, new ones in the free list from `first` on.
+__device__ __forceinline__ uint32_t plan_slot(const fk_page_plan_args &a, uint32_t r, uint32_t pos, uint32_t held,
+                                              uint32_t first) {
+  const auto table = global_at<uint32_t>(a.table) + (uint64_t)r * a.table_len;
+  const uint32_t page = pos / a.block_size, within = pos - page * a.block_size;
+  uint32_t block;
+  if (page < held) {
+    block = table[page];
+  } else {
+    block = global_at<const uint32_t>(a.free_blocks)[first + (page - held)];
+    if (within == 0) table[page] = block;
+  }
+  return plan_u32((uint64_t)block * a.block_size + within);
+}
+
+__device__ __forceinline__ void plan_token(const fk_page_plan_args &a, uint32_t t, uint32_t slot, uint32_t pos,
+                                           uint32_t owner) {
+  global_at<uint32_t>(a.slots)[t] = slot;
+  global_at<uint32_t>(a.positions)[t] = pos;
+  global_at<uint32_t>(a.owner)[t] = owner;
+}
+
+__device__ __forceinline__ void plan_counts(const fk_page_plan_args &a, uint32_t total, uint32_t head, uint32_t taken,
+                                            uint32_t refused) {
+  global_at<uint32_t>(a.starts)[a.requests] = total;
+  const auto c = global_at<uint32_t>(a.counts);
+  c[0] = total;
+  c[1] = taken;
+  c[2] = refused;
+  c[3] = head + taken;
+}
+
+// HELD: at most FK_PLAN_HELD requests.
+#define FK_PLAN_HELD (2 * FK_PLAN_THREADS)
+__device__ __forceinline__ void page_plan_held(const fk_page_plan_args &a) {
+  __shared__ uint32_t token_slots[FK_PLAN_WAVES], block_slots[FK_PLAN_WAVES], refused, taken;
+  // a request's first token, its cached positions, its first new block's place
+  // in the free list (FK_NO_SLOT: it does not fit)
+  __shared__ uint32_t starts[FK_PLAN_HELD], held_at[FK_PLAN_HELD], firsts[FK_PLAN_HELD];
+  const uint32_t tid = threadIdx.x, n = a.requests;
+  const uint32_t head = *global_at<const uint32_t>(a.head);
+  uint32_t c[2], f[2];
+#pragma unroll
+  for (uint32_t i = 0; i < 2; i++) {
+    const uint32_t r = 2 * tid + i;
+    c[i] = r < n ? global_at<const uint32_t>(a.cached)[r] : 0u;
+    f[i] = r < n ? global_at<const uint32_t>(a.fresh)[r] : 0u;
+  }
+  const uint32_t avail = a.free_len > head ? a.free_len - head : 0u;
+  if (tid == 0) refused = taken = 0;
+  uint32_t total;
+  const uint32_t first = group_before(plan_add(f[0], f[1]), token_slots, &total);
+  const PlanRequest q[2] = {plan_request(a, c[0], f[0], first), plan_request(a, c[1], f[1], plan_add(first, f[0]))};
+  // (requests that fit need a block a token at most, so the step's fewer than
+  // 2^32)
+  uint32_t needed, after = group_before(q[0].need + q[1].need, block_slots, &needed);
+  uint32_t out = 0, most = 0;
+#pragma unroll
+  for (uint32_t i = 0; i < 2; i++) {
+    const uint32_t r = 2 * tid + i;
+    const uint32_t before = after;
+    after += q[i].need;
+    const bool fits = q[i].fits && (q[i].need == 0 || after <= avail);
+    const uint32_t start = r < n ? (i ? plan_add(first, f[0]) : first) : 0xFFFFFFFFu;
+    starts[r] = start;
+    held_at[r] = c[i];
+    firsts[r] = fits ? head + before : FK_NO_SLOT;
+    if (r < n) {
+      if (fits && q[i].need) most = after;
+      out += !fits;
+      if (tid % gridDim.x == blockIdx.x) {
+        global_at<uint32_t>(a.lengths)[r] = fits ? c[i] + f[i] : c[i];
+        global_at<uint32_t>(a.starts)[r] = start;
+      }
+    }
+  }
+  if (blockIdx.x == 0) {
+    if (out) atomicAdd(&refused, out);
+    if (most) atomicMax(&taken, most);
+  }
+  __syncthreads();
+  if (blockIdx.x == 0 && tid == 0) plan_counts(a, total, head, taken, refused);
+  for (uint64_t t64 = (uint64_t)blockIdx.x * FK_PLAN_THREADS + tid; t64 < a.tokens;
+       t64 += (uint64_t)gridDim.x * FK_PLAN_THREADS) {
+    const uint32_t t = (uint32_t)t64;
+    uint32_t slot = FK_NO_SLOT, pos = 0, owner = FK_NO_SLOT;
+    if (t < total) {
+      // the last request that starts at or before t: one without tokens starts
+      // where the next does
+      owner = 0;
+#pragma unroll
+      for (uint32_t step = FK_PLAN_HELD / 2; step > 0; step /= 2)
+        if (starts[owner + step] <= t) owner += step;
+      const uint32_t cached = held_at[owner], free_at = firsts[owner];
+      pos = cached + (t - starts[owner]);
+      if (free_at != FK_NO_SLOT) slot = plan_slot(a, owner, pos, plan_pages(cached, a.block_size), free_at);
+    }
+    plan_token(a, t, slot, pos, owner);
+  }
+}
+
 __device__ __forceinline__ void page_plan(const fk_page_plan_args &a) {
-  __shared__ uint64_t token_slots[FK_PLAN_WAVES], block_slots[FK_PLAN_WAVES];
-  __shared__ uint64_t first_token[FK_PLAN_THREADS];  // the tokens before a chunk's first request
-  __shared__ uint64_t first_block[FK_PLAN_THREADS];  // the new blocks before it
+  __shared__ uint32_t token_slots[FK_PLAN_WAVES], block_slots[FK_PLAN_WAVES];
+  __shared__ uint32_t first_token[FK_PLAN_THREADS];  // the tokens before a chunk's first request
+  __shared__ uint32_t first_block[FK_PLAN_THREADS];  // the new blocks before it
   __shared__ uint32_t refused, taken;
   const uint32_t tid = threadIdx.x;
   const uint32_t n = a.requests;
@@ -101,19 +216,19 @@ __device__ __forceinline__ void page_plan(const fk_page_plan_args &a) {
   const uint32_t avail = a.free_len > head ? a.free_len - head : 0u;
   if (tid == 0) refused = taken = 0;
 
-  uint64_t mine = 0, total;
-  for (uint32_t r = r0; r < r1; r++) mine += fresh[r];
-  const uint64_t tokens0 = group_before(mine, token_slots, &total);
-  uint64_t need = 0, needed;
+  uint32_t mine = 0, total;
+  for (uint32_t r = r0; r < r1; r++) mine = plan_add(mine, fresh[r]);
+  const uint32_t tokens0 = group_before(mine, token_slots, &total);
+  uint32_t need = 0, needed;
   {
-    uint64_t at = tokens0;
+    uint32_t at = tokens0;
     for (uint32_t r = r0; r < r1; r++) {
       const PlanRequest q = plan_request(a, r, at);
       need += q.need;
-      at += q.fresh;
+      at = plan_add(at, q.fresh);
     }
   }
-  const uint64_t blocks0 = group_before(need, block_slots, &needed);
+  const uint32_t blocks0 = group_before(need, block_slots, &needed);
   first_token[tid] = tokens0;
   first_block[tid] = blocks0;
   __syncthreads();
@@ -122,19 +237,19 @@ __device__ __forceinline__ void page_plan(const fk_page_plan_args &a) {
   // the first, which walks them all.
   const bool writes = tid % gridDim.x == blockIdx.x, counts = blockIdx.x == 0;
   if (writes || counts) {
-    uint64_t at = tokens0, after = blocks0;
+    uint32_t at = tokens0, after = blocks0;
     uint32_t out = 0, most = 0;
     for (uint32_t r = r0; r < r1; r++) {
       const PlanRequest q = plan_request(a, r, at);
       after += q.need;
       const bool fits = q.fits && (q.need == 0 || after <= avail);
-      if (fits && q.need) most = (uint32_t)after;
+      if (fits && q.need) most = after;
       out += !fits;
       if (writes) {
         global_at<uint32_t>(a.lengths)[r] = fits ? q.cached + q.fresh : q.cached;
-        global_at<uint32_t>(a.starts)[r] = plan_u32(at);
+        global_at<uint32_t>(a.starts)[r] = at;
       }
-      at += q.fresh;
+      at = plan_add(at, q.fresh);
     }
     if (counts) {
       if (out) atomicAdd(&refused, out);
@@ -143,18 +258,9 @@ __device__ __forceinline__ void page_plan(const fk_page_plan_args &a) {
   }
   if (counts) {
     __syncthreads();
-    if (tid == 0) {
-      global_at<uint32_t>(a.starts)[n] = plan_u32(total);
-      const auto c = global_at<uint32_t>(a.counts);
-      c[0] = plan_u32(total);
-      c[1] = taken;
-      c[2] = refused;
-      c[3] = head + taken;
-    }
+    if (tid == 0) plan_counts(a, total, head, taken, refused);
   }
 
-  const auto table = global_at<const uint32_t>(a.table);
-  const auto free_blocks = global_at<const uint32_t>(a.free_blocks);
   for (uint64_t t64 = (uint64_t)blockIdx.x * FK_PLAN_THREADS + tid; t64 < a.tokens;
        t64 += (uint64_t)gridDim.x * FK_PLAN_THREADS) {
     const uint32_t t = (uint32_t)t64;
@@ -167,30 +273,19 @@ __device__ __forceinline__ void page_plan(const fk_page_plan_args &a) {
       for (uint32_t step = FK_PLAN_THREADS / 2; step > 0; step /= 2)
         if (first_token[lo + step] <= t) lo += step;
       uint32_t r = lo * chunk;
-      uint64_t at = first_token[lo], blocks = first_block[lo];
+      uint32_t at = first_token[lo], blocks = first_block[lo];
       PlanRequest q = plan_request(a, r, at);
-      while (at + q.fresh <= t) {
-        at += q.fresh;
+      while (plan_add(at, q.fresh) <= t) {
+        at = plan_add(at, q.fresh);
         blocks += q.need;
         q = plan_request(a, ++r, at);
       }
       owner = r;
-      pos = q.cached + (uint32_t)(t - at);
-      if (q.fits && (q.need == 0 || blocks + q.need <= avail)) {
-        const uint32_t page = pos / a.block_size, within = pos - page * a.block_size;
-        uint32_t block;
-        if (page < q.held) {
-          block = table[(uint64_t)r * a.table_len + page];
-        } else {
-          block = free_blocks[head + (uint32_t)blocks + (page - q.held)];
-          if (within == 0) global_at<uint32_t>(a.table)[(uint64_t)r * a.table_len + page] = block;
-        }
-        slot = plan_u32((uint64_t)block * a.block_size + within);
-      }
+      pos = q.cached + (t - at);
+      if (q.fits && (q.need == 0 || blocks + q.need <= avail))
+        slot = plan_slot(a, r, pos, q.held, head + blocks);
     }
-    global_at<uint32_t>(a.slots)[t] = slot;
-    global_at<uint32_t>(a.positions)[t] = pos;
-    global_at<uint32_t>(a.owner)[t] = owner;
+    plan_token(a, t, slot, pos, owner);
   }
 }
 
