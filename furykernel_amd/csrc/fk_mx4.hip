@@ -49,10 +49,11 @@ __global__ void __launch_bounds__(256, 3) op_mx4_gemm_mid(fk_mx4_gemm_args a) {
 uint64_t codes_bytes(uint32_t rows, uint32_t k) { return (uint64_t)fk::mx4_row_tiles(rows) * fk::mx4_pairs(k) * 2048; }
 uint64_t scales_bytes(uint32_t rows, uint32_t k) { return (uint64_t)fk::mx4_row_tiles(rows) * fk::mx4_pairs(k) * 128; }
 
-// A matrix the kernels' 32-bit counts of tiles hold.
+// A matrix that one launch of a thread for 64 bytes of codes makes: up to 2^25
+// pairs of tiles (1.4 10^11 elements).
 bool matrix(uint32_t rows, uint32_t k) {
   return rows > 0 && k > 0 && rows <= 1u << 30 && k <= 1u << 30 &&
-         (uint64_t)fk::mx4_row_tiles(rows) * fk::mx4_pairs(k) < 1ull << 31;
+         (uint64_t)fk::mx4_row_tiles(rows) * fk::mx4_pairs(k) <= 1ull << 25;
 }
 
 // Rows of `type` from `addr` on, `stride` elements apart, aligned to their

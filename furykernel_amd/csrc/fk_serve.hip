@@ -34,10 +34,10 @@ __global__ void __launch_bounds__(FK_STORE_THREADS) op_paged_store(fk_paged_stor
   fk::paged_store<T, BF16>(a);
 }
 
-template <uint32_t DP, bool FULL, bool BF16>
-__global__ void __launch_bounds__(FK_PAGED_THREADS, DP == 256 ? 1 : 2)
+template <uint32_t DP, uint32_t W, bool FULL, bool BF16>
+__global__ void __launch_bounds__(64 * W, DP == 256 || W == 8 ? 1 : 2)
     op_paged_attend(fk_paged_attend_args a, fk::PagedPlan pl) {
-  fk::paged_attend<DP, FULL, BF16>(a, pl);
+  fk::paged_attend<DP, W, FULL, BF16>(a, pl);
 }
 
 template <uint32_t W, bool BF16>
@@ -50,7 +50,7 @@ __global__ void __launch_bounds__(64 * W)
 // threadgroups, the joins' entries and what the kernels take; 0 threadgroups and the reason if
 // the kernels do not take them.
 struct AttendLaunch {
-  uint32_t width = 0, groups = 0, joins = 0;
+  uint32_t width = 0, waves = 4, groups = 0, joins = 0;
   fk::PagedPlan plan{};
   const char *why = "";
 };
@@ -89,17 +89,23 @@ AttendLaunch attend_launch(const fk_paged_attend_args &a) {
     l.plan.by_pair = pairs <= l.groups;
     l.joins = l.plan.by_pair ? (uint32_t)pairs : l.groups;
     // Few units a pair at most: a threadgroup takes pairs whole, which saves the
-    // prefix sum and the join and costs a unit's time each where the pairs are
-    // few.  Requests of u units (256 keys of 64, 128 of 128 and 256), split and
-    // whole, µs, 8 kv heads (256: 2):
-    //           u = 1          2            3            4           8
-    //   1 of 64   7.4   5.0   9.4   6.8    9.4   9.5   10.0  11.7   10.8  19.9
-    //   1 of 128  8.3   6.0  10.3   7.9   10.6   9.8   10.9  11.3   11.4  19.1
-    //   1 of 256 12.4   9.7  14.5  13.5   14.3  16.5   14.0  19.5   14.3  31.3
-    //   41 of 128 11.6  9.8  15.7  14.3   21.6  17.4   25.2  21.2   38.2  35.5
-    // (many requests of one length gain from it at any length, ragged ones
-    // wait for their longest: the bound is what the host knows).
-    l.plan.whole = (seen + unit - 1) / unit <= (l.width == 256 ? 2 : 3);
+    // prefix sum and the join and costs each further unit's time; of two units
+    // and more by 8 wavefronts, where the pairs do not fill the CUs anyway.
+    // Requests of u units (256 keys of 64, 128 of 128 and 256), 8 kv heads (of
+    // 256: 2), µs split, whole by 4, whole by 8:
+    //               u = 1            2                3                4
+    //    1 of 64    7.4 5.0  5.6     9.4  6.7  6.0    9.5  9.2  8.3    9.8 11.7  9.6
+    //   16 of 64    8.7 6.3  6.5    11.9  8.8  7.9   13.1 11.0 10.2   14.4 13.1 11.2
+    //    1 of 128   8.3 5.9  6.3    10.1  7.2  6.9   10.3  9.2  8.8   10.8 11.1  9.9
+    //   16 of 128   9.2 6.8  7.2    12.6  9.1  8.9   14.2 11.1 11.6   15.2 13.0 12.4
+    //   41 of 128  11.6 9.8         15.7 14.3        21.6 17.4        25.2 21.2
+    //    1 of 256  12.4 9.7         14.5 13.5        14.3 16.5        14.0 19.5
+    // (many requests of one length would gain from it at any length, but ragged
+    // ones would wait for their longest: the table's length is what the host
+    // knows.)
+    const uint64_t each = (seen + unit - 1) / unit;
+    l.waves = l.width != 256 && pairs <= 256 && each >= 2 && each <= 4 ? 8 : 4;
+    l.plan.whole = each <= (l.width == 256 ? 2 : l.waves == 8 ? 4 : 3);
     if (l.plan.whole) l.groups = (uint32_t)(pairs < most ? pairs : most);
   }
   return l;
@@ -109,12 +115,19 @@ size_t attend_bytes(const fk_paged_attend_args &a, const AttendLaunch &l) {
   return l.groups * (sizeof(fk::u32x4) + 2 * (size_t)l.plan.rows * (a.head_dim + 2) * sizeof(float));
 }
 
-template <uint32_t DP, bool BF16>
+template <uint32_t DP, uint32_t W, bool BF16>
 void queue_attend(const fk_paged_attend_args &a, const AttendLaunch &l, hipStream_t s) {
   if (a.head_dim == DP)
-    hipLaunchKernelGGL((op_paged_attend<DP, true, BF16>), dim3(l.groups), dim3(FK_PAGED_THREADS), 0, s, a, l.plan);
+    hipLaunchKernelGGL((op_paged_attend<DP, W, true, BF16>), dim3(l.groups), dim3(64 * W), 0, s, a, l.plan);
   else
-    hipLaunchKernelGGL((op_paged_attend<DP, false, BF16>), dim3(l.groups), dim3(FK_PAGED_THREADS), 0, s, a, l.plan);
+    hipLaunchKernelGGL((op_paged_attend<DP, W, false, BF16>), dim3(l.groups), dim3(64 * W), 0, s, a, l.plan);
+}
+
+template <bool BF16>
+void queue_attend(const fk_paged_attend_args &a, const AttendLaunch &l, hipStream_t s) {
+  if (l.width == 256) queue_attend<256, 4, BF16>(a, l, s);
+  else if (l.width == 128) l.waves == 8 ? queue_attend<128, 8, BF16>(a, l, s) : queue_attend<128, 4, BF16>(a, l, s);
+  else l.waves == 8 ? queue_attend<64, 8, BF16>(a, l, s) : queue_attend<64, 4, BF16>(a, l, s);
 }
 
 template <uint32_t W>
@@ -283,15 +296,8 @@ extern "C" int fk_paged_attend(fk_ctx *ctx, const fk_paged_attend_args *a, fk_st
   const AttendLaunch l = a ? attend_launch(*a) : AttendLaunch{};
   if (int st = admit(ctx, "fk_paged_attend", a, l)) return st;
   const hipStream_t s = stream_of(ctx, stream);
-  if (a->cache_bf16) {
-    if (l.width == 64) queue_attend<64, true>(*a, l, s);
-    else if (l.width == 128) queue_attend<128, true>(*a, l, s);
-    else queue_attend<256, true>(*a, l, s);
-  } else {
-    if (l.width == 64) queue_attend<64, false>(*a, l, s);
-    else if (l.width == 128) queue_attend<128, false>(*a, l, s);
-    else queue_attend<256, false>(*a, l, s);
-  }
+  if (a->cache_bf16) queue_attend<true>(*a, l, s);
+  else queue_attend<false>(*a, l, s);
   if (int st = launched(ctx, "fk_paged_attend")) return st;
   if (l.plan.whole) return FK_OK;
   const uint32_t states = l.groups / l.joins;  // of a pair, about

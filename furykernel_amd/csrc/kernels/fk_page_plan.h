@@ -137,7 +137,7 @@ __device__ __forceinline__ void plan_counts(const fk_page_plan_args &a, uint32_t
 __device__ __forceinline__ void page_plan_held(const fk_page_plan_args &a) {
   __shared__ uint32_t token_slots[FK_PLAN_WAVES], block_slots[FK_PLAN_WAVES], refused, taken;
   // a request's first token, its cached positions, its first new block's place
-  // in the free list (FK_NO_SLOT: it does not fit)
+  // in the free list (below free_len; FK_NO_SLOT: it does not fit)
   __shared__ uint32_t starts[FK_PLAN_HELD], held_at[FK_PLAN_HELD], firsts[FK_PLAN_HELD];
   const uint32_t tid = threadIdx.x, n = a.requests;
   const uint32_t head = *global_at<const uint32_t>(a.head);
@@ -166,7 +166,7 @@ __device__ __forceinline__ void page_plan_held(const fk_page_plan_args &a) {
     const uint32_t start = r < n ? (i ? plan_add(first, f[0]) : first) : 0xFFFFFFFFu;
     starts[r] = start;
     held_at[r] = c[i];
-    firsts[r] = fits ? head + before : FK_NO_SLOT;
+    firsts[r] = fits ? (q[i].need ? head + before : 0u) : FK_NO_SLOT;
     if (r < n) {
       if (fits && q[i].need) most = after;
       out += !fits;

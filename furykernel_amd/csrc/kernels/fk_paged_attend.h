@@ -20,9 +20,9 @@
 // a request, pairs go whole to the threadgroups instead: no prefix sum, no
 // states, no join (the launch's rule has both sides measured).
 //
-// In a threadgroup each of the 4 wavefronts takes a quarter of a pair's tiles
-// with a state of its own; nothing is shared until they meet at the pair's
-// end.  A tile's K and V rows (KT keys) go straight into the wavefront's LDS;
+// In a threadgroup each of the 4 wavefronts (8 where few pairs go whole) takes
+// its share of a pair's tiles with a state of its own; nothing is shared until
+// they meet at the pair's end.  A tile's K and V rows (KT keys) go straight into the wavefront's LDS;
 // the next tile's K is loaded as soon as the scores are made and its V after
 // the values, so loads are in flight all the time without a second buffer.
 // That needs reads of one beside loads into the other, which the compiler
@@ -189,8 +189,8 @@ __device__ __forceinline__ uint16_t paged_round(float x) {
 }
 
 // DP: the head's width in the tiles (64, 128 or 256; head_dim at most that);
-// FULL: head_dim is DP.
-template <uint32_t DP, bool FULL, bool BF16>
+// W: its wavefronts, 4, or 8 of whole pairs; FULL: head_dim is DP.
+template <uint32_t DP, uint32_t W, bool FULL, bool BF16>
 __device__ __forceinline__ void paged_attend(const fk_paged_attend_args &a, const PagedPlan &pl) {
   using Op = PagedOperand<BF16>;
   using vec = typename Op::vec;
@@ -199,10 +199,10 @@ __device__ __forceinline__ void paged_attend(const fk_paged_attend_args &a, cons
   constexpr uint32_t UNITS = DP / 8;             // 16-byte pieces of a row
   constexpr uint32_t KPL = 64 / UNITS;           // rows a load of the wavefront covers
   constexpr uint32_t LOADS = KT / KPL;           // loads a tile's K or V takes
-  constexpr uint32_t UK = KT * FK_PAGED_WAVES;   // keys a unit
-  __shared__ __attribute__((aligned(16))) uint16_t kv[FK_PAGED_WAVES][2][KT * DP];
-  __shared__ float sm[FK_PAGED_WAVES][16], sl[FK_PAGED_WAVES][16];
-  __shared__ uint32_t wave_units[FK_PAGED_WAVES];
+  constexpr uint32_t THREADS = 64 * W;
+  __shared__ __attribute__((aligned(16))) uint16_t kv[W][2][KT * DP];
+  __shared__ float sm[W][16], sl[W][16];
+  __shared__ uint32_t wave_units[W];
   __shared__ u32x4 found;
   const uint32_t lane = threadIdx.x & (FK_WAVE - 1);
   const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x / FK_WAVE);
@@ -219,7 +219,7 @@ __device__ __forceinline__ void paged_attend(const fk_paged_attend_args &a, cons
   auto units_of = [&](uint32_t r) { return units_in(length_of(r)); };
   // (rows of pieces past head_dim are zeros in K, which no load writes)
   if (!FULL)
-    for (uint32_t i = threadIdx.x; i < FK_PAGED_WAVES * KT * UNITS; i += FK_PAGED_THREADS)
+    for (uint32_t i = threadIdx.x; i < W * KT * UNITS; i += THREADS)
       reinterpret_cast<uint4 *>(kv[i / (KT * UNITS)][0])[i % (KT * UNITS)] = make_uint4(0, 0, 0, 0);
   // The run: units begin .. end - 1 of `total`, of which request r's `here`
   // start at `at`.
@@ -228,7 +228,7 @@ __device__ __forceinline__ void paged_attend(const fk_paged_attend_args &a, cons
     __syncthreads();
   } else {
     // The units of each thread's requests, and before them.
-    const uint32_t chunk = (n + FK_PAGED_THREADS - 1) / FK_PAGED_THREADS;
+    const uint32_t chunk = (n + THREADS - 1) / THREADS;
     const uint32_t r0 = min(threadIdx.x * chunk, n), r1 = min(r0 + chunk, n);
     uint32_t mine = 0;
     for (uint32_t r = r0; r < r1; r++) mine += units_of(r);
@@ -242,7 +242,7 @@ __device__ __forceinline__ void paged_attend(const fk_paged_attend_args &a, cons
     __syncthreads();
     uint32_t before = upto - mine;
 #pragma unroll
-    for (uint32_t w = 0; w < FK_PAGED_WAVES; w++) {
+    for (uint32_t w = 0; w < W; w++) {
       before += w < wave ? wave_units[w] : 0u;
       total += wave_units[w];
     }
@@ -264,12 +264,12 @@ __device__ __forceinline__ void paged_attend(const fk_paged_attend_args &a, cons
     // Requests that see nothing: rows of zeros.
     for (uint32_t r = blockIdx.x; r < n; r += gridDim.x)
       if (length_of(r) == 0) {
-        for (uint32_t e = threadIdx.x; e < width; e += FK_PAGED_THREADS) {
+        for (uint32_t e = threadIdx.x; e < width; e += THREADS) {
           if (a.out_f32) global_at<float>(a.out)[r * a.out_stride + e] = 0.0f;
           else global_at<uint16_t>(a.out)[r * a.out_stride + e] = 0;
         }
         if (pl.by_pair)
-          for (uint32_t p = threadIdx.x; p < per_request; p += FK_PAGED_THREADS)
+          for (uint32_t p = threadIdx.x; p < per_request; p += THREADS)
             joins[r * per_request + p] = u32x4{0, 0, 0, 0};
       }
     if (begin == end) {
@@ -307,7 +307,7 @@ __device__ __forceinline__ void paged_attend(const fk_paged_attend_args &a, cons
       if (length == 0) {
         const uint32_t g = pid % per_request / pl.head_tiles, t = pid % pl.head_tiles * 16;
         const uint64_t where = r * a.out_stride + (uint64_t)(g * pl.group + t) * D;
-        for (uint32_t e = threadIdx.x; e < min(pl.group - t, 16u) * D; e += FK_PAGED_THREADS) {
+        for (uint32_t e = threadIdx.x; e < min(pl.group - t, 16u) * D; e += THREADS) {
           if (a.out_f32) global_at<float>(a.out)[where + e] = 0.0f;
           else global_at<uint16_t>(a.out)[where + e] = 0;
         }
@@ -326,10 +326,10 @@ __device__ __forceinline__ void paged_attend(const fk_paged_attend_args &a, cons
       const uint32_t g = pair / pl.head_tiles, h0 = g * pl.group + pair % pl.head_tiles * 16;
       const uint32_t G = min(pl.group - pair % pl.head_tiles * 16, 16u);
       const uint32_t seg1 = min(end, pair0 + per_pair);
-      // the segment's tiles, a quarter to each wavefront
+      // the segment's tiles, shared out to the wavefronts
       const uint32_t s0 = (pos - pair0) * FK_PAGED_WAVES, s1 = min((seg1 - pair0) * FK_PAGED_WAVES, ks.tiles);
-      const uint32_t t0 = ks.tile0 + s0 + wave * (s1 - s0) / FK_PAGED_WAVES;
-      const uint32_t t1 = ks.tile0 + s0 + (wave + 1) * (s1 - s0) / FK_PAGED_WAVES;
+      const uint32_t t0 = ks.tile0 + s0 + wave * (s1 - s0) / W;
+      const uint32_t t1 = ks.tile0 + s0 + (wave + 1) * (s1 - s0) / W;
 
       // Q (B of S = K Qᵀ): lane l holds head l mod 16 (past the group: its
       // last), d 32 h + 8 (l div 16) .. + 7, zeros past the head.
@@ -518,15 +518,15 @@ __device__ __forceinline__ void paged_attend(const fk_paged_attend_args &a, cons
       const bool whole = pos == pair0 && seg1 == pair0 + per_pair;
       const uint32_t side = pair0 < begin ? 0u : 1u;
       const auto to = states + paged_state(blockIdx.x, side, pl.rows, D);
-      for (uint32_t e = threadIdx.x; e < G * D; e += FK_PAGED_THREADS) {
+      for (uint32_t e = threadIdx.x; e < G * D; e += THREADS) {
         const uint32_t q = e / D, d = e - q * D;
         float mm = sm[0][q];
 #pragma unroll
-        for (uint32_t w = 1; w < FK_PAGED_WAVES; w++) mm = __builtin_fmaxf(mm, sm[w][q]);
+        for (uint32_t w = 1; w < W; w++) mm = __builtin_fmaxf(mm, sm[w][q]);
         const float mc = paged_ref(mm);
         float ll = 0.0f, oo = 0.0f;
 #pragma unroll
-        for (uint32_t w = 0; w < FK_PAGED_WAVES; w++) {
+        for (uint32_t w = 0; w < W; w++) {
           const float f = __builtin_amdgcn_exp2f(sm[w][q] - mc);
           ll += sl[w][q] * f;
           oo += reinterpret_cast<const float *>(kv[w][1])[q * DP + d] * f;

@@ -76,7 +76,8 @@ int fk_page_plan(fk_ctx *ctx, const fk_page_plan_args *args, fk_stream *stream);
  * block_size, q and k turned by RoPE (src/FuryKernel/Program/Eval.hs:372-383,
  * NeoX halves, in binary32 by the table's cosines and sines at positions[t]),
  * q rounded once into qr, k and v rounded once into the pools.  Tokens without
- * a slot leave everything as it was; tokens of one slot leave either's row. */
+ * a slot leave everything as it was.  Slots are distinct, as a plan's are (of
+ * two tokens with one slot, each element is one's or the other's). */
 typedef struct fk_paged_store_args {
   uint64_t q, k, v;   /* rows of rows_type; q may be 0: no queries */
   uint64_t slots;     /* u32 [tokens] */

@@ -120,6 +120,15 @@ def test_plan_of_lengths_that_are_nonsense(device, mem):
     hold_plan(device, mem, x)
 
 
+@pytest.mark.parametrize("n", [40, 3000])
+def test_plan_of_a_free_list_taken_past_its_end(device, mem, n):
+    """No block is left; requests whose pages hold their new tokens go on."""
+    x = plan_case(8, n, 60, 3, 16, 7)
+    x["head"] = 0xFFFFFFFF
+    want = hold_plan(device, mem, x)
+    assert 0 < want["counts"][2] < n and np.any(want["slots"] != S.NO_SLOT)
+
+
 def test_plan_of_nothing(device, mem):
     x = plan_case(7, 5, 60, 0, 16, 7)
     x["fresh"][:] = 0
@@ -288,11 +297,24 @@ RAGGED = [0, 1, 2, 15, 16, 17, 31, 32, 33, 63, 64, 65, 0, 127, 128, 129, 255, 25
 @pytest.mark.parametrize("heads,kv,d,block", [
     (4, 4, 64, 16), (8, 2, 64, 7), (7, 1, 64, 1), (16, 1, 128, 16), (12, 4, 128, 24), (17, 1, 128, 64),
     (40, 1, 64, 16), (2, 2, 8, 16), (4, 2, 72, 16), (6, 2, 80, 5), (8, 8, 96, 128), (3, 1, 136, 16), (4, 1, 256, 16),
-    (34, 2, 256, 3)])
+    (34, 2, 256, 3), (4, 2, 64, 1000), (300, 300, 8, 16)])
 def test_attend_of_ragged_requests(device, mem, heads, kv, d, block, cache):
     print(f"attend {heads} {kv} {d} {block} {cache}", flush=True)
     x = attend_inputs(np.random.default_rng(heads + d), RAGGED, heads, kv, d, block, cache)
     hold_attend(device, mem, x, d ** -0.5)
+
+
+@pytest.mark.parametrize("pages", [2, 4, 8, 12, 16, 17, 24, 32, 64, 65, 100])
+@pytest.mark.parametrize("d,kv", [(64, 2), (128, 1), (256, 2), (64, 64)])
+def test_attend_of_tables_of_every_length(device, mem, pages, d, kv):
+    """Tables of few units go whole to the threadgroups, longer ones split:
+    each side of each rule, the lengths short and up to the table's."""
+    print(f"attend table {pages} {d} {kv}", flush=True)
+    top = pages * 16
+    lengths = [x for x in (0, 1, 33, top // 2, top - 1, top, 17) if x <= top]
+    x = attend_inputs(np.random.default_rng(pages), lengths, 2 * kv, kv, d, 16, "bf16", table_len=pages)
+    hold_attend(device, mem, x, d ** -0.5)
+    hold_attend(device, mem, x, d ** -0.5, window=40)
 
 
 @pytest.mark.parametrize("window", [1, 7, 64, 100, 256, 5000])
@@ -311,6 +333,14 @@ def test_attend_of_batches(device, mem, lengths, d, cache):
     print(f"attend batch {len(lengths)} {max(lengths)} {d} {cache}", flush=True)
     x = attend_inputs(np.random.default_rng(len(lengths)), lengths, 4, 2, d, 16, cache)
     hold_attend(device, mem, x, d ** -0.5)
+
+
+def test_attend_of_one_request_with_many_heads(device, mem):
+    """More (request, kv head) pairs than threads, split, whole and empty."""
+    for lengths, table_len in (([2000], 125), ([0], 125), ([90], 6)):
+        print(f"attend many heads {lengths}", flush=True)
+        x = attend_inputs(np.random.default_rng(5), lengths, 300, 300, 16, 16, "bf16", table_len=table_len)
+        hold_attend(device, mem, x, 0.25)
 
 
 def test_attend_rows_apart_and_f32_out(device, mem):
