@@ -49,11 +49,11 @@ __global__ void __launch_bounds__(256, 3) op_mx4_gemm_mid(fk_mx4_gemm_args a) {
 uint64_t codes_bytes(uint32_t rows, uint32_t k) { return (uint64_t)fk::mx4_row_tiles(rows) * fk::mx4_pairs(k) * 2048; }
 uint64_t scales_bytes(uint32_t rows, uint32_t k) { return (uint64_t)fk::mx4_row_tiles(rows) * fk::mx4_pairs(k) * 128; }
 
-// A matrix that one launch of a thread for 64 bytes of codes makes: up to 2^25
-// pairs of tiles (1.4 10^11 elements).
+// A matrix that one launch of a wavefront a tile makes: up to 2^25 pairs of
+// tiles (1.4 10^11 elements), 2^32 threads.
 bool matrix(uint32_t rows, uint32_t k) {
   return rows > 0 && k > 0 && rows <= 1u << 30 && k <= 1u << 30 &&
-         (uint64_t)fk::mx4_row_tiles(rows) * fk::mx4_pairs(k) <= 1ull << 25;
+         (uint64_t)fk::mx4_row_tiles(rows) * fk::mx4_pairs(k) < 1ull << 25;
 }
 
 // Rows of `type` from `addr` on, `stride` elements apart, aligned to their
@@ -70,10 +70,10 @@ uint64_t rows_bytes(uint64_t rows, uint64_t stride, uint64_t width, uint32_t typ
   return ((rows - 1) * stride + width) * fk::mx4_bytes_of((int)type);
 }
 
-// A threadgroup a FK_MX4_THREADS / 64 pairs of tiles.
-uint32_t pair_groups(uint32_t rows, uint32_t k) {
-  const uint64_t pairs = (uint64_t)fk::mx4_row_tiles(rows) * fk::mx4_pairs(k), w = FK_MX4_THREADS / FK_WAVE;
-  return (uint32_t)((pairs + w - 1) / w);
+// Threadgroups of a wavefront a tile.
+uint32_t tile_groups(uint32_t rows, uint32_t k) {
+  const uint64_t tiles = 2ull * fk::mx4_row_tiles(rows) * fk::mx4_pairs(k), w = FK_MX4_THREADS / FK_WAVE;
+  return (uint32_t)((tiles + w - 1) / w);
 }
 
 template <typename F>
@@ -198,7 +198,7 @@ extern "C" size_t fk_mx4_scales_bytes(uint32_t rows, uint32_t k) { return matrix
 
 extern "C" int fk_mx4_quantize(fk_ctx *ctx, const fk_mx4_quantize_args *a, fk_stream *stream) {
   if (int st = admit(ctx, "fk_mx4_quantize", a)) return st;
-  const dim3 grid(pair_groups(a->rows, a->k)), block(FK_MX4_THREADS);
+  const dim3 grid(tile_groups(a->rows, a->k)), block(FK_MX4_THREADS);
   const hipStream_t s = stream_of(ctx, stream);
   of_type(a->x_type, [&](auto t) {
     hipLaunchKernelGGL((op_mx4_quantize<decltype(t)::value>), grid, block, 0, s, *a);
@@ -208,7 +208,7 @@ extern "C" int fk_mx4_quantize(fk_ctx *ctx, const fk_mx4_quantize_args *a, fk_st
 
 extern "C" int fk_mx4_dequantize(fk_ctx *ctx, const fk_mx4_dequantize_args *a, fk_stream *stream) {
   if (int st = admit(ctx, "fk_mx4_dequantize", a)) return st;
-  const dim3 grid(pair_groups(a->rows, a->k)), block(FK_MX4_THREADS);
+  const dim3 grid(tile_groups(a->rows, a->k)), block(FK_MX4_THREADS);
   const hipStream_t s = stream_of(ctx, stream);
   of_type(a->y_type, [&](auto t) {
     hipLaunchKernelGGL((op_mx4_dequantize<decltype(t)::value>), grid, block, 0, s, *a);

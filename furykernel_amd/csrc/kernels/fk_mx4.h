@@ -2,8 +2,8 @@
 // fkrocm_mx4.h has the format and the order they are held in).
 //
 // Both are one pass, so the wide side's stream bounds them.  A wavefront
-// takes 16 rows by 256 elements (two tiles): a lane 8 consecutive elements of
-// a row at a time, 16 lanes a row's 128, so loads are whole lines of 4 rows;
+// takes a tile, 16 rows by 128 elements: a lane 8 consecutive elements of a row
+// at a time, 16 lanes a row's 128, so loads are whole lines of 4 rows;
 // the four lanes of a block share its maximum by quad permutes, and a lane's
 // codes are one word, 64 bytes together in the tile's order.  The conversions
 // are the hardware's scaled ones (v_cvt_scalef32_pk_fp4_f32 and back).
@@ -86,133 +86,124 @@ __device__ __forceinline__ void mx4_store8(uint64_t row, uint64_t i, const float
   }
 }
 
-// The wavefront's two tiles: its row tile, pair of tiles, and where a lane's
-// 8 elements of turn i of tile t lie.
+// The wavefront's tile: its row tile and place along k (the second of the last
+// pair may lie past k), and where a lane's 8 elements of turn i lie.
 struct Mx4Place {
-  uint32_t tile, pair, piece, sub;
+  uint32_t tile, step, piece, sub;
   bool there;
 };
 __device__ __forceinline__ Mx4Place mx4_place(uint32_t rows, uint32_t k) {
   Mx4Place p;
-  const uint32_t pairs = mx4_pairs(k);
+  const uint32_t steps = 2 * mx4_pairs(k);
   const uint64_t w = (uint64_t)blockIdx.x * (FK_MX4_THREADS / FK_WAVE) + threadIdx.x / FK_WAVE;
-  p.there = w < (uint64_t)mx4_row_tiles(rows) * pairs;
-  p.tile = __builtin_amdgcn_readfirstlane((uint32_t)(w / pairs));
-  p.pair = __builtin_amdgcn_readfirstlane((uint32_t)(w % pairs));
+  p.there = w < (uint64_t)mx4_row_tiles(rows) * steps;
+  p.tile = __builtin_amdgcn_readfirstlane((uint32_t)w / steps);
+  p.step = __builtin_amdgcn_readfirstlane((uint32_t)w % steps);
   p.piece = threadIdx.x % 16;
   p.sub = threadIdx.x % FK_WAVE / 16;
   return p;
 }
-// The byte of a lane's word of codes, and of its block's pair of scales.
-__device__ __forceinline__ uint64_t mx4_code_at(const Mx4Place &p, uint32_t k, uint32_t t, uint32_t i) {
-  return ((uint64_t)p.tile * mx4_pairs(k) + p.pair) * 2048 + t * 1024 + (p.piece / 4 * 16 + 4 * i + p.sub) * 16 +
+// The byte of a lane's word of codes, and of its block's scale.
+__device__ __forceinline__ uint64_t mx4_code_at(const Mx4Place &p, uint32_t k, uint32_t i) {
+  return ((uint64_t)p.tile * 2 * mx4_pairs(k) + p.step) * 1024 + (p.piece / 4 * 16 + 4 * i + p.sub) * 16 +
          p.piece % 4 * 4;
 }
 __device__ __forceinline__ uint64_t mx4_scale_at(const Mx4Place &p, uint32_t k, uint32_t i) {
-  return ((uint64_t)p.tile * mx4_pairs(k) + p.pair) * 128 + (p.piece / 4 * 16 + 4 * i + p.sub) * 2;
+  return ((uint64_t)p.tile * mx4_pairs(k) + p.step / 2) * 128 + (p.piece / 4 * 16 + 4 * i + p.sub) * 2 + p.step % 2;
 }
 
 template <int T>
 __device__ __forceinline__ void mx4_quantize(const fk_mx4_quantize_args &a) {
   const Mx4Place p = mx4_place(a.rows, a.k);
   if (!p.there) return;
-  float x[2][4][8];
-#pragma unroll
-  for (uint32_t t = 0; t < 2; t++)
-#pragma unroll
-    for (uint32_t i = 0; i < 4; i++) {
-      const uint32_t row = 16 * p.tile + 4 * i + p.sub, col = p.pair * 256 + t * 128 + p.piece * 8;
-      const uint64_t at = a.x + (uint64_t)row * a.x_stride * mx4_bytes_of(T);
-#pragma unroll
-      for (int j = 0; j < 8; j++) x[t][i][j] = 0.0f;
-      if (row < a.rows && col + 8 <= a.k) {
-        mx4_load8<T>(at, col, x[t][i]);
-      } else if (row < a.rows && col < a.k) {
-#pragma unroll
-        for (uint32_t j = 0; j < 7; j++)
-          if (col + j < a.k) x[t][i][j] = mx4_load<T>(at, col + j);
-      }
-    }
+  const uint32_t col = p.step * 128 + p.piece * 8;
+  float x[4][8];
 #pragma unroll
   for (uint32_t i = 0; i < 4; i++) {
-    uint32_t scales = 0;
+    const uint32_t row = 16 * p.tile + 4 * i + p.sub;
+    const uint64_t at = a.x + (uint64_t)row * a.x_stride * mx4_bytes_of(T);
 #pragma unroll
-    for (uint32_t t = 0; t < 2; t++) {
-      // the largest magnitude as its bits (NaN above infinity above the rest)
-      uint32_t big = 0;
+    for (int j = 0; j < 8; j++) x[i][j] = 0.0f;
+    if (row < a.rows && col + 8 <= a.k) {
+      mx4_load8<T>(at, col, x[i]);
+    } else if (row < a.rows && col < a.k) {
 #pragma unroll
-      for (int j = 0; j < 8; j++) big = max(big, __float_as_uint(x[t][i][j]) & 0x7FFFFFFFu);
-      big = max(big, (uint32_t)dpp_i<0xB1>((int)big));
-      big = max(big, (uint32_t)dpp_i<0x4E>((int)big));
-      const uint32_t e = big >> 23;
-      const uint32_t b = big == 0 ? 127u : (e == 255 ? 255u : (e > 2 ? e - 2 : 0u));
-      // small scales with the elements at 2^64 times themselves: the
-      // conversion takes a normal scale
-      const bool low = b < 64;
-      const float up = low ? 18446744073709551616.0f : 1.0f;
-      const float scale = __uint_as_float((low ? b + 64 : b) << 23);
-      uint32_t code = 0;
-#define FK_MX4_CODE(J) \
-  code = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(code, x[t][i][2 * J] * up, x[t][i][2 * J + 1] * up, scale, J)
-      FK_MX4_CODE(0);
-      FK_MX4_CODE(1);
-      FK_MX4_CODE(2);
-      FK_MX4_CODE(3);
-#undef FK_MX4_CODE
-      *global_at<uint32_t>(a.codes + mx4_code_at(p, a.k, t, i)) = b == 255 ? 0u : code;
-      scales |= b << (8 * t);
+      for (uint32_t j = 0; j < 7; j++)
+        if (col + j < a.k) x[i][j] = mx4_load<T>(at, col + j);
     }
-    if (p.piece % 4 == 0) *global_at<uint16_t>(a.scales + mx4_scale_at(p, a.k, i)) = (uint16_t)scales;
+  }
+#pragma unroll
+  for (uint32_t i = 0; i < 4; i++) {
+    // the largest magnitude as its bits (NaN above infinity above the rest)
+    uint32_t big = 0;
+#pragma unroll
+    for (int j = 0; j < 8; j++) big = max(big, __float_as_uint(x[i][j]) & 0x7FFFFFFFu);
+    big = max(big, (uint32_t)dpp_i<0xB1>((int)big));
+    big = max(big, (uint32_t)dpp_i<0x4E>((int)big));
+    const uint32_t e = big >> 23;
+    const uint32_t b = big == 0 ? 127u : (e == 255 ? 255u : (e > 2 ? e - 2 : 0u));
+    // small scales with the elements at 2^64 times themselves: the conversion
+    // takes a normal scale
+    const bool low = b < 64;
+    const float up = low ? 18446744073709551616.0f : 1.0f;
+    const float scale = __uint_as_float((low ? b + 64 : b) << 23);
+    uint32_t code = 0;
+#define FK_MX4_CODE(J) \
+  code = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(code, x[i][2 * J] * up, x[i][2 * J + 1] * up, scale, J)
+    FK_MX4_CODE(0);
+    FK_MX4_CODE(1);
+    FK_MX4_CODE(2);
+    FK_MX4_CODE(3);
+#undef FK_MX4_CODE
+    *global_at<uint32_t>(a.codes + mx4_code_at(p, a.k, i)) = b == 255 ? 0u : code;
+    if (p.piece % 4 == 0) *global_at<uint8_t>(a.scales + mx4_scale_at(p, a.k, i)) = (uint8_t)b;
   }
 }
 
 template <int T>
 __device__ __forceinline__ void mx4_dequantize(const fk_mx4_dequantize_args &a) {
   const Mx4Place p = mx4_place(a.rows, a.k);
-  if (!p.there) return;
-  uint32_t code[2][4], scales[4];
+  const uint32_t col = p.step * 128 + p.piece * 8;
+  if (!p.there || col >= a.k) return;
+  uint32_t code[4], scales[4];
 #pragma unroll
   for (uint32_t i = 0; i < 4; i++) {
-    scales[i] = *global_at<const uint16_t>(a.scales + mx4_scale_at(p, a.k, i));
-#pragma unroll
-    for (uint32_t t = 0; t < 2; t++) code[t][i] = *global_at<const uint32_t>(a.codes + mx4_code_at(p, a.k, t, i));
+    scales[i] = *global_at<const uint8_t>(a.scales + mx4_scale_at(p, a.k, i));
+    code[i] = *global_at<const uint32_t>(a.codes + mx4_code_at(p, a.k, i));
   }
 #pragma unroll
-  for (uint32_t i = 0; i < 4; i++)
-#pragma unroll
-    for (uint32_t t = 0; t < 2; t++) {
-      const uint32_t row = 16 * p.tile + 4 * i + p.sub, col = p.pair * 256 + t * 128 + p.piece * 8;
-      if (row >= a.rows || col >= a.k) continue;
-      const uint32_t b = scales[i] >> (8 * t) & 255u;
-      // 2^(b - 127), of which b = 0 is no normal number
-      const float scale = b == 255 ? __builtin_nanf("") : __uint_as_float(b ? b << 23 : 0x00400000u);
-      float y[8];
-#define FK_MX4_VALUE(J)                                                                        \
-  {                                                                                            \
-    const mx4_float2 v = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(code[t][i], 1.0f, J);        \
-    y[2 * J] = v[0] * scale;                                                                   \
-    y[2 * J + 1] = v[1] * scale;                                                               \
+  for (uint32_t i = 0; i < 4; i++) {
+    const uint32_t row = 16 * p.tile + 4 * i + p.sub, b = scales[i];
+    if (row >= a.rows) continue;
+    // 2^(b - 127), of which b = 0 is no normal number
+    const float scale = b == 255 ? __builtin_nanf("") : __uint_as_float(b ? b << 23 : 0x00400000u);
+    float y[8];
+#define FK_MX4_VALUE(J)                                                                     \
+  {                                                                                         \
+    const mx4_float2 v = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(code[i], 1.0f, J);        \
+    y[2 * J] = v[0] * scale;                                                                \
+    y[2 * J + 1] = v[1] * scale;                                                            \
   }
-      FK_MX4_VALUE(0);
-      FK_MX4_VALUE(1);
-      FK_MX4_VALUE(2);
-      FK_MX4_VALUE(3);
+    FK_MX4_VALUE(0);
+    FK_MX4_VALUE(1);
+    FK_MX4_VALUE(2);
+    FK_MX4_VALUE(3);
 #undef FK_MX4_VALUE
-      // (the product is made before it is rounded: fused with the rounding to
-      // f16 it adds a zero, and a code of -0 comes out as +0)
+    // (the product is made before it is rounded: fused with the rounding to
+    // f16 it adds a zero, and a code of -0 comes out as +0)
 #pragma unroll
-      for (int j = 0; j < 8; j++) asm volatile("" : "+v"(y[j]));
-      const uint64_t at = a.y + (uint64_t)row * a.y_stride * mx4_bytes_of(T);
-      if (col + 8 <= a.k) {
-        mx4_store8<T>(at, col, y);
-      } else {
+    for (int j = 0; j < 8; j++) asm volatile("" : "+v"(y[j]));
+    const uint64_t at = a.y + (uint64_t)row * a.y_stride * mx4_bytes_of(T);
+    if (col + 8 <= a.k) {
+      mx4_store8<T>(at, col, y);
+    } else {
 #pragma unroll
-        for (uint32_t j = 0; j < 7; j++)
-          if (col + j < a.k) mx4_store<T>(at, col + j, y[j]);
-      }
-      if (a.scales_out && p.piece % 4 == 0)
-        global_at<float>(a.scales_out)[(uint64_t)row * ((a.k >> 5) + ((a.k & 31u) != 0)) + col / 32] = scale;
+      for (uint32_t j = 0; j < 7; j++)
+        if (col + j < a.k) mx4_store<T>(at, col + j, y[j]);
     }
+    if (a.scales_out && p.piece % 4 == 0)
+      global_at<float>(a.scales_out)[(uint64_t)row * ((a.k >> 5) + ((a.k & 31u) != 0)) + col / 32] = scale;
+  }
 }
 
 }  // namespace fk
