@@ -56,18 +56,16 @@ bool matrix(uint32_t rows, uint32_t k) {
          (uint64_t)fk::mx4_row_tiles(rows) * fk::mx4_pairs(k) < 1ull << 25;
 }
 
-// Rows of `type` from `addr` on, `stride` elements apart, aligned to their
-// elements.
-int check_rows(Refusal &no, const char *name, uint64_t addr, uint64_t stride, uint64_t width, uint32_t type) {
+// Rows of `type`, `stride` elements apart, aligned to their elements.
+int check_rows(Refusal &no, const char *name, uint64_t stride, uint64_t width, uint32_t type) {
   if (type > FK_T_BF16) return no(FK_ERR_ARG, "%s of type %u", name, type);
   if (stride < width || stride >= 1ull << 40)
     return no(FK_ERR_ARG, "%s's rows of %llu, %llu apart", name, (unsigned long long)width, (unsigned long long)stride);
-  if (addr == 0 || addr % fk::mx4_bytes_of((int)type))
-    return no(FK_ERR_ARG, "%s is null or not aligned to its elements", name);
   return FK_OK;
 }
-uint64_t rows_bytes(uint64_t rows, uint64_t stride, uint64_t width, uint32_t type) {
-  return ((rows - 1) * stride + width) * fk::mx4_bytes_of((int)type);
+Span rows_of(const char *name, uint64_t addr, uint64_t rows, uint64_t stride, uint64_t width, uint32_t type) {
+  const uint32_t bytes = fk::mx4_bytes_of((int)type);
+  return {name, addr, fk::rows_span(rows, stride, width, bytes), bytes};
 }
 
 // Threadgroups of a wavefront a tile.
@@ -103,9 +101,11 @@ struct Form {
 // The form of the least cost takes 1.02 times the fastest one's time on
 // average over them, at most 1.26 (32 rows by 8192, k 2048: 5.4 µs, 64 x 16
 // blocks 4.3).
-constexpr Form forms[] = {{"few 1x1", FEW, 1, 1, 8, 2.54, 0.25, 0.169}, {"few 4x1", FEW, 4, 1, 8, 2.71, 0.34, 0.127},
-                          {"few 4x2", FEW, 4, 2, 8, 3.34, 0.43, 0.153}, {"few 8x2", FEW, 8, 2, 4, 3.73, 0.65, 0.120},
-                          {"mid 8x8", MID, 8, 8, 768, 3.86, 0.57, 3.10}, {"many 16x16", MANY, 16, 16, 256, 10.3, 0.83, 1.61}};
+constexpr Form forms[] = {
+    {"few 1x1", FEW, 1, 1, 8, 2.54, 0.25, 0.169},  {"few 4x1", FEW, 4, 1, 8, 2.71, 0.34, 0.127},
+    {"few 4x2", FEW, 4, 2, 8, 3.34, 0.43, 0.153},  {"few 8x2", FEW, 8, 2, 4, 3.73, 0.65, 0.120},
+    {"mid 8x8", MID, 8, 8, 768, 3.86, 0.57, 3.10}, {"many 16x16", MANY, 16, 16, 256, 10.3, 0.83, 1.61},
+};
 
 uint64_t tiles_of(const Form &f, uint32_t m, uint32_t n) {
   return (uint64_t)((fk::mx4_row_tiles(m) + f.mb - 1) / f.mb) * ((fk::mx4_row_tiles(n) + f.nb - 1) / f.nb);
@@ -151,44 +151,37 @@ namespace fk {
 
 int check(const fk_mx4_quantize_args &a, Refusal &no) {
   if (!matrix(a.rows, a.k)) return no(FK_ERR_RANGE, "no matrix of %u rows of %u", a.rows, a.k);
-  if (int st = check_rows(no, "x", a.x, a.x_stride, a.k, a.x_type)) return st;
-  const Span x = {"x", a.x, rows_bytes(a.rows, a.x_stride, a.k, a.x_type)};
+  if (int st = check_rows(no, "x", a.x_stride, a.k, a.x_type)) return st;
+  const Span reads[] = {rows_of("x", a.x, a.rows, a.x_stride, a.k, a.x_type)};
   const Span writes[] = {{"codes", a.codes, codes_bytes(a.rows, a.k)}, {"scales", a.scales, scales_bytes(a.rows, a.k)}};
-  for (const Span &w : writes)
-    if (meets(w, x)) return no(FK_ERR_ARG, "%s overlaps x", w.name);
-  return check_spans(no, nullptr, 0, writes, 2, 16);
+  return check_spans(no, reads, 1, writes, 2);
 }
 
 int check(const fk_mx4_dequantize_args &a, Refusal &no) {
   if (!matrix(a.rows, a.k)) return no(FK_ERR_RANGE, "no matrix of %u rows of %u", a.rows, a.k);
-  if (int st = check_rows(no, "y", a.y, a.y_stride, a.k, a.y_type)) return st;
+  if (int st = check_rows(no, "y", a.y_stride, a.k, a.y_type)) return st;
   const Span reads[] = {{"codes", a.codes, codes_bytes(a.rows, a.k)}, {"scales", a.scales, scales_bytes(a.rows, a.k)}};
-  const Span y = {"y", a.y, rows_bytes(a.rows, a.y_stride, a.k, a.y_type)};
-  const Span out = {"scales_out", a.scales_out, a.scales_out ? 4ull * a.rows * ((a.k >> 5) + ((a.k & 31u) != 0)) : 0};
-  if (a.scales_out % 4) return no(FK_ERR_ARG, "scales_out is not 4-byte aligned");
-  for (const Span &w : {y, out})
-    for (const Span &r : reads)
-      if (meets(w, r)) return no(FK_ERR_ARG, "%s overlaps %s", w.name, r.name);
-  if (meets(y, out)) return no(FK_ERR_ARG, "scales_out overlaps y");
-  return check_spans(no, reads, 2, nullptr, 0, 16);
+  const uint64_t blocks = (a.k >> 5) + ((a.k & 31u) != 0);
+  const Span writes[] = {rows_of("y", a.y, a.rows, a.y_stride, a.k, a.y_type),
+                         {"scales_out", a.scales_out, a.scales_out ? 4ull * a.rows * blocks : 0, 4}};
+  return check_spans(no, reads, 2, writes, 2);
 }
 
 int check(const fk_mx4_gemm_args &a, Refusal &no) {
-  if (!matrix(a.m, a.k) || !matrix(a.n, a.k)) return no(FK_ERR_RANGE, "no product of %u and %u rows of %u", a.m, a.n, a.k);
+  if (!matrix(a.m, a.k) || !matrix(a.n, a.k))
+    return no(FK_ERR_RANGE, "no product of %u and %u rows of %u", a.m, a.n, a.k);
   if ((uint64_t)mx4_row_tiles(a.m) * mx4_row_tiles(a.n) >= 1ull << 31)
     return no(FK_ERR_RANGE, "a product of %u by %u: 2^31 tiles and more", a.m, a.n);
   const Form &f = forms[pick(a.m, a.n, a.k)];
   if (f.kind != MANY && tiles_of(f, a.m, a.n) >= 1ull << 23)  // a launch of 2^32 threads
     return no(FK_ERR_RANGE, "a product of %u by %u, k %u: 2^23 threadgroups and more", a.m, a.n, a.k);
-  if (int st = check_rows(no, "c", a.c, a.c_stride, a.n, a.c_type)) return st;
+  if (int st = check_rows(no, "c", a.c_stride, a.n, a.c_type)) return st;
   const Span reads[] = {{"a_codes", a.a_codes, codes_bytes(a.m, a.k)},
                         {"a_scales", a.a_scales, scales_bytes(a.m, a.k)},
                         {"b_codes", a.b_codes, codes_bytes(a.n, a.k)},
                         {"b_scales", a.b_scales, scales_bytes(a.n, a.k)}};
-  const Span c = {"c", a.c, rows_bytes(a.m, a.c_stride, a.n, a.c_type)};
-  for (const Span &r : reads)
-    if (meets(c, r)) return no(FK_ERR_ARG, "c overlaps %s", r.name);
-  return check_spans(no, reads, 4, nullptr, 0, 16);
+  const Span writes[] = {rows_of("c", a.c, a.m, a.c_stride, a.n, a.c_type)};
+  return check_spans(no, reads, 4, writes, 1);
 }
 
 }  // namespace fk
@@ -197,7 +190,7 @@ extern "C" size_t fk_mx4_codes_bytes(uint32_t rows, uint32_t k) { return matrix(
 extern "C" size_t fk_mx4_scales_bytes(uint32_t rows, uint32_t k) { return matrix(rows, k) ? scales_bytes(rows, k) : 0; }
 
 extern "C" int fk_mx4_quantize(fk_ctx *ctx, const fk_mx4_quantize_args *a, fk_stream *stream) {
-  if (int st = admit(ctx, "fk_mx4_quantize", a)) return st;
+  if (int st = admit(ctx, "fk_mx4_quantize", a, stream)) return st;
   const dim3 grid(tile_groups(a->rows, a->k)), block(FK_MX4_THREADS);
   const hipStream_t s = stream_of(ctx, stream);
   of_type(a->x_type, [&](auto t) {
@@ -207,7 +200,7 @@ extern "C" int fk_mx4_quantize(fk_ctx *ctx, const fk_mx4_quantize_args *a, fk_st
 }
 
 extern "C" int fk_mx4_dequantize(fk_ctx *ctx, const fk_mx4_dequantize_args *a, fk_stream *stream) {
-  if (int st = admit(ctx, "fk_mx4_dequantize", a)) return st;
+  if (int st = admit(ctx, "fk_mx4_dequantize", a, stream)) return st;
   const dim3 grid(tile_groups(a->rows, a->k)), block(FK_MX4_THREADS);
   const hipStream_t s = stream_of(ctx, stream);
   of_type(a->y_type, [&](auto t) {
@@ -221,7 +214,7 @@ extern "C" const char *fk_mx4_gemm_form(uint32_t m, uint32_t n, uint32_t k) {
 }
 
 extern "C" int fk_mx4_gemm(fk_ctx *ctx, const fk_mx4_gemm_args *a, fk_stream *stream) {
-  if (int st = admit(ctx, "fk_mx4_gemm", a)) return st;
+  if (int st = admit(ctx, "fk_mx4_gemm", a, stream)) return st;
   const hipStream_t s = stream_of(ctx, stream);
   of_type(a->c_type, [&](auto t) {
     queue_picked<decltype(t)::value>(pick(a->m, a->n, a->k), *a, s, std::make_index_sequence<std::size(forms)>{});

@@ -46,9 +46,9 @@ __global__ void __launch_bounds__(64 * W)
   fk::paged_attend_join<W, BF16>(a, pl, groups);
 }
 
-// The attention's launch for these sizes: head_dim's tile width, its
-// threadgroups, the joins' entries and what the kernels take; 0 threadgroups and the reason if
-// the kernels do not take them.
+// The attention's launch for these sizes: head_dim's tile width, its wavefronts
+// and threadgroups, the joins' entries and what the kernels take; 0
+// threadgroups and the reason if the kernels do not take them.
 struct AttendLaunch {
   uint32_t width = 0, waves = 4, groups = 0, joins = 0;
   fk::PagedPlan plan{};
@@ -148,15 +148,15 @@ static int check(const fk_page_plan_args &a, Refusal &no) {
   if ((uint64_t)a.table_len * a.block_size >= 1ull << 32 || a.tokens == 0xFFFFFFFFu)
     return no(FK_ERR_RANGE, "tables of %u blocks of %u, %u tokens: past 32 bits", a.table_len, a.block_size, a.tokens);
   const uint64_t n = a.requests, t = a.tokens;
-  const Span reads[] = {{"cached", a.cached, 4 * n},
-                        {"fresh", a.fresh, 4 * n},
-                        {"free_blocks", a.free_blocks, 4ull * a.free_len},
-                        {"head", a.head, 4}};
-  const Span writes[] = {{"table", a.table, 4 * n * a.table_len}, {"lengths", a.lengths, 4 * n},
-                         {"starts", a.starts, 4 * (n + 1)},       {"slots", a.slots, 4 * t},
-                         {"positions", a.positions, 4 * t},       {"owner", a.owner, 4 * t},
-                         {"counts", a.counts, 16}};
-  return check_spans(no, reads, 4, writes, 7, 4);
+  const Span reads[] = {{"cached", a.cached, 4 * n, 4},
+                        {"fresh", a.fresh, 4 * n, 4},
+                        {"free_blocks", a.free_blocks, 4ull * a.free_len, 4},
+                        {"head", a.head, 4, 4}};
+  const Span writes[] = {{"table", a.table, 4 * n * a.table_len, 4}, {"lengths", a.lengths, 4 * n, 4},
+                         {"starts", a.starts, 4 * (n + 1), 4},       {"slots", a.slots, 4 * t, 4},
+                         {"positions", a.positions, 4 * t, 4},       {"owner", a.owner, 4 * t, 4},
+                         {"counts", a.counts, 16, 4}};
+  return check_spans(no, reads, 4, writes, 7);
 }
 
 // Units of 16 elements that a token's rows have: one thread's work.
@@ -184,17 +184,23 @@ static int check(const fk_paged_store_args &a, Refusal &no) {
   if ((__uint128_t)store_units(a) * T >= (1ull << 32) - FK_STORE_THREADS)
     return no(FK_ERR_RANGE, "%u tokens of %llu units of 16 elements: past 32 bits", a.tokens,
               (unsigned long long)store_units(a));
-  auto rows = [&](uint64_t stride, uint64_t width) { return T ? ((T - 1) * stride + width) * wide : 0; };
+  // (the kernel counts a row's elements in 32 bits)
+  if (qw >= 1ull << 31 || kw >= 1ull << 31)
+    return no(FK_ERR_RANGE, "%u heads over %u of width %u: rows of 2^31 elements and more", a.heads, a.kv_heads,
+              a.head_dim);
+  auto rows = [&](uint64_t stride, uint64_t width) { return fk::rows_span(T, stride, width, wide); };
   const __uint128_t pool = (__uint128_t)a.blocks * a.block_size * kw * 2;
   if (pool >= 1ull << 48) return no(FK_ERR_RANGE, "a pool of 2^48 bytes and more");
   const Span reads[] = {{"q", a.q, a.q ? rows(a.q_stride, qw) : 0},
                         {"k", a.k, rows(a.k_stride, kw)},
                         {"v", a.v, rows(a.v_stride, kw)},
-                        {"slots", a.slots, 4 * T},
-                        {"positions", a.positions, a.rotated ? 4 * T : 0},
+                        {"slots", a.slots, 4 * T, 4},
+                        {"positions", a.positions, a.rotated ? 4 * T : 0, 4},
                         {"rope", a.rope, a.rotated ? 8ull * a.rope_rows * a.rotated : 0}};
-  const Span writes[] = {{"qr", a.qr, T * qw * 2}, {"kpool", a.kpool, (uint64_t)pool}, {"vpool", a.vpool, (uint64_t)pool}};
-  return check_spans(no, reads, 6, writes, 3, 16);
+  const Span writes[] = {{"qr", a.qr, T * qw * 2},
+                         {"kpool", a.kpool, (uint64_t)pool},
+                         {"vpool", a.vpool, (uint64_t)pool}};
+  return check_spans(no, reads, 6, writes, 3);
 }
 
 static int check(const fk_paged_attend_args &a, const AttendLaunch &l, Refusal &no) {
@@ -212,15 +218,15 @@ static int check(const fk_paged_attend_args &a, const AttendLaunch &l, Refusal &
   if (pool >= 1ull << 48) return no(FK_ERR_RANGE, "a pool of 2^48 bytes and more");
   if (a.starts && a.q_rows == 0) return no(FK_ERR_ARG, "starts of no rows of q");
   const uint64_t q_rows = a.starts ? a.q_rows : n;
-  const Span reads[] = {{"q", a.q, ((q_rows - 1) * a.q_stride + w) * 2},
+  const Span reads[] = {{"q", a.q, fk::rows_span(q_rows, a.q_stride, w, 2)},
                         {"kpool", a.kpool, (uint64_t)pool},
                         {"vpool", a.vpool, (uint64_t)pool},
-                        {"table", a.table, 4 * n * a.table_len},
-                        {"lengths", a.lengths, 4 * n},
-                        {"starts", a.starts, a.starts ? 4 * (n + 1) : 0}};
-  const Span writes[] = {{"out", a.out, ((n - 1) * a.out_stride + w) * (a.out_f32 ? 4 : 2)},
+                        {"table", a.table, 4 * n * a.table_len, 4},
+                        {"lengths", a.lengths, 4 * n, 4},
+                        {"starts", a.starts, a.starts ? 4 * (n + 1) : 0, 4}};
+  const Span writes[] = {{"out", a.out, fk::rows_span(n, a.out_stride, w, a.out_f32 ? 4 : 2)},
                          {"workspace", a.workspace, bytes}};
-  return check_spans(no, reads, 6, writes, 2, 16);
+  return check_spans(no, reads, 6, writes, 2);
 }
 
 }  // namespace fk
@@ -260,7 +266,7 @@ extern "C" int fk_serve_check(const char *entry, const void *args, size_t args_b
 }
 
 extern "C" int fk_page_plan(fk_ctx *ctx, const fk_page_plan_args *a, fk_stream *stream) {
-  if (int st = admit(ctx, "fk_page_plan", a)) return st;
+  if (int st = admit(ctx, "fk_page_plan", a, stream)) return st;
   const uint64_t groups = ((uint64_t)a->tokens + FK_PLAN_THREADS - 1) / FK_PLAN_THREADS;
   const uint32_t g = (uint32_t)(groups < 1 ? 1 : (groups > 256 ? 256 : groups));
   hipLaunchKernelGGL(a->requests <= FK_PLAN_HELD ? op_page_plan_held : op_page_plan, dim3(g), dim3(FK_PLAN_THREADS), 0,
@@ -269,7 +275,7 @@ extern "C" int fk_page_plan(fk_ctx *ctx, const fk_page_plan_args *a, fk_stream *
 }
 
 extern "C" int fk_paged_store(fk_ctx *ctx, const fk_paged_store_args *a, fk_stream *stream) {
-  if (int st = admit(ctx, "fk_paged_store", a)) return st;
+  if (int st = admit(ctx, "fk_paged_store", a, stream)) return st;
   if (a->tokens == 0) return FK_OK;
   const uint64_t units = store_units(*a) * a->tokens;
   const dim3 grid((uint32_t)((units + FK_STORE_THREADS - 1) / FK_STORE_THREADS)), block(FK_STORE_THREADS);
@@ -294,7 +300,7 @@ extern "C" size_t fk_paged_attend_workspace(const fk_paged_attend_args *a) {
 
 extern "C" int fk_paged_attend(fk_ctx *ctx, const fk_paged_attend_args *a, fk_stream *stream) {
   const AttendLaunch l = a ? attend_launch(*a) : AttendLaunch{};
-  if (int st = admit(ctx, "fk_paged_attend", a, l)) return st;
+  if (int st = admit(ctx, "fk_paged_attend", a, stream, l)) return st;
   const hipStream_t s = stream_of(ctx, stream);
   if (a->cache_bf16) queue_attend<true>(*a, l, s);
   else queue_attend<false>(*a, l, s);

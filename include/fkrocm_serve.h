@@ -48,7 +48,8 @@ enum { FK_T_F32 = 0, FK_T_F16 = 1, FK_T_BF16 = 2 };
  * A request does not fit if cached + fresh passes table_len * block_size, if
  * its tokens (or those of one before it) end past `tokens`, or if the blocks
  * that the requests up to it need pass the free list; it takes no block, its
- * length stays cached, its tokens' slots are FK_NO_SLOT. */
+ * length stays cached, its tokens' slots are FK_NO_SLOT (so what a step makes
+ * of them means nothing: it goes into a later step). */
 typedef struct fk_page_plan_args {
   uint64_t cached;      /* u32 [requests] */
   uint64_t fresh;       /* u32 [requests] */
@@ -98,7 +99,7 @@ typedef struct fk_paged_store_args {
   uint32_t cache_bf16; /* the pools and qr hold bf16 (else f16) */
 } fk_paged_store_args;
 
-/* Addresses are 16-byte aligned, rows too (strides). */
+/* Addresses are 16-byte aligned, rows too (strides); slots and positions 4-byte. */
 int fk_paged_store(fk_ctx *ctx, const fk_paged_store_args *args, fk_stream *stream);
 
 /* Attention of one new token a request: out[r] = softmax(scale q[r] Kᵀ) V
@@ -142,7 +143,8 @@ typedef struct fk_paged_attend_args {
 /* The workspace's bytes for these sizes (addresses, scale and strides are not
  * looked at); 0 if the sizes are refused. */
 size_t fk_paged_attend_workspace(const fk_paged_attend_args *args);
-/* Addresses are 16-byte aligned; q_stride a multiple of 8. */
+/* Addresses are 16-byte aligned (table, lengths and starts 4-byte); q_stride a
+ * multiple of 8. */
 int fk_paged_attend(fk_ctx *ctx, const fk_paged_attend_args *args, fk_stream *stream);
 
 /* The checks that an entry makes of its arguments before it queues anything,

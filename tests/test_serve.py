@@ -14,8 +14,8 @@ from furykernel_amd.kernels import LaunchError
 INCLUDE = Path(__file__).resolve().parents[1] / "include"
 HEADER = (INCLUDE / "fkrocm_serve.h").read_text() + (INCLUDE / "fkrocm_mx4.h").read_text()
 STRUCTS = {"fk_mx4_quantize_args": mx4.QuantizeArgs, "fk_mx4_dequantize_args": mx4.DequantizeArgs,
-           "fk_mx4_gemm_args": mx4.GemmArgs, "fk_page_plan_args": paged.PagePlanArgs, "fk_paged_store_args": paged.PagedStoreArgs,
-           "fk_paged_attend_args": paged.PagedAttendArgs}
+           "fk_mx4_gemm_args": mx4.GemmArgs, "fk_page_plan_args": paged.PagePlanArgs,
+           "fk_paged_store_args": paged.PagedStoreArgs, "fk_paged_attend_args": paged.PagedAttendArgs}
 
 
 class FakeDevice:
@@ -48,7 +48,7 @@ def test_the_structs_fields_are_the_headers(name):
 
 
 def attend_sizes(**over):
-    return {**dict(requests=3, heads=8, kv_heads=2, head_dim=64, block_size=16, blocks=20, table_len=5), **over}
+    return {**dict(requests=5, heads=8, kv_heads=2, head_dim=64, block_size=16, blocks=20, table_len=5), **over}
 
 
 def attend(over=(), sizes=(), **kw):
@@ -64,8 +64,8 @@ def attend(over=(), sizes=(), **kw):
 
 def test_attend_takes_what_it_says():
     attend()
-    attend(out_type="f32", over={"out": FakeBuffer(3 * 512 * 4)})
-    attend(q_stride=520, over={"q": FakeBuffer((2 * 520 + 512) * 2)})
+    attend(out_type="f32", over={"out": FakeBuffer(5 * 512 * 4)})
+    attend(q_stride=520, over={"q": FakeBuffer((4 * 520 + 512) * 2)})
     for d in (8, 72, 128, 200, 256):
         attend(sizes={"head_dim": d})
     attend(sizes={"heads": 34, "window": 7})
@@ -84,16 +84,17 @@ def test_attend_refuses_sizes(sizes):
 @pytest.mark.parametrize("name", ["q", "kpool", "vpool", "table", "lengths", "out", "workspace"])
 def test_attend_refuses_buffers(name):
     sizes = attend_sizes()
-    full = {"q": 3072, "kpool": 81920, "vpool": 81920, "table": 60, "lengths": 12, "out": 3072,
+    full = {"q": 5120, "kpool": 81920, "vpool": 81920, "table": 100, "lengths": 20, "out": 5120,
             "workspace": paged.attend_workspace(**sizes)}[name]
     attend({name: FakeBuffer(full)})
-    for bad in (FakeBuffer(full - 1), FakeBuffer(full, FakeDevice()), FakeBuffer(full, ptr=FakeBuffer.at + 8)):
+    off = 2 if name in ("table", "lengths") else 8
+    for bad in (FakeBuffer(full - 1), FakeBuffer(full, FakeDevice()), FakeBuffer(full, ptr=FakeBuffer.at + off)):
         with pytest.raises(LaunchError):
             attend({name: bad})
 
 
 def test_attend_refuses_overlaps_strides_and_types():
-    q = FakeBuffer(3 * 512 * 4)
+    q = FakeBuffer(5 * 512 * 4)
     for over, kw in (({"q": q, "out": q}, {}), ({"lengths": q, "workspace": q}, {}), ({}, {"q_stride": 504}),
                      ({"q": q}, {"q_stride": 516}), ({}, {"out_stride": 511}), ({}, {"cache": "f32"}),
                      ({}, {"cache": "bf16", "out_type": "f16"}), ({}, {"out_stride": 513})):
@@ -102,10 +103,10 @@ def test_attend_refuses_overlaps_strides_and_types():
 
 
 def test_attend_refuses_starts_without_rows():
-    starts, q = FakeBuffer(16), FakeBuffer(7 * 512 * 2)
+    starts, q = FakeBuffer(24), FakeBuffer(7 * 512 * 2)
     attend({"starts": starts, "q": q}, q_rows=7)
-    for over, rows in (({"starts": starts, "q": q}, 0), ({"starts": starts, "q": q}, 8), ({"starts": starts, "q": q}, -1),
-                       ({"starts": FakeBuffer(12), "q": q}, 7)):
+    for over, rows in (({"starts": starts, "q": q}, 0), ({"starts": starts, "q": q}, 8),
+                       ({"starts": starts, "q": q}, -1), ({"starts": FakeBuffer(20), "q": q}, 7)):
         with pytest.raises(LaunchError):
             attend(over, q_rows=rows)
 
@@ -177,7 +178,8 @@ def test_store_takes_what_it_says():
 
 @pytest.mark.parametrize("sizes", [
     {"kv_heads": 0}, {"head_dim": 8}, {"head_dim": 40}, {"head_dim": 272}, {"block_size": 0}, {"blocks": 0},
-    {"blocks": 1 << 31}, {"rotated": 33}, {"rope_rows": 0}, {"tokens": 1 << 28}, {"tokens": -3}])
+    {"blocks": 1 << 31}, {"rotated": 33}, {"rope_rows": 0}, {"tokens": 1 << 28}, {"tokens": -3},
+    {"tokens": 1, "heads": 1 << 25}, {"tokens": 1, "kv_heads": 1 << 25, "blocks": 1}])
 def test_store_refuses_sizes(sizes):
     with pytest.raises(LaunchError):
         store(sizes=sizes)
@@ -186,8 +188,9 @@ def test_store_refuses_sizes(sizes):
 def test_store_refuses_buffers_strides_and_types():
     for name in ("q", "k", "v", "slots", "positions", "rope", "qr", "kpool", "vpool"):
         good = store().held[("q", "k", "v", "slots", "positions", "rope", "qr", "kpool", "vpool").index(name)]
+        off = 2 if name in ("slots", "positions") else 4
         for bad in (FakeBuffer(good.size - 1), FakeBuffer(good.size, FakeDevice()),
-                    FakeBuffer(good.size, ptr=FakeBuffer.at + 4)):
+                    FakeBuffer(good.size, ptr=FakeBuffer.at + off)):
             with pytest.raises(LaunchError):
                 store({name: bad})
     big = FakeBuffer(1 << 20)
@@ -197,6 +200,22 @@ def test_store_refuses_buffers_strides_and_types():
                      ({"kpool": big, "vpool": big}, {}), ({"q": big, "kpool": big}, {}), ({"q": big}, {"q_offset": 1})):
         with pytest.raises(LaunchError):
             store(over, **kw)
+
+
+def test_the_arrays_of_a_step_may_lie_together():
+    # (a plan's outputs in one buffer, a word apart)
+    store({"slots": FakeBuffer(20, ptr=FakeBuffer.at + 4), "positions": FakeBuffer(20, ptr=FakeBuffer.at + 324)})
+    attend({"lengths": FakeBuffer(20, ptr=FakeBuffer.at + 4), "table": FakeBuffer(100, ptr=FakeBuffer.at + 324)})
+
+
+def test_the_checks_refuse_spans_past_any_memory():
+    huge = FakeBuffer(1 << 80)   # what a wrapped size would let through
+    with pytest.raises(LaunchError, match="spans 2"):
+        store({"k": huge}, sizes={"tokens": 1 << 24, "heads": 1, "head_dim": 16, "rotated": 8}, k_stride=1 << 39)
+    with pytest.raises(LaunchError, match="spans 2"):
+        attend({"q": huge, "starts": FakeBuffer(24)}, q_rows=1 << 31, q_stride=1 << 36)
+    with pytest.raises(LaunchError, match="spans 2"):
+        mx4.Quantize(DEVICE, huge, matrix(1 << 24, 32), x_stride=1 << 39)
 
 
 def test_the_check_refuses_unknown_entries_and_sizes_of_arguments():
