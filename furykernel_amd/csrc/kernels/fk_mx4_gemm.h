@@ -101,11 +101,13 @@ __device__ __forceinline__ void mx4_gemm_few(const fk_mx4_gemm_args &a) {
 #pragma unroll
       for (uint32_t i = 0; i < MB; i++)
 #pragma unroll
-        for (uint32_t j = 0; j < NB; j++) acc[i][j] = mx4_mfma<0>(now.b[j][0], now.bs[j], now.a[i][0], now.as[i], acc[i][j]);
+        for (uint32_t j = 0; j < NB; j++)
+          acc[i][j] = mx4_mfma<0>(now.b[j][0], now.bs[j], now.a[i][0], now.as[i], acc[i][j]);
 #pragma unroll
       for (uint32_t i = 0; i < MB; i++)
 #pragma unroll
-        for (uint32_t j = 0; j < NB; j++) acc[i][j] = mx4_mfma<1>(now.b[j][1], now.bs[j], now.a[i][1], now.as[i], acc[i][j]);
+        for (uint32_t j = 0; j < NB; j++)
+          acc[i][j] = mx4_mfma<1>(now.b[j][1], now.bs[j], now.a[i][1], now.as[i], acc[i][j]);
       now = next;
     }
   }
@@ -288,9 +290,11 @@ __device__ __forceinline__ void mx4_gemm_mid(const fk_mx4_gemm_args &a) {
 #pragma unroll
     for (uint32_t h = 0; h < 2; h++) {
 #pragma unroll
-      for (uint32_t i = 0; i < GM; i++) s[i][h] = __builtin_amdgcn_raw_buffer_load_b16(as_src, as_at[i] + 64 * h, pair * 128, 0);
+      for (uint32_t i = 0; i < GM; i++)
+        s[i][h] = __builtin_amdgcn_raw_buffer_load_b16(as_src, as_at[i] + 64 * h, pair * 128, 0);
 #pragma unroll
-      for (uint32_t i = 0; i < GN; i++) t[i][h] = __builtin_amdgcn_raw_buffer_load_b16(bs_src, bs_at[i] + 64 * h, pair * 128, 0);
+      for (uint32_t i = 0; i < GN; i++)
+        t[i][h] = __builtin_amdgcn_raw_buffer_load_b16(bs_src, bs_at[i] + 64 * h, pair * 128, 0);
     }
   };
   scales(sa[0], sb[0], 0);
@@ -334,7 +338,6 @@ __device__ __forceinline__ void mx4_gemm_mid(const fk_mx4_gemm_args &a) {
   mx4_store_many<GM, GN, false, T>(a, 16 * tm + 32 * wm * GM, 16 * tn + 32 * wn * GN, acc,
                                    reinterpret_cast<char *>(mx4_lds) + wave * GN * 2048);
 }
-
 
 template <int T>
 __device__ __forceinline__ void mx4_gemm_many(const fk_mx4_gemm_args &a) {

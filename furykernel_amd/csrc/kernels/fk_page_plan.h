@@ -14,6 +14,7 @@
 // the free list's next, so its number follows from the sums alone: no token
 // waits for a table entry that this launch writes.  A request's new page is
 // written by the token that opens it.
+// 8 requests take 3.7 µs, 1500 with 59 thousand tokens 6.0.
 #pragma once
 
 #include <hip/hip_runtime.h>

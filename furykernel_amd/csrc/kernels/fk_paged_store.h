@@ -5,6 +5,8 @@
 // Elementwise, so the rows' read and the caches' write bound it.  A thread
 // takes 8 elements of a head's first half and the 8 they are paired with:
 // 16-byte loads and stores, and each pair's cosine and sine once for both.
+// 8191 tokens of 32 and 8 heads of 128 in bf16 take 32.5 µs (203 MB, 6.2 TB/s),
+// 8 tokens 2.8: the launch and three loads, one behind another.
 #pragma once
 
 #include "fk_address.h"
