@@ -249,3 +249,35 @@ def test_a_linear_captured_with_its_quantisation(device, mem):
         device.sync()
         assert np.array_equal(y.read(np.uint32), got.view(np.uint32).ravel())
     captured[0].destroy()
+
+
+def test_products_on_two_streams_at_once(device, mem):
+    """Products of one weight by two streams, of different forms: each one's
+    bits those it has alone."""
+    rng = np.random.default_rng(17)
+    n, k = 2050, 1900
+    weights = matrix(device, mem, n, k)
+    mx4.Quantize(device, mem.put(rng.standard_normal((n, k)).astype(np.float32)), weights).enqueue()
+    ops, outs = [], []
+    for m in (8, 1000):
+        rows, y = matrix(device, mem, m, k), mem.empty(4 * m * n)
+        ops.append([mx4.Quantize(device, mem.put(rng.standard_normal((m, k)).astype(np.float32)), rows),
+                    mx4.Gemm(device, rows, weights, y)])
+        outs.append(y)
+    alone = []
+    for pair, y in zip(ops, outs):
+        for op in pair:
+            op.enqueue()
+        device.sync()
+        alone.append(y.read(np.uint32).copy())
+        y.write(np.zeros_like(alone[-1]))
+    device.sync()
+    streams = [device.new_stream(), device.new_stream()]
+    for _ in range(5):
+        for i in range(2):
+            for pair, stream in zip(ops, streams):
+                pair[i].enqueue(stream)
+    for s in streams:
+        device.sync(s)
+    for y, want in zip(outs, alone):
+        assert np.array_equal(y.read(np.uint32), want)

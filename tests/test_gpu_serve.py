@@ -451,6 +451,43 @@ def test_attend_takes_queries_by_a_plans_starts(device, mem):
     assert np.all(got[lengths == 0] == 0) and np.sum(lengths == 0) == 3
 
 
+def test_index_arrays_a_word_off(device, mem):
+    """Tables, lengths, starts, slots and positions at any word of a buffer:
+    the same bits as from its start."""
+    def shifted(array):
+        return mem.put(np.concatenate([np.uint32([0xDEADBEEF]), np.ravel(array), np.uint32([0xDEADBEEF])]))
+
+    x = attend_inputs(np.random.default_rng(15), [40, 500, 1, 77], 8, 2, 64, 16, "f16")
+    starts = np.arange(5, dtype=np.uint32)
+    op, read, _ = bind_attend(device, mem, x, 0.1)
+    op.enqueue()
+    device.sync()
+    want = read()
+    for name, array in (("table", x["table"]), ("lengths", x["lengths"]), ("starts", starts)):
+        setattr(op.args, name, shifted(array).ptr + 4)
+    op.args.q_rows = 4
+    op.enqueue()
+    device.sync()
+    assert np.array_equal(read(), want)
+
+    rng = np.random.default_rng(16)
+    tokens, d = 5, 16
+    slots, positions = np.uint32([3, 9, 0, 30, 7]), np.uint32([1, 0, 4, 2, 2])
+    rows, cs = mem.put(rng.standard_normal((2, tokens, d)).astype(np.float32)), rng.standard_normal((5, 8, 2))
+    got = []
+    for put, off in ((mem.put, 0), (shifted, 4)):
+        pools = [mem.empty(2 * 32 * d) for _ in range(2)]
+        op = paged.PagedStore(device, k=rows, v=rows, v_offset=tokens * d, slots=put(slots), positions=put(positions),
+                              rope=mem.put(cs.astype(np.float32)), rope_rows=5, rotated=8, kpool=pools[0],
+                              vpool=pools[1], tokens=tokens, kv_heads=1, head_dim=d, block_size=16, blocks=2)
+        op.args.slots += off
+        op.args.positions += off
+        op.enqueue()
+        device.sync()
+        got.append([p.read(np.uint16).copy() for p in pools])
+    assert all(np.array_equal(p, q) for p, q in zip(*got))
+
+
 # A step of them together ------------------------------------------------------------
 
 
