@@ -26,8 +26,13 @@ using fk::stream_of;
 
 namespace {
 
-__global__ void __launch_bounds__(FK_PLAN_THREADS) op_page_plan_held(fk_page_plan_args a) { fk::page_plan_held(a); }
-__global__ void __launch_bounds__(FK_PLAN_THREADS) op_page_plan(fk_page_plan_args a) { fk::page_plan(a); }
+template <uint32_t THREADS, uint32_t PER>
+__global__ void __launch_bounds__(THREADS) op_page_plan_held(fk_page_plan_args a, fk::Divisor block, uint32_t groups) {
+  fk::page_plan_held<THREADS, PER>(a, block, groups);
+}
+__global__ void __launch_bounds__(FK_PLAN_THREADS) op_page_plan(fk_page_plan_args a, fk::Divisor block, uint32_t) {
+  fk::page_plan(a, block);
+}
 
 template <int T, bool BF16>
 __global__ void __launch_bounds__(FK_STORE_THREADS) op_paged_store(fk_paged_store_args a) {
@@ -267,10 +272,28 @@ extern "C" int fk_serve_check(const char *entry, const void *args, size_t args_b
 
 extern "C" int fk_page_plan(fk_ctx *ctx, const fk_page_plan_args *a, fk_stream *stream) {
   if (int st = admit(ctx, "fk_page_plan", a, stream)) return st;
-  const uint64_t groups = ((uint64_t)a->tokens + FK_PLAN_THREADS - 1) / FK_PLAN_THREADS;
-  const uint32_t g = (uint32_t)(groups < 1 ? 1 : (groups > 256 ? 256 : groups));
-  hipLaunchKernelGGL(a->requests <= FK_PLAN_HELD ? op_page_plan_held : op_page_plan, dim3(g), dim3(FK_PLAN_THREADS), 0,
-                     stream_of(ctx, stream), *a);
+  auto queue = [&](auto kernel, uint32_t threads) {
+    const uint64_t groups = ((uint64_t)a->tokens + threads - 1) / threads;
+    const uint32_t g = (uint32_t)(groups < 1 ? 1 : (groups > 256 ? 256 : groups));
+    hipLaunchKernelGGL(kernel, dim3(g), dim3(threads), 0, stream_of(ctx, stream), *a, fk::divisor(a->block_size), g);
+  };
+  // The fewest wavefronts that hold the requests, one or two a thread: a barrier
+  // and a sum of few beats another request a thread, but not another two.  µs,
+  // one behind another, by threads x requests a thread:
+  //   requests, tokens    256x1  256x2  512x2  256x4  512x4  1024x2
+  //       8,     8         2.93   3.17   3.36   3.46   3.75   3.99
+  //     200,   200         3.21   3.53   3.72   3.86   4.17   4.18
+  //     500,   500                3.53   3.89   4.09   4.53   4.33
+  //     500, 51480                5.13   5.51   5.55   6.00   6.05
+  //    1000,  1000                       3.89   4.06   4.59   4.74
+  //    1500, 58169                                     6.46   7.01
+  //    2000,  2000                                     5.17   5.30
+  const uint32_t n = a->requests;
+  if (n <= 256) queue(op_page_plan_held<256, 1>, 256);
+  else if (n <= 512) queue(op_page_plan_held<256, 2>, 256);
+  else if (n <= 1024) queue(op_page_plan_held<512, 2>, 512);
+  else if (n <= 2048) queue(op_page_plan_held<512, 4>, 512);
+  else queue(op_page_plan, FK_PLAN_THREADS);
   return launched(ctx, "fk_page_plan");
 }
 

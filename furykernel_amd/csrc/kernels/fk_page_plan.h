@@ -7,25 +7,30 @@
 // prefix sums for itself (no threadgroup waits for another, nothing is kept
 // in memory between) and then takes its own tokens.
 //
-// Up to 2048 requests stay in LDS, two a thread: their lengths are read once,
-// and a token finds its request by bisection there.  Of more, each of the 1024
-// threads holds the sums of n / 1024 consecutive ones; a token finds its
-// thread's chunk by bisection and its request by walking the chunk.  A block is
-// the free list's next, so its number follows from the sums alone: no token
-// waits for a table entry that this launch writes.  A request's new page is
-// written by the token that opens it.
-// 8 requests take 3.7 µs, 1500 with 59 thousand tokens 6.0.
+// Up to 2048 requests stay in LDS, one to four a thread: their lengths are read
+// once, and a token finds its request by bisection there.  Of more, each of
+// the 1024 threads holds the sums of n / 1024 consecutive ones; a token finds
+// its thread's chunk by bisection and its request by walking the chunk.  A
+// block is the free list's next, so its number follows from the sums alone: no
+// token waits for a table entry that this launch writes.  A request's new page
+// is written by the token that opens it.
+//
+// What a thread does before the tokens is one long chain, so its parts are
+// short: quotients by the launch's block size as products, no branches, all
+// that memory gives asked for before the first wait (8 requests of 256
+// threads 3.6 µs with divisions, branches and loads where they are used, 2.9
+// so; 1500 with 59 thousand tokens 7.2 and 6.5).
 #pragma once
 
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
 #include "fk_address.h"
+#include "fk_divisor.h"
 
 #include "../../../include/fkrocm_serve.h"
 
 #define FK_PLAN_THREADS 1024
-#define FK_PLAN_WAVES (FK_PLAN_THREADS / 64)
 
 namespace fk {
 
@@ -36,8 +41,9 @@ struct PlanRequest {
   bool fits;            // its table row and the step's tokens hold it
 };
 
-__device__ __forceinline__ uint32_t plan_pages(uint32_t positions, uint32_t block) {
-  return positions ? (positions - 1) / block + 1 : 0u;
+__device__ __forceinline__ uint32_t plan_pages(uint32_t positions, const Divisor &block) {
+  const uint32_t some = min(positions, 1u);
+  return quotient(positions - some, block) + some;
 }
 
 // Sums of tokens stop at 2^32 - 1, which no step has: what is past it is past
@@ -45,20 +51,22 @@ __device__ __forceinline__ uint32_t plan_pages(uint32_t positions, uint32_t bloc
 __device__ __forceinline__ uint32_t plan_add(uint32_t x, uint32_t y) { return __builtin_elementwise_add_sat(x, y); }
 
 // A request whose tokens start at `start`.
-__device__ __forceinline__ PlanRequest plan_request(const fk_page_plan_args &a, uint32_t cached, uint32_t fresh,
-                                                    uint32_t start) {
+__device__ __forceinline__ PlanRequest plan_request(const fk_page_plan_args &a, const Divisor &block, uint32_t cached,
+                                                    uint32_t fresh, uint32_t start) {
   PlanRequest q;
   q.cached = cached;
   q.fresh = fresh;
   const uint64_t total = (uint64_t)q.cached + q.fresh;
-  q.fits = total <= (uint64_t)a.table_len * a.block_size && plan_add(start, fresh) <= a.tokens;
-  q.held = q.fits ? plan_pages(q.cached, a.block_size) : 0u;
-  q.need = q.fits ? plan_pages((uint32_t)total, a.block_size) - q.held : 0u;
+  q.fits = total <= (uint64_t)a.table_len * block.by && plan_add(start, fresh) <= a.tokens;
+  const uint32_t held = plan_pages(q.cached, block), all = plan_pages((uint32_t)total, block);
+  q.held = q.fits ? held : 0u;
+  q.need = q.fits ? all - held : 0u;
   return q;
 }
 
-__device__ __forceinline__ PlanRequest plan_request(const fk_page_plan_args &a, uint32_t r, uint32_t start) {
-  return plan_request(a, global_at<const uint32_t>(a.cached)[r], global_at<const uint32_t>(a.fresh)[r], start);
+__device__ __forceinline__ PlanRequest plan_request(const fk_page_plan_args &a, const Divisor &block, uint32_t r,
+                                                    uint32_t start) {
+  return plan_request(a, block, global_at<const uint32_t>(a.cached)[r], global_at<const uint32_t>(a.fresh)[r], start);
 }
 
 // A lane's value from DPP control CTRL's lane, 0 where there is none or the
@@ -80,6 +88,7 @@ __device__ __forceinline__ uint32_t wave_upto(uint32_t v) {
 
 // The sum of the threads before this one, and the threadgroup's; `slots`
 // holds a value a wavefront and is used once.
+template <uint32_t THREADS>
 __device__ __forceinline__ uint32_t group_before(uint32_t v, uint32_t *slots, uint32_t *total) {
   const uint32_t upto = wave_upto(v), wave = threadIdx.x / 64, lane = threadIdx.x & 63;
   // (before this lane: the lane below's sum, which a difference would lose
@@ -89,7 +98,7 @@ __device__ __forceinline__ uint32_t group_before(uint32_t v, uint32_t *slots, ui
   __syncthreads();
   uint32_t before = 0, all = 0;
 #pragma unroll
-  for (uint32_t w = 0; w < FK_PLAN_WAVES; w++) {
+  for (uint32_t w = 0; w < THREADS / 64; w++) {
     before = plan_add(before, w < wave ? slots[w] : 0u);
     all = plan_add(all, slots[w]);
   }
@@ -102,10 +111,10 @@ __device__ __forceinline__ uint32_t plan_u32(uint64_t x) { return x < 0xFFFFFFFF
 
 // Token t of a request whose position is pos: its slot.  `held` blocks are in
 // the table, new ones in the free list from `first` on.
-__device__ __forceinline__ uint32_t plan_slot(const fk_page_plan_args &a, uint32_t r, uint32_t pos, uint32_t held,
-                                              uint32_t first) {
+__device__ __forceinline__ uint32_t plan_slot(const fk_page_plan_args &a, const Divisor &size, uint32_t r,
+                                              uint32_t pos, uint32_t held, uint32_t first) {
   const auto table = global_at<uint32_t>(a.table) + (uint64_t)r * a.table_len;
-  const uint32_t page = pos / a.block_size, within = pos - page * a.block_size;
+  const uint32_t page = quotient(pos, size), within = pos - page * size.by;
   uint32_t block;
   if (page < held) {
     block = table[page];
@@ -113,7 +122,7 @@ __device__ __forceinline__ uint32_t plan_slot(const fk_page_plan_args &a, uint32
     block = global_at<const uint32_t>(a.free_blocks)[first + (page - held)];
     if (within == 0) table[page] = block;
   }
-  return plan_u32((uint64_t)block * a.block_size + within);
+  return plan_u32((uint64_t)block * size.by + within);
 }
 
 __device__ __forceinline__ void plan_token(const fk_page_plan_args &a, uint32_t t, uint32_t slot, uint32_t pos,
@@ -133,45 +142,68 @@ __device__ __forceinline__ void plan_counts(const fk_page_plan_args &a, uint32_t
   c[3] = head + taken;
 }
 
-// HELD: at most FK_PLAN_HELD requests.
-#define FK_PLAN_HELD (2 * FK_PLAN_THREADS)
-__device__ __forceinline__ void page_plan_held(const fk_page_plan_args &a) {
-  __shared__ uint32_t token_slots[FK_PLAN_WAVES], block_slots[FK_PLAN_WAVES], refused, taken;
+// At most PER THREADS requests, PER a thread.
+template <uint32_t THREADS, uint32_t PER>
+__device__ __forceinline__ void page_plan_held(const fk_page_plan_args &a, const Divisor &block, uint32_t groups) {
+  constexpr uint32_t HELD = PER * THREADS;
+  __shared__ uint32_t token_slots[THREADS / 64], block_slots[THREADS / 64], refused, taken;
   // a request's first token, its cached positions, its first new block's place
   // in the free list (below free_len; FK_NO_SLOT: it does not fit)
-  __shared__ uint32_t starts[FK_PLAN_HELD], held_at[FK_PLAN_HELD], firsts[FK_PLAN_HELD];
+  __shared__ uint32_t starts[HELD], held_at[HELD], firsts[HELD];
   const uint32_t tid = threadIdx.x, n = a.requests;
-  const uint32_t head = *global_at<const uint32_t>(a.head);
-  uint32_t c[2], f[2];
+  uint32_t head = *global_at<const uint32_t>(a.head), free_len = a.free_len;
+  uint32_t c[PER], f[PER];
 #pragma unroll
-  for (uint32_t i = 0; i < 2; i++) {
-    const uint32_t r = 2 * tid + i;
-    c[i] = r < n ? global_at<const uint32_t>(a.cached)[r] : 0u;
-    f[i] = r < n ? global_at<const uint32_t>(a.fresh)[r] : 0u;
+  for (uint32_t i = 0; i < PER; i++) {
+    // (past the last: the last again, put to 0 below, so that the loads need no
+    // branches)
+    const uint32_t r = min(PER * tid + i, n - 1);
+    c[i] = global_at<const uint32_t>(a.cached)[r];
+    f[i] = global_at<const uint32_t>(a.fresh)[r];
   }
-  const uint32_t avail = a.free_len > head ? a.free_len - head : 0u;
+  // (everything on its way before the first wait)
+  asm volatile("" : "+s"(head), "+s"(free_len));
+#pragma unroll
+  for (uint32_t i = 0; i < PER; i++) {
+    c[i] = PER * tid + i < n ? c[i] : 0u;
+    f[i] = PER * tid + i < n ? f[i] : 0u;
+  }
+  const uint32_t avail = free_len > head ? free_len - head : 0u;
   if (tid == 0) refused = taken = 0;
-  uint32_t total;
-  const uint32_t first = group_before(plan_add(f[0], f[1]), token_slots, &total);
-  const PlanRequest q[2] = {plan_request(a, c[0], f[0], first), plan_request(a, c[1], f[1], plan_add(first, f[0]))};
+  uint32_t mine = f[0], total;
+#pragma unroll
+  for (uint32_t i = 1; i < PER; i++) mine = plan_add(mine, f[i]);
+  uint32_t first[PER];
+  first[0] = group_before<THREADS>(mine, token_slots, &total);
+#pragma unroll
+  for (uint32_t i = 1; i < PER; i++) first[i] = plan_add(first[i - 1], f[i - 1]);
   // (requests that fit need a block a token at most, so the step's fewer than
   // 2^32)
-  uint32_t needed, after = group_before(q[0].need + q[1].need, block_slots, &needed);
-  uint32_t out = 0, most = 0;
+  PlanRequest q[PER];
+  uint32_t need = 0, needed;
 #pragma unroll
-  for (uint32_t i = 0; i < 2; i++) {
-    const uint32_t r = 2 * tid + i;
+  for (uint32_t i = 0; i < PER; i++) {
+    q[i] = plan_request(a, block, c[i], f[i], first[i]);
+    need += q[i].need;
+  }
+  uint32_t after = group_before<THREADS>(need, block_slots, &needed);
+  uint32_t out = 0, most = 0;
+  // a wavefront's requests' own outputs: by the threadgroup of its number
+  const bool writes = min(__builtin_amdgcn_readfirstlane(tid / 64), groups - 1) == blockIdx.x;
+#pragma unroll
+  for (uint32_t i = 0; i < PER; i++) {
+    const uint32_t r = PER * tid + i;
     const uint32_t before = after;
     after += q[i].need;
     const bool fits = q[i].fits && (q[i].need == 0 || after <= avail);
-    const uint32_t start = r < n ? (i ? plan_add(first, f[0]) : first) : 0xFFFFFFFFu;
+    const uint32_t start = r < n ? first[i] : 0xFFFFFFFFu;
     starts[r] = start;
     held_at[r] = c[i];
     firsts[r] = fits ? (q[i].need ? head + before : 0u) : FK_NO_SLOT;
     if (r < n) {
       if (fits && q[i].need) most = after;
       out += !fits;
-      if (tid % gridDim.x == blockIdx.x) {
+      if (writes) {
         global_at<uint32_t>(a.lengths)[r] = fits ? c[i] + f[i] : c[i];
         global_at<uint32_t>(a.starts)[r] = start;
       }
@@ -183,8 +215,8 @@ __device__ __forceinline__ void page_plan_held(const fk_page_plan_args &a) {
   }
   __syncthreads();
   if (blockIdx.x == 0 && tid == 0) plan_counts(a, total, head, taken, refused);
-  for (uint64_t t64 = (uint64_t)blockIdx.x * FK_PLAN_THREADS + tid; t64 < a.tokens;
-       t64 += (uint64_t)gridDim.x * FK_PLAN_THREADS) {
+  for (uint64_t t64 = (uint64_t)blockIdx.x * THREADS + tid; t64 < a.tokens;
+       t64 += (uint64_t)groups * THREADS) {
     const uint32_t t = (uint32_t)t64;
     uint32_t slot = FK_NO_SLOT, pos = 0, owner = FK_NO_SLOT;
     if (t < total) {
@@ -192,18 +224,18 @@ __device__ __forceinline__ void page_plan_held(const fk_page_plan_args &a) {
       // where the next does
       owner = 0;
 #pragma unroll
-      for (uint32_t step = FK_PLAN_HELD / 2; step > 0; step /= 2)
+      for (uint32_t step = HELD / 2; step > 0; step /= 2)
         if (starts[owner + step] <= t) owner += step;
       const uint32_t cached = held_at[owner], free_at = firsts[owner];
       pos = cached + (t - starts[owner]);
-      if (free_at != FK_NO_SLOT) slot = plan_slot(a, owner, pos, plan_pages(cached, a.block_size), free_at);
+      if (free_at != FK_NO_SLOT) slot = plan_slot(a, block, owner, pos, plan_pages(cached, block), free_at);
     }
     plan_token(a, t, slot, pos, owner);
   }
 }
 
-__device__ __forceinline__ void page_plan(const fk_page_plan_args &a) {
-  __shared__ uint32_t token_slots[FK_PLAN_WAVES], block_slots[FK_PLAN_WAVES];
+__device__ __forceinline__ void page_plan(const fk_page_plan_args &a, const Divisor &block) {
+  __shared__ uint32_t token_slots[FK_PLAN_THREADS / 64], block_slots[FK_PLAN_THREADS / 64];
   __shared__ uint32_t first_token[FK_PLAN_THREADS];  // the tokens before a chunk's first request
   __shared__ uint32_t first_block[FK_PLAN_THREADS];  // the new blocks before it
   __shared__ uint32_t refused, taken;
@@ -219,17 +251,17 @@ __device__ __forceinline__ void page_plan(const fk_page_plan_args &a) {
 
   uint32_t mine = 0, total;
   for (uint32_t r = r0; r < r1; r++) mine = plan_add(mine, fresh[r]);
-  const uint32_t tokens0 = group_before(mine, token_slots, &total);
+  const uint32_t tokens0 = group_before<FK_PLAN_THREADS>(mine, token_slots, &total);
   uint32_t need = 0, needed;
   {
     uint32_t at = tokens0;
     for (uint32_t r = r0; r < r1; r++) {
-      const PlanRequest q = plan_request(a, r, at);
+      const PlanRequest q = plan_request(a, block, r, at);
       need += q.need;
       at = plan_add(at, q.fresh);
     }
   }
-  const uint32_t blocks0 = group_before(need, block_slots, &needed);
+  const uint32_t blocks0 = group_before<FK_PLAN_THREADS>(need, block_slots, &needed);
   first_token[tid] = tokens0;
   first_block[tid] = blocks0;
   __syncthreads();
@@ -241,7 +273,7 @@ __device__ __forceinline__ void page_plan(const fk_page_plan_args &a) {
     uint32_t at = tokens0, after = blocks0;
     uint32_t out = 0, most = 0;
     for (uint32_t r = r0; r < r1; r++) {
-      const PlanRequest q = plan_request(a, r, at);
+      const PlanRequest q = plan_request(a, block, r, at);
       after += q.need;
       const bool fits = q.fits && (q.need == 0 || after <= avail);
       if (fits && q.need) most = after;
@@ -275,16 +307,16 @@ __device__ __forceinline__ void page_plan(const fk_page_plan_args &a) {
         if (first_token[lo + step] <= t) lo += step;
       uint32_t r = lo * chunk;
       uint32_t at = first_token[lo], blocks = first_block[lo];
-      PlanRequest q = plan_request(a, r, at);
+      PlanRequest q = plan_request(a, block, r, at);
       while (plan_add(at, q.fresh) <= t) {
         at = plan_add(at, q.fresh);
         blocks += q.need;
-        q = plan_request(a, ++r, at);
+        q = plan_request(a, block, ++r, at);
       }
       owner = r;
       pos = q.cached + (t - at);
       if (q.fits && (q.need == 0 || blocks + q.need <= avail))
-        slot = plan_slot(a, r, pos, q.held, head + blocks);
+        slot = plan_slot(a, block, r, pos, q.held, head + blocks);
     }
     plan_token(a, t, slot, pos, owner);
   }

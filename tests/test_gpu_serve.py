@@ -90,8 +90,8 @@ def hold_plan(device, mem, x):
 
 @pytest.mark.parametrize("n,longest,chunk,block,spare", [
     (1, 0, 1, 16, 0), (1, 0, 1, 1, 3), (1, 5000, 3000, 16, 100), (2, 31, 33, 16, 0), (63, 40, 9, 7, 5),
-    (256, 300, 1, 16, 0), (1000, 100, 40, 24, 17), (1023, 9, 3, 1, 0), (1024, 50, 20, 8, 1), (1025, 50, 20, 128, 2),
-    (3001, 30, 7, 16, 999), (20000, 20, 12, 16, 50)])
+    (256, 300, 1, 16, 0), (257, 60, 4, 5, 3), (512, 60, 4, 5, 0), (513, 60, 4, 11, 9), (1000, 100, 40, 24, 17), (1023, 9, 3, 1, 0), (1024, 50, 20, 8, 1), (1025, 50, 20, 128, 2),
+    (2048, 40, 5, 3, 0), (2049, 40, 5, 3, 70), (1500, 700, 80, 16, 777), (3001, 30, 7, 16, 999), (20000, 20, 12, 16, 50)])
 def test_plan_is_its_definition(device, mem, n, longest, chunk, block, spare):
     print(f"plan {n} {longest} {chunk} {block} {spare}", flush=True)
     x = plan_case(n + block, n, longest, chunk, block, -(-(longest + chunk) // block) + 1, spare)
@@ -103,30 +103,38 @@ def test_plan_is_its_definition(device, mem, n, longest, chunk, block, spare):
     ("blocks", dict(spare_blocks=-9)), ("no blocks", dict(spare_blocks=-10 ** 6)), ("table", dict(table_len=2)),
     ("tokens", dict(spare_tokens=-30)), ("no tokens", dict(spare_tokens=-10 ** 6)),
     ("all", dict(spare_blocks=-30, table_len=3, spare_tokens=-100))])
-def test_plan_refuses_requests_that_do_not_fit(device, mem, why, over):
-    x = plan_case(5, 300, 60, 30, 16, **{"table_len": 7, **over})
+@pytest.mark.parametrize("n", [150, 300, 700, 1500, 2500])
+def test_plan_refuses_requests_that_do_not_fit(device, mem, why, over, n):
+    x = plan_case(5, n, 60, 30, 16, **{"table_len": 7, **over})
     if why == "no blocks":
         x["free"] = x["free"][:2]     # fewer than are taken already
     want = hold_plan(device, mem, x)
-    assert 0 < want["counts"][2] <= 300
+    assert 0 < want["counts"][2] <= n
 
 
-def test_plan_of_lengths_that_are_nonsense(device, mem):
-    x = plan_case(6, 40, 60, 30, 16, 7)
+@pytest.mark.parametrize("n", [40, 400, 1000, 2000, 2500])
+def test_plan_of_lengths_that_are_nonsense(device, mem, n):
+    x = plan_case(6, n, 60, 30, 16, 7)
     rng = np.random.default_rng(1)
     for name in ("cached", "fresh"):
-        x[name][rng.integers(0, 40, 5)] = rng.choice([0xFFFFFFFF, 0x80000000, 113], 5)
+        x[name][rng.integers(0, n, 5)] = rng.choice([0xFFFFFFFF, 0x80000000, 113], 5)
     x["table"][:, :3] = 0xFFFFFFF0    # slots past 32 bits are no slots
     hold_plan(device, mem, x)
 
 
-@pytest.mark.parametrize("n", [40, 3000])
+@pytest.mark.parametrize("n", [40, 400, 1000, 2000, 3000])
 def test_plan_of_a_free_list_taken_past_its_end(device, mem, n):
     """No block is left; requests whose pages hold their new tokens go on."""
     x = plan_case(8, n, 60, 3, 16, 7)
     x["head"] = 0xFFFFFFFF
     want = hold_plan(device, mem, x)
     assert 0 < want["counts"][2] < n and np.any(want["slots"] != S.NO_SLOT)
+
+
+@pytest.mark.parametrize("block", [1, 2, 3, 5, 7, 11, 16, 24, 100, 641, 1000, 4095, 65537])
+def test_plan_of_blocks_of_any_size(device, mem, block):
+    x = plan_case(9, 70, 9000, 3, block, -(-9003 // block) + 1, 5)
+    hold_plan(device, mem, x)
 
 
 def test_plan_of_nothing(device, mem):
