@@ -6,6 +6,10 @@ The pieces, from the bottom:
   context, code-object modules, resident arenas, copies, launches, events,
   graphs, the kernels' manifest and ABI hashes, native launch tables, and the
   one-call decode attention of ``include/fkrocm_ops.h``.
+* ``paged`` — the operators of a served batch over paged caches
+  (``include/fkrocm_serve.h``): page plan, RoPE and store, attention.
+* ``mx4`` — 4-bit microscaled matrices (``include/fkrocm_mx4.h``): made, read
+  back, multiplied.
 * ``kernels`` — the launch table of the hand-written gfx950 kernels
   (``fk_kernels.hsaco``, ``fk_attend.hsaco``) and their launchers.
 * ``manifest`` — each kernel's manifest as the reference's JSON.
