@@ -94,23 +94,28 @@ AttendLaunch attend_launch(const fk_paged_attend_args &a) {
     l.plan.by_pair = pairs <= l.groups;
     l.joins = l.plan.by_pair ? (uint32_t)pairs : l.groups;
     // Few units a pair at most: a threadgroup takes pairs whole, which saves the
-    // prefix sum and the join and costs each further unit's time; of two units
-    // and more by 8 wavefronts, where the pairs do not fill the CUs anyway.
-    // Requests of u units (256 keys of 64, 128 of 128 and 256), 8 kv heads (of
-    // 256: 2), µs split, whole by 4, whole by 8:
-    //               u = 1            2                3                4
-    //    1 of 64    7.4 5.0  5.6     9.4  6.7  6.0    9.5  9.2  8.3    9.8 11.7  9.6
-    //   16 of 64    8.7 6.3  6.5    11.9  8.8  7.9   13.1 11.0 10.2   14.4 13.1 11.2
-    //    1 of 128   8.3 5.9  6.3    10.1  7.2  6.9   10.3  9.2  8.8   10.8 11.1  9.9
-    //   16 of 128   9.2 6.8  7.2    12.6  9.1  8.9   14.2 11.1 11.6   15.2 13.0 12.4
-    //   41 of 128  11.6 9.8         15.7 14.3        21.6 17.4        25.2 21.2
-    //    1 of 256  12.4 9.7         14.5 13.5        14.3 16.5        14.0 19.5
-    // (many requests of one length would gain from it at any length, but ragged
-    // ones would wait for their longest: the table's length is what the host
-    // knows.)
+    // prefix sum and the join and costs each further unit's time, and a long
+    // pair's to the launch; where the pairs do not fill the CUs by 8 wavefronts,
+    // which share all but three units better than 4.  Requests of up to u units
+    // (256 keys of 64, 128 of 128), evenly spread (the one has u), µs split,
+    // whole by 4, whole by 8:
+    //    pairs, width    u = 2           3               4               5               6
+    //      8 of 64    9.3  6.4  6.0   9.3  8.1  8.3   9.7  9.9  8.7   9.9 11.6 11.1  10.0 13.1 11.4
+    //     80 of 64   10.4  7.3  7.1  10.5  8.6  9.0  10.8 10.5  9.5  11.2 11.8 11.1  12.6 13.7 12.1
+    //    164 of 64   11.6  7.9  7.6  13.2  9.5  9.7  13.7 11.1 10.2  14.0 12.7 12.4  18.1 14.2 12.9
+    //    328 of 64   13.4 10.5 12.7  16.8 12.1 14.7  18.8 15.1 15.6  19.5 18.6 20.2  22.3 18.6 20.4
+    //      8 of 128  10.1  7.2  6.9  10.2  8.5  8.6  10.5  9.8  8.9  10.5 11.2 10.6  10.6 12.5 10.9
+    //     80 of 128  10.7  7.6  7.4  11.1  8.9  9.2  11.4 10.2  9.5  12.1 11.5 11.1  13.1 13.0 11.8
+    //    164 of 128  12.5  8.4  8.4  14.4  9.8 10.2  15.3 11.3 11.0  15.2 12.6 12.5  19.4 14.1 13.5
+    //    328 of 128  14.0  9.3 12.5  18.8 12.7 15.2  19.7 15.6 17.1  20.7 17.3 18.2  24.6 18.7 20.8
+    // Of 256 (128 keys), 2, 32 and 82 pairs of all u units, split and whole by 4:
+    // 13.7 11.8, 14.7 12.7 and 15.9 13.1 at 2, 13.4 14.1, 14.9 15.3 and 17.3 15.8
+    // at 3.  (Many pairs gain at more units too, but one of the table's length
+    // among short ones would cost more: that is what the host knows.)
     const uint64_t each = (seen + unit - 1) / unit;
-    l.waves = l.width != 256 && pairs <= 256 && each >= 2 && each <= 4 ? 8 : 4;
-    l.plan.whole = each <= (l.width == 256 ? 2 : l.waves == 8 ? 4 : 3);
+    l.waves = l.width != 256 && pairs <= 256 && each >= 2 && each != 3 ? 8 : 4;
+    l.plan.whole = each <= (l.width == 256 ? 2 : pairs < 64 ? 4 : 6);
+    if (!l.plan.whole) l.waves = 4;
     if (l.plan.whole) l.groups = (uint32_t)(pairs < most ? pairs : most);
   }
   return l;

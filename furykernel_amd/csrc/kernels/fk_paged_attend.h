@@ -298,10 +298,13 @@ __device__ __forceinline__ void paged_attend(const fk_paged_attend_args &a, cons
   const uint32_t v_lds = (uint32_t)(uintptr_t)(FK_PAGED_LDS uint16_t *)vbuf;
   u32x4 last_join = {0, 0, 0, 0};
 
-  uint32_t pid = blockIdx.x;
+  uint32_t pid = blockIdx.x, entries = 0;
   do {
     if (pl.whole) {
       r = pid / per_request;
+      // a whole table of no more than a wavefront's lanes, beside the length
+      if (a.table_len <= FK_WAVE)
+        entries = global_at<const uint32_t>(a.table)[(uint64_t)r * a.table_len + min(lane, a.table_len - 1)];
       length = length_of(r);
       here = units_in(length);
       at = 0;
@@ -349,19 +352,26 @@ __device__ __forceinline__ void paged_attend(const fk_paged_attend_args &a, cons
 
       const auto row = global_at<const uint32_t>(a.table) + (uint64_t)r * a.table_len;
       const uint32_t last_entry = (ks.last - 1) / a.block_size;
-      uint32_t entry0 = 0, entries = 0;   // the table entries entry0 + lane, none yet
-      bool held = false;
+      // The table entries entry0 + lane, from the first tile's on unless they are
+      // there already, landed with Q: no tile without a load of them waits for
+      // one.
+      uint32_t entry0 = 0;
+      if (!pl.whole || a.table_len > FK_WAVE) {
+        entry0 = min(max(t0 * KT, ks.first) / a.block_size, last_entry);
+        entries = row[min(entry0 + lane, last_entry)];
+      }
+      __builtin_amdgcn_s_waitcnt(FK_PAGED_VMCNT(0));
+      asm volatile("" : "+v"(entries));
+#pragma unroll
+      for (uint32_t h = 0; h < DP / 32; h++) asm volatile("" : "+v"(qf[h]));
+      entries = min(entries, a.blocks - 1);
       uint64_t off[LOADS];                // the tile's rows in the pools, in bytes
       // K's piece u at place u ^ (key's) of its row, V's 32-byte pairs of pieces
       // likewise, so that the reads below meet different banks.
       auto rows_of = [&](uint32_t tile) {
-        const uint32_t key0 = max(tile * KT, ks.first), key1 = min(tile * KT + KT, ks.last) - 1;
-        const uint32_t need0 = key0 / a.block_size, need1 = key1 / a.block_size;
-        if (!held || need1 > entry0 + 63) {
-          entry0 = need0;
+        if ((min(tile * KT + KT, ks.last) - 1) / a.block_size > entry0 + 63) {
+          entry0 = max(tile * KT, ks.first) / a.block_size;
           entries = min(row[min(entry0 + lane, last_entry)], a.blocks - 1);
-          held = true;
-          // landed here, so that no tile without this load waits for one
           __builtin_amdgcn_s_waitcnt(FK_PAGED_VMCNT(0));
           asm volatile("" : "+v"(entries));
         }
@@ -374,6 +384,7 @@ __device__ __forceinline__ void paged_attend(const fk_paged_attend_args &a, cons
           within[q] = key - entry * a.block_size;
           block[q] = __builtin_amdgcn_ds_bpermute((entry - entry0) * 4, entries);
         }
+        __builtin_amdgcn_sched_barrier(0);  // all asked for before the first is waited for
 #pragma unroll
         for (uint32_t q = 0; q < LOADS; q++)
           off[q] = (((uint64_t)block[q] * a.kv_heads + g) * a.block_size + within[q]) * (2 * D);

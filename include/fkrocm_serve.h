@@ -110,7 +110,7 @@ int fk_paged_store(fk_ctx *ctx, const fk_paged_store_args *args, fk_stream *stre
  * without a new token (or with tokens past q_rows) counts as empty.  A length
  * of 0 gives a row of zeros; a length past table_len * block_size counts as
  * that.  A table entry past `blocks` reads
- * the pool's last block; entries behind a length are not read.
+ * the pool's last block; what entries behind a length hold does not matter.
  *
  * Scores, the running maximum, the sums and the weighted values are binary32
  * (probabilities go to the matrix cores as two 16-bit parts, 16 bits and more

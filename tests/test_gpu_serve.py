@@ -312,8 +312,8 @@ def test_attend_of_ragged_requests(device, mem, heads, kv, d, block, cache):
     hold_attend(device, mem, x, d ** -0.5)
 
 
-@pytest.mark.parametrize("pages", [2, 4, 8, 12, 16, 17, 24, 32, 64, 65, 100])
-@pytest.mark.parametrize("d,kv", [(64, 2), (128, 1), (256, 2), (64, 64)])
+@pytest.mark.parametrize("pages", [2, 4, 8, 12, 16, 17, 24, 32, 40, 48, 49, 64, 65, 80, 96, 97, 100])
+@pytest.mark.parametrize("d,kv", [(64, 2), (128, 1), (256, 2), (64, 64), (64, 16), (128, 16), (128, 50)])
 def test_attend_of_tables_of_every_length(device, mem, pages, d, kv):
     """Tables of few units go whole to the threadgroups, longer ones split:
     each side of each rule, the lengths short and up to the table's."""
