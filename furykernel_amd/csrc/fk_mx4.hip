@@ -31,8 +31,10 @@ __global__ void __launch_bounds__(FK_MX4_THREADS) op_mx4_dequantize(fk_mx4_dequa
   fk::mx4_dequantize<T>(a);
 }
 
+// (two wavefronts a SIMD: 8 x 2 with two pairs in flight would take one's
+// registers and its CU alone; 200 rows by 8192, k 2048 8.7 µs, so 7.0)
 template <uint32_t MB, uint32_t NB, uint32_t W, int T>
-__global__ void __launch_bounds__(64 * W) op_mx4_gemm_few(fk_mx4_gemm_args a) {
+__global__ void __launch_bounds__(64 * W, 2) op_mx4_gemm_few(fk_mx4_gemm_args a) {
   fk::mx4_gemm_few<MB, NB, W, T>(a);
 }
 
@@ -89,22 +91,24 @@ struct Form {
   const char *name;
   Kind kind;
   uint32_t mb, nb, by;
-  double base, step, work;
+  double base, step, turn, work;
 };
-// What each costs, in µs, fitted to its times on 98 products (1 to 8192 rows
+// What each costs, in µs, fitted to its times on 229 products (1 to 8192 rows
 // by 512 to 16384, k of 2048 to 8192, the operands from memory each time):
-//   few         base, `step` for each pair of tiles of k a wavefront takes, and
-//               `work` for a thousand KB that all threadgroups read (mb + nb
-//               blocks a pair each: what a tile reads again, others read too)
+//   few         base, for each pair of tiles of k a wavefront takes `step` and
+//               `turn` for every threadgroup of its CU, and `work` for a
+//               thousand KB that all threadgroups read (mb + nb blocks a pair
+//               each: what a tile reads again, others read too)
 //   mid, many   `step` a pair, `work` for 10^5 blocks times pairs, and `base`
 //               for every time the tiles fill the chip
-// The form of the least cost takes 1.02 times the fastest one's time on
-// average over them, at most 1.26 (32 rows by 8192, k 2048: 5.4 µs, 64 x 16
-// blocks 4.3).
+// The form of the least cost takes 1.003 times the fastest one's time on
+// average over them, at most 1.18 (512 rows by 5000, k 2048: 14.6 µs, mid
+// 12.4).  Between 64 x 16 and 128 x 32 blocks, 32 x 32 ones would be 0.5 %
+// faster on average.
 constexpr Form forms[] = {
-    {"few 1x1", FEW, 1, 1, 8, 2.54, 0.25, 0.169},  {"few 4x1", FEW, 4, 1, 8, 2.71, 0.34, 0.127},
-    {"few 4x2", FEW, 4, 2, 8, 3.34, 0.43, 0.153},  {"few 8x2", FEW, 8, 2, 4, 3.73, 0.65, 0.120},
-    {"mid 8x8", MID, 8, 8, 768, 3.86, 0.57, 3.10}, {"many 16x16", MANY, 16, 16, 256, 10.3, 0.83, 1.61},
+    {"few 1x1", FEW, 1, 1, 8, 2.598, 0.129, 0.091, 0.160}, {"few 4x1", FEW, 4, 1, 8, 2.587, 0.182, 0.512, 0.074},
+    {"few 4x2", FEW, 4, 2, 4, 2.558, 0, 0.580, 0.060},     {"few 8x2", FEW, 8, 2, 4, 2.743, 0, 1.047, 0.025},
+    {"mid 8x8", MID, 8, 8, 768, 5.416, 0.467, 0, 2.579},   {"many 16x16", MANY, 16, 16, 256, 11.667, 0.763, 0, 1.376},
 };
 
 uint64_t tiles_of(const Form &f, uint32_t m, uint32_t n) {
@@ -113,7 +117,9 @@ uint64_t tiles_of(const Form &f, uint32_t m, uint32_t n) {
 
 double cost(const Form &f, uint32_t m, uint32_t n, uint32_t k) {
   const double t = (double)tiles_of(f, m, n), pairs = fk::mx4_pairs(k);
-  if (f.kind == FEW) return f.base + f.step * std::ceil(pairs / f.by) + f.work * 1e-3 * t * pairs * (f.mb + f.nb);
+  if (f.kind == FEW)
+    return f.base + std::ceil(pairs / f.by) * (f.step + f.turn * std::ceil(t / 256)) +
+           f.work * 1e-3 * t * pairs * (f.mb + f.nb);
   return f.base * std::ceil(t / f.by) + f.step * pairs + f.work * 1e-5 * t * f.mb * f.nb * pairs;
 }
 

@@ -193,6 +193,24 @@ def test_products_whose_sums_fit_are_exact(device, mem, m, n, k):
         assert same.all(), (kind, int((~same).sum()), np.argwhere(~same)[:4].tolist())
 
 
+# Of each form whose wavefronts share k: sizes, and the wavefronts.
+TURNS = [("few 1x1", 5, 200, 8), ("few 4x1", 100, 1000, 8), ("few 4x2", 100, 2500, 4), ("few 8x2", 500, 1500, 4)]
+
+
+@pytest.mark.parametrize("form,m,n,w", TURNS)
+def test_products_of_one_to_six_pairs_of_tiles_a_wavefront(device, mem, form, m, n, w):
+    """As above, k ending in each turn of a wavefront's loop."""
+    rng = np.random.default_rng(m)
+    for pairs in (w + 1, 2 * w - 1, 2 * w, 2 * w + 1, 3 * w, 3 * w + 2, 4 * w, 4 * w + 1, 5 * w, 6 * w - 1):
+        k = 256 * pairs - 37
+        print(f"gemm turns {form} {m} {n} {k}", flush=True)
+        assert runtime.library().fk_mx4_gemm_form(m, n, k).decode() == form
+        (ca, sa), (cb, sb) = random_matrix(rng, m, k, 0), random_matrix(rng, n, k, 0)
+        want = M.values(ca, sa, k).astype(np.float32) @ M.values(cb, sb, k).T.astype(np.float32)
+        got = product(device, mem, put_matrix(device, mem, ca, sa, k), put_matrix(device, mem, cb, sb, k), m, n, "f32")
+        assert np.array_equal(got.view(np.float32), want)
+
+
 @pytest.mark.parametrize("m,n,k", [(1, 64, 4096), (9, 300, 2048), (40, 200, 1000), (256, 512, 2048), (300, 700, 900)])
 def test_products_over_scales_apart(device, mem, m, n, k):
     """Scales 2^-20 .. 2^20: off by the additions' roundings, k of them of at
