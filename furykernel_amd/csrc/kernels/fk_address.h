@@ -16,4 +16,12 @@ __device__ __forceinline__ global_ptr<T> global_at(uint64_t address) {
   return (global_ptr<T>)address;
 }
 
+// A load of what a launch takes once, with ONCE: it leaves the caches to what
+// is used again.
+template <bool ONCE, typename T>
+__device__ __forceinline__ T load_from(global_ptr<const T> p) {
+  if constexpr (ONCE) return __builtin_nontemporal_load(p);
+  else return *p;
+}
+
 }  // namespace fk

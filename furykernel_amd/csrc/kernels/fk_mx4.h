@@ -7,9 +7,9 @@
 // the four lanes of a block share its maximum by quad permutes, and a lane's
 // codes are one word, 64 bytes together in the tile's order.  The conversions
 // are the hardware's scaled ones (v_cvt_scalef32_pk_fp4_f32 and back).
-// Measured on 8192 x 8192: bf16 made in 28.3 µs (6.0 TB/s), read back in 26.4
-// (6.4); f32 52 (5.8) and 71 (4.3: 268 MB of stores, more than the chip's last
-// cache holds; whole 64-byte pieces a store, by quad permutes, take 69).
+// Measured on 8192 x 8192, out of memory each time: bf16 made in 33.0 µs (5.2
+// TB/s), read back in 32.7; f32 56.9 and 66.4 (73.9 in stores of 16 bytes
+// apart).
 #pragma once
 
 #include "fk_address.h"
@@ -44,19 +44,19 @@ __device__ __forceinline__ float mx4_load(uint64_t row, uint64_t i) {
   else return __uint_as_float((uint32_t)global_at<const uint16_t>(row)[i] << 16);
 }
 // Eight from element i on.
-template <int T>
+template <int T, bool ONCE>
 __device__ __forceinline__ void mx4_load8(uint64_t row, uint64_t i, float (&x)[8]) {
   if constexpr (T == FK_T_F32) {
     const auto p = global_at<const mx4_float4>(row + 4 * i);
-    const mx4_float4 a = p[0], b = p[1];
+    const mx4_float4 a = load_from<ONCE, mx4_float4>(p), b = load_from<ONCE, mx4_float4>(p + 1);
 #pragma unroll
     for (int j = 0; j < 4; j++) x[j] = a[j], x[4 + j] = b[j];
   } else if constexpr (T == FK_T_F16) {
-    const mx4_half8 h = *global_at<const mx4_half8>(row + 2 * i);
+    const mx4_half8 h = load_from<ONCE, mx4_half8>(global_at<const mx4_half8>(row + 2 * i));
 #pragma unroll
     for (int j = 0; j < 8; j++) x[j] = (float)h[j];
   } else {
-    const mx4_u32x4 w = *global_at<const mx4_u32x4>(row + 2 * i);
+    const mx4_u32x4 w = load_from<ONCE, mx4_u32x4>(global_at<const mx4_u32x4>(row + 2 * i));
 #pragma unroll
     for (int j = 0; j < 4; j++) {
       x[2 * j] = __uint_as_float(w[j] << 16);
@@ -115,7 +115,7 @@ __device__ __forceinline__ uint64_t mx4_scale_at(const Mx4Place &p, uint32_t k, 
   return ((uint64_t)p.tile * mx4_pairs(k) + p.step / 2) * 128 + (p.piece / 4 * 16 + 4 * i + p.sub) * 2 + p.step % 2;
 }
 
-template <int T>
+template <int T, bool ONCE>
 __device__ __forceinline__ void mx4_quantize(const fk_mx4_quantize_args &a) {
   const Mx4Place p = mx4_place(a.rows, a.k);
   if (!p.there) return;
@@ -128,7 +128,7 @@ __device__ __forceinline__ void mx4_quantize(const fk_mx4_quantize_args &a) {
 #pragma unroll
     for (int j = 0; j < 8; j++) x[i][j] = 0.0f;
     if (row < a.rows && col + 8 <= a.k) {
-      mx4_load8<T>(at, col, x[i]);
+      mx4_load8<T, ONCE>(at, col, x[i]);
     } else if (row < a.rows && col < a.k) {
 #pragma unroll
       for (uint32_t j = 0; j < 7; j++)
@@ -197,7 +197,22 @@ __device__ __forceinline__ void mx4_dequantize(const fk_mx4_dequantize_args &a) 
 #pragma unroll
     for (int j = 0; j < 8; j++) asm volatile("" : "+v"(y[j]));
     const uint64_t at = a.y + (uint64_t)row * a.y_stride * mx4_bytes_of(T);
-    if (col + 8 <= a.k) {
+    if (T == FK_T_F32 && p.step * 128 + p.piece / 4 * 32 + 32 <= a.k) {
+      // a whole block: its four lanes' 128 bytes as two stores of 64 together
+      const uint32_t q = p.piece % 4;
+      mx4_float4 w[2];
+#pragma unroll
+      for (int j = 0; j < 4; j++) {
+        // (quad_perm [0, 0, 1, 1] and [2, 2, 3, 3])
+        const float lo[2] = {dpp_f<0x50>(y[j]), dpp_f<0xFA>(y[j])};
+        const float hi[2] = {dpp_f<0x50>(y[4 + j]), dpp_f<0xFA>(y[4 + j])};
+        w[0][j] = q % 2 ? hi[0] : lo[0];
+        w[1][j] = q % 2 ? hi[1] : lo[1];
+      }
+      const auto to = global_at<mx4_float4>(at + 4ull * (p.step * 128 + p.piece / 4 * 32));
+      to[q] = w[0];
+      to[4 + q] = w[1];
+    } else if (col + 8 <= a.k) {
       mx4_store8<T>(at, col, y);
     } else {
 #pragma unroll

@@ -169,10 +169,11 @@ __device__ __forceinline__ void mx4_gemm_few(const fk_mx4_gemm_args &a) {
 //   one threadgroup a CU: four stages, the next step's operands read and a
 //   later step's loaded between a step's matrix operations, and tile after
 //   tile with the next one's first loads under the stores.  Half the traffic
-//   for each product: 8192 x 8192, operands from memory, k 8192 235 µs (4.7
-//   PFLOP/s; mid 298), k 2048 86 (3.2; mid 103).  With no loads, reads or
-//   scales at all its matrix operations take 200 µs of the 235: the clock that
-//   the chip's power leaves them (1.9 GHz of 2.4) bounds it.
+//   for each product: 8192 x 8192 to f16, the same operands each time, k 8192
+//   235 to 246 µs (4.5 to 4.7 PFLOP/s; mid 300), k 2048 86 (3.2; mid 91), from
+//   memory each time 258 and 85.  With no loads, reads or scales at all its
+//   matrix operations take 200 µs of the 235: the clock that the chip's power
+//   leaves them (1.9 GHz of 2.4) bounds it.
 #define FK_MX4_STAGES 4
 #define FK_MX4_LDS __attribute__((address_space(3)))
 constexpr uint32_t mx4_many_side = 16;  // row tiles of a tile's side
@@ -200,7 +201,9 @@ __device__ __forceinline__ fk_float16v mx4_mfma32(u32x4 b, uint32_t bs, u32x4 a,
 // A wavefront's 32 GM rows of 32 GN columns into C, through its own share of
 // an LDS stage: of 32 rows at a time RB bytes each are written as the
 // operation left them, a lane 4 columns of a row, and read back a row's
-// consecutive 16 bytes a lane, so that stores are RB whole bytes of a row.
+// consecutive 16 bytes a lane, so that stores are RB whole bytes of a row (of the
+// many, past the caches: 8192 x 8192, operands from memory, k 2048 97 µs, so 85;
+// k 8192 264 and 258).
 template <uint32_t GM, uint32_t GN, bool AGPR, int T>
 __device__ __forceinline__ void mx4_store_many(const fk_mx4_gemm_args &a, uint32_t m0, uint32_t n0,
                                                fk_float16v (&acc)[GM][GN], char *stage) {
@@ -247,7 +250,8 @@ __device__ __forceinline__ void mx4_store_many(const fk_mx4_gemm_args &a, uint32
         const uint64_t at = a.c + ((uint64_t)m * a.c_stride + n) * BYTES;
         if (m < a.m && n < a.n) {
           if (n + EACH <= a.n) {
-            *global_at<mx4_u32x4>(at) = w;
+            if constexpr (AGPR) __builtin_nontemporal_store(w, global_at<mx4_u32x4>(at));
+            else *global_at<mx4_u32x4>(at) = w;
           } else {
 #pragma unroll
             for (uint32_t e = 0; e < EACH - 1; e++)

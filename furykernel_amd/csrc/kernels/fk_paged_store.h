@@ -5,8 +5,11 @@
 // Elementwise, so the rows' read and the caches' write bound it.  A thread
 // takes 8 elements of a head's first half and the 8 they are paired with:
 // 16-byte loads and stores, and each pair's cosine and sine once for both.
-// 8191 tokens of 32 and 8 heads of 128 in bf16 take 32.5 µs (203 MB, 6.2 TB/s),
-// 8 tokens 2.8: the launch and three loads, one behind another.
+// Rows of 16 bits and the caches' elements pass the caches by: 8191 tokens of 32
+// and 8 heads of 128 in bf16, out of memory each time, took 41.7 µs, so 35.9
+// (203 MB, 5.7 TB/s); f32 rows, two loads a line, lose by it (4096 tokens of
+// heads of 64 16.4 µs, 17.5).  8 tokens take 2.8: the launch and three loads,
+// one behind another.
 #pragma once
 
 #include "fk_address.h"
@@ -32,11 +35,11 @@ __device__ __forceinline__ void load8(uint64_t rows, uint64_t at, float (&x)[8])
 #pragma unroll
     for (int i = 0; i < 4; i++) x[i] = a[i], x[4 + i] = b[i];
   } else if constexpr (T == FK_T_F16) {
-    const store_half8 h = *global_at<const store_half8>(rows + 2 * at);
+    const store_half8 h = load_from<true, store_half8>(global_at<const store_half8>(rows + 2 * at));
 #pragma unroll
     for (int i = 0; i < 8; i++) x[i] = (float)h[i];
   } else {
-    const u32x4 w = *global_at<const u32x4>(rows + 2 * at);
+    const u32x4 w = load_from<true, u32x4>(global_at<const u32x4>(rows + 2 * at));
 #pragma unroll
     for (int i = 0; i < 4; i++) {
       x[2 * i] = __uint_as_float(w[i] << 16);
@@ -52,12 +55,12 @@ __device__ __forceinline__ void store8(uint64_t to, const float (&x)[8]) {
     store_bf16x8 h;
 #pragma unroll
     for (int i = 0; i < 8; i++) h[i] = (__bf16)x[i];
-    *global_at<store_bf16x8>(to) = h;
+    __builtin_nontemporal_store(h, global_at<store_bf16x8>(to));
   } else {
     store_half8 h;
 #pragma unroll
     for (int i = 0; i < 8; i++) h[i] = (_Float16)x[i];
-    *global_at<store_half8>(to) = h;
+    __builtin_nontemporal_store(h, global_at<store_half8>(to));
   }
 }
 

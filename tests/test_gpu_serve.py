@@ -90,8 +90,9 @@ def hold_plan(device, mem, x):
 
 @pytest.mark.parametrize("n,longest,chunk,block,spare", [
     (1, 0, 1, 16, 0), (1, 0, 1, 1, 3), (1, 5000, 3000, 16, 100), (2, 31, 33, 16, 0), (63, 40, 9, 7, 5),
-    (256, 300, 1, 16, 0), (257, 60, 4, 5, 3), (512, 60, 4, 5, 0), (513, 60, 4, 11, 9), (1000, 100, 40, 24, 17), (1023, 9, 3, 1, 0), (1024, 50, 20, 8, 1), (1025, 50, 20, 128, 2),
-    (2048, 40, 5, 3, 0), (2049, 40, 5, 3, 70), (1500, 700, 80, 16, 777), (3001, 30, 7, 16, 999), (20000, 20, 12, 16, 50)])
+    (256, 300, 1, 16, 0), (257, 60, 4, 5, 3), (512, 60, 4, 5, 0), (513, 60, 4, 11, 9),
+    (1000, 100, 40, 24, 17), (1023, 9, 3, 1, 0), (1024, 50, 20, 8, 1), (1025, 50, 20, 128, 2), (2048, 40, 5, 3, 0),
+    (2049, 40, 5, 3, 70), (1500, 700, 80, 16, 777), (3001, 30, 7, 16, 999), (20000, 20, 12, 16, 50)])
 def test_plan_is_its_definition(device, mem, n, longest, chunk, block, spare):
     print(f"plan {n} {longest} {chunk} {block} {spare}", flush=True)
     x = plan_case(n + block, n, longest, chunk, block, -(-(longest + chunk) // block) + 1, spare)
