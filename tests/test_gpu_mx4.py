@@ -164,8 +164,8 @@ SHAPES = [(1, 1, 1), (1, 16, 32), (2, 17, 300), (3, 100, 128), (8, 8192, 2048), 
           (17, 33, 64), (31, 130, 1000), (33, 64, 512), (64, 512, 256), (65, 257, 513), (100, 1001, 3080),
           (128, 512, 96), (129, 384, 2048), (200, 100, 5000), (255, 300, 1536), (256, 256, 128), (257, 513, 640),
           (300, 1030, 2304), (512, 768, 4096), (1000, 40, 130), (1030, 2050, 300), (250, 2040, 2048),
-          (500, 2030, 1900), (200, 8192, 2048), (201, 8191, 2049), (30, 16380, 2040), (27, 16001, 700), (500, 8190, 2048), (4000, 2050, 1900),
-          (5000, 8192, 3080), (4097, 8111, 2500), (4090, 4090, 8190)]
+          (500, 2030, 1900), (200, 8192, 2048), (201, 8191, 2049), (30, 16380, 2040), (27, 16001, 700),
+          (500, 8190, 2048), (4000, 2050, 1900), (5000, 8192, 3080), (4097, 8111, 2500), (4090, 4090, 8190)]
 
 
 def test_the_products_shapes_reach_every_form():
