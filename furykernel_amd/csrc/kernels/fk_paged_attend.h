@@ -42,11 +42,14 @@
 // transposing reads.  The probabilities go in as two 16-bit parts, p cut off
 // and what that leaves, which keeps 16 bits of them in bf16 and 21 in f16: the
 // operation has matrix cycles to spare and the result nearly the precision of
-// binary32 products.  Both parts of a p above 0 are above 0 (the second is
-// taken from p (1 + 2^-20), which the sum counts too), so that a value of
-// infinity gives infinity and not the difference of two.  A reference 15
-// below the running maximum keeps f16's smallest step at 2^-39 of the largest
-// probability.
+// binary32 products.  A reference 15 below the running maximum keeps f16's
+// smallest step at 2^-39 of the largest probability.
+//
+// A part of 0 times a value of infinity is no number, where the probability
+// itself would give infinity.  A wavefront whose tiles gave such a sum makes
+// them again with the parts that are 0 at the type's smallest step, those of
+// keys of a score of -infinity excepted: infinite values then give infinity,
+// whatever their keys' weights, and rows whose sums are finite never come here.
 #pragma once
 
 #include "fk_address.h"
@@ -153,6 +156,12 @@ FK_PAGED_READ8(paged_read8_tr, "ds_read_b64_tr_b16", u32x2)
 // seen no score.
 __device__ __forceinline__ float paged_ref(float m) { return m == -__builtin_inff() ? 0.0f : m; }
 
+// A state's value times its factor, onto another: one that infinite values made
+// stays so where the factor is too small for a binary32.
+__device__ __forceinline__ float paged_plus(float sum, float o, float f) {
+  return sum + (__builtin_isinf(o) ? o : o * f);
+}
+
 // Eight 16-bit operands of a matrix operation.
 template <bool BF16>
 struct PagedOperand;
@@ -160,6 +169,7 @@ template <>
 struct PagedOperand<false> {
   typedef _Float16 elem;
   typedef fk_half8 vec;
+  static constexpr uint32_t tiny = 1;  // 2^-24, where a reference's probability is 2^15
   static __device__ __forceinline__ fk_float4v mfma(vec a, vec b, fk_float4v c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
   }
@@ -176,6 +186,7 @@ template <>
 struct PagedOperand<true> {
   typedef __bf16 elem;
   typedef fk_paged_bf16x8 vec;
+  static constexpr uint32_t tiny = 27 << 7;  // 2^-100
   static __device__ __forceinline__ fk_float4v mfma(vec a, vec b, fk_float4v c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
   }
@@ -358,10 +369,13 @@ __device__ __forceinline__ void paged_attend(const fk_paged_attend_args &a, cons
       // there already, landed with Q: no tile without a load of them waits for
       // one.
       uint32_t entry0 = 0;
-      if (!pl.whole || a.table_len > FK_WAVE) {
-        entry0 = min(max(t0 * KT, ks.first) / a.block_size, last_entry);
-        entries = row[min(entry0 + lane, last_entry)];
-      }
+      auto first_entries = [&] {
+        if (!pl.whole || a.table_len > FK_WAVE) {
+          entry0 = min(max(t0 * KT, ks.first) / a.block_size, last_entry);
+          entries = row[min(entry0 + lane, last_entry)];
+        }
+      };
+      first_entries();
       __builtin_amdgcn_s_waitcnt(FK_PAGED_VMCNT(0));
       asm volatile("" : "+v"(entries));
 #pragma unroll
@@ -405,117 +419,155 @@ __device__ __forceinline__ void paged_attend(const fk_paged_attend_args &a, cons
       };
 
       fk_float4v o[DP / 16];
+      float m, l;
+      // The wavefront's tiles; whether a sum of a row that has weights is not a
+      // number (a second making of its own: a branch in each tile and 30 registers
+      // more took 41 requests of up to 700 keys 9.6 µs, so 9.25; 8.95 without).
+      auto make = [&](auto once_more) __attribute__((always_inline)) {
+        constexpr bool again = decltype(once_more)::value;
 #pragma unroll
-      for (uint32_t d = 0; d < DP / 16; d++) o[d] = fk_float4v{0.0f, 0.0f, 0.0f, 0.0f};
-      float m = -__builtin_inff(), l = 0.0f;
-
-      if (t0 < t1) {
-        rows_of(t0);
-        load(kpool, kbuf, true);
-        load(vpool, vbuf, false);
-      }
-      for (uint32_t t = t0; t < t1; t++) {
-        const bool more = t + 1 < t1;
-        __builtin_amdgcn_s_waitcnt(FK_PAGED_VMCNT(LOADS));  // K landed, V's loads in flight
-        asm volatile("" ::: "memory");
-        // S: groups of 16 keys; register i of group s is key 16 s + 4 (l div 16)
-        // + i of the tile, head l mod 16.
-        fk_float4v sc[KT / 16];
-#pragma unroll
-        for (uint32_t s = 0; s < KT / 16; s++) sc[s] = fk_float4v{0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-        for (uint32_t c = 0; c < KT * DP / 4096; c++) {
-          // of 4 addresses and STEP rows further: at 64, pieces h of groups s and
-          // s + 1 (and s + 2); else four pieces of a group (and the next)
-          constexpr uint32_t HS = DP == 64 ? 2 : 4, ROWS = DP == 64 ? 32 : 16;
-          uint32_t at[4];
-          u32x4 w[8];
-#pragma unroll
-          for (uint32_t i = 0; i < 4; i++)
-            at[i] = k_lds + (lane % 16 + i / HS * 16) * (2 * DP) + ((4 * (c * HS + i % HS) + lane / 16) ^ k_turn) * 16;
-          paged_read8<ROWS * 2 * DP>(at, w);
-#pragma unroll
-          for (uint32_t i = 0; i < 8; i++) {
-            const uint32_t s = i % 4 / HS + i / 4 * (ROWS / 16), h = c * HS + i % HS;
-            sc[s] = Op::mfma(__builtin_bit_cast(vec, w[i]), qf[h], sc[s]);
-          }
-        }
-        // The reads are done before the next tile's loads land on them.
-#pragma unroll
-        for (uint32_t s = 0; s < KT / 16; s++) asm volatile("" : "+v"(sc[s])::"memory");
-        if (more) {
-          rows_of(t + 1);
+        for (uint32_t d = 0; d < DP / 16; d++) o[d] = fk_float4v{0.0f, 0.0f, 0.0f, 0.0f};
+        m = -__builtin_inff(), l = 0.0f;
+        if (t0 < t1) {
+          rows_of(t0);
           load(kpool, kbuf, true);
+          load(vpool, vbuf, false);
         }
-        float mt = -__builtin_inff();
-#pragma unroll
-        for (uint32_t s = 0; s < KT / 16; s++)
-#pragma unroll
-          for (int i = 0; i < 4; i++) {
-            const uint32_t k = t * KT + 16 * s + 4 * (lane / 16) + i;
-            sc[s][i] = k < ks.last && k >= ks.first ? sc[s][i] * c : -__builtin_inff();
-            mt = __builtin_fmaxf(mt, sc[s][i]);
-          }
-        const float mn = __builtin_fmaxf(m, paged_max(mt) - 15.0f);
-        const float mc = paged_ref(mn);
-        const float alpha = __builtin_amdgcn_exp2f(m - mc);
-        m = mn;
-        vec ph[KT / 32], pr[KT / 32];
-        float sum = 0.0f;
-#pragma unroll
-        for (uint32_t s = 0; s < KT / 16; s++)
-#pragma unroll
-          for (int i = 0; i < 4; i += 2) {
-            const float p0 = __builtin_amdgcn_exp2f(sc[s][i] - mc), p1 = __builtin_amdgcn_exp2f(sc[s][i + 1] - mc);
-            const float w0 = p0 * 1.00000095367431640625f, w1 = p1 * 1.00000095367431640625f;
-            sum += w0 + w1;
-            float c0, c1;
-            Op::cut(p0, p1, ph[s / 2], s % 2 * 4 + i, &c0, &c1);
-            pr[s / 2][s % 2 * 4 + i] = (elem)(w0 - c0);
-            pr[s / 2][s % 2 * 4 + i + 1] = (elem)(w1 - c1);
-          }
-        l = l * alpha + paged_sum(sum);
-#pragma unroll
-        for (uint32_t d = 0; d < DP / 16; d++) o[d] *= alpha;
-        if (more) __builtin_amdgcn_s_waitcnt(FK_PAGED_VMCNT(LOADS));  // V landed, the next K in flight
-        else __builtin_amdgcn_s_waitcnt(FK_PAGED_VMCNT(0));
-        asm volatile("" ::: "memory");
-        if (t * KT < ks.first || t * KT + KT > ks.last) {
-          // Rows outside the request's keys hold other values: zeros, so that
-          // an infinity there is nothing to a probability of 0.
-#pragma unroll
-          for (uint32_t q = 0; q < LOADS; q++) {
-            const uint32_t k = t * KT + q * KPL + krow;
-            if (k < ks.first || k >= ks.last)
-              reinterpret_cast<uint4 *>(vbuf)[q * 64 + lane] = make_uint4(0, 0, 0, 0);
-          }
+        for (uint32_t t = t0; t < t1; t++) {
+          const bool more = t + 1 < t1;
+          __builtin_amdgcn_s_waitcnt(FK_PAGED_VMCNT(LOADS));  // K landed, V's loads in flight
           asm volatile("" ::: "memory");
-        }
-        // Oᵀ += Vᵀ Pᵀ.  Transposed reads: within 16 lanes, lane 4 k + q reads key
-        // K0 + k, d D0 + 4 q .. + 3 and receives keys K0 .. K0 + 3 of d D0 + (its
-        // index): keys 32 h + 4 (l div 16) .. + 3 and 16 further, ph[h]'s order.
+          // S: groups of 16 keys; register i of group s is key 16 s + 4 (l div 16)
+          // + i of the tile, head l mod 16.
+          fk_float4v sc[KT / 16];
 #pragma unroll
-        for (uint32_t c = 0; c < KT * DP / 2048; c++) {
-          // of 4 addresses and 16 rows further: at 64, two 16s of d by two 32s of
-          // keys; else four 16s of d
-          constexpr uint32_t DS = DP == 64 ? 2 : 4;
-          uint32_t at[4];
-          u32x2 w[8];
+          for (uint32_t s = 0; s < KT / 16; s++) sc[s] = fk_float4v{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-          for (uint32_t i = 0; i < 4; i++)
-            at[i] = v_lds + (tk + i / DS * 32) * (2 * DP) + ((16 * (c * DS + i % DS) + td) ^ (v_turn << 4)) * 2;
-          paged_read8_tr<16 * 2 * DP>(at, w);
+          for (uint32_t c = 0; c < KT * DP / 4096; c++) {
+            // of 4 addresses and STEP rows further: at 64, pieces h of groups s and
+            // s + 1 (and s + 2); else four pieces of a group (and the next)
+            constexpr uint32_t HS = DP == 64 ? 2 : 4, ROWS = DP == 64 ? 32 : 16;
+            uint32_t at[4];
+            u32x4 w[8];
 #pragma unroll
-          for (uint32_t i = 0; i < 4; i++) {
-            const uint32_t d = c * DS + i % DS, h = i / DS;
-            const vec vf = __builtin_bit_cast(vec, u32x4{w[i][0], w[i][1], w[4 + i][0], w[4 + i][1]});
-            o[d] = Op::mfma(vf, ph[h], o[d]);
-            o[d] = Op::mfma(vf, pr[h], o[d]);
+            for (uint32_t i = 0; i < 4; i++)
+              at[i] = k_lds + (lane % 16 + i / HS * 16) * (2 * DP) +
+                      ((4 * (c * HS + i % HS) + lane / 16) ^ k_turn) * 16;
+            paged_read8<ROWS * 2 * DP>(at, w);
+#pragma unroll
+            for (uint32_t i = 0; i < 8; i++) {
+              const uint32_t s = i % 4 / HS + i / 4 * (ROWS / 16), h = c * HS + i % HS;
+              sc[s] = Op::mfma(__builtin_bit_cast(vec, w[i]), qf[h], sc[s]);
+            }
           }
-        }
+          // The reads are done before the next tile's loads land on them.
 #pragma unroll
-        for (uint32_t d = 0; d < DP / 16; d++) asm volatile("" : "+v"(o[d])::"memory");
-        if (more) load(vpool, vbuf, false);
+          for (uint32_t s = 0; s < KT / 16; s++) asm volatile("" : "+v"(sc[s])::"memory");
+          if (more) {
+            rows_of(t + 1);
+            load(kpool, kbuf, true);
+          }
+          float mt = -__builtin_inff();
+#pragma unroll
+          for (uint32_t s = 0; s < KT / 16; s++)
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+              const uint32_t k = t * KT + 16 * s + 4 * (lane / 16) + i;
+              sc[s][i] = k < ks.last && k >= ks.first ? sc[s][i] * c : -__builtin_inff();
+              mt = __builtin_fmaxf(mt, sc[s][i]);
+            }
+          const float mn = __builtin_fmaxf(m, paged_max(mt) - 15.0f);
+          const float mc = paged_ref(mn);
+          float alpha = __builtin_amdgcn_exp2f(m - mc);
+          if (again) alpha = __builtin_fmaxf(alpha, 0x1p-126f);
+          m = mn;
+          vec ph[KT / 32], pr[KT / 32];
+          float sum = 0.0f;
+#pragma unroll
+          for (uint32_t s = 0; s < KT / 16; s++)
+#pragma unroll
+            for (int i = 0; i < 4; i += 2) {
+              const float p0 = __builtin_amdgcn_exp2f(sc[s][i] - mc), p1 = __builtin_amdgcn_exp2f(sc[s][i + 1] - mc);
+              sum += p0 + p1;
+              float c0, c1;
+              Op::cut(p0, p1, ph[s / 2], s % 2 * 4 + i, &c0, &c1);
+              pr[s / 2][s % 2 * 4 + i] = (elem)(p0 - c0);
+              pr[s / 2][s % 2 * 4 + i + 1] = (elem)(p1 - c1);
+            }
+          if (again) {
+#pragma unroll
+            for (uint32_t h = 0; h < KT / 32; h++) {
+              u32x4 parts[2] = {__builtin_bit_cast(u32x4, ph[h]), __builtin_bit_cast(u32x4, pr[h])};
+#pragma unroll
+              for (uint32_t i = 0; i < 8; i++)
+#pragma unroll
+                for (uint32_t x = 0; x < 2; x++) {
+                  const uint32_t at = 16 * (i % 2);
+                  if (sc[2 * h + i / 4][i % 4] > -__builtin_inff() && (parts[x][i / 2] >> at & 0xFFFFu) == 0)
+                    parts[x][i / 2] |= Op::tiny << at;
+                }
+              ph[h] = __builtin_bit_cast(vec, parts[0]);
+              pr[h] = __builtin_bit_cast(vec, parts[1]);
+            }
+          }
+          l = l * alpha + paged_sum(sum);
+#pragma unroll
+          for (uint32_t d = 0; d < DP / 16; d++) o[d] *= alpha;
+          if (more) __builtin_amdgcn_s_waitcnt(FK_PAGED_VMCNT(LOADS));  // V landed, the next K in flight
+          else __builtin_amdgcn_s_waitcnt(FK_PAGED_VMCNT(0));
+          asm volatile("" ::: "memory");
+          if (t * KT < ks.first || t * KT + KT > ks.last) {
+            // Rows outside the request's keys hold other values: zeros, so that
+            // an infinity there is nothing to a probability of 0.
+#pragma unroll
+            for (uint32_t q = 0; q < LOADS; q++) {
+              const uint32_t k = t * KT + q * KPL + krow;
+              if (k < ks.first || k >= ks.last)
+                reinterpret_cast<uint4 *>(vbuf)[q * 64 + lane] = make_uint4(0, 0, 0, 0);
+            }
+            asm volatile("" ::: "memory");
+          }
+          // Oᵀ += Vᵀ Pᵀ.  Transposed reads: within 16 lanes, lane 4 k + q reads key
+          // K0 + k, d D0 + 4 q .. + 3 and receives keys K0 .. K0 + 3 of d D0 + (its
+          // index): keys 32 h + 4 (l div 16) .. + 3 and 16 further, ph[h]'s order.
+#pragma unroll
+          for (uint32_t c = 0; c < KT * DP / 2048; c++) {
+            // of 4 addresses and 16 rows further: at 64, two 16s of d by two 32s of
+            // keys; else four 16s of d
+            constexpr uint32_t DS = DP == 64 ? 2 : 4;
+            uint32_t at[4];
+            u32x2 w[8];
+#pragma unroll
+            for (uint32_t i = 0; i < 4; i++)
+              at[i] = v_lds + (tk + i / DS * 32) * (2 * DP) + ((16 * (c * DS + i % DS) + td) ^ (v_turn << 4)) * 2;
+            paged_read8_tr<16 * 2 * DP>(at, w);
+#pragma unroll
+            for (uint32_t i = 0; i < 4; i++) {
+              const uint32_t d = c * DS + i % DS, h = i / DS;
+              const vec vf = __builtin_bit_cast(vec, u32x4{w[i][0], w[i][1], w[4 + i][0], w[4 + i][1]});
+              o[d] = Op::mfma(vf, ph[h], o[d]);
+              o[d] = Op::mfma(vf, pr[h], o[d]);
+            }
+          }
+#pragma unroll
+          for (uint32_t d = 0; d < DP / 16; d++) asm volatile("" : "+v"(o[d])::"memory");
+          if (more) load(vpool, vbuf, false);
+        }
+        if (again) return false;
+        // (not a number where one of the head's own d is not)
+        fk_float4v any = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (uint32_t d = 0; d < DP / 16; d++)
+          if (FULL || 16 * d + 4 * (lane / 16) < D) any += o[d];
+        const float sum = (any[0] + any[1]) + (any[2] + any[3]);
+        return __builtin_amdgcn_ballot_w64(sum != sum && l == l) != 0;
+      };
+      if (make(fk_bool_tag<false>{})) {
+        first_entries();
+        __builtin_amdgcn_s_waitcnt(FK_PAGED_VMCNT(0));
+        asm volatile("" : "+v"(entries));
+        entries = min(entries, a.blocks - 1);
+        make(fk_bool_tag<true>{});
       }
 
       // The wavefronts' states meet, each in the place of its V rows: head l
@@ -545,7 +597,7 @@ __device__ __forceinline__ void paged_attend(const fk_paged_attend_args &a, cons
         for (uint32_t w = 0; w < W; w++) {
           const float f = __builtin_amdgcn_exp2f(sm[w][q] - mc);
           ll += sl[w][q] * f;
-          oo += reinterpret_cast<const float *>(kv[w][1])[q * DP + d] * f;
+          oo = paged_plus(oo, reinterpret_cast<const float *>(kv[w][1])[q * DP + d], f);
         }
         if (whole) {
           const uint64_t where = r * a.out_stride + (uint64_t)(h0 + q) * D + d;
@@ -616,13 +668,13 @@ __device__ __forceinline__ void paged_attend_join(const fk_paged_attend_args &a,
     const float f0 = __builtin_amdgcn_exp2f(mm - mc);
     ll *= f0;
 #pragma unroll
-    for (uint32_t i = 0; i < 4; i++) oo[i] *= f0;
+    for (uint32_t i = 0; i < 4; i++) oo[i] = paged_plus(0.0f, oo[i], f0);
 #pragma unroll
     for (uint32_t s = 0; s < U; s++) {
       const float f = __builtin_amdgcn_exp2f(m[s] - mc);
       ll += l[s] * f;
 #pragma unroll
-      for (uint32_t i = 0; i < 4; i++) oo[i] += o[s][i] * f;
+      for (uint32_t i = 0; i < 4; i++) oo[i] = paged_plus(oo[i], o[s][i], f);
     }
     mm = mn;
   }
@@ -646,7 +698,7 @@ __device__ __forceinline__ void paged_attend_join(const fk_paged_attend_args &a,
   for (uint32_t d = threadIdx.x; d < D; d += 64 * W) {
     float o = 0.0f;
 #pragma unroll
-    for (uint32_t w = 0; w < W; w++) o += so[w][d] * f[w];
+    for (uint32_t w = 0; w < W; w++) o = paged_plus(o, so[w][d], f[w]);
     const uint64_t where = j[1] * a.out_stride + (uint64_t)((j[2] >> 4) + q) * D + d;
     if (a.out_f32) global_at<float>(a.out)[where] = o / l;
     else global_at<uint16_t>(a.out)[where] = paged_round<BF16>(o / l);

@@ -115,7 +115,8 @@ int fk_paged_store(fk_ctx *ctx, const fk_paged_store_args *args, fk_stream *stre
  * Scores, the running maximum, the sums and the weighted values are binary32
  * (probabilities go to the matrix cores as two 16-bit parts, 16 bits and more
  * of each), rounded once on the way out.  The same lengths give the same
- * bits, whatever else the pool holds. */
+ * bits, whatever else the pool holds.  An infinite value gives infinity
+ * whatever its key's finite score. */
 typedef struct fk_paged_attend_args {
   uint64_t q;         /* rows of [heads][head_dim], the caches' type: a request's each, or with starts q_rows */
   uint64_t kpool, vpool;

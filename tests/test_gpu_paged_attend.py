@@ -1,0 +1,99 @@
+"""The paged attention (include/fkrocm_serve.h: fk_paged_attend) on the GPU
+where its values leave the ordinary: infinities of unlikely keys."""
+
+import numpy as np
+import pytest
+
+import serve_cases as S
+from test_gpu_serve import attend_inputs, bind_attend, mem  # noqa: F401  (mem is a fixture)
+
+pytestmark = pytest.mark.gpu
+
+
+def position(x, r, p):
+    """Where the pools hold position p of request r: (block, place in it)."""
+    return x["table"][r, p // x["block"]], p % x["block"]
+
+
+# Request 0's keys of chosen scores, below one of 0 by as much; past 87 a
+# weight is no normal binary32, past 103 none at all.
+BELOW = [0.0, 5.0, 13.5, 14.25, 17.5, 20.0, 27.0, 40.0, 60.0, 86.0, 95.0, 120.0]
+
+
+@pytest.mark.parametrize("cache", ["f16", "bf16"])
+@pytest.mark.parametrize("d,lengths,table_len", [(64, [90, 40], 6), (128, [90, 40], 6), (256, [30, 17], 4),
+                                                 (80, [90, 40], 6), (64, [5000, 300], 320), (128, [5000, 9], 320),
+                                                 (256, [3000, 5], 200), (200, [3000, 64], 200)])
+def test_infinite_values_of_unlikely_keys(device, mem, d, lengths, table_len, cache):
+    """An infinite value gives infinity whatever its key's weight: any finite
+    score's is above 0.  A key of score -infinity has a weight of 0, and 0
+    times infinity is no number; both infinities in one element are none
+    either.  Elsewhere the finite values' attention, within its bound."""
+    print(f"attend infinities {d} {lengths} {cache}", flush=True)
+    bf16 = cache == "bf16"
+    rng = np.random.default_rng(d + len(lengths))
+    x = attend_inputs(rng, lengths, 2, 1, d, 16, cache, table_len=table_len)
+    top = lengths[0]
+    # scores from element 0 alone: -64 of every key but the chosen, which
+    # lie over the whole length
+    at = np.linspace(0, top - 1, len(BELOW)).round().astype(int)[::-1]
+    lost = next(p for p in range(top // 2, top) if p not in at)
+    assert len(set(at)) == len(BELOW)
+    x["q"][0] = S.narrow(np.zeros((2, d)), bf16)
+    x["q"][0, :, 0] = S.narrow(np.ones(2), bf16)
+    for p in range(top):
+        b, i = position(x, 0, p)
+        x["k"][b, 0, i, 0] = S.narrow([-64.0], bf16)[0]
+    inf = 0x7F80 if bf16 else 0x7C00
+    for j, (p, below) in enumerate(zip(at, BELOW)):
+        b, i = position(x, 0, p)
+        x["k"][b, 0, i, 0] = S.narrow([-below], bf16)[0]
+        x["v"][b, 0, i, 2 * j] = inf | (0x8000 if j % 3 == 0 else 0)
+    both, none, nought = 30, 31, 33
+    for p, column, bits in ((at[2], both, inf), (at[7], both, inf | 0x8000), (at[9], none, inf + 1), (lost, nought, inf)):
+        b, i = position(x, 0, p)
+        x["v"][b, 0, i, column] = bits
+    b, i = position(x, 0, lost)
+    x["k"][b, 0, i, 0] = inf | 0x8000
+    op, read, _ = bind_attend(device, mem, x, 1.0, out_type="f32")
+    op.enqueue()
+    device.sync()
+    got = read()
+    columns = 2 * np.arange(len(BELOW))
+    want = np.where(np.arange(len(BELOW)) % 3 == 0, -np.inf, np.inf)
+    assert np.array_equal(got[0][:, columns], np.broadcast_to(want, (2, len(BELOW)))), got[0][:, columns]
+    assert np.isnan(got[0][:, [both, none, nought]]).all()
+    rest = np.setdiff1d(np.arange(d), np.concatenate([columns, [both, none, nought]]))
+    wide = {i: S.widen(x[i], bf16) for i in ("q", "k", "v")}
+    b, i = position(x, 0, lost)
+    wide["k"][b, 0, i, 0] = -1e5               # (the oracle's weight: 0 all the same)
+    with np.errstate(invalid="ignore"):
+        out, spread, reach = S.attend(*wide.values(), x["table"], x["lengths"], 16, 1.0)
+    # a key's parts that would be 0 stand at 2^-39 of the largest weight (f16),
+    # two of them
+    reach = np.minimum(reach, 130.0)
+    tol = S.attend_tolerance(out, spread, reach, x["lengths"], d, 2.0 ** -24) + top * 2.0 ** -38 * 6
+    for r in range(2):
+        cols = rest if r == 0 else np.arange(d)
+        err = np.abs(got[r][:, cols] - out[r][:, cols])
+        assert np.all(err <= tol[r][:, cols]), (r, err.max())
+
+
+def test_rows_of_infinite_scores_and_values(device, mem):
+    """A row all of whose scores are -infinity, and one with a score of
+    infinity, are no numbers, with infinite values in their keys too."""
+    x = attend_inputs(np.random.default_rng(4), [40, 40], 2, 1, 64, 16, "f16")
+    x["q"][:] = S.narrow(np.zeros((2, 2, 64)), False)
+    x["q"][:, :, 0] = S.narrow(np.ones(2), False)
+    for p in range(40):
+        b, i = position(x, 0, p)
+        x["k"][b, 0, i, 0] = 0xFC00
+    b, i = position(x, 1, 7)
+    x["k"][b, 0, i, 0] = 0x7C00
+    for r in range(2):
+        b, i = position(x, r, 20)
+        x["v"][b, 0, i, 3] = 0x7C00
+    op, read, _ = bind_attend(device, mem, x, 1.0)
+    op.enqueue()
+    device.sync()
+    assert np.isnan(read()).all()
