@@ -39,11 +39,13 @@
 //
 // Matrix operations (v_mfma_f32_16x16x32): S = K Qᵀ, then Oᵀ = Vᵀ Pᵀ with the
 // probabilities in the registers that made them, V transposed by the LDS's
-// transposing reads.  The probabilities go in as two 16-bit parts, p cut off
-// and what that leaves, which keeps 16 bits of them in bf16 and 21 in f16: the
-// operation has matrix cycles to spare and the result nearly the precision of
-// binary32 products.  A reference 15 below the running maximum keeps f16's
-// smallest step at 2^-39 of the largest probability.
+// transposing reads.  The probabilities go in as 16-bit parts, p cut off and
+// what that leaves: three in bf16, which hold all 24 bits of a binary32 (two
+// hold 16, and took as long: 64 requests of up to 16384 keys 232 µs), two in
+// f16, which hold 21, as many as a binary32 exponential keeps of scores of
+// about 10 (three: 41 requests of up to 700 keys 9.55 µs, so 9.25).  A reference
+// 15 below the running maximum keeps f16's smallest step at 2^-39 of the largest
+// probability.
 //
 // A part of 0 times a value of infinity is no number, where the probability
 // itself would give infinity.  A wavefront whose tiles gave such a sum makes
@@ -173,13 +175,14 @@ struct PagedOperand<false> {
   static __device__ __forceinline__ fk_float4v mfma(vec a, vec b, fk_float4v c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
   }
-  // p0 and p1 cut off to 16 bits, as elements i and i + 1 and as they were.
-  static __device__ __forceinline__ void cut(float p0, float p1, vec &to, int i, float *c0, float *c1) {
+  // The parts of two probabilities, a word each: cut off, and what that leaves
+  // to the nearest.
+  static constexpr uint32_t parts = 2;
+  static __device__ __forceinline__ void cut(float p0, float p1, uint32_t (&to)[parts]) {
+    typedef _Float16 half2 __attribute__((ext_vector_type(2)));
     const auto h = __builtin_amdgcn_cvt_pkrtz(p0, p1);
-    to[i] = (elem)h[0];
-    to[i + 1] = (elem)h[1];
-    *c0 = (float)h[0];
-    *c1 = (float)h[1];
+    to[0] = __builtin_bit_cast(uint32_t, h);
+    to[1] = __builtin_bit_cast(uint32_t, half2{(_Float16)(p0 - (float)h[0]), (_Float16)(p1 - (float)h[1])});
   }
 };
 template <>
@@ -190,12 +193,16 @@ struct PagedOperand<true> {
   static __device__ __forceinline__ fk_float4v mfma(vec a, vec b, fk_float4v c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
   }
-  static __device__ __forceinline__ void cut(float p0, float p1, vec &to, int i, float *c0, float *c1) {
-    const uint32_t u0 = __float_as_uint(p0) & 0xFFFF0000u, u1 = __float_as_uint(p1) & 0xFFFF0000u;
-    to[i] = __builtin_bit_cast(elem, (uint16_t)(u0 >> 16));
-    to[i + 1] = __builtin_bit_cast(elem, (uint16_t)(u1 >> 16));
-    *c0 = __uint_as_float(u0);
-    *c1 = __uint_as_float(u1);
+  // (each part eight bits: the third is all that the first two leave)
+  static constexpr uint32_t parts = 3;
+  static __device__ __forceinline__ void cut(float p0, float p1, uint32_t (&to)[parts]) {
+#pragma unroll
+    for (uint32_t x = 0; x < parts; x++) {
+      const uint32_t u0 = __float_as_uint(p0), u1 = __float_as_uint(p1);
+      to[x] = __builtin_amdgcn_perm(u1, u0, 0x07060302);  // the upper halves
+      p0 -= __uint_as_float(u0 & 0xFFFF0000u);
+      p1 -= __uint_as_float(u1 & 0xFFFF0000u);
+    }
   }
 };
 
@@ -210,7 +217,6 @@ template <uint32_t DP, uint32_t W, bool FULL, bool BF16>
 __device__ __forceinline__ void paged_attend(const fk_paged_attend_args &a, const PagedPlan &pl) {
   using Op = PagedOperand<BF16>;
   using vec = typename Op::vec;
-  using elem = typename Op::elem;
   constexpr uint32_t KT = DP == 64 ? 64 : 32;    // keys a tile: 8 KB of K at 64 and 128, 16 KB at 256
   constexpr uint32_t UNITS = DP / 8;             // 16-byte pieces of a row
   constexpr uint32_t KPL = 64 / UNITS;           // rows a load of the wavefront covers
@@ -481,7 +487,7 @@ __device__ __forceinline__ void paged_attend(const fk_paged_attend_args &a, cons
           float alpha = __builtin_amdgcn_exp2f(m - mc);
           if (again) alpha = __builtin_fmaxf(alpha, 0x1p-126f);
           m = mn;
-          vec ph[KT / 32], pr[KT / 32];
+          u32x4 parts[KT / 32][Op::parts];
           float sum = 0.0f;
 #pragma unroll
           for (uint32_t s = 0; s < KT / 16; s++)
@@ -489,26 +495,22 @@ __device__ __forceinline__ void paged_attend(const fk_paged_attend_args &a, cons
             for (int i = 0; i < 4; i += 2) {
               const float p0 = __builtin_amdgcn_exp2f(sc[s][i] - mc), p1 = __builtin_amdgcn_exp2f(sc[s][i + 1] - mc);
               sum += p0 + p1;
-              float c0, c1;
-              Op::cut(p0, p1, ph[s / 2], s % 2 * 4 + i, &c0, &c1);
-              pr[s / 2][s % 2 * 4 + i] = (elem)(p0 - c0);
-              pr[s / 2][s % 2 * 4 + i + 1] = (elem)(p1 - c1);
+              uint32_t words[Op::parts];
+              Op::cut(p0, p1, words);
+#pragma unroll
+              for (uint32_t x = 0; x < Op::parts; x++) parts[s / 2][x][s % 2 * 2 + i / 2] = words[x];
             }
           if (again) {
 #pragma unroll
-            for (uint32_t h = 0; h < KT / 32; h++) {
-              u32x4 parts[2] = {__builtin_bit_cast(u32x4, ph[h]), __builtin_bit_cast(u32x4, pr[h])};
+            for (uint32_t h = 0; h < KT / 32; h++)
 #pragma unroll
               for (uint32_t i = 0; i < 8; i++)
 #pragma unroll
-                for (uint32_t x = 0; x < 2; x++) {
+                for (uint32_t x = 0; x < Op::parts; x++) {
                   const uint32_t at = 16 * (i % 2);
-                  if (sc[2 * h + i / 4][i % 4] > -__builtin_inff() && (parts[x][i / 2] >> at & 0xFFFFu) == 0)
-                    parts[x][i / 2] |= Op::tiny << at;
+                  if (sc[2 * h + i / 4][i % 4] > -__builtin_inff() && (parts[h][x][i / 2] >> at & 0xFFFFu) == 0)
+                    parts[h][x][i / 2] |= Op::tiny << at;
                 }
-              ph[h] = __builtin_bit_cast(vec, parts[0]);
-              pr[h] = __builtin_bit_cast(vec, parts[1]);
-            }
           }
           l = l * alpha + paged_sum(sum);
 #pragma unroll
@@ -529,7 +531,7 @@ __device__ __forceinline__ void paged_attend(const fk_paged_attend_args &a, cons
           }
           // Oᵀ += Vᵀ Pᵀ.  Transposed reads: within 16 lanes, lane 4 k + q reads key
           // K0 + k, d D0 + 4 q .. + 3 and receives keys K0 .. K0 + 3 of d D0 + (its
-          // index): keys 32 h + 4 (l div 16) .. + 3 and 16 further, ph[h]'s order.
+          // index): keys 32 h + 4 (l div 16) .. + 3 and 16 further, parts[h]'s order.
 #pragma unroll
           for (uint32_t c = 0; c < KT * DP / 2048; c++) {
             // of 4 addresses and 16 rows further: at 64, two 16s of d by two 32s of
@@ -545,8 +547,9 @@ __device__ __forceinline__ void paged_attend(const fk_paged_attend_args &a, cons
             for (uint32_t i = 0; i < 4; i++) {
               const uint32_t d = c * DS + i % DS, h = i / DS;
               const vec vf = __builtin_bit_cast(vec, u32x4{w[i][0], w[i][1], w[4 + i][0], w[4 + i][1]});
-              o[d] = Op::mfma(vf, ph[h], o[d]);
-              o[d] = Op::mfma(vf, pr[h], o[d]);
+#pragma unroll
+              for (uint32_t x = 0; x < Op::parts; x++)
+                o[d] = Op::mfma(vf, __builtin_bit_cast(vec, parts[h][x]), o[d]);
             }
           }
 #pragma unroll

@@ -113,10 +113,10 @@ int fk_paged_store(fk_ctx *ctx, const fk_paged_store_args *args, fk_stream *stre
  * the pool's last block; what entries behind a length hold does not matter.
  *
  * Scores, the running maximum, the sums and the weighted values are binary32
- * (probabilities go to the matrix cores as two 16-bit parts, 16 bits and more
- * of each), rounded once on the way out.  The same lengths give the same
- * bits, whatever else the pool holds.  An infinite value gives infinity
- * whatever its key's finite score. */
+ * (probabilities go to the matrix cores as 16-bit parts, which hold 24 bits of
+ * them with bf16 caches, 21 with f16 ones), rounded once on the way out.  The
+ * same lengths give the same bits, whatever else the pool holds.  An infinite
+ * value gives infinity whatever its key's finite score. */
 typedef struct fk_paged_attend_args {
   uint64_t q;         /* rows of [heads][head_dim], the caches' type: a request's each, or with starts q_rows */
   uint64_t kpool, vpool;

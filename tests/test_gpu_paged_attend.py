@@ -1,5 +1,6 @@
 """The paged attention (include/fkrocm_serve.h: fk_paged_attend) on the GPU
-where its values leave the ordinary: infinities of unlikely keys."""
+at the edges of its numbers: the bits its probabilities keep, infinities of
+unlikely keys."""
 
 import numpy as np
 import pytest
@@ -13,6 +14,36 @@ pytestmark = pytest.mark.gpu
 def position(x, r, p):
     """Where the pools hold position p of request r: (block, place in it)."""
     return x["table"][r, p // x["block"]], p % x["block"]
+
+
+@pytest.mark.parametrize("d", [64, 128, 256])
+@pytest.mark.parametrize("cache", ["f16", "bf16"])
+def test_probabilities_keep_their_bits(device, mem, d, cache):
+    """Two keys, of score 0 and value 0 and of score x in -2 .. 0 and value v,
+    both exact: out = v p / (1 + p), p = e^x, in f32.  Roundings of 2^-24: the
+    scale to log2 units 2 and the score 1 (of |x| at most: 6 together), the
+    reference's subtraction from at most 16 log2 units 6 (half of 2^-20, times ln 2),
+    the exponential 1 ulp (2); p's parts exact (bf16) or off by 2^-11 of the
+    2^-10 of p that the first leaves (f16: 8); their sum 3, the sum 1 + p 1, the
+    quotient 1, the result 1."""
+    print(f"attend bits {d} {cache}", flush=True)
+    bf16, n, heads = cache == "bf16", 300, 16
+    rng = np.random.default_rng(d)
+    x = attend_inputs(rng, [2] * n, heads, 1, d, 16, cache)
+    x["q"][:] = 0
+    x["q"][:, np.arange(heads), np.arange(heads)] = S.narrow(np.ones(heads), bf16)
+    score, value = S.narrow(-2 * rng.random((n, d)), bf16), S.narrow(1 + rng.random((n, d)), bf16)
+    for r in range(n):
+        b = x["table"][r, 0]
+        x["k"][b, 0, 0], x["v"][b, 0, 0] = 0, 0
+        x["k"][b, 0, 1], x["v"][b, 0, 1] = score[r], value[r]
+    op, read, _ = bind_attend(device, mem, x, 1.0, out_type="f32")
+    op.enqueue()
+    device.sync()
+    p = np.exp(S.widen(score, bf16)[:, :heads, None])
+    want = S.widen(value, bf16)[:, None] * p / (1 + p)
+    err = np.abs(read() / want - 1).max()
+    assert err <= (20 if bf16 else 28) * 2.0 ** -24, np.log2(err)
 
 
 # Request 0's keys of chosen scores, below one of 0 by as much; past 87 a
@@ -70,9 +101,9 @@ def test_infinite_values_of_unlikely_keys(device, mem, d, lengths, table_len, ca
     with np.errstate(invalid="ignore"):
         out, spread, reach = S.attend(*wide.values(), x["table"], x["lengths"], 16, 1.0)
     # a key's parts that would be 0 stand at 2^-39 of the largest weight (f16),
-    # two of them
+    # two of them, of values below 5
     reach = np.minimum(reach, 130.0)
-    tol = S.attend_tolerance(out, spread, reach, x["lengths"], d, 2.0 ** -24) + top * 2.0 ** -38 * 6
+    tol = S.attend_tolerance(out, spread, reach, x["lengths"], d, 2.0 ** -24) + top * 2 * 2.0 ** -39 * 5
     for r in range(2):
         cols = rest if r == 0 else np.arange(d)
         err = np.abs(got[r][:, cols] - out[r][:, cols])
