@@ -43,9 +43,9 @@
 // what that leaves: three in bf16, which hold all 24 bits of a binary32 (two
 // hold 16, and took as long: 64 requests of up to 16384 keys 232 µs), two in
 // f16, which hold 21, as many as a binary32 exponential keeps of scores of
-// about 10 (three: 41 requests of up to 700 keys 9.55 µs, so 9.25).  A reference
-// 15 below the running maximum keeps f16's smallest step at 2^-39 of the largest
-// probability.
+// about 10 (three: 41 requests of up to 700 keys 9.55 µs, so 9.25).  In f16 a
+// reference 15 below the running maximum keeps the smallest step at 2^-39 of the
+// largest probability.
 //
 // A part of 0 times a value of infinity is no number, where the probability
 // itself would give infinity.  A wavefront whose tiles gave such a sum makes
@@ -171,7 +171,8 @@ template <>
 struct PagedOperand<false> {
   typedef _Float16 elem;
   typedef fk_half8 vec;
-  static constexpr uint32_t tiny = 1;  // 2^-24, where a reference's probability is 2^15
+  static constexpr float shift = 15.0f;  // the reference below the running maximum: probabilities to 2^15
+  static constexpr uint32_t tiny = 1;    // 2^-24
   static __device__ __forceinline__ fk_float4v mfma(vec a, vec b, fk_float4v c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
   }
@@ -189,6 +190,7 @@ template <>
 struct PagedOperand<true> {
   typedef __bf16 elem;
   typedef fk_paged_bf16x8 vec;
+  static constexpr float shift = 0.0f;       // (values may be as large as a binary32's)
   static constexpr uint32_t tiny = 27 << 7;  // 2^-100
   static __device__ __forceinline__ fk_float4v mfma(vec a, vec b, fk_float4v c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
@@ -482,7 +484,7 @@ __device__ __forceinline__ void paged_attend(const fk_paged_attend_args &a, cons
               sc[s][i] = k < ks.last && k >= ks.first ? sc[s][i] * c : -__builtin_inff();
               mt = __builtin_fmaxf(mt, sc[s][i]);
             }
-          const float mn = __builtin_fmaxf(m, paged_max(mt) - 15.0f);
+          const float mn = __builtin_fmaxf(m, paged_max(mt) - Op::shift);
           const float mc = paged_ref(mn);
           float alpha = __builtin_amdgcn_exp2f(m - mc);
           if (again) alpha = __builtin_fmaxf(alpha, 0x1p-126f);

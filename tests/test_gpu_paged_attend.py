@@ -6,7 +6,7 @@ import numpy as np
 import pytest
 
 import serve_cases as S
-from test_gpu_serve import attend_inputs, bind_attend, mem  # noqa: F401  (mem is a fixture)
+from test_gpu_serve import attend_inputs, bind_attend, hold_attend, mem  # noqa: F401  (mem is a fixture)
 
 pytestmark = pytest.mark.gpu
 
@@ -128,3 +128,15 @@ def test_rows_of_infinite_scores_and_values(device, mem):
     op.enqueue()
     device.sync()
     assert np.isnan(read()).all()
+
+
+@pytest.mark.parametrize("out_type", [None, "f32"])
+@pytest.mark.parametrize("d,lengths", [(64, [1, 2, 40, 300]), (128, [1, 2, 40, 300]), (256, [1, 300, 5]),
+                                       (64, [3000, 7]), (128, [3000])])
+def test_values_near_the_largest_bf16(device, mem, d, lengths, out_type):
+    """Values of about 2^115 (2^112 of 3000 keys): a row's weights of 1 and
+    less times them add to less than 2^128, so the row is finite."""
+    print(f"attend large values {d} {lengths} {out_type}", flush=True)
+    x = attend_inputs(np.random.default_rng(d), lengths, 4, 2, d, 16, "bf16")
+    x["v"] = S.narrow(S.widen(x["v"], True) * 2.0 ** (115 if max(lengths) < 1000 else 112), True)
+    hold_attend(device, mem, x, d ** -0.5, out_type=out_type)
