@@ -330,9 +330,12 @@ __device__ __forceinline__ void mx4_gemm_mid(const fk_mx4_gemm_args &a) {
   codes(0, 0);
   codes(1, 1);
   uint32_t at = 0, to = 2;   // the stage a step reads, and the one it loads
+  // A step loads the stage that the step before it read, so a wavefront comes
+  // to its barrier with its reads done (their products may follow).
 #define FK_MX4_MID(TILE, WAIT, S)                                                                             \
   do {                                                                                                        \
     FK_MX4_VMCNT(WAIT);                                                                                       \
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");                                                        \
     FK_MX4_BARRIER();                                                                                         \
     __builtin_amdgcn_sched_barrier(0);                                                                        \
     if (TILE == 0) scales(sa[1], sb[1], min(p + 1, pairs - 1));                                               \
