@@ -12,8 +12,12 @@
 
 namespace fk {
 
+// The context's device, and nothing left of what an earlier call on this
+// thread (a refused allocation, another library's) failed with: `launched`
+// would take it for the launch's.
 inline int use_device(fk_ctx *ctx) {
   const hipError_t e = hipSetDevice(ctx->device);
+  (void)hipGetLastError();
   return e == hipSuccess ? FK_OK : fk_fail(ctx, FK_ERR_HIP, "hipSetDevice: %s", hipGetErrorString(e));
 }
 

@@ -62,6 +62,7 @@ size_t check_attend(fk_ctx *ctx, const fk_attend_args *a, const char *what) {
 
 int launch_attend(fk_ctx *ctx, const fk_attend_args *a, float *partials, hipStream_t s, const char *what) {
   const fk_step_attend_params &p = a->p;
+  (void)hipGetLastError();  // an earlier call's, which is none of this launch's
   hipLaunchKernelGGL(op_attend, dim3(p.kv_heads * p.splits), dim3(FK_ATTN_THREADS), 0, s,
                      reinterpret_cast<const float *>(a->q), reinterpret_cast<const float *>(a->knew),
                      reinterpret_cast<const float *>(a->vnew), reinterpret_cast<uint16_t *>(a->kc),
