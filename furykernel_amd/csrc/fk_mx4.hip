@@ -143,6 +143,16 @@ uint32_t pick(uint32_t m, uint32_t n, uint32_t k) {
   return best;
 }
 
+// Why the kernels do not take a product of these sizes; null if they do.
+const char *refused(uint32_t m, uint32_t n, uint32_t k) {
+  if (!matrix(m, k) || !matrix(n, k)) return "no such matrices";
+  if ((uint64_t)fk::mx4_row_tiles(m) * fk::mx4_row_tiles(n) >= 1ull << 31) return "2^31 tiles and more";
+  const Form &f = forms[pick(m, n, k)];
+  if (f.kind != MANY && tiles_of(f, m, n) >= 1ull << 23)  // a launch of 2^32 threads
+    return "2^23 threadgroups and more";
+  return nullptr;
+}
+
 template <uint32_t I, int T>
 void queue_form(const fk_mx4_gemm_args &a, hipStream_t s) {
   constexpr Form f = forms[I];
@@ -184,13 +194,8 @@ int check(const fk_mx4_dequantize_args &a, Refusal &no) {
 }
 
 int check(const fk_mx4_gemm_args &a, Refusal &no) {
-  if (!matrix(a.m, a.k) || !matrix(a.n, a.k))
-    return no(FK_ERR_RANGE, "no product of %u and %u rows of %u", a.m, a.n, a.k);
-  if ((uint64_t)mx4_row_tiles(a.m) * mx4_row_tiles(a.n) >= 1ull << 31)
-    return no(FK_ERR_RANGE, "a product of %u by %u: 2^31 tiles and more", a.m, a.n);
-  const Form &f = forms[pick(a.m, a.n, a.k)];
-  if (f.kind != MANY && tiles_of(f, a.m, a.n) >= 1ull << 23)  // a launch of 2^32 threads
-    return no(FK_ERR_RANGE, "a product of %u by %u, k %u: 2^23 threadgroups and more", a.m, a.n, a.k);
+  if (const char *why = refused(a.m, a.n, a.k))
+    return no(FK_ERR_RANGE, "a product of %u by %u rows of %u: %s", a.m, a.n, a.k, why);
   if (int st = check_rows(no, "c", a.c_stride, a.n, a.c_type)) return st;
   const Span reads[] = {{"a_codes", a.a_codes, codes_bytes(a.m, a.k)},
                         {"a_scales", a.a_scales, scales_bytes(a.m, a.k)},
@@ -227,7 +232,7 @@ extern "C" int fk_mx4_dequantize(fk_ctx *ctx, const fk_mx4_dequantize_args *a, f
 }
 
 extern "C" const char *fk_mx4_gemm_form(uint32_t m, uint32_t n, uint32_t k) {
-  return matrix(m, k) && matrix(n, k) ? forms[pick(m, n, k)].name : "";
+  return refused(m, n, k) ? "" : forms[pick(m, n, k)].name;
 }
 
 extern "C" int fk_mx4_gemm(fk_ctx *ctx, const fk_mx4_gemm_args *a, fk_stream *stream) {
