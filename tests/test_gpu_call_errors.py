@@ -26,8 +26,9 @@ def test_a_refused_allocation_is_not_the_next_operators_error(device, mem):
     attend.enqueue()
     device.sync()
     want = read()
-    words = {name: mem.empty(4 * n) for name, n in dict(
-        cached=2, fresh=2, free=4, head=1, table=4, lengths=2, starts=3, slots=2, positions=2, owner=2, counts=4).items()}
+    sizes = dict(cached=2, fresh=2, free=4, head=1, table=4, lengths=2, starts=3, slots=2, positions=2, owner=2,
+                 counts=4)
+    words = {name: mem.empty(4 * n) for name, n in sizes.items()}
     for name, values in dict(cached=[3, 0], fresh=[1, 1], free=[5, 6, 7, 8], head=[0], table=[4, 0, 0, 0]).items():
         words[name].write(np.uint32(values))
     plan = paged.PagePlan(device, **words, requests=2, tokens=2, table_len=2, block_size=16, free_len=4)

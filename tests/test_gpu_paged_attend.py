@@ -81,7 +81,8 @@ def test_infinite_values_of_unlikely_keys(device, mem, d, lengths, table_len, ca
         x["k"][b, 0, i, 0] = S.narrow([-below], bf16)[0]
         x["v"][b, 0, i, 2 * j] = inf | (0x8000 if j % 3 == 0 else 0)
     both, none, nought = 30, 31, 33
-    for p, column, bits in ((at[2], both, inf), (at[7], both, inf | 0x8000), (at[9], none, inf + 1), (lost, nought, inf)):
+    for p, column, bits in ((at[2], both, inf), (at[7], both, inf | 0x8000), (at[9], none, inf + 1),
+                            (lost, nought, inf)):
         b, i = position(x, 0, p)
         x["v"][b, 0, i, column] = bits
     b, i = position(x, 0, lost)
