@@ -51,11 +51,11 @@ __global__ void __launch_bounds__(256, 3) op_mx4_gemm_mid(fk_mx4_gemm_args a) {
 uint64_t codes_bytes(uint32_t rows, uint32_t k) { return (uint64_t)fk::mx4_row_tiles(rows) * fk::mx4_pairs(k) * 2048; }
 uint64_t scales_bytes(uint32_t rows, uint32_t k) { return (uint64_t)fk::mx4_row_tiles(rows) * fk::mx4_pairs(k) * 128; }
 
-// A matrix that one launch of a wavefront a tile makes: up to 2^25 pairs of
-// tiles (1.4 10^11 elements), 2^32 threads.
+// A matrix that one launch of a wavefront a tile makes: fewer than 2^25 - 1 pairs
+// of tiles (1.4 10^11 elements), 2^32 threads in whole threadgroups.
 bool matrix(uint32_t rows, uint32_t k) {
   return rows > 0 && k > 0 && rows <= 1u << 30 && k <= 1u << 30 &&
-         (uint64_t)fk::mx4_row_tiles(rows) * fk::mx4_pairs(k) < 1ull << 25;
+         (uint64_t)fk::mx4_row_tiles(rows) * fk::mx4_pairs(k) < (1ull << 25) - 1;
 }
 
 // Rows of `type`, `stride` elements apart, aligned to their elements.

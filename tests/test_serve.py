@@ -292,3 +292,11 @@ def test_the_form_of_a_refused_product_is_none():
         args = mx4.GemmArgs(*(i << 44 for i in range(1, 6)), n, m, n, k, 0)
         taken = lib.fk_serve_check(b"fk_mx4_gemm", ctypes.byref(args), ctypes.sizeof(args), None, 0) == 0
         assert bool(lib.fk_mx4_gemm_form(m, n, k)) == taken
+
+
+def test_no_matrix_takes_a_launch_of_more_threads_than_there_are():
+    """A wavefront of 64 threads a tile, two tiles a pair, whole threadgroups of
+    four: fewer than 2^32 threads."""
+    lib = runtime.library()
+    for tiles, taken in (((1 << 25) - 3, True), ((1 << 25) - 2, True), ((1 << 25) - 1, False), (1 << 25, False)):
+        assert bool(lib.fk_mx4_codes_bytes(16 * tiles, 1)) == taken == bool(lib.fk_mx4_scales_bytes(16 * tiles, 1))
