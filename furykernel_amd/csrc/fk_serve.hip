@@ -326,6 +326,11 @@ extern "C" size_t fk_paged_attend_workspace(const fk_paged_attend_args *a) {
   return a ? attend_bytes(*a, attend_launch(*a)) : 0;
 }
 
+extern "C" const char *fk_paged_attend_form(const fk_paged_attend_args *a) {
+  const AttendLaunch l = a ? attend_launch(*a) : AttendLaunch{};
+  return l.groups == 0 ? "" : (!l.plan.whole ? "split" : (l.waves == 8 ? "whole 8" : "whole 4"));
+}
+
 extern "C" int fk_paged_attend(fk_ctx *ctx, const fk_paged_attend_args *a, fk_stream *stream) {
   const AttendLaunch l = a ? attend_launch(*a) : AttendLaunch{};
   if (int st = admit(ctx, "fk_paged_attend", a, stream, l)) return st;

@@ -171,6 +171,13 @@ def attend_workspace(requests: int, heads: int, kv_heads: int, head_dim: int, bl
     return n
 
 
+def attend_form(**sizes: int) -> str:
+    """How a PagedAttend of ``attend_workspace``'s sizes is shared out
+    (fk_paged_attend_form)."""
+    attend_workspace(**sizes)
+    return runtime.library().fk_paged_attend_form(ctypes.byref(PagedAttendArgs(**sizes))).decode()
+
+
 class PagedAttend(runtime.Operation):
     """Attention of one new token a request over its pages (fk_paged_attend):
     out[r] = softmax(scale q[r] Kᵀ) V over positions 0 .. lengths[r] - 1 (with

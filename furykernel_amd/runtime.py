@@ -140,6 +140,7 @@ ENTRY_POINTS: list[tuple[str, object, list]] = [
     ("fk_page_plan", _int, [_vp, _vp, _vp]),
     ("fk_paged_store", _int, [_vp, _vp, _vp]),
     ("fk_paged_attend_workspace", _sz, [_vp]),
+    ("fk_paged_attend_form", ctypes.c_char_p, [_vp]),
     ("fk_paged_attend", _int, [_vp, _vp, _vp]),
     ("fk_mx4_codes_bytes", _sz, [_u32, _u32]),
     ("fk_mx4_scales_bytes", _sz, [_u32, _u32]),

@@ -144,6 +144,11 @@ typedef struct fk_paged_attend_args {
 /* The workspace's bytes for these sizes (addresses, scale and strides are not
  * looked at); 0 if the sizes are refused. */
 size_t fk_paged_attend_workspace(const fk_paged_attend_args *args);
+/* How a call of these sizes is shared out: "split" (runs of keys, and a second
+ * launch that joins them), "whole 4" or "whole 8" (each request and kv head to
+ * one threadgroup of as many wavefronts), "" if the sizes are refused; for
+ * profiles and tests. */
+const char *fk_paged_attend_form(const fk_paged_attend_args *args);
 /* Addresses are 16-byte aligned (table, lengths and starts 4-byte); q_stride a
  * multiple of 8. */
 int fk_paged_attend(fk_ctx *ctx, const fk_paged_attend_args *args, fk_stream *stream);

@@ -1,11 +1,13 @@
 """The paged attention (include/fkrocm_serve.h: fk_paged_attend) on the GPU
 at the edges of its numbers: the bits its probabilities keep, infinities of
-unlikely keys."""
+unlikely keys, large values; and where its keys are split over threadgroups,
+with a plan's starts, in windows, and captured."""
 
 import numpy as np
 import pytest
 
 import serve_cases as S
+from furykernel_amd import paged
 from test_gpu_serve import attend_inputs, bind_attend, hold_attend, mem  # noqa: F401  (mem is a fixture)
 
 pytestmark = pytest.mark.gpu
@@ -141,3 +143,132 @@ def test_values_near_the_largest_bf16(device, mem, d, lengths, out_type):
     x = attend_inputs(np.random.default_rng(d), lengths, 4, 2, d, 16, "bf16")
     x["v"] = S.narrow(S.widen(x["v"], True) * 2.0 ** (115 if max(lengths) < 1000 else 112), True)
     hold_attend(device, mem, x, d ** -0.5, out_type=out_type)
+
+
+# The attention whose keys are split over threadgroups and joined --------------------
+
+
+def sizes_of(x, window=0):
+    return dict(requests=len(x["lengths"]), heads=x["heads"], kv_heads=x["kv"], head_dim=x["d"],
+                block_size=x["block"], blocks=x["k"].shape[0], table_len=x["table"].shape[1], window=window)
+
+
+@pytest.mark.parametrize("d,cache", [(64, "f16"), (128, "bf16"), (256, "f16")])
+@pytest.mark.parametrize("lengths,kv", [([3000, 0, 9000, 5, 700, 64, 2048], 2), ([1], 1),
+                                        ([40, 0, 300, 7, 2100, 90] * 60, 2)])
+def test_split_attention_takes_queries_by_a_plans_starts(device, mem, d, cache, lengths, kv):
+    """As the whole one: a request's last token's row, nothing of a request
+    without one or with tokens past the rows there are; pairs fewer and more
+    than the threadgroups, twice into one workspace with other requests empty."""
+    print(f"attend split starts {len(lengths)} {kv} {d} {cache}", flush=True)
+    bf16, n, heads = cache == "bf16", len(lengths), 3 * kv
+    rng = np.random.default_rng(n + d)
+    x = attend_inputs(rng, lengths, heads, kv, d, 16, cache, table_len=max(130, -(-max(lengths) // 16)))
+    sizes = sizes_of(x)
+    assert paged.attend_form(**sizes) == "split"
+    w, q_rows = heads * d, 2 * n
+    rows = S.narrow(rng.standard_normal((q_rows, heads, d)), bf16)
+    starts, out = mem.empty(4 * n + 4), mem.empty(2 * n * w)
+    op = paged.PagedAttend(device, q=mem.put(rows), kpool=mem.put(x["k"]), vpool=mem.put(x["v"]),
+                           table=mem.put(x["table"]), lengths=mem.put(x["lengths"]), starts=starts, q_rows=q_rows,
+                           out=out, workspace=mem.empty(paged.attend_workspace(**sizes)), scale=d ** -0.5, cache=cache,
+                           **sizes)
+    wide = [S.widen(x[i], bf16) for i in ("k", "v")]
+    for turn in range(2):
+        fresh = rng.integers(0, 4, n)
+        fresh[0] = turn + 1 if n > 1 else 1
+        begin = np.concatenate([[0], fresh.cumsum()])
+        if n > 1:
+            begin[-1] = max(begin[-1], q_rows + 3)      # the last one's tokens end past the rows
+        starts.write(begin.astype(np.uint32))
+        op.enqueue()
+        device.sync()
+        seen = np.where((np.diff(begin) > 0) & (begin[1:] <= q_rows), x["lengths"], 0)
+        q = S.widen(rows[np.clip(begin[1:] - 1, 0, q_rows - 1)], bf16)
+        o, spread, reach = S.attend(q, *wide, x["table"], seen, 16, d ** -0.5)
+        got = S.widen(out.read(np.uint16, n * w).reshape(n, heads, d), bf16)
+        tol = S.attend_tolerance(o, spread, reach, seen, d, S.half_step(cache))
+        bad = ~(np.abs(got - o) <= tol)
+        assert not bad.any(), (turn, int(bad.sum()), np.argwhere(bad)[:4].tolist())
+        assert np.all(got[seen == 0] == 0) and (n == 1 or (seen == 0).sum() > 1)
+
+
+@pytest.mark.parametrize("window", [1500, 2049, 3000])
+@pytest.mark.parametrize("d,block,cache", [(64, 16, "bf16"), (128, 24, "f16"), (256, 16, "bf16"), (72, 7, "f16")])
+def test_split_attention_in_a_window(device, mem, window, d, block, cache):
+    print(f"attend split window {window} {d} {block} {cache}", flush=True)
+    lengths = [3000, 0, 9000, 5, window, window + 1, 1, 6000]
+    x = attend_inputs(np.random.default_rng(window), lengths, 6, 2, d, block, cache)
+    assert paged.attend_form(**sizes_of(x, window)) == "split"
+    hold_attend(device, mem, x, d ** -0.5, window=window)
+
+
+@pytest.mark.parametrize("cache,d,block,window", [("f16", 64, 16, 0), ("bf16", 128, 24, 0), ("bf16", 64, 16, 1600)])
+def test_a_captured_step_of_split_attention(device, mem, cache, d, block, window):
+    """Plan, store and attend, whose two launches share a workspace, captured
+    once and replayed over requests of up to 3000 positions that grow, rest and
+    come in, with eager calls on the same buffers between: every replay's rows
+    those of the definition over the caches as they then are."""
+    rng = np.random.default_rng(21)
+    bf16 = cache == "bf16"
+    heads, kv, tokens = 4, 2, 9
+    cached = np.array([0, 1900, block * 40, 3000, 5], np.uint32)
+    n, table_len = len(cached), -(-3040 // block)
+    x = attend_inputs(rng, [int(c) for c in cached], heads, kv, d, block, cache, spare=30, table_len=table_len)
+    sizes = sizes_of(x, window)
+    assert paged.attend_form(**sizes) == "split"
+    blocks = sizes["blocks"]
+    used = {int(b) for r in range(n) for b in x["table"][r, :-(-int(cached[r]) // block)]}
+    free = np.array([b for b in range(blocks) if b not in used], np.uint32)
+    head, table, width = 0, x["table"], (heads + 2 * kv) * d
+    b = dict(cached=mem.put(cached), fresh=mem.put(np.ones(n, np.uint32)), free=mem.put(free),
+             head=mem.put(np.zeros(1, np.uint32)), table=mem.put(table), lengths=mem.empty(4 * n),
+             starts=mem.empty(4 * n + 4), slots=mem.empty(4 * tokens), positions=mem.empty(4 * tokens),
+             owner=mem.empty(4 * tokens), counts=mem.put(np.zeros(4, np.uint32)))
+    rows, qr, out = mem.empty(4 * tokens * width), mem.empty(2 * tokens * heads * d), mem.empty(2 * n * heads * d)
+    kpool, vpool = mem.put(x["k"]), mem.put(x["v"])
+    plan = paged.PagePlan(device, **b, requests=n, tokens=tokens, table_len=table_len, block_size=block,
+                          free_len=len(free))
+    store = paged.PagedStore(device, q=rows, k=rows, v=rows, k_offset=heads * d, v_offset=(heads + kv) * d,
+                             q_stride=width, k_stride=width, v_stride=width, slots=b["slots"], qr=qr, kpool=kpool,
+                             vpool=vpool, tokens=tokens, heads=heads, kv_heads=kv, head_dim=d, block_size=block,
+                             blocks=blocks, rows_type="f32", cache=cache)
+    attend = paged.PagedAttend(device, q=qr, kpool=kpool, vpool=vpool, table=b["table"], lengths=b["lengths"], out=out,
+                               workspace=mem.empty(paged.attend_workspace(**sizes)), scale=d ** -0.5, cache=cache,
+                               starts=b["starts"], q_rows=tokens, **sizes)
+    stream = device.new_stream()
+    with device.capture(stream) as captured:
+        for op in (plan, store, attend):
+            op.enqueue(stream)
+        b["cached"].copy_from(b["lengths"], 4 * n, stream=stream)
+        b["head"].copy_from(b["counts"], 4, src_offset=12, stream=stream)
+    for step in range(5):
+        fresh = np.ones(n, np.uint32)
+        fresh[step] = step % 3                      # a request rests, another brings two tokens
+        new = rng.standard_normal((tokens, width)).astype(np.float32)
+        rows.write(new)
+        b["fresh"].write(fresh)
+        device.sync()
+        captured[0].replay(stream)
+        device.sync(stream)
+        want = S.plan(cached, fresh, free, head, table, tokens, block)
+        for k in ("lengths", "starts", "slots"):
+            assert np.array_equal(b[k].read(np.uint32, want[k].size), want[k]), (step, k)
+        table, head, cached = want["table"], int(want["counts"][3]), want["lengths"]
+        for t in range(int(want["counts"][0])):
+            at, within = divmod(int(want["slots"][t]), block)
+            for pool, first in ((x["k"], heads), (x["v"], heads + kv)):
+                pool[at, :, within] = S.narrow(new[t, first * d:(first + kv) * d].reshape(kv, d), bf16)
+        qs = S.widen(S.narrow(new[:, :heads * d], bf16), bf16).reshape(tokens, heads, d)
+        seen = np.where(fresh > 0, cached, 0)
+        o, spread, reach = S.attend(qs[np.maximum(want["starts"][1:].astype(int) - 1, 0)], S.widen(x["k"], bf16),
+                                    S.widen(x["v"], bf16), table, seen, block, d ** -0.5, window)
+        got = out.read(np.uint16, n * heads * d)
+        tol = S.attend_tolerance(o, spread, reach, cached, d, S.half_step(cache))
+        bad = ~(np.abs(S.widen(got.reshape(n, heads, d), bf16) - o) <= tol)
+        assert not bad.any(), (step, int(bad.sum()), np.argwhere(bad)[:4].tolist())
+        out.write(np.zeros_like(got))
+        attend.enqueue()
+        device.sync()
+        assert np.array_equal(out.read(np.uint16, n * heads * d), got)
+    captured[0].destroy()

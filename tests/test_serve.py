@@ -300,3 +300,13 @@ def test_no_matrix_takes_a_launch_of_more_threads_than_there_are():
     lib = runtime.library()
     for tiles, taken in (((1 << 25) - 3, True), ((1 << 25) - 2, True), ((1 << 25) - 1, False), (1 << 25, False)):
         assert bool(lib.fk_mx4_codes_bytes(16 * tiles, 1)) == taken == bool(lib.fk_mx4_scales_bytes(16 * tiles, 1))
+
+
+def test_the_attentions_form_by_its_sizes():
+    for form, over in (("whole 4", {"table_len": 16}), ("whole 8", {"table_len": 32}), ("split", {"table_len": 400}),
+                       ("whole 8", {"table_len": 400, "window": 200}), ("split", {"head_dim": 256, "table_len": 17})):
+        assert paged.attend_form(**attend_sizes(**over)) == form
+    with pytest.raises(LaunchError):
+        paged.attend_form(**attend_sizes(heads=7))
+    lib = runtime.library()
+    assert lib.fk_paged_attend_form(None) == b"" == lib.fk_paged_attend_form(ctypes.byref(paged.PagedAttendArgs()))
