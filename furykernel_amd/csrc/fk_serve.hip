@@ -100,17 +100,17 @@ AttendLaunch attend_launch(const fk_paged_attend_args &a) {
     // (256 keys of 64, 128 of 128), evenly spread (the one has u), µs split,
     // whole by 4, whole by 8:
     //    pairs, width    u = 2           3               4               5               6
-    //      8 of 64    9.3  6.4  6.0   9.3  8.1  8.3   9.7  9.9  8.7   9.9 11.6 11.1  10.0 13.1 11.4
-    //     80 of 64   10.4  7.3  7.1  10.5  8.6  9.0  10.8 10.5  9.5  11.2 11.8 11.1  12.6 13.7 12.1
-    //    164 of 64   11.6  7.9  7.6  13.2  9.5  9.7  13.7 11.1 10.2  14.0 12.7 12.4  18.1 14.2 12.9
-    //    328 of 64   13.4 10.5 12.7  16.8 12.1 14.7  18.8 15.1 15.6  19.5 18.6 20.2  22.3 18.6 20.4
-    //      8 of 128  10.1  7.2  6.9  10.2  8.5  8.6  10.5  9.8  8.9  10.5 11.2 10.6  10.6 12.5 10.9
-    //     80 of 128  10.7  7.6  7.4  11.1  8.9  9.2  11.4 10.2  9.5  12.1 11.5 11.1  13.1 13.0 11.8
-    //    164 of 128  12.5  8.4  8.4  14.4  9.8 10.2  15.3 11.3 11.0  15.2 12.6 12.5  19.4 14.1 13.5
-    //    328 of 128  14.0  9.3 12.5  18.8 12.7 15.2  19.7 15.6 17.1  20.7 17.3 18.2  24.6 18.7 20.8
-    // Of 256 (128 keys), 2, 32 and 82 pairs of all u units, split and whole by 4:
-    // 13.7 11.8, 14.7 12.7 and 15.9 13.1 at 2, 13.4 14.1, 14.9 15.3 and 17.3 15.8
-    // at 3.  (Many pairs gain at more units too, but one of the table's length
+    //      8 of 64   10.0  7.2  6.9  10.3  8.8  8.9  10.6 10.4  9.2  10.6 12.1 11.3  10.6 13.7 11.6
+    //     80 of 64   10.7  7.6  7.3  11.0  9.1  9.3  11.5 10.7  9.8  11.9 12.2 11.8  13.6 14.0 12.4
+    //    164 of 64   11.6  7.9  7.8  13.3  9.5 10.0  13.8 11.1 10.5  14.4 12.8 12.9  16.7 14.5 13.0
+    //    328 of 64   13.9  9.2 12.8  18.1 11.2 15.3  17.6 13.6 16.3  20.4 16.2 18.8  22.0 18.1 19.6
+    //      8 of 128  11.0  7.8  7.2  11.1  9.2  9.1  11.4 10.6  9.5  11.3 12.1 11.1  11.4 13.5 11.7
+    //     80 of 128  11.5  8.1  7.5  11.9  9.5  9.3  12.5 11.0  9.9  12.9 12.2 11.5  14.3 13.8 12.3
+    //    164 of 128  12.5  8.4  7.9  14.1  9.9  9.9  14.6 11.4 10.5  15.0 13.0 12.3  17.9 14.2 13.2
+    //    328 of 128  14.7  9.7 13.3  19.7 11.7 15.5  18.8 14.0 16.7  22.1 16.2 18.9  23.8 18.2 19.9
+    // (f16; bf16 within 4 % of it).  Of 256 (128 keys), 2, 32 and 82 pairs of all
+    // u units, split and whole by 4: 14.5 11.9, 15.0 12.5 and 16.4 13.4 at 2, 14.4
+    // 14.5, 15.8 15.1 and 17.9 15.9 at 3.  (Many pairs gain at more units too, but one of the table's length
     // among short ones would cost more: that is what the host knows.)
     const uint64_t each = (seen + unit - 1) / unit;
     l.waves = l.width != 256 && pairs <= 256 && each >= 2 && each != 3 ? 8 : 4;

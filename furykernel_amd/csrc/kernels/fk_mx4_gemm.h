@@ -165,6 +165,9 @@ __device__ __forceinline__ void mx4_gemm_few(const fk_mx4_gemm_args &a) {
 // - mx4_gemm_mid: three stages, the operands read as they are needed, and
 //   three threadgroups a CU, one's loads, reads and stores under another's
 //   matrix operations.  For what few 256 x 256 tiles would leave to few CUs.
+//   (Before every other step the compiler's waits for the scales drain the loads
+//   that the written wait would leave in flight, so the third stage hides less
+//   than it could.)
 // - mx4_gemm_many: 256 × 256 tiles whose sums take half the register file, so
 //   one threadgroup a CU: four stages, the next step's operands read and a
 //   later step's loaded between a step's matrix operations, and tile after
@@ -508,7 +511,10 @@ __device__ __forceinline__ void mx4_gemm_many(const fk_mx4_gemm_args &a) {
   // looks at has loads and stores in their order, so the waits of a tile's
   // first pair of steps leave out the stores that went out behind its first
   // loads, whose number is known where the tile before was whole: with the
-  // operands from memory each time, 8192 x 8192, k 2048 104.7 µs, so 93.6.
+  // operands from memory each time, 8192 x 8192, k 2048 104.7 µs, so 93.6.  (The
+  // compiler's own waits for the tile's first scales count none of the stores,
+  // which are conditional, and still hold the first products until all but a few
+  // are out.)
   constexpr uint32_t STORES = 32 * GB * 32 * GB * mx4_bytes_of(T) / (16 * FK_WAVE);  // of a whole tile, a wavefront's
 #define FK_MX4_UNDER(N) ((N) + STORES < 63 ? (N) + STORES : 63)
   bool under = false;

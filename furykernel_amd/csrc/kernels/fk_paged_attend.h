@@ -29,8 +29,8 @@
 // That needs reads of one beside loads into the other, which the compiler
 // would not let pass each other: they are written out (a tile took 2.4 µs where
 // latency alone counts, now 2.0).
-// Measured: one request of 131072 keys, 32 heads over 8 of 128, 84 µs (537 MB,
-// 6.4 TB/s) and 4.6 for the join; 64 requests of up to 16384, 229 and 4.8
+// Measured: one request of 131072 keys, 32 heads over 8 of 128, 82 µs (537 MB,
+// 6.5 TB/s) and 4.6 for the join; 64 requests of up to 16384, 228 and 5.9
 // (1.46 GB, 6.4 TB/s).  A tile's block lookups all go out before the first is
 // waited for, and a run's first table entries beside Q (a short table beside
 // the lengths): 41 requests of 512 keys of 64 13.4 µs, so 11.8.

@@ -7,7 +7,8 @@
 // 16-byte loads and stores, and each pair's cosine and sine once for both.
 // Rows of 16 bits and the caches' elements pass the caches by: 8191 tokens of 32
 // and 8 heads of 128 in bf16, out of memory each time, took 41.7 µs, so 35.9
-// (203 MB, 5.7 TB/s); f32 rows, two loads a line, lose by it (4096 tokens of
+// (203 MB, 5.7 TB/s; the store alone, without what an attention that reads the
+// rows next would save); f32 rows, two loads a line, lose by it (4096 tokens of
 // heads of 64 16.4 µs, 17.5).  8 tokens take 2.8: the launch and three loads,
 // one behind another.
 #pragma once

@@ -46,10 +46,11 @@ enum { FK_T_F32 = 0, FK_T_F16 = 1, FK_T_BF16 = 2 };
  * block_size.  Tokens behind the last: owner and slot FK_NO_SLOT, position 0.
  *
  * A request does not fit if cached + fresh passes table_len * block_size, if
- * its tokens (or those of one before it) end past `tokens`, or if the blocks
- * that the requests up to it need pass the free list; it takes no block, its
- * length stays cached, its tokens' slots are FK_NO_SLOT (so what a step makes
- * of them means nothing: it goes into a later step). */
+ * its tokens (or those of one before it) end past `tokens`, or if it needs new
+ * blocks and those that the requests up to it need pass the free list (one
+ * whose tokens all go into blocks it holds fits whatever the list holds); it
+ * takes no block, its length stays cached, its tokens' slots are FK_NO_SLOT (so
+ * what a step makes of them means nothing: it goes into a later step). */
 typedef struct fk_page_plan_args {
   uint64_t cached;      /* u32 [requests] */
   uint64_t fresh;       /* u32 [requests] */
@@ -109,8 +110,8 @@ int fk_paged_store(fk_ctx *ctx, const fk_paged_store_args *args, fk_stream *stre
  * that of its last new token, row starts[r + 1] - 1 of q_rows, and a request
  * without a new token (or with tokens past q_rows) counts as empty.  A length
  * of 0 gives a row of zeros; a length past table_len * block_size counts as
- * that.  A table entry past `blocks` reads
- * the pool's last block; what entries behind a length hold does not matter.
+ * that.  A table entry past `blocks` reads the pool's last block; what entries
+ * behind a length hold does not matter.
  *
  * Scores, the running maximum, the sums and the weighted values are binary32
  * (probabilities go to the matrix cores as 16-bit parts, which hold 24 bits of
