@@ -54,18 +54,19 @@ BELOW = [0.0, 5.0, 13.5, 14.25, 17.5, 20.0, 27.0, 40.0, 60.0, 86.0, 95.0, 120.0]
 
 
 @pytest.mark.parametrize("cache", ["f16", "bf16"])
-@pytest.mark.parametrize("d,lengths,table_len", [(64, [90, 40], 6), (128, [90, 40], 6), (256, [30, 17], 4),
-                                                 (80, [90, 40], 6), (64, [5000, 300], 320), (128, [5000, 9], 320),
-                                                 (256, [3000, 5], 200), (200, [3000, 64], 200)])
-def test_infinite_values_of_unlikely_keys(device, mem, d, lengths, table_len, cache):
+@pytest.mark.parametrize("d,lengths,table_len,block", [
+    (64, [90, 40], 6, 16), (128, [90, 40], 6, 16), (256, [30, 17], 4, 16), (80, [90, 40], 6, 16),
+    (64, [5000, 300], 320, 16), (128, [5000, 9], 320, 16), (256, [3000, 5], 200, 16), (200, [3000, 64], 200, 16),
+    (64, [700, 40], 700, 1), (128, [500, 3], 500, 1), (64, [2000, 40], 2000, 1), (128, [5000, 40], 2, 2500)])
+def test_infinite_values_of_unlikely_keys(device, mem, d, lengths, table_len, block, cache):
     """An infinite value gives infinity whatever its key's weight: any finite
     score's is above 0.  A key of score -infinity has a weight of 0, and 0
     times infinity is no number; both infinities in one element are none
     either.  Elsewhere the finite values' attention, within its bound."""
-    print(f"attend infinities {d} {lengths} {cache}", flush=True)
+    print(f"attend infinities {d} {lengths} {block} {cache}", flush=True)
     bf16 = cache == "bf16"
     rng = np.random.default_rng(d + len(lengths))
-    x = attend_inputs(rng, lengths, 2, 1, d, 16, cache, table_len=table_len)
+    x = attend_inputs(rng, lengths, 2, 1, d, block, cache, table_len=table_len)
     top = lengths[0]
     # scores from element 0 alone: -64 of every key but the chosen, which
     # lie over the whole length
@@ -102,7 +103,7 @@ def test_infinite_values_of_unlikely_keys(device, mem, d, lengths, table_len, ca
     b, i = position(x, 0, lost)
     wide["k"][b, 0, i, 0] = -1e5               # (the oracle's weight: 0 all the same)
     with np.errstate(invalid="ignore"):
-        out, spread, reach = S.attend(*wide.values(), x["table"], x["lengths"], 16, 1.0)
+        out, spread, reach = S.attend(*wide.values(), x["table"], x["lengths"], block, 1.0)
     # a key's parts that would be 0 stand at 2^-39 of the largest weight (f16),
     # two of them, of values below 5
     reach = np.minimum(reach, 130.0)
@@ -201,6 +202,19 @@ def test_split_attention_in_a_window(device, mem, window, d, block, cache):
     x = attend_inputs(np.random.default_rng(window), lengths, 6, 2, d, block, cache)
     assert paged.attend_form(**sizes_of(x, window)) == "split"
     hold_attend(device, mem, x, d ** -0.5, window=window)
+
+
+@pytest.mark.parametrize("heads,kv,d,block,cache", [(40, 2, 64, 16, "f16"), (17, 1, 128, 16, "bf16"),
+                                                    (33, 1, 256, 24, "f16"), (6, 2, 64, 4096, "bf16"),
+                                                    (48, 3, 72, 1, "bf16"), (512, 16, 64, 16, "f16")])
+@pytest.mark.parametrize("lengths", [[9000, 0, 5, 700, 2500], [3000]])
+def test_split_attention_of_many_heads_a_kv_head(device, mem, heads, kv, d, block, cache, lengths):
+    """Groups of more than 16 query heads, the last ones few; large blocks and
+    ones of a position."""
+    print(f"attend split heads {heads} {kv} {d} {block} {cache} {lengths}", flush=True)
+    x = attend_inputs(np.random.default_rng(heads), lengths, heads, kv, d, block, cache)
+    assert paged.attend_form(**sizes_of(x)) == "split"
+    hold_attend(device, mem, x, d ** -0.5)
 
 
 @pytest.mark.parametrize("cache,d,block,window", [("f16", 64, 16, 0), ("bf16", 128, 24, 0), ("bf16", 64, 16, 1600)])
