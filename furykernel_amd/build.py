@@ -15,6 +15,7 @@ from __future__ import annotations
 import os
 import subprocess
 import sys
+from concurrent.futures import ThreadPoolExecutor
 from pathlib import Path
 
 PACKAGE = Path(__file__).resolve().parent
@@ -50,19 +51,16 @@ def _run(cmd: list[str]) -> None:
 
 def build_runtime() -> Path:
     """The C ABI's library: the runtime and manifest (host code) and the
-    operations (fk_ops.hip, fk_serve.hip, fk_mx4.hip, whose kernels are built
-    with the kernels' flags)."""
+    operations (fk_ops.hip, fk_serve.hip, fk_mx4.hip, fk_fp8.hip, fk_paged8.hip,
+    whose kernels are built with the kernels' flags), four at a time."""
     tmp = RUNTIME_SO.with_suffix(".so.tmp")
-    objs = []
-    for src in (CSRC / "fk_runtime.cpp", CSRC / "fk_manifest.cpp"):
-        obj = PACKAGE / f".{src.stem}.o"
-        _run([HIPCC, "-c", "-fPIC", "-O2", "-std=c++17", "-Wno-unused-value", "-Wno-unused-result",
-              f"-I{ROOT / 'include'}", str(src), "-o", str(obj)])
-        objs.append(obj)
-    for src in (CSRC / "fk_ops.hip", CSRC / "fk_serve.hip", CSRC / "fk_mx4.hip"):
-        obj = PACKAGE / f".{src.stem}.o"
-        _run([HIPCC, "-c", "-fPIC", *KERNEL_FLAGS, f"-I{ROOT / 'include'}", str(src), "-o", str(obj)])
-        objs.append(obj)
+    host = ["-O2", "-std=c++17", "-Wno-unused-value", "-Wno-unused-result"]
+    units = [(CSRC / f"{name}.cpp", host) for name in ("fk_runtime", "fk_manifest")] + \
+        [(CSRC / f"{name}.hip", KERNEL_FLAGS) for name in ("fk_ops", "fk_serve", "fk_mx4", "fk_fp8", "fk_paged8")]
+    objs = [PACKAGE / f".{src.stem}.o" for src, _ in units]
+    with ThreadPoolExecutor(4) as pool:
+        list(pool.map(_run, ([HIPCC, "-c", "-fPIC", *flags, f"-I{ROOT / 'include'}", str(src), "-o", str(obj)]
+                             for (src, flags), obj in zip(units, objs))))
     _run([HIPCC, "-shared", "-fPIC", f"--offload-arch={ARCH}", *map(str, objs), "-o", str(tmp), "-lhiprtc"])
     for o in objs:
         o.unlink()

@@ -6,8 +6,11 @@
 
 #include <cstdarg>
 #include <cstdio>
+#include <type_traits>
 
+#include "../../include/fkrocm_fp8.h"
 #include "../../include/fkrocm_mx4.h"
+#include "../../include/fkrocm_paged8.h"
 #include "fk_internal.h"
 
 namespace fk {
@@ -76,6 +79,26 @@ inline int check_spans(Refusal &no, const Span *reads, size_t n_reads, const Spa
   return FK_OK;
 }
 
+// Rows of an FK_T_* type, `stride` elements apart, aligned to their elements.
+inline uint32_t type_bytes(uint32_t type) { return type == FK_T_F32 ? 4 : 2; }
+inline int check_rows(Refusal &no, const char *name, uint64_t stride, uint64_t width, uint32_t type) {
+  if (type > FK_T_BF16) return no(FK_ERR_ARG, "%s of type %u", name, type);
+  if (stride < width || stride >= 1ull << 40)
+    return no(FK_ERR_ARG, "%s's rows of %llu, %llu apart", name, (unsigned long long)width, (unsigned long long)stride);
+  return FK_OK;
+}
+inline Span rows_of(const char *name, uint64_t addr, uint64_t rows, uint64_t stride, uint64_t width, uint32_t type) {
+  return {name, addr, rows_span(rows, stride, width, type_bytes(type)), type_bytes(type)};
+}
+
+// f with an FK_T_* type as a constant.
+template <typename F>
+void of_type(uint32_t type, F &&f) {
+  if (type == FK_T_F32) f(std::integral_constant<int, FK_T_F32>{});
+  else if (type == FK_T_F16) f(std::integral_constant<int, FK_T_F16>{});
+  else f(std::integral_constant<int, FK_T_BF16>{});
+}
+
 // A call's arguments as its entry takes them, or the refusal on the context.
 template <typename Args, typename... More>
 int admit(fk_ctx *ctx, const char *what, const Args *a, fk_stream *stream, const More &...more) {
@@ -89,9 +112,16 @@ int admit(fk_ctx *ctx, const char *what, const Args *a, fk_stream *stream, const
 
 }  // namespace fk
 
-// The checks of fk_mx4.hip's entries, for fk_serve_check.
+// The checks of the other files' entries, for fk_serve_check.
 namespace fk {
 int check(const fk_mx4_quantize_args &a, Refusal &no);
 int check(const fk_mx4_dequantize_args &a, Refusal &no);
 int check(const fk_mx4_gemm_args &a, Refusal &no);
+int check(const fk_fp8_quantize_args &a, Refusal &no);
+int check(const fk_fp8_dequantize_args &a, Refusal &no);
+int check(const fk_fp8_add_norm_args &a, Refusal &no);
+int check(const fk_fp8_gemm_args &a, Refusal &no);
+int check(const fk_paged_store8_args &a, Refusal &no);
+int check(const fk_paged_load8_args &a, Refusal &no);
+int check(const fk_paged_attend8_args &a, Refusal &no);
 }  // namespace fk

@@ -1,0 +1,289 @@
+// fk_fp8.hip — the 8-bit matrices' operators as one C call each
+// (include/fkrocm_fp8.h), their kernels compiled into the C ABI's library.
+
+#include "../../include/fkrocm_fp8.h"
+
+#include <hip/hip_runtime.h>
+
+#include <cmath>
+#include <iterator>
+#include <utility>
+
+#include "fk_admit.h"
+#include "kernels/fk_fp8.h"
+#include "kernels/fk_fp8_gemm.h"
+
+using fk::admit;
+using fk::check_rows;
+using fk::launched;
+using fk::of_type;
+using fk::Refusal;
+using fk::rows_of;
+using fk::Span;
+using fk::stream_of;
+
+namespace {
+
+template <int T>
+__global__ void __launch_bounds__(FK_FP8_THREADS) op_fp8_quantize(fk_fp8_quantize_args a) {
+  fk::fp8_quantize<T>(a);
+}
+
+template <int T>
+__global__ void __launch_bounds__(FK_FP8_THREADS) op_fp8_dequantize(fk_fp8_dequantize_args a) {
+  fk::fp8_dequantize<T>(a);
+}
+
+template <int T, uint32_t H>
+__global__ void __launch_bounds__(1024) op_fp8_add_norm(fk_fp8_add_norm_args a) {
+  fk::fp8_add_norm<T, H>(a);
+}
+
+template <uint32_t MB, uint32_t NB, uint32_t W, int T>
+__global__ void __launch_bounds__(64 * W, 2) op_fp8_gemm_few(fk_fp8_gemm_args a) {
+  fk::fp8_gemm_few<MB, NB, W, T>(a);
+}
+
+template <uint32_t GM, uint32_t GN, int T>
+__global__ void __launch_bounds__(256, 3) op_fp8_gemm_mid(fk_fp8_gemm_args a) {
+  fk::fp8_gemm_mid<GM, GN, T>(a);
+}
+
+template <int T>
+__global__ void __launch_bounds__(256, 1) op_fp8_gemm_many(fk_fp8_gemm_args a) {
+  fk::fp8_gemm_many<T>(a);
+}
+
+uint64_t codes_bytes(uint32_t rows, uint32_t k) { return (uint64_t)fk::fp8_row_tiles(rows) * fk::fp8_blocks(k) * 2048; }
+uint64_t scales_bytes(uint32_t rows, uint32_t k) { return (uint64_t)fk::fp8_row_tiles(rows) * fk::fp8_quads(k) * 64; }
+
+// A matrix that one launch of a wavefront for each 16 rows of a block makes, in
+// fewer than 2^32 threads of whole threadgroups (1.4 10^11 elements).
+bool matrix(uint32_t rows, uint32_t k) {
+  return rows > 0 && k > 0 && rows <= 1u << 30 && k <= 1u << 30 &&
+         (uint64_t)fk::fp8_row_tiles(rows) * fk::fp8_blocks(k) < (1ull << 26) - 4;
+}
+
+// Threadgroups of a wavefront for each 16 rows of a block.
+uint32_t block_groups(uint32_t rows, uint32_t k) {
+  const uint64_t n = (uint64_t)fk::fp8_row_tiles(rows) * fk::fp8_blocks(k), w = FK_FP8_THREADS / FK_WAVE;
+  return (uint32_t)((n + w - 1) / w);
+}
+
+// The norm's launch: 16 rows' threadgroups on one XCD, 8 such tiles in turn.
+constexpr uint32_t norm_most = 8 * 1024 * FK_FP8_NORM_HELD;
+struct NormLaunch {
+  uint32_t groups, threads, held;
+};
+NormLaunch norm_launch(const fk_fp8_add_norm_args &a) {
+  const uint32_t pieces = 16 * fk::fp8_blocks(a.k);
+  NormLaunch l;
+  l.groups = (fk::fp8_row_tiles(a.rows) + 7) / 8 * 128;
+  l.threads = pieces <= 256 * 4 ? 256 : 1024;
+  if (pieces < 256) l.threads = (pieces + 63) / 64 * 64;
+  const uint32_t each = (pieces + l.threads - 1) / l.threads;
+  l.held = each <= 1 ? 1 : (each <= 2 ? 2 : FK_FP8_NORM_HELD);
+  return l;
+}
+
+// The forms of the product: blocks of 16 of a threadgroup's tile, the
+// wavefronts that share a tile's k (few) or the threadgroups the chip holds at
+// once (mid, many).
+enum Kind { FEW, MID, MANY };
+struct Form {
+  const char *name;
+  Kind kind;
+  uint32_t mb, nb, by;
+  // of C of 16 bits, and of f32 (a step of 0 and less: not that C)
+  struct Cost {
+    double base, step, turn, work;
+  } cost[2];
+};
+// What each costs, in µs:
+//   few         base, for each block of k a wavefront takes `step` and `turn` for
+//               every threadgroup of its CU, and `work` for a thousand KB that
+//               all threadgroups read (mb + nb tiles a block each)
+//   mid, many   `step` a block, `work` for 10^5 tiles times blocks, and `base`
+//               for every time the tiles fill the chip
+constexpr Form forms[] = {
+    {"few 1x1", FEW, 1, 1, 8, {{2.598, 0.129, 0.091, 0.160}, {2.598, 0.129, 0.091, 0.160}}},
+    {"few 4x1", FEW, 4, 1, 8, {{2.587, 0.182, 0.512, 0.074}, {2.587, 0.182, 0.512, 0.074}}},
+    {"few 4x2", FEW, 4, 2, 4, {{2.558, 0, 0.580, 0.060}, {2.558, 0, 0.580, 0.060}}},
+    {"few 8x2", FEW, 8, 2, 4, {{2.743, 0, 1.047, 0.025}, {-1, 0, 0, 0}}},
+    {"mid 8x8", MID, 8, 8, 768, {{5.416, 0.467, 0, 2.579}, {5.416, 0.467, 0, 2.579}}},
+    {"many 16x16", MANY, 16, 16, 256, {{11.667, 0.763, 0, 1.376}, {11.667, 0.763, 0, 1.376}}},
+};
+
+uint64_t tiles_of(const Form &f, uint32_t m, uint32_t n) {
+  return (uint64_t)((fk::fp8_row_tiles(m) + f.mb - 1) / f.mb) * ((fk::fp8_row_tiles(n) + f.nb - 1) / f.nb);
+}
+
+double cost(const Form &f, uint32_t m, uint32_t n, uint32_t k, uint32_t type) {
+  const Form::Cost &c = f.cost[type == FK_T_F32];
+  const double t = (double)tiles_of(f, m, n), blocks = fk::fp8_blocks(k);
+  if (f.kind == FEW)
+    return c.base + std::ceil(blocks / f.by) * (c.step + c.turn * std::ceil(t / 256)) +
+           c.work * 1e-3 * t * blocks * (f.mb + f.nb);
+  return c.base * std::ceil(t / f.by) + c.step * blocks + c.work * 1e-5 * t * f.mb * f.nb * blocks;
+}
+
+// mid and many address a tile's slab with 32 bits.
+constexpr bool takes(const Form &f, uint32_t k, uint32_t type) {
+  return f.cost[type == FK_T_F32].base > 0 && (f.kind == FEW || fk::fp8_blocks(k) < 1u << 16);
+}
+
+uint32_t pick(uint32_t m, uint32_t n, uint32_t k, uint32_t type) {
+  uint32_t best = 0;
+  for (uint32_t i = 1; i < std::size(forms); i++)
+    if (takes(forms[i], k, type) && cost(forms[i], m, n, k, type) < cost(forms[best], m, n, k, type)) best = i;
+  return best;
+}
+
+// Why the kernels do not take a product of these sizes; null if they do.
+const char *refused(uint32_t m, uint32_t n, uint32_t k, uint32_t type) {
+  if (!matrix(m, k) || !matrix(n, k)) return "no such matrices";
+  if ((uint64_t)fk::fp8_row_tiles(m) * fk::fp8_row_tiles(n) >= 1ull << 31) return "2^31 tiles and more";
+  const Form &f = forms[pick(m, n, k, type)];
+  if (f.kind != MANY && tiles_of(f, m, n) >= 1ull << 23)  // a launch of 2^32 threads
+    return "2^23 threadgroups and more";
+  return nullptr;
+}
+
+template <uint32_t I, int T>
+void queue_form(const fk_fp8_gemm_args &a, hipStream_t s) {
+  constexpr Form f = forms[I];
+  const uint32_t tiles = (uint32_t)tiles_of(f, a.m, a.n);
+  if constexpr (f.kind == FEW && takes(f, 1, T))
+    hipLaunchKernelGGL((op_fp8_gemm_few<f.mb, f.nb, f.by, T>), dim3(tiles), dim3(64 * f.by), 0, s, a);
+  else if constexpr (f.kind == MID)
+    hipLaunchKernelGGL((op_fp8_gemm_mid<f.mb / 4, f.nb / 4, T>), dim3(tiles), dim3(256),
+                       (fk::fp8_mid_lds<f.mb / 4, f.nb / 4>()), s, a);
+  else if constexpr (f.kind == MANY)
+    hipLaunchKernelGGL((op_fp8_gemm_many<T>), dim3(tiles < f.by ? tiles : f.by), dim3(256), fk::fp8_many_lds, s, a);
+}
+
+template <int T, size_t... I>
+void queue_picked(uint32_t form, const fk_fp8_gemm_args &a, hipStream_t s, std::index_sequence<I...>) {
+  ((form == I ? queue_form<I, T>(a, s) : void()), ...);
+}
+
+template <int T, uint32_t H>
+void queue_norm(const fk_fp8_add_norm_args &a, const NormLaunch &l, hipStream_t s) {
+  hipLaunchKernelGGL((op_fp8_add_norm<T, H>), dim3(l.groups), dim3(l.threads), 0, s, a);
+}
+
+}  // namespace
+
+namespace fk {
+
+int check(const fk_fp8_quantize_args &a, Refusal &no) {
+  if (!matrix(a.rows, a.k)) return no(FK_ERR_RANGE, "no matrix of %u rows of %u", a.rows, a.k);
+  if (int st = check_rows(no, "x", a.x_stride, a.k, a.x_type)) return st;
+  const Span reads[] = {rows_of("x", a.x, a.rows, a.x_stride, a.k, a.x_type)};
+  const Span writes[] = {{"codes", a.codes, codes_bytes(a.rows, a.k)}, {"scales", a.scales, scales_bytes(a.rows, a.k)}};
+  return check_spans(no, reads, 1, writes, 2);
+}
+
+int check(const fk_fp8_dequantize_args &a, Refusal &no) {
+  if (!matrix(a.rows, a.k)) return no(FK_ERR_RANGE, "no matrix of %u rows of %u", a.rows, a.k);
+  if (int st = check_rows(no, "y", a.y_stride, a.k, a.y_type)) return st;
+  const Span reads[] = {{"codes", a.codes, codes_bytes(a.rows, a.k)}, {"scales", a.scales, scales_bytes(a.rows, a.k)}};
+  const Span writes[] = {rows_of("y", a.y, a.rows, a.y_stride, a.k, a.y_type),
+                         {"scales_out", a.scales_out, a.scales_out ? 4ull * a.rows * fk::fp8_blocks(a.k) : 0, 4}};
+  return check_spans(no, reads, 2, writes, 2);
+}
+
+int check(const fk_fp8_add_norm_args &a, Refusal &no) {
+  if (!matrix(a.rows, a.k) || a.k > norm_most)
+    return no(FK_ERR_RANGE, "no matrix of %u rows of %u (at most %u)", a.rows, a.k, norm_most);
+  if (fk::fp8_row_tiles(a.rows) >= 1u << 18)  // a launch of 2^32 threads
+    return no(FK_ERR_RANGE, "%u rows: 2^22 and more", a.rows);
+  if (!(a.eps >= 0.0f) || std::isinf(a.eps)) return no(FK_ERR_ARG, "eps = %g", (double)a.eps);
+  if (int st = check_rows(no, "x", a.x_stride, a.k, a.x_type)) return st;
+  if (a.residual)
+    if (int st = check_rows(no, "residual", a.residual_stride, a.k, a.x_type)) return st;
+  if (a.sum)
+    if (int st = check_rows(no, "sum", a.sum_stride, a.k, a.x_type)) return st;
+  // (over x or the residual, element by element, the sum is no overlap: each is
+  // read by the thread that writes it, before)
+  const bool over_x = a.sum == a.x && a.sum_stride == a.x_stride;
+  const bool over_r = a.sum == a.residual && a.sum_stride == a.residual_stride;
+  const Span x = rows_of("x", a.x, a.rows, a.x_stride, a.k, a.x_type);
+  const Span r = rows_of("residual", a.residual, a.residual ? a.rows : 0, a.residual_stride, a.k, a.x_type);
+  const Span sum = rows_of("sum", a.sum, a.sum ? a.rows : 0, a.sum_stride, a.k, a.x_type);
+  const Span gamma = {"gamma", a.gamma, a.gamma ? 4ull * a.k : 0};
+  const Span codes = {"codes", a.codes, codes_bytes(a.rows, a.k)};
+  const Span scales = {"scales", a.scales, scales_bytes(a.rows, a.k)};
+  {
+    const Span reads[] = {x, r, gamma}, writes[] = {codes, scales};
+    if (int st = check_spans(no, reads, 3, writes, 2)) return st;
+  }
+  Span reads[4] = {codes, scales, gamma};
+  size_t n = 3;
+  if (!over_x && !(a.residual == a.x && over_r)) reads[n++] = x;
+  const Span one[] = {sum};
+  if (int st = check_spans(no, reads, n, one, 1)) return st;
+  const Span other[] = {r};
+  return over_r || (a.residual == a.x && over_x) ? FK_OK : check_spans(no, other, 1, one, 1);
+}
+
+int check(const fk_fp8_gemm_args &a, Refusal &no) {
+  if (const char *why = refused(a.m, a.n, a.k, a.c_type))
+    return no(FK_ERR_RANGE, "a product of %u by %u rows of %u: %s", a.m, a.n, a.k, why);
+  if (int st = check_rows(no, "c", a.c_stride, a.n, a.c_type)) return st;
+  const Span reads[] = {{"a_codes", a.a_codes, codes_bytes(a.m, a.k)},
+                        {"a_scales", a.a_scales, scales_bytes(a.m, a.k)},
+                        {"b_codes", a.b_codes, codes_bytes(a.n, a.k)},
+                        {"b_scales", a.b_scales, scales_bytes(a.n, a.k)}};
+  const Span writes[] = {rows_of("c", a.c, a.m, a.c_stride, a.n, a.c_type)};
+  return check_spans(no, reads, 4, writes, 1);
+}
+
+}  // namespace fk
+
+extern "C" size_t fk_fp8_codes_bytes(uint32_t rows, uint32_t k) { return matrix(rows, k) ? codes_bytes(rows, k) : 0; }
+extern "C" size_t fk_fp8_scales_bytes(uint32_t rows, uint32_t k) { return matrix(rows, k) ? scales_bytes(rows, k) : 0; }
+
+extern "C" int fk_fp8_quantize(fk_ctx *ctx, const fk_fp8_quantize_args *a, fk_stream *stream) {
+  if (int st = admit(ctx, "fk_fp8_quantize", a, stream)) return st;
+  const dim3 grid(block_groups(a->rows, a->k)), block(FK_FP8_THREADS);
+  of_type(a->x_type, [&](auto t) {
+    hipLaunchKernelGGL((op_fp8_quantize<decltype(t)::value>), grid, block, 0, stream_of(ctx, stream), *a);
+  });
+  return launched(ctx, "fk_fp8_quantize");
+}
+
+extern "C" int fk_fp8_dequantize(fk_ctx *ctx, const fk_fp8_dequantize_args *a, fk_stream *stream) {
+  if (int st = admit(ctx, "fk_fp8_dequantize", a, stream)) return st;
+  const dim3 grid(block_groups(a->rows, a->k)), block(FK_FP8_THREADS);
+  of_type(a->y_type, [&](auto t) {
+    hipLaunchKernelGGL((op_fp8_dequantize<decltype(t)::value>), grid, block, 0, stream_of(ctx, stream), *a);
+  });
+  return launched(ctx, "fk_fp8_dequantize");
+}
+
+extern "C" int fk_fp8_add_norm(fk_ctx *ctx, const fk_fp8_add_norm_args *a, fk_stream *stream) {
+  if (int st = admit(ctx, "fk_fp8_add_norm", a, stream)) return st;
+  const NormLaunch l = norm_launch(*a);
+  const hipStream_t s = stream_of(ctx, stream);
+  of_type(a->x_type, [&](auto t) {
+    constexpr int T = decltype(t)::value;
+    if (l.held == 1) queue_norm<T, 1>(*a, l, s);
+    else if (l.held == 2) queue_norm<T, 2>(*a, l, s);
+    else queue_norm<T, FK_FP8_NORM_HELD>(*a, l, s);
+  });
+  return launched(ctx, "fk_fp8_add_norm");
+}
+
+extern "C" const char *fk_fp8_gemm_form(uint32_t m, uint32_t n, uint32_t k, uint32_t c_type) {
+  return c_type > FK_T_BF16 || refused(m, n, k, c_type) ? "" : forms[pick(m, n, k, c_type)].name;
+}
+
+extern "C" int fk_fp8_gemm(fk_ctx *ctx, const fk_fp8_gemm_args *a, fk_stream *stream) {
+  if (int st = admit(ctx, "fk_fp8_gemm", a, stream)) return st;
+  const hipStream_t s = stream_of(ctx, stream);
+  of_type(a->c_type, [&](auto t) {
+    queue_picked<decltype(t)::value>(pick(a->m, a->n, a->k, a->c_type), *a, s, std::make_index_sequence<std::size(forms)>{});
+  });
+  return launched(ctx, "fk_fp8_gemm");
+}

@@ -14,8 +14,11 @@
 #include "kernels/fk_mx4_gemm.h"
 
 using fk::admit;
+using fk::check_rows;
 using fk::launched;
+using fk::of_type;
 using fk::Refusal;
+using fk::rows_of;
 using fk::Span;
 using fk::stream_of;
 
@@ -58,18 +61,6 @@ bool matrix(uint32_t rows, uint32_t k) {
          (uint64_t)fk::mx4_row_tiles(rows) * fk::mx4_pairs(k) < (1ull << 25) - 1;
 }
 
-// Rows of `type`, `stride` elements apart, aligned to their elements.
-int check_rows(Refusal &no, const char *name, uint64_t stride, uint64_t width, uint32_t type) {
-  if (type > FK_T_BF16) return no(FK_ERR_ARG, "%s of type %u", name, type);
-  if (stride < width || stride >= 1ull << 40)
-    return no(FK_ERR_ARG, "%s's rows of %llu, %llu apart", name, (unsigned long long)width, (unsigned long long)stride);
-  return FK_OK;
-}
-Span rows_of(const char *name, uint64_t addr, uint64_t rows, uint64_t stride, uint64_t width, uint32_t type) {
-  const uint32_t bytes = fk::mx4_bytes_of((int)type);
-  return {name, addr, fk::rows_span(rows, stride, width, bytes), bytes};
-}
-
 // Threadgroups of a wavefront a tile.
 uint32_t tile_groups(uint32_t rows, uint32_t k) {
   const uint64_t tiles = 2ull * fk::mx4_row_tiles(rows) * fk::mx4_pairs(k), w = FK_MX4_THREADS / FK_WAVE;
@@ -84,13 +75,6 @@ uint32_t tile_groups(uint32_t rows, uint32_t k) {
 bool passes_by(const fk_mx4_quantize_args &a) {
   const uint64_t bytes = fk::mx4_bytes_of((int)a.x_type);
   return (uint64_t)a.rows * a.k * bytes >= 1ull << 23 && a.x % 16 == 0 && a.x_stride * bytes % 16 == 0;
-}
-
-template <typename F>
-void of_type(uint32_t type, F &&f) {
-  if (type == FK_T_F32) f(std::integral_constant<int, FK_T_F32>{});
-  else if (type == FK_T_F16) f(std::integral_constant<int, FK_T_F16>{});
-  else f(std::integral_constant<int, FK_T_BF16>{});
 }
 
 // The forms of the product: blocks of 16 of a threadgroup's tile, the

@@ -4,7 +4,6 @@
 // Each entry checks its arguments against what its kernels take, on the host
 // and before anything is queued, then launches on the caller's stream.
 
-#include "../../include/fkrocm_mx4.h"
 #include "../../include/fkrocm_serve.h"
 
 #include <hip/hip_runtime.h>
@@ -268,6 +267,20 @@ extern "C" int fk_serve_check(const char *entry, const void *args, size_t args_b
     st = check(*static_cast<const fk_mx4_dequantize_args *>(args), no);
   } else if (is("fk_mx4_gemm", sizeof(fk_mx4_gemm_args))) {
     st = check(*static_cast<const fk_mx4_gemm_args *>(args), no);
+  } else if (is("fk_fp8_quantize", sizeof(fk_fp8_quantize_args))) {
+    st = check(*static_cast<const fk_fp8_quantize_args *>(args), no);
+  } else if (is("fk_fp8_dequantize", sizeof(fk_fp8_dequantize_args))) {
+    st = check(*static_cast<const fk_fp8_dequantize_args *>(args), no);
+  } else if (is("fk_fp8_add_norm", sizeof(fk_fp8_add_norm_args))) {
+    st = check(*static_cast<const fk_fp8_add_norm_args *>(args), no);
+  } else if (is("fk_fp8_gemm", sizeof(fk_fp8_gemm_args))) {
+    st = check(*static_cast<const fk_fp8_gemm_args *>(args), no);
+  } else if (is("fk_paged_store8", sizeof(fk_paged_store8_args))) {
+    st = check(*static_cast<const fk_paged_store8_args *>(args), no);
+  } else if (is("fk_paged_load8", sizeof(fk_paged_load8_args))) {
+    st = check(*static_cast<const fk_paged_load8_args *>(args), no);
+  } else if (is("fk_paged_attend8", sizeof(fk_paged_attend8_args))) {
+    st = check(*static_cast<const fk_paged_attend8_args *>(args), no);
   } else if (st == FK_OK) {
     st = no(FK_ERR_NOT_FOUND, "no operator %s", entry ? entry : "(null)");
   }

@@ -1,0 +1,248 @@
+// fk_fp8.h — 8-bit matrices made and read back (include/fkrocm_fp8.h has the
+// format and the order they are held in): of plain rows, and as the RMSNorm of
+// a residual stream.
+//
+// One pass each, so the wide side's stream bounds them.
+#pragma once
+
+#include "fk_e4m3.h"
+#include "fk_mx4.h"
+
+#include "../../../include/fkrocm_fp8.h"
+
+#define FK_FP8_THREADS 256
+#define FK_FP8_NORM_HELD 4  // the most pieces of 8 elements that a thread of the norm holds
+
+namespace fk {
+
+__host__ __device__ __forceinline__ uint32_t fp8_row_tiles(uint32_t rows) { return (rows >> 4) + ((rows & 15u) != 0); }
+// Blocks of 128 along k, and groups of four of them.
+__host__ __device__ __forceinline__ uint32_t fp8_blocks(uint32_t k) { return (k >> 7) + ((k & 127u) != 0); }
+__host__ __device__ __forceinline__ uint32_t fp8_quads(uint32_t k) { return (fp8_blocks(k) + 3) / 4; }
+
+// The byte of a row's elements 8 piece .. + 7 (8 codes), and of a block's scale.
+__device__ __forceinline__ uint64_t fp8_code_at(uint32_t row, uint32_t piece, uint32_t blocks) {
+  return ((uint64_t)(row / 16) * blocks * 2 + piece / 8) * 1024 + (piece % 8 / 2 * 16 + row % 16) * 16 + piece % 2 * 8;
+}
+__device__ __forceinline__ uint64_t fp8_scale_at(uint32_t row, uint32_t block, uint32_t quads) {
+  return ((uint64_t)(row / 16) * quads + block / 4) * 64 + row % 16 * 4 + block % 4;
+}
+
+// The maximum over the 16 lanes of a block.
+__device__ __forceinline__ uint32_t fp8_row_max(uint32_t x) {
+  x = max(x, (uint32_t)dpp_i<0xB1>((int)x));
+  x = max(x, (uint32_t)dpp_i<0x4E>((int)x));
+  x = max(x, (uint32_t)dpp_i<0x141>((int)x));
+  return max(x, (uint32_t)dpp_i<0x140>((int)x));
+}
+
+// A lane's 8 elements, whose block the 16 lanes of its row share: codes and
+// the scale's byte.
+__device__ __forceinline__ u32x2 fp8_encode(const float (&x)[8], uint32_t &byte) {
+  uint32_t big = 0;
+#pragma unroll
+  for (int j = 0; j < 8; j++) big = max(big, e4m3_size(x[j]));
+  byte = e4m3_exponent(fp8_row_max(big));
+  const float scale = e4m3_scale(byte);
+  return u32x2{e4m3_codes(x[0], x[1], x[2], x[3], scale), e4m3_codes(x[4], x[5], x[6], x[7], scale)};
+}
+
+// Eight elements from `col` on of a row of k, zeros behind it.
+template <int T, bool ONCE>
+__device__ __forceinline__ void fp8_load8(uint64_t row, uint32_t col, uint32_t k, float (&x)[8]) {
+#pragma unroll
+  for (int j = 0; j < 8; j++) x[j] = 0.0f;
+  if (col + 8 <= k) {
+    mx4_load8<T, ONCE>(row, col, x);
+  } else if (col < k) {
+#pragma unroll
+    for (uint32_t j = 0; j < 7; j++)
+      if (col + j < k) x[j] = mx4_load<T>(row, col + j);
+  }
+}
+template <int T>
+__device__ __forceinline__ void fp8_store8(uint64_t row, uint32_t col, uint32_t k, const float (&x)[8]) {
+  if (col + 8 <= k) {
+    mx4_store8<T>(row, col, x);
+  } else {
+#pragma unroll
+    for (uint32_t j = 0; j < 7; j++)
+      if (col + j < k) mx4_store<T>(row, col + j, x[j]);
+  }
+}
+
+// The wavefront's 16 rows by a block, and a lane's piece of 8 elements and its
+// row of turn i (4 rows a turn).
+struct Fp8Place {
+  uint32_t tile, block, piece, sub;
+  bool there;
+};
+__device__ __forceinline__ Fp8Place fp8_place(uint32_t rows, uint32_t k) {
+  Fp8Place p;
+  const uint32_t blocks = fp8_blocks(k);
+  const uint64_t w = (uint64_t)blockIdx.x * (FK_FP8_THREADS / FK_WAVE) + threadIdx.x / FK_WAVE;
+  p.there = w < (uint64_t)fp8_row_tiles(rows) * blocks;
+  p.tile = __builtin_amdgcn_readfirstlane((uint32_t)w / blocks);
+  p.block = __builtin_amdgcn_readfirstlane((uint32_t)w % blocks);
+  p.piece = threadIdx.x % 16;
+  p.sub = threadIdx.x % FK_WAVE / 16;
+  return p;
+}
+
+template <int T>
+__device__ __forceinline__ void fp8_quantize(const fk_fp8_quantize_args &a) {
+  const Fp8Place p = fp8_place(a.rows, a.k);
+  if (!p.there) return;
+  const uint32_t blocks = fp8_blocks(a.k), quads = fp8_quads(a.k);
+  const uint32_t col = p.block * 128 + p.piece * 8;
+  float x[4][8];
+#pragma unroll
+  for (uint32_t i = 0; i < 4; i++) {
+    const uint32_t row = 16 * p.tile + 4 * i + p.sub;
+    const uint64_t at = a.x + (uint64_t)row * a.x_stride * mx4_bytes_of(T);
+    fp8_load8<T, false>(at, row < a.rows ? col : a.k, a.k, x[i]);
+  }
+#pragma unroll
+  for (uint32_t i = 0; i < 4; i++) {
+    const uint32_t row = 16 * p.tile + 4 * i + p.sub;
+    uint32_t byte;
+    const u32x2 codes = fp8_encode(x[i], byte);
+    *global_at<u32x2>(a.codes + fp8_code_at(row, p.block * 16 + p.piece, blocks)) = codes;
+    // (the last block's lanes 1 to 3 write those of the blocks that fill its four up)
+    const uint32_t block = p.block + p.piece;
+    if (p.piece == 0 || (p.block == blocks - 1 && block < 4 * quads))
+      *global_at<uint8_t>(a.scales + fp8_scale_at(row, block, quads)) =
+          (uint8_t)(p.piece == 0 && row < a.rows ? byte : 127u);
+  }
+}
+
+template <int T>
+__device__ __forceinline__ void fp8_dequantize(const fk_fp8_dequantize_args &a) {
+  const Fp8Place p = fp8_place(a.rows, a.k);
+  const uint32_t col = p.block * 128 + p.piece * 8;
+  if (!p.there || col >= a.k) return;
+  const uint32_t blocks = fp8_blocks(a.k), quads = fp8_quads(a.k);
+  u32x2 codes[4];
+  uint32_t bytes[4];
+#pragma unroll
+  for (uint32_t i = 0; i < 4; i++) {
+    const uint32_t row = 16 * p.tile + 4 * i + p.sub;
+    codes[i] = *global_at<const u32x2>(a.codes + fp8_code_at(row, p.block * 16 + p.piece, blocks));
+    bytes[i] = *global_at<const uint8_t>(a.scales + fp8_scale_at(row, p.block, quads));
+  }
+#pragma unroll
+  for (uint32_t i = 0; i < 4; i++) {
+    const uint32_t row = 16 * p.tile + 4 * i + p.sub;
+    if (row >= a.rows) continue;
+    const float scale = e4m3_scale(bytes[i]);
+    float y[8], z[2][4];
+    e4m3_values(codes[i][0], z[0]);
+    e4m3_values(codes[i][1], z[1]);
+#pragma unroll
+    for (int j = 0; j < 8; j++) {
+      y[j] = z[j / 4][j % 4] * scale;
+      // (the product is made before it is rounded: fused with the rounding to
+      // f16 it adds a zero, and a code of -0 comes out as +0)
+      asm volatile("" : "+v"(y[j]));
+    }
+    fp8_store8<T>(a.y + (uint64_t)row * a.y_stride * mx4_bytes_of(T), col, a.k, y);
+    if (a.scales_out && p.piece == 0) global_at<float>(a.scales_out)[(uint64_t)row * blocks + p.block] = scale;
+  }
+}
+
+// The row of a threadgroup of the norm: the 16 rows of a tile, whose codes
+// share lines of memory, on one XCD (a launch's threadgroups go to the 8 in
+// turn), so that each line is whole in one L2 before it leaves.
+__device__ __forceinline__ uint32_t fp8_norm_row(uint32_t group) {
+  const uint32_t i = group / 8;
+  return (i / 16 * 8 + group % 8) * 16 + i % 16;
+}
+
+// A row's sum over a threadgroup, the same in every thread.
+__device__ __forceinline__ float fp8_norm_sum(float x, float *slots) {
+  x = wave_sum(x);
+  const uint32_t waves = blockDim.x / FK_WAVE;
+  if (waves == 1) return x;
+  if (threadIdx.x % FK_WAVE == 0) slots[threadIdx.x / FK_WAVE] = x;
+  __syncthreads();
+  float sum = slots[0];
+  for (uint32_t w = 1; w < waves; w++) sum += slots[w];
+  return sum;
+}
+
+// x rounded to T and widened again.
+template <int T>
+__device__ __forceinline__ float fp8_rounded(float x) {
+  if constexpr (T == FK_T_F32) return x;
+  else if constexpr (T == FK_T_F16) return (float)(_Float16)x;
+  else return (float)(__bf16)x;
+}
+
+// A row of T, H pieces of 8 elements a thread, held from the first load to the
+// codes: piece t + i threads.
+template <int T, uint32_t H>
+__device__ __forceinline__ void fp8_add_norm(const fk_fp8_add_norm_args &a) {
+  __shared__ float slots[16];
+  const uint32_t row = fp8_norm_row(blockIdx.x);
+  const uint32_t blocks = fp8_blocks(a.k), quads = fp8_quads(a.k), pieces = 16 * blocks;
+  const uint32_t threads = blockDim.x;
+  if (row >= 16 * fp8_row_tiles(a.rows)) return;
+  const uint64_t scales = a.scales + fp8_scale_at(row, 0, quads);
+  // the bytes of the blocks that fill the last four up
+  if (threadIdx.x < 4 * quads - blocks)
+    *global_at<uint8_t>(scales + (uint64_t)(quads - 1) * 64 + (3 - threadIdx.x)) = 127;
+  if (row >= a.rows) {
+    for (uint32_t i = threadIdx.x; i < pieces; i += threads) {
+      *global_at<u32x2>(a.codes + fp8_code_at(row, i, blocks)) = u32x2{0, 0};
+      if (i % 16 == 0) *global_at<uint8_t>(a.scales + fp8_scale_at(row, i / 16, quads)) = 127;
+    }
+    return;
+  }
+  constexpr uint32_t B = mx4_bytes_of(T);
+  float h[H][8], r[H][8];
+#pragma unroll
+  for (uint32_t i = 0; i < H; i++) {
+    const uint32_t col = 8 * (threadIdx.x + i * threads);
+    fp8_load8<T, false>(a.x + row * a.x_stride * B, col, a.k, h[i]);
+    if (a.residual) fp8_load8<T, false>(a.residual + row * a.residual_stride * B, col, a.k, r[i]);
+  }
+  float squares = 0.0f;
+#pragma unroll
+  for (uint32_t i = 0; i < H; i++) {
+    const uint32_t col = 8 * (threadIdx.x + i * threads);
+    if (a.residual) {
+#pragma unroll
+      for (int j = 0; j < 8; j++) h[i][j] = fp8_rounded<T>(h[i][j] + r[i][j]);
+    }
+    if (a.sum) fp8_store8<T>(a.sum + row * a.sum_stride * B, col, a.k, h[i]);
+#pragma unroll
+    for (int j = 0; j < 8; j++) squares += h[i][j] * h[i][j];
+  }
+  const float mean = fp8_norm_sum(squares, slots) / (float)a.k;
+  const float scale = 1.0f / __builtin_sqrtf(mean + a.eps);
+#pragma unroll
+  for (uint32_t i = 0; i < H; i++) {
+    const uint32_t piece = threadIdx.x + i * threads;
+    if (piece >= pieces) break;  // (16 lanes together)
+    float g[8];
+    if (a.gamma) {
+      fp8_load8<FK_T_F32, false>(a.gamma, 8 * piece, a.k, g);
+#pragma unroll
+      for (int j = 0; j < 8; j++) h[i][j] = h[i][j] * scale * g[j];
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; j++) h[i][j] = h[i][j] * scale;
+    }
+    if (8 * piece + 8 > a.k) {
+      // (what lies behind the row is 0 whatever the row's factor)
+#pragma unroll
+      for (uint32_t j = 0; j < 8; j++) h[i][j] = 8 * piece + j < a.k ? h[i][j] : 0.0f;
+    }
+    uint32_t byte;
+    const u32x2 codes = fp8_encode(h[i], byte);
+    *global_at<u32x2>(a.codes + fp8_code_at(row, piece, blocks)) = codes;
+    if (piece % 16 == 0) *global_at<uint8_t>(a.scales + fp8_scale_at(row, piece / 16, quads)) = (uint8_t)byte;
+  }
+}
+
+}  // namespace fk

@@ -27,9 +27,9 @@ __device__ __forceinline__ fk_float4v mx4_mfma(u32x4 b, uint32_t bs, u32x4 a, ui
                                                           (int)as);
 }
 
-// Four consecutive columns n .. n + 3 of row m of C.
-template <int T>
-__device__ __forceinline__ void mx4_store_c(const fk_mx4_gemm_args &a, uint32_t m, uint32_t n, fk_float4v v) {
+// Four consecutive columns n .. n + 3 of row m of C (of a call's arguments).
+template <int T, typename Args>
+__device__ __forceinline__ void mx4_store_c(const Args &a, uint32_t m, uint32_t n, fk_float4v v) {
   if (m >= a.m || n >= a.n) return;
   const uint64_t at = a.c + ((uint64_t)m * a.c_stride + n) * mx4_bytes_of(T);
   if (n + 4 <= a.n) {
@@ -207,9 +207,9 @@ __device__ __forceinline__ fk_float16v mx4_mfma32(u32x4 b, uint32_t bs, u32x4 a,
 // consecutive 16 bytes a lane, so that stores are RB whole bytes of a row (of the
 // many, past the caches: 8192 x 8192, operands from memory, k 2048 97 µs, so 85;
 // k 8192 264 and 258).
-template <uint32_t GM, uint32_t GN, bool AGPR, int T>
-__device__ __forceinline__ void mx4_store_many(const fk_mx4_gemm_args &a, uint32_t m0, uint32_t n0,
-                                               fk_float16v (&acc)[GM][GN], char *stage) {
+template <uint32_t GM, uint32_t GN, bool AGPR, int T, typename Args>
+__device__ __forceinline__ void mx4_store_many(const Args &a, uint32_t m0, uint32_t n0, fk_float16v (&acc)[GM][GN],
+                                               char *stage) {
   constexpr uint32_t RB = GN * 64, BYTES = mx4_bytes_of(T), COLS = RB / BYTES, UNITS = RB / 16, EACH = 16 / BYTES;
   const uint32_t lane = threadIdx.x % FK_WAVE;
   // 16-byte unit u of row m at place u ^ turn(m): no bank twice in 16 lanes

@@ -213,6 +213,117 @@ __device__ __forceinline__ uint16_t paged_round(float x) {
   return __builtin_bit_cast(uint16_t, (typename PagedOperand<BF16>::elem)x);
 }
 
+// A threadgroup's run of units, begin .. end - 1, in runs of `run`: its first
+// request, the first of that one's `here` units and its length.
+struct PagedRun {
+  uint32_t run = 1, begin = 0, end = 0, request = 0, at = 0, here = 0, length = 0;
+};
+
+// The run of a threadgroup of W wavefronts, by a prefix sum of the requests'
+// units (units_in: of a length); false if it is empty.  Requests that see
+// nothing get their rows of zeros, and their pairs' entries of the joins.
+template <uint32_t W, typename Units>
+__device__ __forceinline__ bool paged_share(const fk_paged_attend_args &a, const PagedPlan &pl, Units units_in,
+                                            uint32_t width, uint32_t per_request, PagedRun &x) {
+  constexpr uint32_t THREADS = 64 * W;
+  __shared__ uint32_t wave_units[W];
+  __shared__ u32x4 found;
+  const uint32_t lane = threadIdx.x & (FK_WAVE - 1);
+  const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x / FK_WAVE);
+  const uint32_t n = a.requests;
+  const auto joins = global_at<u32x4>(a.workspace);
+  auto length_of = [&](uint32_t r) { return paged_length(a, r); };
+  auto units_of = [&](uint32_t r) { return units_in(length_of(r)); };
+  // The units of each thread's requests, and before them.
+  uint32_t total = 0;
+  const uint32_t chunk = (n + THREADS - 1) / THREADS;
+  const uint32_t r0 = min(threadIdx.x * chunk, n), r1 = min(r0 + chunk, n);
+  uint32_t mine = 0;
+  for (uint32_t r = r0; r < r1; r++) mine += units_of(r);
+  uint32_t upto = mine;
+#pragma unroll
+  for (int d = 1; d < 64; d *= 2) {
+    const uint32_t o = __shfl_up(upto, d, 64);
+    if (lane >= (uint32_t)d) upto += o;
+  }
+  if (lane == 63) wave_units[wave] = upto;
+  __syncthreads();
+  uint32_t before = upto - mine;
+#pragma unroll
+  for (uint32_t w = 0; w < W; w++) {
+    before += w < wave ? wave_units[w] : 0u;
+    total += wave_units[w];
+  }
+  // This threadgroup's run of units, its request found by the thread that
+  // holds it.
+  x.run = max((total + gridDim.x - 1) / gridDim.x, 1u);
+  x.begin = min(blockIdx.x * x.run, total);
+  x.end = min(x.begin + x.run, total);
+  if (before <= x.begin && x.begin < before + mine) {
+    uint32_t r = r0, at = before, here = units_of(r);
+    while (at + here <= x.begin) {
+      at += here;
+      here = units_of(++r);
+    }
+    found = u32x4{r, at, here, length_of(r)};
+  }
+  __syncthreads();
+
+  // Requests that see nothing: rows of zeros.
+  for (uint32_t r = blockIdx.x; r < n; r += gridDim.x)
+    if (length_of(r) == 0) {
+      for (uint32_t e = threadIdx.x; e < width; e += THREADS) {
+        if (a.out_f32) global_at<float>(a.out)[r * a.out_stride + e] = 0.0f;
+        else global_at<uint16_t>(a.out)[r * a.out_stride + e] = 0;
+      }
+      if (pl.by_pair)
+        for (uint32_t p = threadIdx.x; p < per_request; p += THREADS)
+          joins[r * per_request + p] = u32x4{0, 0, 0, 0};
+    }
+  if (x.begin == x.end) {
+    if (!pl.by_pair && threadIdx.x == 0) joins[blockIdx.x] = u32x4{0, 0, 0, 0};
+    return false;
+  }
+  x.request = __builtin_amdgcn_readfirstlane(found[0]);
+  x.at = __builtin_amdgcn_readfirstlane(found[1]);
+  x.here = __builtin_amdgcn_readfirstlane(found[2]);
+  x.length = __builtin_amdgcn_readfirstlane(found[3]);
+  return true;
+}
+
+// A pair's states of W wavefronts (state_of: a wavefront's values by head and d
+// in rows of DP; sm, sl: maxima and sums by head) added up: into the out rows
+// from `where` on if the pair is whole, or into the workspace's `to`.
+template <uint32_t DP, uint32_t W, bool BF16, typename State>
+__device__ __forceinline__ void paged_meet(const fk_paged_attend_args &a, State state_of, const float (&sm)[W][16],
+                                           const float (&sl)[W][16], uint32_t G, uint32_t D, bool whole,
+                                           uint64_t where, global_ptr<float> to, uint32_t rows) {
+  for (uint32_t e = threadIdx.x; e < G * D; e += 64 * W) {
+    const uint32_t q = e / D, d = e - q * D;
+    float mm = sm[0][q];
+#pragma unroll
+    for (uint32_t w = 1; w < W; w++) mm = __builtin_fmaxf(mm, sm[w][q]);
+    const float mc = paged_ref(mm);
+    float ll = 0.0f, oo = 0.0f;
+#pragma unroll
+    for (uint32_t w = 0; w < W; w++) {
+      const float f = __builtin_amdgcn_exp2f(sm[w][q] - mc);
+      ll += sl[w][q] * f;
+      oo = paged_plus(oo, state_of(w)[q * DP + d], f);
+    }
+    if (whole) {
+      if (a.out_f32) global_at<float>(a.out)[where + e] = oo / ll;
+      else global_at<uint16_t>(a.out)[where + e] = paged_round<BF16>(oo / ll);
+    } else {
+      to[q * D + d] = oo;
+      if (d == 0) {
+        to[rows * D + 2 * q] = mm;
+        to[rows * D + 2 * q + 1] = ll;
+      }
+    }
+  }
+}
+
 // DP: the head's width in the tiles (64, 128 or 256; head_dim at most that);
 // W: its wavefronts, 4, or 8 of whole pairs; FULL: head_dim is DP.
 template <uint32_t DP, uint32_t W, bool FULL, bool BF16>
@@ -226,8 +337,6 @@ __device__ __forceinline__ void paged_attend(const fk_paged_attend_args &a, cons
   constexpr uint32_t THREADS = 64 * W;
   __shared__ __attribute__((aligned(16))) uint16_t kv[W][2][KT * DP];
   __shared__ float sm[W][16], sl[W][16];
-  __shared__ uint32_t wave_units[W];
-  __shared__ u32x4 found;
   const uint32_t lane = threadIdx.x & (FK_WAVE - 1);
   const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x / FK_WAVE);
   const uint32_t n = a.requests, D = FULL ? DP : a.head_dim;
@@ -240,71 +349,19 @@ __device__ __forceinline__ void paged_attend(const fk_paged_attend_args &a, cons
   auto units_in = [&](uint32_t length) {
     return (paged_keys<KT>(length, a.window, pl.length).tiles + FK_PAGED_WAVES - 1) / FK_PAGED_WAVES * per_request;
   };
-  auto units_of = [&](uint32_t r) { return units_in(length_of(r)); };
   // (rows of pieces past head_dim are zeros in K, which no load writes)
   if (!FULL)
     for (uint32_t i = threadIdx.x; i < W * KT * UNITS; i += THREADS)
       reinterpret_cast<uint4 *>(kv[i / (KT * UNITS)][0])[i % (KT * UNITS)] = make_uint4(0, 0, 0, 0);
-  // The run: units begin .. end - 1 of `total`, of which request r's `here`
-  // start at `at`.
-  uint32_t run = 1, total = 0, begin = 0, end = 0, r = 0, at = 0, here = 0, length = 0;
+  // The run: units begin .. end - 1, of which request r's `here` start at `at`.
+  PagedRun mine;
   if (pl.whole) {
     __syncthreads();
-  } else {
-    // The units of each thread's requests, and before them.
-    const uint32_t chunk = (n + THREADS - 1) / THREADS;
-    const uint32_t r0 = min(threadIdx.x * chunk, n), r1 = min(r0 + chunk, n);
-    uint32_t mine = 0;
-    for (uint32_t r = r0; r < r1; r++) mine += units_of(r);
-    uint32_t upto = mine;
-#pragma unroll
-    for (int d = 1; d < 64; d *= 2) {
-      const uint32_t o = __shfl_up(upto, d, 64);
-      if (lane >= (uint32_t)d) upto += o;
-    }
-    if (lane == 63) wave_units[wave] = upto;
-    __syncthreads();
-    uint32_t before = upto - mine;
-#pragma unroll
-    for (uint32_t w = 0; w < W; w++) {
-      before += w < wave ? wave_units[w] : 0u;
-      total += wave_units[w];
-    }
-    // This threadgroup's run of units, its request found by the thread that
-    // holds it.
-    run = max((total + gridDim.x - 1) / gridDim.x, 1u);
-    begin = min(blockIdx.x * run, total);
-    end = min(begin + run, total);
-    if (before <= begin && begin < before + mine) {
-      uint32_t r = r0, at = before, here = units_of(r);
-      while (at + here <= begin) {
-        at += here;
-        here = units_of(++r);
-      }
-      found = u32x4{r, at, here, length_of(r)};
-    }
-    __syncthreads();
-
-    // Requests that see nothing: rows of zeros.
-    for (uint32_t r = blockIdx.x; r < n; r += gridDim.x)
-      if (length_of(r) == 0) {
-        for (uint32_t e = threadIdx.x; e < width; e += THREADS) {
-          if (a.out_f32) global_at<float>(a.out)[r * a.out_stride + e] = 0.0f;
-          else global_at<uint16_t>(a.out)[r * a.out_stride + e] = 0;
-        }
-        if (pl.by_pair)
-          for (uint32_t p = threadIdx.x; p < per_request; p += THREADS)
-            joins[r * per_request + p] = u32x4{0, 0, 0, 0};
-      }
-    if (begin == end) {
-      if (!pl.by_pair && threadIdx.x == 0) joins[blockIdx.x] = u32x4{0, 0, 0, 0};
-      return;
-    }
-    r = __builtin_amdgcn_readfirstlane(found[0]);
-    at = __builtin_amdgcn_readfirstlane(found[1]);
-    here = __builtin_amdgcn_readfirstlane(found[2]);
-    length = __builtin_amdgcn_readfirstlane(found[3]);
+  } else if (!paged_share<W>(a, pl, units_in, width, per_request, mine)) {
+    return;
   }
+  const uint32_t run = mine.run;
+  uint32_t begin = mine.begin, end = mine.end, r = mine.request, at = mine.at, here = mine.here, length = mine.length;
 
   uint16_t *const kbuf = kv[wave][0], *const vbuf = kv[wave][1];
   const auto kpool = global_at<const char>(a.kpool);
@@ -590,32 +647,9 @@ __device__ __forceinline__ void paged_attend(const fk_paged_attend_args &a, cons
       __syncthreads();
       const bool whole = pos == pair0 && seg1 == pair0 + per_pair;
       const uint32_t side = pair0 < begin ? 0u : 1u;
-      const auto to = states + paged_state(blockIdx.x, side, pl.rows, D);
-      for (uint32_t e = threadIdx.x; e < G * D; e += THREADS) {
-        const uint32_t q = e / D, d = e - q * D;
-        float mm = sm[0][q];
-#pragma unroll
-        for (uint32_t w = 1; w < W; w++) mm = __builtin_fmaxf(mm, sm[w][q]);
-        const float mc = paged_ref(mm);
-        float ll = 0.0f, oo = 0.0f;
-#pragma unroll
-        for (uint32_t w = 0; w < W; w++) {
-          const float f = __builtin_amdgcn_exp2f(sm[w][q] - mc);
-          ll += sl[w][q] * f;
-          oo = paged_plus(oo, reinterpret_cast<const float *>(kv[w][1])[q * DP + d], f);
-        }
-        if (whole) {
-          const uint64_t where = r * a.out_stride + (uint64_t)(h0 + q) * D + d;
-          if (a.out_f32) global_at<float>(a.out)[where] = oo / ll;
-          else global_at<uint16_t>(a.out)[where] = paged_round<BF16>(oo / ll);
-        } else {
-          to[q * D + d] = oo;
-          if (d == 0) {
-            to[pl.rows * D + 2 * q] = mm;
-            to[pl.rows * D + 2 * q + 1] = ll;
-          }
-        }
-      }
+      auto state_of = [&](uint32_t w) { return reinterpret_cast<const float *>(kv[w][1]); };
+      paged_meet<DP, W, BF16>(a, state_of, sm, sl, G, D, whole, r * a.out_stride + (uint64_t)h0 * D,
+                              states + paged_state(blockIdx.x, side, pl.rows, D), pl.rows);
       if (!pl.whole && pos == pair0) {
         // the pair starts here: it ends here too, or in the threadgroup of its
         // last unit

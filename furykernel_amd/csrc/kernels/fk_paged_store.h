@@ -65,6 +65,35 @@ __device__ __forceinline__ void store8(uint64_t to, const float (&x)[8]) {
   }
 }
 
+// Elements e .. e + 7 of a head's first half and those they are paired with,
+// turned by row `pos` of the table where they are among the `rotated` pairs.
+__device__ __forceinline__ void store_turn(uint64_t rope, uint32_t pos, uint32_t rotated, uint32_t e, float (&x)[8],
+                                           float (&y)[8]) {
+  const uint64_t cs = rope + 8 * ((uint64_t)pos * rotated + e);
+  float c[8], s[8];
+  if (rotated % 8 == 0) {
+    // whole eights, so four 16-byte loads
+#pragma unroll
+    for (int j = 0; j < 4; j++) {
+      const store_float4 w = global_at<const store_float4>(cs)[j];
+      c[2 * j] = w.x, s[2 * j] = w.y, c[2 * j + 1] = w.z, s[2 * j + 1] = w.w;
+    }
+  } else {
+    // the last pair in the place of those past it, which stay as they are
+#pragma unroll
+    for (int j = 0; j < 8; j++) {
+      const store_float2 w = global_at<const store_float2>(cs)[min((uint32_t)j, rotated - 1 - e)];
+      c[j] = w.x, s[j] = w.y;
+    }
+  }
+#pragma unroll
+  for (int j = 0; j < 8; j++) {
+    const float first = x[j] * c[j] - y[j] * s[j], second = y[j] * c[j] + x[j] * s[j];
+    x[j] = e + j < rotated ? first : x[j];
+    y[j] = e + j < rotated ? second : y[j];
+  }
+}
+
 // T: the rows' type.  Unit u of a token: head u / (head_dim / 16) of q, then
 // k's, then v's, and its elements 8 (u mod (head_dim / 16)) .. + 7 with those
 // half a head further.
@@ -92,30 +121,7 @@ __device__ __forceinline__ void paged_store(const fk_paged_store_args &a) {
   load8<T>(rows, at + half, y);
   const uint32_t slot = global_at<const uint32_t>(a.slots)[token];
   if (!is_v && e < rotated) {
-    const uint32_t pos = min(global_at<const uint32_t>(a.positions)[token], a.rope_rows - 1);
-    const uint64_t cs = a.rope + 8 * ((uint64_t)pos * rotated + e);
-    float c[8], s[8];
-    if (rotated % 8 == 0) {
-      // whole eights, so four 16-byte loads
-#pragma unroll
-      for (int j = 0; j < 4; j++) {
-        const store_float4 w = global_at<const store_float4>(cs)[j];
-        c[2 * j] = w.x, s[2 * j] = w.y, c[2 * j + 1] = w.z, s[2 * j + 1] = w.w;
-      }
-    } else {
-      // the last pair in the place of those past it, which stay as they are
-#pragma unroll
-      for (int j = 0; j < 8; j++) {
-        const store_float2 w = global_at<const store_float2>(cs)[min((uint32_t)j, rotated - 1 - e)];
-        c[j] = w.x, s[j] = w.y;
-      }
-    }
-#pragma unroll
-    for (int j = 0; j < 8; j++) {
-      const float first = x[j] * c[j] - y[j] * s[j], second = y[j] * c[j] + x[j] * s[j];
-      x[j] = e + j < rotated ? first : x[j];
-      y[j] = e + j < rotated ? second : y[j];
-    }
+    store_turn(a.rope, min(global_at<const uint32_t>(a.positions)[token], a.rope_rows - 1), rotated, e, x, y);
   }
   if (slot >= a.blocks * a.block_size) return;
   uint64_t to;

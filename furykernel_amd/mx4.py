@@ -16,7 +16,7 @@ import ctypes
 
 from . import runtime
 from .kernels import LaunchError
-from .paged import _U32, _U64, TYPES, admit, element, need, whole
+from .paged import _U32, _U64, TYPES, admit, element, need, row_stride, whole
 
 
 class QuantizeArgs(ctypes.Structure):
@@ -60,13 +60,6 @@ class Mx4Matrix:
                 need(entry, f"{name}'s scales", self.scales, lib.fk_mx4_scales_bytes(self.rows, self.k), device))
 
 
-def _stride(entry: str, name: str, stride: int | None, width: int) -> int:
-    stride = width if stride is None else stride
-    if not width <= stride < 1 << 40:
-        raise LaunchError(f"{entry}: {name} = {stride} of rows of {width}")
-    return stride
-
-
 class Quantize(runtime.Operation):
     """Rows x [rows][k] of `x_type`, `x_stride` elements apart and `x_offset`
     elements into their buffer, to `to` (fk_mx4_quantize)."""
@@ -75,7 +68,7 @@ class Quantize(runtime.Operation):
                  x_offset: int = 0):
         e = "fk_mx4_quantize"
         wide = element(e, x_type)
-        x_stride = _stride(e, "x_stride", x_stride, to.k)
+        x_stride = row_stride(e, "x_stride", x_stride, to.k)
         codes, scales = to._held(e, "the matrix", device)
         at = need(e, "x", x, ((to.rows - 1) * x_stride + to.k) * wide, device, x_offset * wide)
         args = QuantizeArgs(at, codes, scales, x_stride, to.rows, to.k, TYPES[x_type])
@@ -92,7 +85,7 @@ class Dequantize(runtime.Operation):
                  scales: runtime.Buffer | None = None):
         e = "fk_mx4_dequantize"
         wide = element(e, y_type)
-        y_stride = _stride(e, "y_stride", y_stride, held.k)
+        y_stride = row_stride(e, "y_stride", y_stride, held.k)
         codes, from_scales = held._held(e, "the matrix", device)
         at = need(e, "y", y, ((held.rows - 1) * y_stride + held.k) * wide, device)
         out = 0 if scales is None else need(e, "scales", scales, 4 * held.rows * -(-held.k // 32), device)
@@ -111,7 +104,7 @@ class Gemm(runtime.Operation):
         wide = element(e, c_type)
         if a.k != b.k:
             raise LaunchError(f"{e}: rows of {a.k} and of {b.k}")
-        c_stride = _stride(e, "c_stride", c_stride, b.rows)
+        c_stride = row_stride(e, "c_stride", c_stride, b.rows)
         at = need(e, "c", c, ((a.rows - 1) * c_stride + b.rows) * wide, device)
         args = GemmArgs(*a._held(e, "A", device), *b._held(e, "B", device), at, c_stride, a.rows, b.rows, a.k,
                         TYPES[c_type])

@@ -49,6 +49,14 @@ def element(entry: str, name: str, types=("f32", "f16", "bf16")) -> int:
     return ELEM_BYTES[name]
 
 
+def row_stride(entry: str, name: str, stride: int | None, width: int) -> int:
+    """Elements from row to row: the width, or what holds a row."""
+    stride = width if stride is None else stride
+    if not width <= stride < 1 << 40:
+        raise LaunchError(f"{entry}: {name} = {stride} of rows of {width}")
+    return stride
+
+
 def admit(entry: str, args: ctypes.Structure) -> None:
     """The library's own checks of a call's arguments (fk_serve_check)."""
     try:

@@ -148,6 +148,18 @@ ENTRY_POINTS: list[tuple[str, object, list]] = [
     ("fk_mx4_dequantize", _int, [_vp, _vp, _vp]),
     ("fk_mx4_gemm", _int, [_vp, _vp, _vp]),
     ("fk_mx4_gemm_form", ctypes.c_char_p, [_u32, _u32, _u32]),
+    ("fk_fp8_codes_bytes", _sz, [_u32, _u32]),
+    ("fk_fp8_scales_bytes", _sz, [_u32, _u32]),
+    ("fk_fp8_quantize", _int, [_vp, _vp, _vp]),
+    ("fk_fp8_dequantize", _int, [_vp, _vp, _vp]),
+    ("fk_fp8_add_norm", _int, [_vp, _vp, _vp]),
+    ("fk_fp8_gemm", _int, [_vp, _vp, _vp]),
+    ("fk_fp8_gemm_form", ctypes.c_char_p, [_u32, _u32, _u32, _u32]),
+    ("fk_paged_store8", _int, [_vp, _vp, _vp]),
+    ("fk_paged_load8", _int, [_vp, _vp, _vp]),
+    ("fk_paged_attend8_workspace", _sz, [_vp]),
+    ("fk_paged_attend8_form", ctypes.c_char_p, [_vp]),
+    ("fk_paged_attend8", _int, [_vp, _vp, _vp]),
     ("fk_serve_check", _int, [ctypes.c_char_p, _vp, _sz, ctypes.c_char_p, _sz]),
     ("fk_rtc_compile", _int, [ctypes.c_char_p, ctypes.c_char_p, ctypes.POINTER(ctypes.c_char_p), _int, _PP,
                               ctypes.POINTER(_sz), ctypes.POINTER(ctypes.c_char_p)]),
