@@ -106,12 +106,12 @@ struct Form {
 //   mid, many   `step` a block, `work` for 10^5 tiles times blocks, and `base`
 //               for every time the tiles fill the chip
 constexpr Form forms[] = {
-    {"few 1x1", FEW, 1, 1, 8, {{2.598, 0.129, 0.091, 0.160}, {2.598, 0.129, 0.091, 0.160}}},
-    {"few 4x1", FEW, 4, 1, 8, {{2.587, 0.182, 0.512, 0.074}, {2.587, 0.182, 0.512, 0.074}}},
-    {"few 4x2", FEW, 4, 2, 4, {{2.558, 0, 0.580, 0.060}, {2.558, 0, 0.580, 0.060}}},
-    {"few 8x2", FEW, 8, 2, 4, {{2.743, 0, 1.047, 0.025}, {-1, 0, 0, 0}}},
-    {"mid 8x8", MID, 8, 8, 768, {{5.416, 0.467, 0, 2.579}, {5.416, 0.467, 0, 2.579}}},
-    {"many 16x16", MANY, 16, 16, 256, {{11.667, 0.763, 0, 1.376}, {11.667, 0.763, 0, 1.376}}},
+    {"few 1x1", FEW, 1, 1, 8, {{1.802, 0.265, 0.282, 0.107}, {1.999, 0.136, 0.441, 0.074}}},
+    {"few 4x1", FEW, 4, 1, 8, {{1.685, 0.173, 0.995, 0.045}, {1.758, 0.234, 1.102, 0.040}}},
+    {"few 4x2", FEW, 4, 2, 4, {{2.825, 0, 0.600, 0.066}, {2.998, 0, 0.672, 0.066}}},
+    {"few 8x2", FEW, 8, 2, 4, {{3.099, 0, 1.246, 0.017}, {-1, 0, 0, 0}}},
+    {"mid 8x8", MID, 8, 8, 768, {{3.098, 0.513, 0, 3.668}, {4.752, 0.516, 0, 5.155}}},
+    {"many 16x16", MANY, 16, 16, 256, {{8.477, 0.789, 0, 1.838}, {12.483, 1.317, 0, 3.669}}},
 };
 
 uint64_t tiles_of(const Form &f, uint32_t m, uint32_t n) {

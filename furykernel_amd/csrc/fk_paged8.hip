@@ -29,10 +29,10 @@ __global__ void __launch_bounds__(FK_LOAD8_THREADS)
   fk::paged_load8<T>(a, block, units);
 }
 
-template <uint32_t DP, uint32_t W, bool FULL, bool BF16>
-__global__ void __launch_bounds__(64 * W, DP == 256 ? 1 : 2)
+template <uint32_t DP, uint32_t EIGHTS, bool FULL, bool BF16, uint32_t PARTS>
+__global__ void __launch_bounds__(64 * FK_PAGED_WAVES, DP == 256 ? 1 : 2)
     op_pages8_attend(fk_paged_attend_args a, uint64_t scales, fk::PagedPlan pl) {
-  fk::paged_attend8<DP, W, FULL, BF16>(a, scales, pl);
+  fk::paged_attend8<DP, EIGHTS, FULL, BF16, PARTS>(a, scales, pl);
 }
 
 template <uint32_t W, bool BF16>
@@ -70,10 +70,10 @@ StoreLaunch store_launch(const fk_paged_store8_args &a) {
 }
 
 // The attention's launch, as fk_serve.hip's: head_dim's tile width, its
-// wavefronts and threadgroups, the joins' entries and what the kernels take; 0
+// threadgroups, the joins' entries and what the kernels take; 0
 // threadgroups and the reason if the kernels do not take them.
 struct AttendLaunch {
-  uint32_t width = 0, waves = 4, groups = 0, joins = 0;
+  uint32_t width = 0, groups = 0, joins = 0;
   fk::PagedPlan plan{};
   const char *why = "";
 };
@@ -105,14 +105,34 @@ AttendLaunch attend_launch(const fk_paged_attend8_args &a) {
       l.why = "fewer than 2^31 units of keys";
       return l;
     }
-    // as many as the chip's 256 compute units hold at once
-    const uint64_t most = l.width == 256 ? 256 : 512;
-    l.groups = (uint32_t)(units < most ? (uint64_t)units : most);
+    // Threadgroups: one a CU of heads past 128 (more registers) and of few pairs
+    // (whose states are then fewer to join), two, or three of heads of 64, whose
+    // tiles cost more operations a byte.  µs by 1, 2 and 3 a CU: one request of
+    // 131072 keys, 8 pairs of 128, 46.5 48.1 53.7; 512 pairs of 128 and up to
+    // 16384 129.1 130.9 130.1, of 64 84.8 78.2 75.2; 128 of 256 74.7 81.1 80.9; 160
+    // of 128 and up to 3000 23.8 21.2 23.2.
     const uint64_t pairs = (uint64_t)a.requests * a.kv_heads * l.plan.head_tiles;
+    const uint64_t most = l.width == 64 ? 768 : (l.width == 256 || pairs <= 16 ? 256 : 512);
+    l.groups = (uint32_t)(units < most ? (uint64_t)units : most);
     l.plan.by_pair = pairs <= l.groups;
     l.joins = l.plan.by_pair ? (uint32_t)pairs : l.groups;
+    // Few units a pair at most: a threadgroup takes pairs whole, which saves the
+    // prefix sum and the join and costs each further unit's time, and a long
+    // pair's to the launch.  µs whole and split of requests of up to u units (256
+    // keys of 64, 128 of 128 and 256), evenly spread | of one unit but for one:
+    //   pairs, width   u = 4                  6                      8                      12
+    //     8 of 64    7.6  9.5              9.5  9.5             11.4  9.7             15.2  9.9
+    //    80 of 64    8.7 12.4| 8.1 10.3   10.5 12.6|10.0 10.2   12.3 13.3|12.0 10.4   16.1 13.6|15.5 10.5
+    //   328 of 64   13.3 16.8| 9.0 11.9   15.2 19.5|11.0 12.0   18.1 19.8|12.3 12.0   27.7 24.9|15.9 12.2
+    //     8 of 128   7.1  9.8              8.5  9.8              9.8 10.2             12.5 10.1
+    //    80 of 128   7.6 12.2| 7.2 10.0    8.9 12.6| 8.8 10.0   10.3 13.0| 9.9 10.0   13.1 13.3|12.7 10.2
+    //   328 of 128  12.6 16.7| 8.3 11.9   14.0 21.8|10.2 11.7   16.7 19.7|10.8 11.9   24.0 26.0|12.9 12.1
+    //     8 of 256  12.0 12.8             14.6 12.8             17.3 13.1             21.8 13.2
+    //    80 of 256  12.8 18.0|12.1 12.7   15.6 19.0|14.8 12.9   18.1 20.3|17.2 12.8   23.2 20.8|22.2 13.2
+    //   328 of 256  24.6 32.4|17.4 19.4   27.5 37.8|21.4 19.5   31.7 43.8|22.4 19.5   45.0 48.2|27.2 19.8
     const uint64_t each = (seen + unit - 1) / unit;
-    l.plan.whole = each <= 2;
+    l.plan.whole = each <= (l.width == 64 ? (pairs < 64 ? 6 : 8)
+                            : l.width == 128 ? (pairs < 128 ? 8 : 12) : (pairs < 64 ? 4 : 6));
     if (l.plan.whole) l.groups = (uint32_t)(pairs < most ? pairs : most);
   }
   return l;
@@ -134,19 +154,24 @@ fk_paged_attend_args shared_args(const fk_paged_attend8_args &a) {
   return s;
 }
 
-template <uint32_t DP, bool BF16>
+// The keys of a group: a tile's where blocks are of whole tiles, 16, or 8 (and
+// heads that do not fill their tiles).
+template <uint32_t DP, bool BF16, uint32_t PARTS>
 void queue_attend(const fk_paged_attend_args &a, uint64_t scales, const AttendLaunch &l, hipStream_t s) {
-  if (a.head_dim == DP)
-    hipLaunchKernelGGL((op_pages8_attend<DP, 4, true, BF16>), dim3(l.groups), dim3(256), 0, s, a, scales, l.plan);
-  else
-    hipLaunchKernelGGL((op_pages8_attend<DP, 4, false, BF16>), dim3(l.groups), dim3(256), 0, s, a, scales, l.plan);
+  constexpr uint32_t tile = fk::attend8_keys(DP);
+  auto queue = [&](auto kernel) {
+    hipLaunchKernelGGL(kernel, dim3(l.groups), dim3(64 * FK_PAGED_WAVES), 0, s, a, scales, l.plan);
+  };
+  if (a.head_dim != DP || a.block_size % 16) queue(op_pages8_attend<DP, 1, false, BF16, PARTS>);
+  else if (a.block_size % tile) queue(op_pages8_attend<DP, 2, true, BF16, PARTS>);
+  else queue(op_pages8_attend<DP, tile / 8, true, BF16, PARTS>);
 }
 
-template <bool BF16>
+template <bool BF16, uint32_t PARTS>
 void queue_attend(const fk_paged_attend_args &a, uint64_t scales, const AttendLaunch &l, hipStream_t s) {
-  if (l.width == 256) queue_attend<256, BF16>(a, scales, l, s);
-  else if (l.width == 128) queue_attend<128, BF16>(a, scales, l, s);
-  else queue_attend<64, BF16>(a, scales, l, s);
+  if (l.width == 256) queue_attend<256, BF16, PARTS>(a, scales, l, s);
+  else if (l.width == 128) queue_attend<128, BF16, PARTS>(a, scales, l, s);
+  else queue_attend<64, BF16, PARTS>(a, scales, l, s);
 }
 
 template <uint32_t W>
@@ -310,8 +335,8 @@ extern "C" int fk_paged_attend8(fk_ctx *ctx, const fk_paged_attend8_args *a, fk_
   const AttendLaunch l = attend_launch(*a);
   const fk_paged_attend_args s = shared_args(*a);
   const hipStream_t on = stream_of(ctx, stream);
-  if (a->q_bf16) queue_attend<true>(s, a->scales, l, on);
-  else queue_attend<false>(s, a->scales, l, on);
+  if (a->q_bf16) a->out_f32 ? queue_attend<true, 3>(s, a->scales, l, on) : queue_attend<true, 2>(s, a->scales, l, on);
+  else a->out_f32 ? queue_attend<false, 3>(s, a->scales, l, on) : queue_attend<false, 2>(s, a->scales, l, on);
   if (int st = launched(ctx, "fk_paged_attend8")) return st;
   if (l.plan.whole) return FK_OK;
   const uint32_t states = l.groups / l.joins;  // of a pair, about

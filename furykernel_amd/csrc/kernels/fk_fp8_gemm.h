@@ -357,7 +357,7 @@ __device__ __forceinline__ void fp8_gemm_many(const fk_fp8_gemm_args &a) {
   _Pragma("unroll") for (uint32_t j_ = 0; j_ < GB; j_++) asm volatile("" : "+a"(acc[i_][j_]))
 #define FK_FP8_SCALES(SA, SB, P)                                                                              \
   _Pragma("unroll") for (uint32_t i_ = 0; i_ < GB; i_++) {                                                    \
-    const uint32_t so_ = (P) / 4 * 64 + (P) % 4;                                                              \
+    const uint32_t so_ = __builtin_amdgcn_readfirstlane((P) / 4 * 64 + (P) % 4);                              \
     SA[i_] = __builtin_amdgcn_raw_buffer_load_b8(as.scales, as_at[i_], so_, 0);                               \
     SB[i_] = __builtin_amdgcn_raw_buffer_load_b8(bs.scales, bs_at[i_], so_, 0);                               \
   }

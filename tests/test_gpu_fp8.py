@@ -261,10 +261,10 @@ def hold_product(device, mem, rng, m, n, k, kind, pad=0, spread=3):
         hold_values(device, mem, (a[0], a[1] * 2.0 ** -16), b, m, n, k, kind, pad)
 
 
-def hold_values(device, mem, a, b, m, n, k, kind, pad):
+def hold_values(device, mem, a, b, m, n, k, kind, pad, rows=slice(None)):
     print(f"product {m} {n} {k} {kind} {fp8.gemm_form(m, n, k, kind)}", flush=True)
-    got = product(device, mem, a, b, m, n, k, kind, pad)
-    av, bv = F.values(*a, k), F.values(*b, k)
+    got = product(device, mem, a, b, m, n, k, kind, pad)[rows]
+    av, bv = F.values(a[0][rows], a[1][rows], k), F.values(*b, k)
     want, size = av @ bv.T, np.abs(av) @ np.abs(bv).T
     # k additions of binary32, cut off or rounded (2^-23 each); of 16 bits the cut
     # of eight products of k, and the result's rounding
@@ -295,6 +295,15 @@ def test_products_of_every_form(device, mem, kind):
                     (700, 1500, 400), (2100, 1700, 200), (4100, 4200, 136), (9000, 300, 250), (6200, 8300, 520)):
         seen.add(fp8.gemm_form(m, n, k, kind).split()[0])
         hold_product(device, mem, np.random.default_rng(m), m, n, k, kind)
+    for m, n, k in ((4000, 4090, 1030), (4090, 8100, 1160), (8190, 8190, 1290), (8190, 16300, 2000)):
+        if not fp8.gemm_form(m, n, k, kind).startswith("many"):
+            continue
+        seen.add("many")
+        rng = np.random.default_rng(m)
+        rows = np.unique(np.concatenate([rng.integers(0, m, 60), [0, m - 1]]))
+        a, b = random_matrix(rng, m, k, 3), random_matrix(rng, n, k, 3)
+        hold_values(device, mem, (a[0], a[1] * 2.0 ** -14), b, m, n, k, kind, 1, rows)
+        break
     assert seen == {"few", "mid", "many"}
 
 
