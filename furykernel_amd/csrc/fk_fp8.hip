@@ -44,9 +44,9 @@ __global__ void __launch_bounds__(64 * W, 2) op_fp8_gemm_few(fk_fp8_gemm_args a)
   fk::fp8_gemm_few<MB, NB, W, T>(a);
 }
 
-template <uint32_t GM, uint32_t GN, int T>
-__global__ void __launch_bounds__(256, 3) op_fp8_gemm_mid(fk_fp8_gemm_args a) {
-  fk::fp8_gemm_mid<GM, GN, T>(a);
+template <uint32_t GM, uint32_t GN, uint32_t STAGES, int T>
+__global__ void __launch_bounds__(256, STAGES == 3 ? 3 : 1) op_fp8_gemm_mid(fk_fp8_gemm_args a) {
+  fk::fp8_gemm_mid<GM, GN, STAGES, T>(a);
 }
 
 template <int T>
@@ -87,31 +87,38 @@ NormLaunch norm_launch(const fk_fp8_add_norm_args &a) {
 }
 
 // The forms of the product: blocks of 16 of a threadgroup's tile, the
-// wavefronts that share a tile's k (few) or the threadgroups the chip holds at
-// once (mid, many).
+// wavefronts that share a tile's k (few), the stages of its ring (mid).
 enum Kind { FEW, MID, MANY };
 struct Form {
   const char *name;
   Kind kind;
-  uint32_t mb, nb, by;
-  // of C of 16 bits, and of f32 (a step of 0 and less: not that C)
+  uint32_t mb, nb, by, stages;
+  // of C of 16 bits, and of f32 (a base below 0: not that C)
   struct Cost {
-    double base, step, turn, work;
+    double base, step, turn, tile, work;
   } cost[2];
 };
-// What each costs, in µs:
-//   few         base, for each block of k a wavefront takes `step` and `turn` for
-//               every threadgroup of its CU, and `work` for a thousand KB that
-//               all threadgroups read (mb + nb tiles a block each)
-//   mid, many   `step` a block, `work` for 10^5 tiles times blocks, and `base`
-//               for every time the tiles fill the chip
+// What each costs, in µs, fitted to its times on 221 products (1 to 8192 rows by
+// 512 to 16384, k of 512 to 8192, the operands from memory each time).  With
+// `turns` the threadgroups of the CU that has most,
+//   few         base, for each block of k a wavefront takes `step` and `turn` a
+//               turn, `tile` a turn, and `work` for a thousand tiles of 2 KB that
+//               all threadgroups read
+//   mid, many   base, `tile` a turn, and for each block of k the largest of `step`
+//               (its latency), `turn` a turn and `work` a threadgroup of each CU
+// The form of the least cost takes 1.013 (f32 1.005) times the fastest one's
+// time on average over them, at most 1.40 (8192 rows by 5000, k 512: 46 µs, mid
+// 33; f32 1.22).
 constexpr Form forms[] = {
-    {"few 1x1", FEW, 1, 1, 8, {{1.802, 0.265, 0.282, 0.107}, {1.999, 0.136, 0.441, 0.074}}},
-    {"few 4x1", FEW, 4, 1, 8, {{1.685, 0.173, 0.995, 0.045}, {1.758, 0.234, 1.102, 0.040}}},
-    {"few 4x2", FEW, 4, 2, 4, {{2.825, 0, 0.600, 0.066}, {2.998, 0, 0.672, 0.066}}},
-    {"few 8x2", FEW, 8, 2, 4, {{3.099, 0, 1.246, 0.017}, {-1, 0, 0, 0}}},
-    {"mid 8x8", MID, 8, 8, 768, {{3.098, 0.513, 0, 3.668}, {4.752, 0.516, 0, 5.155}}},
-    {"many 16x16", MANY, 16, 16, 256, {{8.477, 0.789, 0, 1.838}, {12.483, 1.317, 0, 3.669}}},
+    {"few 1x1", FEW, 1, 1, 8, 0, {{1.837, 0.282, 0.241, 0.036, 0.116}, {1.889, 0.253, 0.292, 0.138, 0.099}}},
+    {"few 2x1", FEW, 2, 1, 8, 0, {{1.640, 0.353, 0.423, 0.184, 0.077}, {1.501, 0.331, 0.492, 0.383, 0.069}}},
+    {"few 2x2", FEW, 2, 2, 8, 0, {{1.967, 0.184, 0.913, 0.009, 0.073}, {1.117, 0.311, 0.823, 0.977, 0.079}}},
+    {"few 4x2", FEW, 4, 2, 4, 0, {{1.903, 0, 0.755, 0.679, 0.029}, {1.997, 0.033, 0.783, 0.864, 0.026}}},
+    {"few 8x2", FEW, 8, 2, 8, 0, {{0.137, 0.323, 2.090, 1.823, 0.028}, {-1, 0, 0, 0, 0}}},
+    {"mid 8x8", MID, 8, 8, 0, 3, {{0.416, 0.761, 0.572, 1.831, 0.487}, {0.825, 0.930, 0.743, 3.080, 0.816}}},
+    {"mid 8x8 deep", MID, 8, 8, 0, 8, {{0.657, 0.436, 0.502, 3.304, 0.759}, {0.331, 0.532, 0.823, 4.938, 1.077}}},
+    {"mid 4x8 deep", MID, 4, 8, 0, 10, {{0.978, 0.098, 0.403, 2.276, 0.603}, {1.337, 0.301, 0.551, 2.981, 0.727}}},
+    {"many 16x16", MANY, 16, 16, 0, 0, {{0, 0.573, 1.209, 8.095, 1.599}, {0, 2.339, 2.355, 12.070, 3.078}}},
 };
 
 uint64_t tiles_of(const Form &f, uint32_t m, uint32_t n) {
@@ -120,16 +127,16 @@ uint64_t tiles_of(const Form &f, uint32_t m, uint32_t n) {
 
 double cost(const Form &f, uint32_t m, uint32_t n, uint32_t k, uint32_t type) {
   const Form::Cost &c = f.cost[type == FK_T_F32];
-  const double t = (double)tiles_of(f, m, n), blocks = fk::fp8_blocks(k);
+  const double t = (double)tiles_of(f, m, n), blocks = fk::fp8_blocks(k), turns = std::ceil(t / 256);
+  const double ends = c.base + c.tile * turns;
   if (f.kind == FEW)
-    return c.base + std::ceil(blocks / f.by) * (c.step + c.turn * std::ceil(t / 256)) +
-           c.work * 1e-3 * t * blocks * (f.mb + f.nb);
-  return c.base * std::ceil(t / f.by) + c.step * blocks + c.work * 1e-5 * t * f.mb * f.nb * blocks;
+    return ends + std::ceil(blocks / f.by) * (c.step + c.turn * turns) + c.work * 1e-3 * t * blocks * (f.mb + f.nb);
+  return ends + blocks * std::fmax(c.step, std::fmax(c.turn * turns, c.work * t / 256));
 }
 
 // mid and many address a tile's slab with 32 bits.
 constexpr bool takes(const Form &f, uint32_t k, uint32_t type) {
-  return f.cost[type == FK_T_F32].base > 0 && (f.kind == FEW || fk::fp8_blocks(k) < 1u << 16);
+  return f.cost[type == FK_T_F32].base >= 0 && (f.kind == FEW || fk::fp8_blocks(k) < 1u << 16);
 }
 
 uint32_t pick(uint32_t m, uint32_t n, uint32_t k, uint32_t type) {
@@ -156,10 +163,10 @@ void queue_form(const fk_fp8_gemm_args &a, hipStream_t s) {
   if constexpr (f.kind == FEW && takes(f, 1, T))
     hipLaunchKernelGGL((op_fp8_gemm_few<f.mb, f.nb, f.by, T>), dim3(tiles), dim3(64 * f.by), 0, s, a);
   else if constexpr (f.kind == MID)
-    hipLaunchKernelGGL((op_fp8_gemm_mid<f.mb / 4, f.nb / 4, T>), dim3(tiles), dim3(256),
-                       (fk::fp8_mid_lds<f.mb / 4, f.nb / 4>()), s, a);
+    hipLaunchKernelGGL((op_fp8_gemm_mid<f.mb / 4, f.nb / 4, f.stages, T>), dim3(tiles), dim3(256),
+                       (fk::fp8_mid_lds<f.mb / 4, f.nb / 4, f.stages>()), s, a);
   else if constexpr (f.kind == MANY)
-    hipLaunchKernelGGL((op_fp8_gemm_many<T>), dim3(tiles < f.by ? tiles : f.by), dim3(256), fk::fp8_many_lds, s, a);
+    hipLaunchKernelGGL((op_fp8_gemm_many<T>), dim3(tiles < 256 ? tiles : 256), dim3(256), fk::fp8_many_lds, s, a);
 }
 
 template <int T, size_t... I>

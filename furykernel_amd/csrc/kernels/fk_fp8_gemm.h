@@ -187,17 +187,26 @@ __device__ __forceinline__ void fp8_gemm_few(const fk_fp8_gemm_args &a) {
 // threadgroup of 4 wavefronts, two by two, takes a tile of 64 GM rows and 64 GN
 // columns, each wavefront GM × GN blocks.  A step is one tile of k (64): the
 // operands' 1 KB tiles go straight into a ring of LDS stages and are read back
-// 16 bytes a lane, no bank twice.  The scales come to registers, a block's byte
-// a lane, a block (two steps) ahead.  Two kernels, by what hides what: mid, three
-// stages and several threadgroups a CU; many, one threadgroup a CU with the
-// sums in half its registers, a step's operands read and a later one's loaded
-// between the matrix operations.
+// 16 bytes a lane, no bank twice.  The scales come to registers ahead of their
+// blocks, a byte or four blocks' bytes a lane.  Two kernels, by what hides what:
+//
+// - fp8_gemm_mid: a ring of as many stages as the tile wants.  Three, and three
+//   threadgroups a CU, one's loads, reads and stores under another's matrix
+//   operations; or, where the tiles do not fill the CUs that often, as many as
+//   the LDS holds for one threadgroup, so that a step's loads have the time of
+//   seven others to land: 400 rows by 5000, k 8192 52 µs by three stages, 36 by
+//   eight; 200 rows 51, and 29 in tiles of 64 rows.  What bounds it there is
+//   what a CU takes in, about 60 KB a µs (as the few rows' form).
+// - fp8_gemm_many: 256 × 256 tiles whose sums take half the register file, one
+//   threadgroup a CU, four stages, the next step's operands read and a later
+//   step's loaded between a step's matrix operations, and tile after tile with
+//   the next one's first loads under the stores.
 #define FK_FP8_STAGES 4
 constexpr uint32_t fp8_many_side = 16;  // row tiles of a tile's side
 constexpr uint32_t fp8_many_lds = FK_FP8_STAGES * 2 * fp8_many_side * 1024;
-template <uint32_t GM, uint32_t GN>
+template <uint32_t GM, uint32_t GN, uint32_t STAGES>
 constexpr uint32_t fp8_mid_lds() {
-  return 3 * 4 * (GM + GN) * 1024;
+  return STAGES * 4 * (GM + GN) * 1024;
 }
 
 // An operand's source: up to ROWS row tiles from `tile` on, as buffers of codes
@@ -215,8 +224,9 @@ __device__ __forceinline__ Fp8Source fp8_source(uint64_t codes, uint64_t scales,
   return s;
 }
 
-template <uint32_t GM, uint32_t GN, int T>
+template <uint32_t GM, uint32_t GN, uint32_t STAGES, int T>
 __device__ __forceinline__ void fp8_gemm_mid(const fk_fp8_gemm_args &a) {
+  static_assert(GN >= 2, "the stores' rows of a wavefront are of 128 bytes at least");
   extern __shared__ u32x4 fp8_lds[];
   constexpr uint32_t RA = 4 * GM, RN = 4 * GN;     // row tiles of the slabs
   constexpr uint32_t SLAB = RA * 1024, STAGE = (RA + RN) * 1024;
@@ -251,9 +261,8 @@ __device__ __forceinline__ void fp8_gemm_mid(const fk_fp8_gemm_args &a) {
     for (uint32_t j = 0; j < GN; j++)
 #pragma unroll
       for (int r = 0; r < 16; r++) acc[i][j][r] = 0.0f;
-  uint32_t sa[2][GM], sb[2][GN];
-  const uint32_t steps = 2 * blocks, last = steps - 1;
-  auto codes = [&](uint32_t step, uint32_t stage) {
+  const uint32_t last = 2 * blocks - 1;
+  auto codes = [&](uint32_t step, uint32_t stage) __attribute__((always_inline)) {
     const uint32_t so = min(step, last) * 1024;
 #pragma unroll
     for (uint32_t q = 0; q < GM; q++)
@@ -262,46 +271,71 @@ __device__ __forceinline__ void fp8_gemm_mid(const fk_fp8_gemm_args &a) {
     for (uint32_t q = 0; q < GN; q++)
       __builtin_amdgcn_raw_ptr_buffer_load_lds(bs.codes, b_to + stage * STAGE + q * 1024, 16, b_at[q], so, 0, 0);
   };
-  auto scales = [&](uint32_t (&s)[GM], uint32_t (&t)[GN], uint32_t block) {
-    const uint32_t so = block / 4 * 64 + block % 4;
+  // Four blocks' scales, a byte each.
+  auto scales = [&](uint32_t (&s)[GM], uint32_t (&t)[GN], uint32_t quad) __attribute__((always_inline)) {
 #pragma unroll
-    for (uint32_t i = 0; i < GM; i++) s[i] = __builtin_amdgcn_raw_buffer_load_b8(as.scales, as_at[i], so, 0);
+    for (uint32_t i = 0; i < GM; i++) s[i] = __builtin_amdgcn_raw_buffer_load_b32(as.scales, as_at[i], quad * 64, 0);
 #pragma unroll
-    for (uint32_t i = 0; i < GN; i++) t[i] = __builtin_amdgcn_raw_buffer_load_b8(bs.scales, bs_at[i], so, 0);
+    for (uint32_t i = 0; i < GN; i++) t[i] = __builtin_amdgcn_raw_buffer_load_b32(bs.scales, bs_at[i], quad * 64, 0);
   };
-  scales(sa[0], sb[0], 0);
-  codes(0, 0);
-  codes(1, 1);
-  uint32_t at = 0, to = 2;   // the stage a step reads, and the one it loads
+  uint32_t sa[GM], sb[GN], next_a[GM], next_b[GN];
+  scales(sa, sb, 0);
+#pragma unroll
+  for (uint32_t t = 0; t + 1 < STAGES; t++) codes(t, t);
+  uint32_t at = 0, to = STAGES - 1;   // the stage a step reads, and the one it loads
   // A step loads the stage that the step before it read, so a wavefront comes
-  // to its barrier with its reads done (their products may follow).
-#define FK_FP8_MID(FIRST, WAIT, S)                                                                            \
-  do {                                                                                                        \
-    FK_MX4_VMCNT(WAIT);                                                                                       \
-    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");                                                        \
-    FK_MX4_BARRIER();                                                                                         \
-    __builtin_amdgcn_sched_barrier(0);                                                                        \
-    if (FIRST) scales(sa[1], sb[1], min(p + 1, blocks - 1));                                                  \
-    codes((S) + 2, to);                                                                                       \
-    const u32x4 *s_ = fp8_lds + at * (STAGE / 16);                                                            \
-    fk_fp8_u32x8 fa[GM], fb[GN];                                                                              \
-    _Pragma("unroll") for (uint32_t j = 0; j < GN; j++) fb[j] = fp8_join(s_[rb + 128 * j], s_[rb + 128 * j + 32]); \
-    _Pragma("unroll") for (uint32_t i = 0; i < GM; i++) fa[i] = fp8_join(s_[ra + 128 * i], s_[ra + 128 * i + 32]); \
-    fp8_multiply<T, 0, GM>(acc, fb, sb[0], fa, sa[0]);                                                        \
-    at = at == 2 ? 0 : at + 1;                                                                                \
-    to = to == 2 ? 0 : to + 1;                                                                                \
-  } while (0)
-  for (uint32_t p = 0; p < blocks; p++) {
-    FK_FP8_MID(true, GM + GN, 2 * p);
-    FK_FP8_MID(false, 2 * (GM + GN), 2 * p + 1);
+  // to its barrier with its reads done (their products may follow).  Its own
+  // stage has landed once no more than the loads behind it are in flight (the
+  // scales' among them make that early, never late).
+  auto step = [&](uint32_t s, uint32_t byte) __attribute__((always_inline)) {
+    FK_MX4_VMCNT((STAGES - 2) * (GM + GN));
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    FK_MX4_BARRIER();
+    __builtin_amdgcn_sched_barrier(0);
+    codes(s + STAGES - 1, to);
+    const u32x4 *from = fp8_lds + at * (STAGE / 16);
+    fk_fp8_u32x8 fa[GM], fb[GN];
+    uint32_t xa[GM], xb[GN];
 #pragma unroll
-    for (uint32_t i = 0; i < GM; i++) sa[0][i] = sa[1][i];
+    for (uint32_t j = 0; j < GN; j++) {
+      fb[j] = fp8_join(from[rb + 128 * j], from[rb + 128 * j + 32]);
+      xb[j] = sb[j] >> (8 * byte) & 255u;
+    }
 #pragma unroll
-    for (uint32_t i = 0; i < GN; i++) sb[0][i] = sb[1][i];
+    for (uint32_t i = 0; i < GM; i++) {
+      fa[i] = fp8_join(from[ra + 128 * i], from[ra + 128 * i + 32]);
+      xa[i] = sa[i] >> (8 * byte) & 255u;
+    }
+    fp8_multiply<T, 0, GM>(acc, fb, xb, fa, xa);
+    at = at == STAGES - 1 ? 0 : at + 1;
+    to = to == STAGES - 1 ? 0 : to + 1;
+  };
+  auto turn = [&] __attribute__((always_inline)) {
+#pragma unroll
+    for (uint32_t i = 0; i < GM; i++) sa[i] = next_a[i];
+#pragma unroll
+    for (uint32_t j = 0; j < GN; j++) sb[j] = next_b[j];
+  };
+  // Whole fours of blocks, their scales loaded a four ahead: waited for nearer,
+  // the counter would hold the codes' loads behind them too.
+  uint32_t p = 0;
+  for (; p + 4 <= blocks; p += 4) {
+    scales(next_a, next_b, min(p / 4 + 1, quads - 1));
+#pragma unroll
+    for (uint32_t b = 0; b < 4; b++) {
+      step(2 * (p + b), b);
+      step(2 * (p + b) + 1, b);
+    }
+    turn();
   }
+#pragma unroll
+  for (uint32_t b = 0; b < 3; b++)
+    if (p + b < blocks) {
+      step(2 * (p + b), b);
+      step(2 * (p + b) + 1, b);
+    }
   __builtin_amdgcn_s_waitcnt(0);
   FK_MX4_BARRIER();
-#undef FK_FP8_MID
   mx4_store_many<GM, GN, false, T>(a, 16 * tm + 32 * wm * GM, 16 * tn + 32 * wn * GN, acc,
                                    reinterpret_cast<char *>(fp8_lds) + wave * GN * 2048);
 }
