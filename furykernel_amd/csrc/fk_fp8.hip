@@ -34,9 +34,9 @@ __global__ void __launch_bounds__(FK_FP8_THREADS) op_fp8_dequantize(fk_fp8_dequa
   fk::fp8_dequantize<T>(a);
 }
 
-template <int T, uint32_t H>
+template <int T, uint32_t ROWS, uint32_t H>
 __global__ void __launch_bounds__(1024) op_fp8_add_norm(fk_fp8_add_norm_args a) {
-  fk::fp8_add_norm<T, H>(a);
+  fk::fp8_add_norm<T, ROWS, H>(a);
 }
 
 template <uint32_t MB, uint32_t NB, uint32_t W, int T>
@@ -70,19 +70,24 @@ uint32_t block_groups(uint32_t rows, uint32_t k) {
   return (uint32_t)((n + w - 1) / w);
 }
 
-// The norm's launch: 16 rows' threadgroups on one XCD, 8 such tiles in turn.
-constexpr uint32_t norm_most = 8 * 1024 * FK_FP8_NORM_HELD;
+// The norm's launch: rows a threadgroup, blocks a lane, and tiles of 16 rows by
+// 8, one an XCD.  Where the rows fill the card, rows of 17 to 64 blocks go by two,
+// with two blocks a lane (8192 x 4096 bf16 47.6 us, by one 51.1; of 16 blocks, f32,
+// 46 and 45); few rows, which wait on their own chain of steps, by one, with as few
+// blocks a lane as there are threads for (1 x 5000 4.1 us with one block, 4.9 with
+// two, 6.7 with four; by two rows 5.7).
+constexpr uint32_t norm_most = 4 * 16 * FK_FP8_NORM_HELD * 128;
 struct NormLaunch {
-  uint32_t groups, threads, held;
+  uint32_t rows, held, threads, groups;
 };
 NormLaunch norm_launch(const fk_fp8_add_norm_args &a) {
-  const uint32_t pieces = 16 * fk::fp8_blocks(a.k);
   NormLaunch l;
-  l.groups = (fk::fp8_row_tiles(a.rows) + 7) / 8 * 128;
-  l.threads = pieces <= 256 * 4 ? 256 : 1024;
-  if (pieces < 256) l.threads = (pieces + 63) / 64 * 64;
-  const uint32_t each = (pieces + l.threads - 1) / l.threads;
-  l.held = each <= 1 ? 1 : (each <= 2 ? 2 : FK_FP8_NORM_HELD);
+  const uint32_t blocks = fk::fp8_blocks(a.k);
+  l.rows = a.rows >= 1024 && blocks > 16 && blocks <= 64 ? 2 : 1;
+  const uint32_t each = (blocks * l.rows + 3) / 4;  // blocks for the wavefronts' 16 lanes
+  l.held = l.rows == 2 ? 2 : (each <= 16 ? 1 : (each <= 32 ? 2 : FK_FP8_NORM_HELD));
+  l.threads = 64 * ((each + l.held - 1) / l.held);
+  l.groups = (fk::fp8_row_tiles(a.rows) + 7) / 8 * (128 / l.rows);
   return l;
 }
 
@@ -174,11 +179,10 @@ void queue_picked(uint32_t form, const fk_fp8_gemm_args &a, hipStream_t s, std::
   ((form == I ? queue_form<I, T>(a, s) : void()), ...);
 }
 
-template <int T, uint32_t H>
+template <int T, uint32_t ROWS, uint32_t H>
 void queue_norm(const fk_fp8_add_norm_args &a, const NormLaunch &l, hipStream_t s) {
-  hipLaunchKernelGGL((op_fp8_add_norm<T, H>), dim3(l.groups), dim3(l.threads), 0, s, a);
+  hipLaunchKernelGGL((op_fp8_add_norm<T, ROWS, H>), dim3(l.groups), dim3(l.threads), 0, s, a);
 }
-
 }  // namespace
 
 namespace fk {
@@ -275,9 +279,10 @@ extern "C" int fk_fp8_add_norm(fk_ctx *ctx, const fk_fp8_add_norm_args *a, fk_st
   const hipStream_t s = stream_of(ctx, stream);
   of_type(a->x_type, [&](auto t) {
     constexpr int T = decltype(t)::value;
-    if (l.held == 1) queue_norm<T, 1>(*a, l, s);
-    else if (l.held == 2) queue_norm<T, 2>(*a, l, s);
-    else queue_norm<T, FK_FP8_NORM_HELD>(*a, l, s);
+    if (l.rows == 2) queue_norm<T, 2, 2>(*a, l, s);
+    else if (l.held == 1) queue_norm<T, 1, 1>(*a, l, s);
+    else if (l.held == 2) queue_norm<T, 1, 2>(*a, l, s);
+    else queue_norm<T, 1, FK_FP8_NORM_HELD>(*a, l, s);
   });
   return launched(ctx, "fk_fp8_add_norm");
 }

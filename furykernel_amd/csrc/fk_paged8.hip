@@ -19,7 +19,7 @@ using fk::stream_of;
 namespace {
 
 template <int T, bool BF16, uint32_t W>
-__global__ void __launch_bounds__(W == 8 ? 512 : 256) op_pages8_store(fk_paged_store8_args a, fk::Store8Plan pl) {
+__global__ void __launch_bounds__(W == 1 ? 256 : 64 * W) op_pages8_store(fk_paged_store8_args a, fk::Store8Plan pl) {
   fk::paged_store8<T, BF16, W>(a, pl);
 }
 
@@ -51,10 +51,10 @@ struct StoreLaunch {
 
 StoreLaunch store_launch(const fk_paged_store8_args &a) {
   StoreLaunch l;
-  // as many wavefronts as hold a whole block's rows
+  // as many wavefronts as hold a whole block's rows, a piece of 8 and 8 elements a thread
   const uint64_t pieces = (uint64_t)a.block_size * a.head_dim / 16;
-  l.waves = pieces <= 64 * FK_STORE8_HELD ? 1 : (pieces <= 256 * FK_STORE8_HELD ? 4 : 8);
-  l.threads = l.waves == 8 ? 512 : 256;
+  l.waves = pieces <= 64 ? 1 : (pieces <= 128 ? 2 : (pieces <= 256 ? 4 : 8));
+  l.threads = l.waves == 1 ? 256 : 64 * l.waves;
   const uint64_t T = a.tokens, units = 2ull * a.kv_heads, most = 8192 / l.waves;
   // a token a chunk while that is what fills the chip
   const uint64_t chunk = T * units / most;
@@ -303,6 +303,7 @@ extern "C" int fk_paged_store8(fk_ctx *ctx, const fk_paged_store8_args *a, fk_st
     constexpr int T = decltype(t)::value;
     auto queue = [&](auto kernel) { hipLaunchKernelGGL(kernel, grid, block, 0, s, *a, l.plan); };
     if (l.waves == 1) a->q_bf16 ? queue(op_pages8_store<T, true, 1>) : queue(op_pages8_store<T, false, 1>);
+    else if (l.waves == 2) a->q_bf16 ? queue(op_pages8_store<T, true, 2>) : queue(op_pages8_store<T, false, 2>);
     else if (l.waves == 4) a->q_bf16 ? queue(op_pages8_store<T, true, 4>) : queue(op_pages8_store<T, false, 4>);
     else a->q_bf16 ? queue(op_pages8_store<T, true, 8>) : queue(op_pages8_store<T, false, 8>);
   });

@@ -10,11 +10,25 @@ namespace fk {
 typedef short e4m3_short2 __attribute__((ext_vector_type(2)));
 typedef float e4m3_float2 __attribute__((ext_vector_type(2)));
 
-// A value's part in its block's largest: its magnitude's bits, 0 if it is not
-// finite.
-__device__ __forceinline__ uint32_t e4m3_size(float x) {
-  const uint32_t u = __float_as_uint(x) & 0x7FFFFFFFu;
-  return u < 0x7F800000u ? u : 0u;
+// The bits of the largest finite magnitude of eight values; those that are
+// not finite are made NaN.  Few wavefronts hold any, so the others do not pay for
+// looking at each (7 operations an element fewer: the norm of 8191 x 5000 bf16
+// 65.3 us, 67.4 without).
+__device__ __forceinline__ uint32_t e4m3_largest(float (&x)[8]) {
+  constexpr uint32_t INF = 0x7F800000u;
+  uint32_t big = 0;
+#pragma unroll
+  for (int j = 0; j < 8; j++) big = max(big, __float_as_uint(x[j]) & 0x7FFFFFFFu);
+  if (__builtin_amdgcn_ballot_w64(big >= INF)) {
+    big = 0;
+#pragma unroll
+    for (int j = 0; j < 8; j++) {
+      const uint32_t u = __float_as_uint(x[j]) & 0x7FFFFFFFu;
+      x[j] = u < INF ? x[j] : __builtin_nanf("");
+      big = max(big, u < INF ? u : 0u);
+    }
+  }
+  return big;
 }
 
 // The scale's biased exponent for a largest magnitude of these bits: m 2^e is
@@ -26,13 +40,12 @@ __device__ __forceinline__ uint32_t e4m3_exponent(uint32_t big) {
 }
 __device__ __forceinline__ float e4m3_scale(uint32_t exponent) { return __uint_as_float(exponent << 23); }
 
-// Four values to codes, x / scale to the nearest, halfway cases to the even
-// code; NaN where not finite.
+// Four values, finite or NaN, to codes: x / scale to the nearest, halfway cases
+// to the even code.
 __device__ __forceinline__ uint32_t e4m3_codes(float x0, float x1, float x2, float x3, float scale) {
-  auto nan = [](float x) { return (__float_as_uint(x) & 0x7F800000u) == 0x7F800000u ? __builtin_nanf("") : x; };
   e4m3_short2 w = {0, 0};
-  w = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(w, nan(x0), nan(x1), scale, false);
-  w = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(w, nan(x2), nan(x3), scale, true);
+  w = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(w, x0, x1, scale, false);
+  w = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(w, x2, x3, scale, true);
   return __builtin_bit_cast(uint32_t, w);
 }
 

@@ -11,7 +11,7 @@
 #include "../../../include/fkrocm_fp8.h"
 
 #define FK_FP8_THREADS 256
-#define FK_FP8_NORM_HELD 4  // the most pieces of 8 elements that a thread of the norm holds
+#define FK_FP8_NORM_HELD 4  // the most blocks that a lane of the norm holds a piece of
 
 namespace fk {
 
@@ -38,11 +38,8 @@ __device__ __forceinline__ uint32_t fp8_row_max(uint32_t x) {
 
 // A lane's 8 elements, whose block the 16 lanes of its row share: codes and
 // the scale's byte.
-__device__ __forceinline__ u32x2 fp8_encode(const float (&x)[8], uint32_t &byte) {
-  uint32_t big = 0;
-#pragma unroll
-  for (int j = 0; j < 8; j++) big = max(big, e4m3_size(x[j]));
-  byte = e4m3_exponent(fp8_row_max(big));
+__device__ __forceinline__ u32x2 fp8_encode(float (&x)[8], uint32_t &byte) {
+  byte = e4m3_exponent(fp8_row_max(e4m3_largest(x)));
   const float scale = e4m3_scale(byte);
   return u32x2{e4m3_codes(x[0], x[1], x[2], x[3], scale), e4m3_codes(x[4], x[5], x[6], x[7], scale)};
 }
@@ -150,23 +147,40 @@ __device__ __forceinline__ void fp8_dequantize(const fk_fp8_dequantize_args &a) 
   }
 }
 
-// The row of a threadgroup of the norm: the 16 rows of a tile, whose codes
-// share lines of memory, on one XCD (a launch's threadgroups go to the 8 in
-// turn), so that each line is whole in one L2 before it leaves.
+// The norm: s = x + residual, y = s / sqrt(mean(s^2) + eps) * gamma, as codes.
+// A row is held in registers from the first load to the codes, so that it is
+// read once: 16 lanes a block of 128, H blocks a lane, and a wavefront's four 16s
+// four blocks of one row or, with ROWS 2, two of two rows.  Bound by what it moves:
+// 7 bytes an element of bf16 with a residual and the sum (a copy reaches 5 to
+// 6 TB/s).  A lane's 8 codes are half of a piece of 16, 256 bytes from the row's
+// next, so that a row's codes leave as many short writes; two rows' pieces lie
+// together.  The 16 rows of a tile go to threadgroups on one XCD (a launch's go to
+// the 8 in turn), so that each line of codes is whole in one L2 before it leaves.
+//   8191 x 5000 bf16: 65 us, 4.4 TB/s (one row a threadgroup, 2 blocks a lane 67,
+//   1 or 4 blocks 74; four rows 92: too few of so large threadgroups fit a CU);
+//   8192 x 4096 47 us, 5.0 TB/s (one row 52, four 48); 8 x 2048 f32 3.5 us.
+template <uint32_t ROWS>
 __device__ __forceinline__ uint32_t fp8_norm_row(uint32_t group) {
+  constexpr uint32_t each = 16 / ROWS;
   const uint32_t i = group / 8;
-  return (i / 16 * 8 + group % 8) * 16 + i % 16;
+  return (i / each * 8 + group % 8) * 16 + i % each * ROWS;
 }
 
-// A row's sum over a threadgroup, the same in every thread.
-__device__ __forceinline__ float fp8_norm_sum(float x, float *slots) {
-  x = wave_sum(x);
-  const uint32_t waves = blockDim.x / FK_WAVE;
-  if (waves == 1) return x;
-  if (threadIdx.x % FK_WAVE == 0) slots[threadIdx.x / FK_WAVE] = x;
+// A row's sum over a threadgroup, the same in every lane of the row.
+template <uint32_t ROWS>
+__device__ __forceinline__ float fp8_norm_sum(float x, float (&slots)[16][4]) {
+  x = x + dpp_f<0xB1>(x);
+  x = x + dpp_f<0x4E>(x);
+  x = x + dpp_f<0x141>(x);
+  x = x + dpp_f<0x140>(x);
+  const uint32_t lane = threadIdx.x % FK_WAVE, waves = blockDim.x / FK_WAVE;
+  if (lane % 16 == 0) slots[threadIdx.x / FK_WAVE][lane / 16] = x;
   __syncthreads();
-  float sum = slots[0];
-  for (uint32_t w = 1; w < waves; w++) sum += slots[w];
+  float sum = 0.0f;
+  for (uint32_t w = 0; w < waves; w++) {
+    if constexpr (ROWS == 2) sum += slots[w][lane / 32 * 2] + slots[w][lane / 32 * 2 + 1];
+    else sum += (slots[w][0] + slots[w][1]) + (slots[w][2] + slots[w][3]);
+  }
   return sum;
 }
 
@@ -178,38 +192,29 @@ __device__ __forceinline__ float fp8_rounded(float x) {
   else return (float)(__bf16)x;
 }
 
-// A row of T, H pieces of 8 elements a thread, held from the first load to the
-// codes: piece t + i threads.
-template <int T, uint32_t H>
+template <int T, uint32_t ROWS, uint32_t H>
 __device__ __forceinline__ void fp8_add_norm(const fk_fp8_add_norm_args &a) {
-  __shared__ float slots[16];
-  const uint32_t row = fp8_norm_row(blockIdx.x);
-  const uint32_t blocks = fp8_blocks(a.k), quads = fp8_quads(a.k), pieces = 16 * blocks;
-  const uint32_t threads = blockDim.x;
-  if (row >= 16 * fp8_row_tiles(a.rows)) return;
-  const uint64_t scales = a.scales + fp8_scale_at(row, 0, quads);
-  // the bytes of the blocks that fill the last four up
-  if (threadIdx.x < 4 * quads - blocks)
-    *global_at<uint8_t>(scales + (uint64_t)(quads - 1) * 64 + (3 - threadIdx.x)) = 127;
-  if (row >= a.rows) {
-    for (uint32_t i = threadIdx.x; i < pieces; i += threads) {
-      *global_at<u32x2>(a.codes + fp8_code_at(row, i, blocks)) = u32x2{0, 0};
-      if (i % 16 == 0) *global_at<uint8_t>(a.scales + fp8_scale_at(row, i / 16, quads)) = 127;
-    }
-    return;
-  }
+  __shared__ float slots[16][4];
   constexpr uint32_t B = mx4_bytes_of(T);
+  const uint32_t blocks = fp8_blocks(a.k), quads = fp8_quads(a.k), waves = blockDim.x / FK_WAVE;
+  const uint32_t lane = threadIdx.x % FK_WAVE, wave = threadIdx.x / FK_WAVE;
+  const uint32_t row = fp8_norm_row<ROWS>(blockIdx.x) + (lane / 16 * ROWS / 4);
+  if (row >= 16 * fp8_row_tiles(a.rows)) return;  // (whole threadgroups)
+  const bool there = row < a.rows;
+  // The blocks of a lane, and its piece of each.
+  auto block_of = [&](uint32_t i) { return 4 / ROWS * (wave + i * waves) + lane / 16 % (4 / ROWS); };
+  const uint32_t within = 8 * (lane % 16);
   float h[H][8], r[H][8];
 #pragma unroll
   for (uint32_t i = 0; i < H; i++) {
-    const uint32_t col = 8 * (threadIdx.x + i * threads);
-    fp8_load8<T, false>(a.x + row * a.x_stride * B, col, a.k, h[i]);
-    if (a.residual) fp8_load8<T, false>(a.residual + row * a.residual_stride * B, col, a.k, r[i]);
+    const uint32_t col = there ? 128 * block_of(i) + within : a.k;
+    fp8_load8<T, true>(a.x + row * a.x_stride * B, col, a.k, h[i]);
+    if (a.residual) fp8_load8<T, true>(a.residual + row * a.residual_stride * B, col, a.k, r[i]);
   }
   float squares = 0.0f;
 #pragma unroll
   for (uint32_t i = 0; i < H; i++) {
-    const uint32_t col = 8 * (threadIdx.x + i * threads);
+    const uint32_t col = there ? 128 * block_of(i) + within : a.k;
     if (a.residual) {
 #pragma unroll
       for (int j = 0; j < 8; j++) h[i][j] = fp8_rounded<T>(h[i][j] + r[i][j]);
@@ -218,30 +223,34 @@ __device__ __forceinline__ void fp8_add_norm(const fk_fp8_add_norm_args &a) {
 #pragma unroll
     for (int j = 0; j < 8; j++) squares += h[i][j] * h[i][j];
   }
-  const float mean = fp8_norm_sum(squares, slots) / (float)a.k;
+  const float mean = fp8_norm_sum<ROWS>(squares, slots) / (float)a.k;
   const float scale = 1.0f / __builtin_sqrtf(mean + a.eps);
 #pragma unroll
   for (uint32_t i = 0; i < H; i++) {
-    const uint32_t piece = threadIdx.x + i * threads;
-    if (piece >= pieces) break;  // (16 lanes together)
+    const uint32_t block = block_of(i), col = 128 * block + within;
+    if (block >= blocks) break;  // (the 16 lanes of a block together)
     float g[8];
     if (a.gamma) {
-      fp8_load8<FK_T_F32, false>(a.gamma, 8 * piece, a.k, g);
+      fp8_load8<FK_T_F32, false>(a.gamma, col, a.k, g);
 #pragma unroll
       for (int j = 0; j < 8; j++) h[i][j] = h[i][j] * scale * g[j];
     } else {
 #pragma unroll
       for (int j = 0; j < 8; j++) h[i][j] = h[i][j] * scale;
     }
-    if (8 * piece + 8 > a.k) {
-      // (what lies behind the row is 0 whatever the row's factor)
+    if (!there || col + 8 > a.k) {
+      // (what lies behind the rows and the row is 0 whatever the factor)
 #pragma unroll
-      for (uint32_t j = 0; j < 8; j++) h[i][j] = 8 * piece + j < a.k ? h[i][j] : 0.0f;
+      for (uint32_t j = 0; j < 8; j++) h[i][j] = there && col + j < a.k ? h[i][j] : 0.0f;
     }
     uint32_t byte;
     const u32x2 codes = fp8_encode(h[i], byte);
-    *global_at<u32x2>(a.codes + fp8_code_at(row, piece, blocks)) = codes;
-    if (piece % 16 == 0) *global_at<uint8_t>(a.scales + fp8_scale_at(row, piece / 16, quads)) = (uint8_t)byte;
+    *global_at<u32x2>(a.codes + fp8_code_at(row, col / 8, blocks)) = codes;
+    // (the last block's lanes 1 to 3 write the scales of those that fill its four up)
+    const uint32_t scaled = block + lane % 16;
+    if (lane % 16 == 0 || (block == blocks - 1 && scaled < 4 * quads))
+      *global_at<uint8_t>(a.scales + fp8_scale_at(row, scaled, quads)) =
+          (uint8_t)(lane % 16 == 0 && there ? byte : 127u);
   }
 }
 

@@ -4,11 +4,20 @@
 // The store.  A block's scale needs the largest magnitude of its new rows
 // before the first code, so W wavefronts take a run (the step's tokens of one
 // block) for one head's keys or values: they make the rows, hold them in
-// registers where the run is at most 2 pieces a thread, meet at the largest,
+// registers where the run is at most a piece a thread, meet at the largest,
 // and write the codes.  Rows held before a scale that grew are brought to it
 // by the same wavefronts; the scales are powers of two, so only codes that fall
 // below the new scale's smallest step change their value.  The queries are
 // elementwise and go to threadgroups of their own in the same launch.
+//
+// Bound by what it moves (a head's row of bf16: 3 bytes an element of k and v, 4
+// of q) where there are many tokens, by its chain of loads (slots; rows and
+// turns; then the codes) where there are few.  6443 tokens of 32 + 16 heads of 128
+// in blocks of 16: 30.3 us, 4.8 TB/s (its queries alone 22.7, its runs alone
+// 16.9; with two pieces a thread, and so half the wavefronts, and each token's slot
+// and position read where they are used, 43.6).  8 tokens: 3.8 us.
+// The load is bound by its writes: 32767 tokens of 8 heads of 128 to bf16 31.6 us,
+// 6.4 TB/s.
 #pragma once
 
 #include "fk_divisor.h"
@@ -16,8 +25,6 @@
 #include "fk_paged_store.h"
 
 #include "../../../include/fkrocm_paged8.h"
-
-#define FK_STORE8_HELD 2  // pieces of 8 and 8 elements a thread holds
 
 namespace fk {
 
@@ -28,17 +35,21 @@ struct Store8Plan {
   uint32_t chunk;       // tokens whose runs (begun among them) a run's wavefronts take
 };
 
+// A token's position, if there are any.
+__device__ __forceinline__ uint32_t store8_position(const fk_paged_store8_args &a, uint32_t token) {
+  return a.rotated ? global_at<const uint32_t>(a.positions)[token] : 0u;
+}
+
 // T: the rows' type.  One piece of a row: elements e .. e + 7 of a head and
 // those half a head further, turned if they are a query's or a key's.
 template <int T>
 __device__ __forceinline__ void store8_piece(const fk_paged_store8_args &a, uint64_t rows, uint64_t stride,
-                                             uint32_t token, uint32_t head, uint32_t e, bool turned, float (&x)[8],
-                                             float (&y)[8]) {
+                                             uint32_t token, uint32_t position, uint32_t head, uint32_t e,
+                                             bool turned, float (&x)[8], float (&y)[8]) {
   const uint64_t at = token * stride + head * a.head_dim + e;
   load8<T>(rows, at, x);
   load8<T>(rows, at + a.head_dim / 2, y);
-  if (turned && e < a.rotated)
-    store_turn(a.rope, min(global_at<const uint32_t>(a.positions)[token], a.rope_rows - 1), a.rotated, e, x, y);
+  if (turned && e < a.rotated) store_turn(a.rope, min(position, a.rope_rows - 1), a.rotated, e, x, y);
 }
 
 template <int T, bool BF16>
@@ -50,7 +61,7 @@ __device__ __forceinline__ void store8_queries(const fk_paged_store8_args &a, ui
   const uint32_t u = i - token * units, h = u / per, e = 8 * (u - h * per);
   const uint32_t slot = global_at<const uint32_t>(a.slots)[token];
   float x[8], y[8];
-  store8_piece<T>(a, a.q, a.q_stride, token, h, e, true, x, y);
+  store8_piece<T>(a, a.q, a.q_stride, token, store8_position(a, token), h, e, true, x, y);
   if (slot >= a.blocks * a.block_size) return;
   const uint64_t to = a.qr + 2 * (((uint64_t)token * a.heads + h) * a.head_dim + e);
   store8<BF16>(to, x);
@@ -68,7 +79,7 @@ __device__ __forceinline__ uint32_t wave_most(uint32_t v) {
   return max(a, b);
 }
 
-// W wavefronts a run: 1 (four runs' a threadgroup), 4 or 8.
+// W wavefronts a run: 1 (four runs' a threadgroup), 2, 4 or 8.
 template <int T, uint32_t W>
 __device__ __forceinline__ void store8_runs(const fk_paged_store8_args &a, const Store8Plan &pl) {
   __shared__ uint32_t most[W];
@@ -92,57 +103,67 @@ __device__ __forceinline__ void store8_runs(const fk_paged_store8_args &a, const
   constexpr uint32_t NONE = 0xFFFFFFFFu;
   auto block_of = [&](uint32_t slot) { return slot < places ? quotient(slot, pl.block) : NONE; };
 
-  // The chunk's tokens that begin runs, a lane each.
-  uint64_t begins;
-  {
-    const uint32_t t = first + lane;
-    const bool mine = lane < pl.chunk && t < tokens;
-    const uint32_t here = mine ? block_of(slots[t]) : NONE;
-    const uint32_t before = mine && t > 0 ? block_of(slots[t - 1]) : NONE;
-    begins = __builtin_amdgcn_ballot_w64(here != NONE && here != before);
-  }
+  // 64 tokens from `base` on, a lane each: what the runs within them need of
+  // them is read once, and together.
+  uint32_t base = first, my_slot, my_block, my_position;
+  auto look = [&]() {
+    const uint32_t t = min(base + lane, tokens - 1);
+    my_slot = slots[t];
+    my_position = is_v ? 0u : store8_position(a, t);
+    my_block = block_of(my_slot);
+  };
+  const uint32_t before = slots[max(min(first + lane, tokens - 1), 1u) - 1];
+  look();
+  // The chunk's tokens that begin runs.
+  const uint32_t my_token = first + lane;
+  uint64_t begins = __builtin_amdgcn_ballot_w64(lane < pl.chunk && my_token < tokens && my_block != NONE &&
+                                                (my_token == 0 || my_block != block_of(before)));
+  const uint32_t my_row = thread / per, my_e = 8 * (thread - my_row * per);
   for (; begins; begins &= begins - 1) {
     const uint32_t t0 = first + __builtin_ctzll(begins);
-    const uint32_t slot0 = __builtin_amdgcn_readfirstlane(slots[t0]);
-    const uint32_t block = quotient(slot0, pl.block), place0 = slot0 - block * a.block_size;
-    uint32_t n = 0;  // its tokens
-    for (;;) {
-      const uint32_t t = t0 + n + lane;
-      const uint64_t same = __builtin_amdgcn_ballot_w64(t < tokens && block_of(slots[min(t, tokens - 1)]) == block);
-      if (~same == 0) {
-        n += 64;
-      } else {
-        n += __builtin_ctzll(~same);
-        break;
+    const uint32_t block = __builtin_amdgcn_readlane((int)my_block, (int)(t0 - base));
+    // Its tokens from `from` on among the 64 that the lanes hold there.
+    auto tokens_at = [&](uint32_t from) {
+      const uint64_t run = __builtin_amdgcn_ballot_w64(base + lane < tokens && my_block == block) >> (from - base);
+      return ~run ? (uint32_t)__builtin_ctzll(~run) : 64u;
+    };
+    uint32_t n = tokens_at(t0);
+    if (t0 != base && t0 + n == base + 64) {  // a run that may go on: the lanes from its start
+      base = t0;
+      look();
+      n = tokens_at(t0);
+    }
+    const uint32_t offset = t0 - base;
+    const uint32_t place0 = (uint32_t)__builtin_amdgcn_readlane((int)my_slot, (int)offset) - block * a.block_size;
+    if (n == 64) {
+      uint64_t run;
+      for (;; n += 64) {
+        const uint32_t t = t0 + n + lane;
+        run = __builtin_amdgcn_ballot_w64(t < tokens && block_of(slots[min(t, tokens - 1)]) == block);
+        if (~run) break;
       }
+      n += __builtin_ctzll(~run);
     }
     const uint64_t at = (uint64_t)block * a.kv_heads + head;
     const auto scale_at = global_at<uint32_t>(a.scales + 8 * at + 4 * is_v);
     const uint32_t old = place0 ? *scale_at : 0u;
     const uint32_t pieces = n * per;
-    float x[FK_STORE8_HELD][8], y[FK_STORE8_HELD][8];
-    auto make = [&](uint32_t i, float (&u)[8], float (&v)[8]) {
-      const uint32_t row = i / per;
-      store8_piece<T>(a, rows, stride, t0 + row, head, 8 * (i - row * per), !is_v, u, v);
+    float x[8], y[8];
+    auto make = [&](uint32_t row, uint32_t e, uint32_t position) {
+      store8_piece<T>(a, rows, stride, t0 + row, position, head, e, !is_v, x, y);
+      return max(e4m3_largest(x), e4m3_largest(y));
     };
-    auto largest = [&](const float (&u)[8], const float (&v)[8], uint32_t big) {
-#pragma unroll
-      for (int j = 0; j < 8; j++) big = max(big, max(e4m3_size(u[j]), e4m3_size(v[j])));
-      return big;
-    };
-    const bool held = pieces <= FK_STORE8_HELD * THREADS;
-    uint32_t big = 0;
+    const bool held = pieces <= THREADS && n <= 64;
+    uint32_t big = 0, my_place = 0;  // (the place of the thread's row if the run is held)
     if (held) {
-#pragma unroll
-      for (uint32_t h = 0; h < FK_STORE8_HELD; h++)
-        if (thread + h * THREADS < pieces) {
-          make(thread + h * THREADS, x[h], y[h]);
-          big = largest(x[h], y[h], big);
-        }
+      const int from = 4 * (int)(offset + min(my_row, n - 1));
+      my_place = (uint32_t)__builtin_amdgcn_ds_bpermute(from, (int)my_slot) - block * a.block_size;
+      const uint32_t position = (uint32_t)__builtin_amdgcn_ds_bpermute(from, (int)my_position);
+      if (thread < pieces) big = make(my_row, my_e, position);
     } else {
       for (uint32_t i = thread; i < pieces; i += THREADS) {
-        make(i, x[0], y[0]);
-        big = largest(x[0], y[0], big);
+        const uint32_t row = i / per;
+        big = max(big, make(row, 8 * (i - row * per), is_v ? 0u : store8_position(a, t0 + row)));
       }
     }
     big = wave_most(big);
@@ -174,21 +195,19 @@ __device__ __forceinline__ void store8_runs(const fk_paged_store8_args &a, const
         *p = w;
       }
     }
-    auto put = [&](uint32_t i, const float (&u)[8], const float (&v)[8]) {
-      const uint32_t row = i / per, e = 8 * (i - row * per);
-      const uint64_t to = pool + (at * a.block_size + (slots[t0 + row] - block * a.block_size)) * d + e;
-      *global_at<u32x2>(to) = u32x2{e4m3_codes(u[0], u[1], u[2], u[3], scale), e4m3_codes(u[4], u[5], u[6], u[7], scale)};
+    auto put = [&](uint32_t place, uint32_t e) {
+      const uint64_t to = pool + (at * a.block_size + place) * d + e;
+      *global_at<u32x2>(to) = u32x2{e4m3_codes(x[0], x[1], x[2], x[3], scale), e4m3_codes(x[4], x[5], x[6], x[7], scale)};
       *global_at<u32x2>(to + d / 2) =
-          u32x2{e4m3_codes(v[0], v[1], v[2], v[3], scale), e4m3_codes(v[4], v[5], v[6], v[7], scale)};
+          u32x2{e4m3_codes(y[0], y[1], y[2], y[3], scale), e4m3_codes(y[4], y[5], y[6], y[7], scale)};
     };
     if (held) {
-#pragma unroll
-      for (uint32_t h = 0; h < FK_STORE8_HELD; h++)
-        if (thread + h * THREADS < pieces) put(thread + h * THREADS, x[h], y[h]);
+      if (thread < pieces) put(my_place, my_e);
     } else {
       for (uint32_t i = thread; i < pieces; i += THREADS) {
-        make(i, x[0], y[0]);
-        put(i, x[0], y[0]);
+        const uint32_t row = i / per, e = 8 * (i - row * per);
+        make(row, e, is_v ? 0u : store8_position(a, t0 + row));
+        put(slots[t0 + row] - block * a.block_size, e);
       }
     }
     if constexpr (W > 1) __syncthreads();  // the largest are read before the next run's

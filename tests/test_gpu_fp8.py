@@ -195,6 +195,13 @@ def test_add_norm(device, mem, n, k, kind):
 
 
 @pytest.mark.parametrize("kind", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("n,k", [(1024, 2049), (1033, 2600), (2049, 4100), (1030, 8192), (1025, 2048)])
+def test_add_norm_of_rows_that_fill_the_card(device, mem, n, k, kind):
+    print(f"norm {n} {k} {kind}", flush=True)
+    hold_norm(device, mem, np.random.default_rng(n + k), n, k, kind, gamma=kind != "f16", pads=(0, 8, 16))
+
+
+@pytest.mark.parametrize("kind", ["f32", "f16", "bf16"])
 @pytest.mark.parametrize("residual,gamma,over,pads", [
     (False, True, "none", (0, 0, 0)), (False, False, "", (3, 0, 5)), (True, True, "none", (1, 3, 0)),
     (True, False, "x", (7, 2, 0)), (True, True, "residual", (1, 8, 0)), (False, True, "x", (0, 0, 0)),

@@ -112,6 +112,15 @@ def test_store_bit_for_bit(device, mem, wants, heads, kv, d, block, rows_type, q
         hold_store(device, mem, rng, wants, heads, kv, d, block, rows_type, q_type, rotated, pad)
 
 
+@pytest.mark.parametrize("wants,kv,d,block", [
+    ([700, 1, 64, 39, 41, 1] * 12, 32, 16, 40), ([130, 1, 1, 63] * 50, 32, 16, 64), ([900, 2] * 10, 33, 32, 136),
+    ([1] * 9000, 32, 16, 8), ([3000, 1, 77], 64, 48, 72)])
+def test_store_of_many_tokens_a_wavefront(device, mem, wants, kv, d, block):
+    """Up to 64 tokens whose runs a wavefront takes, runs within them and past them."""
+    print(f"store8 {wants[:6]} {kv} {d} {block}", flush=True)
+    hold_store(device, mem, np.random.default_rng(block), wants, 2, kv, d, block, "bf16", "f16", d // 4)
+
+
 def test_store_without_queries_again_and_of_no_tokens(device, mem):
     rng = np.random.default_rng(4)
     hold_store(device, mem, rng, [5, 40, 1], 2, 2, 64, 16, "f32", "f16", 32, queries=False)
