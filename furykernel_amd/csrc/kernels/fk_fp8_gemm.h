@@ -17,7 +17,7 @@
 // by up to 7 2^-14 of such a largest product: 1 to 5 10^-5 of C for normal
 // rows, with some columns 20 times as large.  C of 16 bits, rounded at 2^-9 or
 // 2^-12, takes that for twice the rate.  C of f32 does not: its operands are
-// widened to bf16, scales and all, which is exact, and go to
+// widened to bf16, scales and all, which is exact from 2^-126 on, and go to
 // v_mfma_f32_16x16x32_bf16 and 32x32x16, whose sums are binary32's.
 #pragma once
 

@@ -364,6 +364,18 @@ def test_products_of_scales_at_their_ends(device, mem, kind):
     assert np.all(np.abs(got - want) <= (2.0 ** -7 if kind == "bf16" else 2.0 ** -15) * size)
 
 
+@pytest.mark.parametrize("m,n", [(20, 40), (300, 520), (1100, 1030)])
+def test_f32_products_of_the_smallest_scale(device, mem, m, n):
+    """Elements below 2^-126, which bfloat16 holds in part or not at all: 2^-126
+    times the other operand's at most from each."""
+    rng = np.random.default_rng(9)
+    a, b = random_matrix(rng, m, 256, 0), random_matrix(rng, n, 256, 0)
+    a, b = (a[0], np.full_like(a[1], 2.0 ** -126)), (b[0], np.full_like(b[1], 2.0 ** 112))
+    got, (av, bv) = product(device, mem, a, b, m, n, 256, "f32"), (F.values(*x, 256) for x in (a, b))
+    tol = 256 * 2.0 ** -23 * (np.abs(av) @ np.abs(bv).T) + 2.0 ** -126 * np.abs(bv).sum(1)
+    assert np.all(np.abs(got - av @ bv.T) <= tol)
+
+
 def test_a_nan_is_its_row_and_columns_only(device, mem):
     rng = np.random.default_rng(8)
     for m, n, kind in ((20, 50, "f32"), (20, 50, "f16"), (600, 700, "f32"), (600, 700, "bf16")):

@@ -485,6 +485,40 @@ def test_attend_past_4_gib_of_pool(device, mem):
             assert np.array_equal(g, values[b, :, place].astype(np.float32), equal_nan=True), i
 
 
+@pytest.mark.parametrize("block", [16, 64])
+def test_store_past_4_gib_of_pool(device, mem, block):
+    """Runs that begin a block and that go on in one, past 32 bits of offset."""
+    kv, d, blocks = 8, 128, 5200000 // block           # 5.3 GB a pool
+    rng, bytes_of = np.random.default_rng(11), kv * block * d
+    far, begun = [blocks - 1, blocks - 70000 // block, 1], np.array([0, 5, 7])
+    codes, scales = zip(*(held_pool(rng, 3, kv, block, d, begun, np.ones(3)) for _ in "kv"))
+    bufs = {n: mem.keep(device.alloc(blocks * bytes_of)) for n in ("kpool", "vpool")}
+    bufs["scales"] = mem.keep(device.alloc(blocks * kv * 8))
+    for i, b in enumerate(far):
+        for n, c in zip(("kpool", "vpool"), codes):
+            bufs[n].write(c[i], offset=b * bytes_of)
+        bufs["scales"].write(np.stack([s[i] for s in scales], -1).astype(np.float32), offset=b * kv * 8)
+    place = [(i, p) for i, first in enumerate(begun) for p in range(first, 8)]
+    x = (rng.standard_normal((len(place), 2 * kv * d)) * 4).astype(np.float32)
+    want = [c.copy() for c in codes]
+    want_scales = [s.copy() for s in scales]
+    for j, (w, s) in enumerate(zip(want, want_scales)):
+        F.store(x[:, j * kv * d:(j + 1) * kv * d].reshape(-1, kv, d),
+                np.array([i * block + p for i, p in place], np.uint32), w, s, block)
+    slots = np.array([far[i] * block + p for i, p in place], np.uint32)
+    row = mem.put(x)
+    paged8.PagedStore8(device, k=row, v=row, **bufs, slots=mem.put(slots), v_offset=kv * d, k_stride=2 * kv * d,
+                       v_stride=2 * kv * d, tokens=len(place), kv_heads=kv, head_dim=d, block_size=block,
+                       blocks=blocks).enqueue()
+    device.sync()
+    for i, b in enumerate(far):
+        for n, w in zip(("kpool", "vpool"), want):
+            got = bufs[n].read(np.uint8, bytes_of, offset=b * bytes_of).reshape(w[i].shape)
+            assert np.all(F.same_codes(got, w[i])), (i, n)
+        got = bufs["scales"].read(np.float32, 2 * kv, offset=b * kv * 8).reshape(kv, 2)
+        assert np.array_equal(got, np.stack([s[i] for s in want_scales], -1).astype(np.float32)), i
+
+
 # A run of them ---------------------------------------------------------------------
 
 
