@@ -111,19 +111,21 @@ struct Form {
 //               all threadgroups read
 //   mid, many   base, `tile` a turn, and for each block of k the largest of `step`
 //               (its latency), `turn` a turn and `work` a threadgroup of each CU
-// The form of the least cost takes 1.013 (f32 1.005) times the fastest one's
-// time on average over them, at most 1.40 (8192 rows by 5000, k 512: 46 µs, mid
-// 33; f32 1.22).
+// The form of the least cost takes 1.014 (f32 1.007) times the fastest one's
+// time on average over them, at most 1.33 (8192 rows by 5000, k 512: 48 µs, mid
+// 36; f32 88 and 66).
 constexpr Form forms[] = {
-    {"few 1x1", FEW, 1, 1, 8, 0, {{1.837, 0.282, 0.241, 0.036, 0.116}, {1.889, 0.253, 0.292, 0.138, 0.099}}},
-    {"few 2x1", FEW, 2, 1, 8, 0, {{1.640, 0.353, 0.423, 0.184, 0.077}, {1.501, 0.331, 0.492, 0.383, 0.069}}},
-    {"few 2x2", FEW, 2, 2, 8, 0, {{1.967, 0.184, 0.913, 0.009, 0.073}, {1.117, 0.311, 0.823, 0.977, 0.079}}},
-    {"few 4x2", FEW, 4, 2, 4, 0, {{1.903, 0, 0.755, 0.679, 0.029}, {1.997, 0.033, 0.783, 0.864, 0.026}}},
-    {"few 8x2", FEW, 8, 2, 8, 0, {{0.137, 0.323, 2.090, 1.823, 0.028}, {-1, 0, 0, 0, 0}}},
-    {"mid 8x8", MID, 8, 8, 0, 3, {{0.416, 0.761, 0.572, 1.831, 0.487}, {0.825, 0.930, 0.743, 3.080, 0.816}}},
-    {"mid 8x8 deep", MID, 8, 8, 0, 8, {{0.657, 0.436, 0.502, 3.304, 0.759}, {0.331, 0.532, 0.823, 4.938, 1.077}}},
-    {"mid 4x8 deep", MID, 4, 8, 0, 10, {{0.978, 0.098, 0.403, 2.276, 0.603}, {1.337, 0.301, 0.551, 2.981, 0.727}}},
-    {"many 16x16", MANY, 16, 16, 0, 0, {{0, 0.573, 1.209, 8.095, 1.599}, {0, 2.339, 2.355, 12.070, 3.078}}},
+    {"few 1x1", FEW, 1, 1, 8, 0, {{1.861, 0.270, 0.254, 0.025, 0.114}, {1.914, 0.238, 0.302, 0.132, 0.099}}},
+    {"few 2x1", FEW, 2, 1, 8, 0, {{1.664, 0.341, 0.438, 0.167, 0.077}, {1.507, 0.349, 0.485, 0.384, 0.067}}},
+    {"few 2x2", FEW, 2, 2, 8, 0, {{1.954, 0.168, 0.933, 0, 0.074}, {1.274, 0.200, 0.942, 0.825, 0.076}}},
+    {"few 4x2", FEW, 4, 2, 4, 0, {{1.898, 0, 0.755, 0.684, 0.030}, {2.024, 0.040, 0.777, 0.856, 0.026}}},
+    {"few 8x2", FEW, 8, 2, 8, 0, {{0.100, 0.357, 2.063, 1.846, 0.029}, {-1, 0, 0, 0, 0}}},
+    {"few 4x3", FEW, 4, 3, 8, 0, {{0.373, 0.456, 1.320, 1.762, 0.071}, {0.140, 0.471, 1.245, 2.318, 0.091}}},
+    {"few 4x4", FEW, 4, 4, 8, 0, {{0.019, 0.327, 1.755, 2.398, 0.081}, {0, 0.604, 1.545, 2.883, 0.099}}},
+    {"mid 8x8", MID, 8, 8, 0, 3, {{0.299, 0.762, 0.581, 1.930, 0.303}, {0.463, 0.945, 0.775, 3.474, 0.816}}},
+    {"mid 8x8 deep", MID, 8, 8, 0, 8, {{0.678, 0.491, 0.505, 3.238, 0.776}, {0.464, 0.747, 0.822, 4.858, 1.119}}},
+    {"mid 4x8 deep", MID, 4, 8, 0, 10, {{0.985, 0.093, 0.403, 2.246, 0.601}, {1.367, 0.159, 0.561, 2.909, 0.742}}},
+    {"many 16x16", MANY, 16, 16, 0, 0, {{0, 0.599, 1.197, 8.499, 1.648}, {0, 0.934, 2.391, 12.069, 3.153}}},
 };
 
 uint64_t tiles_of(const Form &f, uint32_t m, uint32_t n) {

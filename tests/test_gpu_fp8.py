@@ -315,6 +315,21 @@ def test_products_of_every_form(device, mem, kind):
 
 
 @pytest.mark.parametrize("kind", ["f32", "f16", "bf16"])
+def test_each_forms_products(device, mem, kind):
+    """Odd sizes of every form of the rule's, by its name."""
+    sizes = [(3, 509, 130), (17, 3001, 130), (17, 5003, 130), (47, 5003, 130), (17, 9001, 300), (97, 8190, 515),
+             (299, 3001, 8190), (799, 1013, 130), (4099, 3001, 130), (17, 16390, 130), (97, 16390, 130),
+             (3, 16390, 130), (3, 16390, 1030), (97, 16390, 1030), (97, 16390, 2060)]
+    names = {"few 1x1", "few 2x1", "few 2x2", "few 4x2", "few 4x3", "few 4x4", "mid 8x8", "mid 8x8 deep",
+             "mid 4x8 deep", "many 16x16"} | (set() if kind == "f32" else {"few 8x2"})
+    assert {fp8.gemm_form(*s, kind) for s in sizes} == names
+    for s in sizes:
+        rng = np.random.default_rng(s[1])
+        a, b = random_matrix(rng, s[0], s[2], 3), random_matrix(rng, s[1], s[2], 3)
+        hold_values(device, mem, (a[0], a[1] * 2.0 ** -14), b, *s, kind, 3)
+
+
+@pytest.mark.parametrize("kind", ["f32", "f16", "bf16"])
 @pytest.mark.parametrize("m,n,k", [(7, 130, 1100), (130, 260, 1100), (600, 700, 1100), (2050, 1030, 1100)])
 def test_whole_number_products_are_exact(device, mem, m, n, k, kind):
     """Small whole numbers, scales of 1/2 to 2 a block: every product and partial
