@@ -104,28 +104,31 @@ struct Form {
   } cost[2];
 };
 // What each costs, in µs, fitted to its times on 221 products (1 to 8192 rows by
-// 512 to 16384, k of 512 to 8192, the operands from memory each time).  With
+// 512 to 16384, k of 512 to 8192, the operands from memory each time), then
+// moved, each no further from its times than by 6 % of the fit's own misses, to
+// where the least cost names the fastest form most often.  With
 // `turns` the threadgroups of the CU that has most,
 //   few         base, for each block of k a wavefront takes `step` and `turn` a
 //               turn, `tile` a turn, and `work` for a thousand tiles of 2 KB that
 //               all threadgroups read
 //   mid, many   base, `tile` a turn, and for each block of k the largest of `step`
 //               (its latency), `turn` a turn and `work` a threadgroup of each CU
-// The form of the least cost takes 1.014 (f32 1.007) times the fastest one's
-// time on average over them, at most 1.33 (8192 rows by 5000, k 512: 48 µs, mid
-// 36; f32 88 and 66).
+// The form of the least cost takes 1.004 (f32 1.003) times the fastest one's
+// time on average over them, at most 1.13; over 96 others (3 to 6000 rows by 1000,
+// 4096 and 12000, k of 1024 to 12288) 1.011 (1.005), at most 1.16.
 constexpr Form forms[] = {
-    {"few 1x1", FEW, 1, 1, 8, 0, {{1.861, 0.270, 0.254, 0.025, 0.114}, {1.914, 0.238, 0.302, 0.132, 0.099}}},
-    {"few 2x1", FEW, 2, 1, 8, 0, {{1.664, 0.341, 0.438, 0.167, 0.077}, {1.507, 0.349, 0.485, 0.384, 0.067}}},
-    {"few 2x2", FEW, 2, 2, 8, 0, {{1.954, 0.168, 0.933, 0, 0.074}, {1.274, 0.200, 0.942, 0.825, 0.076}}},
-    {"few 4x2", FEW, 4, 2, 4, 0, {{1.898, 0, 0.755, 0.684, 0.030}, {2.024, 0.040, 0.777, 0.856, 0.026}}},
-    {"few 8x2", FEW, 8, 2, 8, 0, {{0.100, 0.357, 2.063, 1.846, 0.029}, {-1, 0, 0, 0, 0}}},
-    {"few 4x3", FEW, 4, 3, 8, 0, {{0.373, 0.456, 1.320, 1.762, 0.071}, {0.140, 0.471, 1.245, 2.318, 0.091}}},
-    {"few 4x4", FEW, 4, 4, 8, 0, {{0.019, 0.327, 1.755, 2.398, 0.081}, {0, 0.604, 1.545, 2.883, 0.099}}},
-    {"mid 8x8", MID, 8, 8, 0, 3, {{0.299, 0.762, 0.581, 1.930, 0.303}, {0.463, 0.945, 0.775, 3.474, 0.816}}},
-    {"mid 8x8 deep", MID, 8, 8, 0, 8, {{0.678, 0.491, 0.505, 3.238, 0.776}, {0.464, 0.747, 0.822, 4.858, 1.119}}},
-    {"mid 4x8 deep", MID, 4, 8, 0, 10, {{0.985, 0.093, 0.403, 2.246, 0.601}, {1.367, 0.159, 0.561, 2.909, 0.742}}},
-    {"many 16x16", MANY, 16, 16, 0, 0, {{0, 0.599, 1.197, 8.499, 1.648}, {0, 0.934, 2.391, 12.069, 3.153}}},
+    {"few 1x1", FEW, 1, 1, 8, 0, {{1.853, 0.397, 0.099, 0.093, 0.139}, {1.754, 0.219, 0.317, 0.208, 0.091}}},
+    {"few 1x2", FEW, 1, 2, 8, 0, {{2.075, 0.191, 0.543, 0.096, 0.120}, {1.965, 0.292, 0.520, 0.257, 0.124}}},
+    {"few 2x1", FEW, 2, 1, 8, 0, {{1.387, 0.513, 0.430, 0.211, 0.061}, {1.313, 0.390, 0.449, 0.369, 0.071}}},
+    {"few 2x2", FEW, 2, 2, 8, 0, {{1.607, 0.315, 0.720, 0.292, 0.082}, {1.162, 0.436, 0.790, 1.052, 0.067}}},
+    {"few 4x2", FEW, 4, 2, 4, 0, {{2.099, 0.056, 0.597, 0.494, 0.059}, {1.972, 0.014, 0.894, 0.997, 0}}},
+    {"few 8x2", FEW, 8, 2, 8, 0, {{0.028, 0.332, 2.227, 1.728, 0.020}, {-1, 0, 0, 0, 0}}},
+    {"few 4x3", FEW, 4, 3, 8, 0, {{0.410, 0.636, 1.366, 1.613, 0.048}, {0.154, 0.635, 0.967, 2.560, 0.103}}},
+    {"few 4x4", FEW, 4, 4, 8, 0, {{0.124, 0.795, 1.188, 2.440, 0.083}, {0.184, 0.554, 1.837, 2.738, 0.071}}},
+    {"mid 8x8", MID, 8, 8, 0, 3, {{0.258, 0.813, 0.553, 1.668, 0.169}, {0.324, 0.980, 0.722, 3.243, 0.795}}},
+    {"mid 8x8 deep", MID, 8, 8, 0, 8, {{0.344, 0.358, 0.531, 3.591, 0.685}, {0.116, 0.213, 0.867, 5.308, 1.075}}},
+    {"mid 4x8 deep", MID, 4, 8, 0, 10, {{1.102, 0.074, 0.415, 2.430, 0.559}, {1.293, 0.059, 0.531, 3.237, 0.761}}},
+    {"many 16x16", MANY, 16, 16, 0, 0, {{0.058, 0.006, 1.172, 8.585, 1.594}, {0.129, 1.084, 2.401, 11.874, 3.147}}},
 };
 
 uint64_t tiles_of(const Form &f, uint32_t m, uint32_t n) {

@@ -89,10 +89,12 @@ __device__ __forceinline__ void fp8_multiply(Acc (&acc)[M][N], const fk_fp8_u32x
 
 // Few rows: a threadgroup takes MB × NB blocks of 16 × 16, its W wavefronts
 // every W-th block of k, the operands straight from memory, two blocks in
-// flight; the wavefronts' sums are added in their order in LDS.  8 rows are bound
-// by the weights' stream (by 8192, k 2048, f32: 4.9 µs, 17 MB); more by what a CU
-// takes in, about 60 KB a µs, so a block is as wide as leaves all CUs one (100
-// rows by 5000, k 8192, f32: blocks of 4 x 2 31.6 µs, of 4 x 3, 210 of them, 22.6).
+// flight; the wavefronts' sums are added in their order in LDS.  Bound by the
+// weights' stream where there are many of them (8 rows by 16384, k 8192: 23 µs,
+// 5.8 TB/s), else by what a CU takes in, about 60 KB a µs: twice the wavefronts,
+// and so loads in flight, gained nothing.  So a block is as wide as leaves all CUs
+// one: 100 rows by 5000, k 8192, f32 in blocks of 4 x 2 31.6 µs, of 4 x 3, 210 of
+// them, 22.6; 8 rows in 313 of 1 x 1 12.0, in 157 of 1 x 2 10.6.
 template <uint32_t MB, uint32_t NB, uint32_t W, int T>
 __device__ __forceinline__ void fp8_gemm_few(const fk_fp8_gemm_args &a) {
   __shared__ fk_float4v sums[W][MB * NB][FK_WAVE];
@@ -109,11 +111,16 @@ __device__ __forceinline__ void fp8_gemm_few(const fk_fp8_gemm_args &a) {
     for (uint32_t j = 0; j < NB; j++) acc[i][j] = fk_float4v{0.0f, 0.0f, 0.0f, 0.0f};
   // (tiles past the last repeat it; nothing of theirs is stored)
   uint64_t ac[MB], bc[NB], as[MB], bs[NB];
+  // A's lanes of rows past the last take it again, whose lines are there (8 rows
+  // by 2048, k 8192 7.4 µs without that, 6.5 so; the tallest blocks have no
+  // registers for it).
+  uint32_t a_lane[MB];
 #pragma unroll
   for (uint32_t i = 0; i < MB; i++) {
     const uint64_t t = min(tm + i, rows_a - 1);
     ac[i] = a.a_codes + t * blocks * 2048;
     as[i] = a.a_scales + t * quads * 64;
+    a_lane[i] = MB < 8 ? lane / 16 * 16 + min(lane % 16, a.m - 16 * (uint32_t)t - 1) : lane;
   }
 #pragma unroll
   for (uint32_t j = 0; j < NB; j++) {
@@ -137,7 +144,7 @@ __device__ __forceinline__ void fp8_gemm_few(const fk_fp8_gemm_args &a) {
 #pragma unroll
     for (uint32_t i = 0; i < MB; i++) {
       const auto from = global_at<const u32x4>(ac[i] + codes);
-      x.a[i] = fp8_join(from[lane], from[64 + lane]);
+      x.a[i] = fp8_join(from[a_lane[i]], from[64 + a_lane[i]]);
       x.as[i] = global_at<const uint8_t>(as[i] + scale)[lane % 16 * 4];
     }
     return x;

@@ -317,10 +317,11 @@ def test_products_of_every_form(device, mem, kind):
 @pytest.mark.parametrize("kind", ["f32", "f16", "bf16"])
 def test_each_forms_products(device, mem, kind):
     """Odd sizes of every form of the rule's, by its name."""
-    sizes = [(3, 509, 130), (17, 3001, 130), (17, 5003, 130), (47, 5003, 130), (17, 9001, 300), (97, 8190, 515),
-             (299, 3001, 8190), (799, 1013, 130), (4099, 3001, 130), (17, 16390, 130), (97, 16390, 130),
-             (3, 16390, 130), (3, 16390, 1030), (97, 16390, 1030), (97, 16390, 2060)]
-    names = {"few 1x1", "few 2x1", "few 2x2", "few 4x2", "few 4x3", "few 4x4", "mid 8x8", "mid 8x8 deep",
+    sizes = [(3, 509, 130), (17, 509, 515), (3, 16390, 130), (17, 3001, 130), (17, 5003, 130), (3, 8190, 1030),
+             (47, 5003, 130), (17, 16390, 130), (17, 8190, 300), (47, 9001, 130), (17, 16390, 300), (17, 12001, 515),
+             (17, 16390, 515), (97, 8190, 300), (97, 8190, 515), (299, 3001, 515), (4099, 3001, 130),
+             (97, 16390, 1030), (97, 16390, 2060)]
+    names = {"few 1x1", "few 1x2", "few 2x1", "few 2x2", "few 4x2", "few 4x3", "few 4x4", "mid 8x8", "mid 8x8 deep",
              "mid 4x8 deep", "many 16x16"} | (set() if kind == "f32" else {"few 8x2"})
     assert {fp8.gemm_form(*s, kind) for s in sizes} == names
     for s in sizes:
