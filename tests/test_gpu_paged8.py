@@ -10,7 +10,8 @@ import pytest
 
 import fp8_cases as F
 import serve_cases as S
-from furykernel_amd import paged, paged8
+from furykernel_amd import fp8, paged, paged8
+from test_gpu_fp8 import matrix as mem_matrix
 from test_gpu_mx4 import held
 from test_gpu_serve import SENTINEL, Memory, mem  # noqa: F401  (mem is a fixture)
 
@@ -600,6 +601,89 @@ def test_a_captured_step_of_8_bit_caches(device, mem, q_type, d, block, window):
         attend.enqueue()
         device.sync()
         assert np.array_equal(out.read(np.uint16, n * heads * d), got)
+    captured[0].destroy()
+
+
+@pytest.mark.parametrize("kind,out_type", [("f32", "f16"), ("bf16", "bf16")])
+def test_a_captured_layer_over_8_bit_caches(device, mem, kind, out_type):
+    """A layer as a server runs it: plan, the stream's norm, q k v, store,
+    attention, its product onto the stream, the next norm and a product.
+    Captured and replayed over requests that grow from nothing, with the same
+    calls made eagerly over buffers of their own between: the same bits, codes
+    and scales after every step."""
+    rng = np.random.default_rng(31)
+    n, hidden, heads, kv, d, block, table_len = 5, 200, 6, 2, 64, 8, 6
+    tokens, blocks, width, wide = 9, 40, (heads + 2 * kv) * d, 264
+    word = 4 if kind == "f32" else 2
+    weights = {name: (rng.standard_normal(shape) * shape[1] ** -0.5).astype(np.float32)
+               for name, shape in (("qkv", (width, hidden)), ("o", (hidden, heads * d)), ("up", (wide, hidden)))}
+    gamma = (1 + 0.1 * rng.standard_normal((2, hidden))).astype(np.float32)
+    cs = rng.standard_normal((64, d // 2, 2)).astype(np.float32)
+
+    def layer():
+        m = {}
+        for name, w in weights.items():
+            m[name] = mem_matrix(device, mem, *w.shape)
+            fp8.Quantize(device, mem.put(w), m[name]).enqueue()
+        b = dict(cached=mem.put(np.zeros(n, np.uint32)), fresh=mem.put(np.ones(n, np.uint32)),
+                 free=mem.put(np.arange(blocks, dtype=np.uint32)), head=mem.put(np.zeros(1, np.uint32)),
+                 table=mem.put(np.zeros((n, table_len), np.uint32)), lengths=mem.empty(4 * n),
+                 starts=mem.empty(4 * n + 4), slots=mem.empty(4 * tokens), positions=mem.empty(4 * tokens),
+                 owner=mem.empty(4 * tokens), counts=mem.put(np.zeros(4, np.uint32)))
+        x, rows, o = (mem.put(np.zeros(tokens * c * word, np.uint8)) for c in (hidden, width, hidden))
+        qr, y = (mem.put(np.zeros(2 * c * heads * d, np.uint8)) for c in (tokens, n))
+        up = mem.put(np.zeros(n * wide * 4, np.uint8))
+        pool = dict(kpool=mem.put(np.zeros(blocks * block * kv * d, np.uint8)),
+                    vpool=mem.put(np.zeros(blocks * block * kv * d, np.uint8)),
+                    scales=mem.put(np.zeros(blocks * kv * 2, np.float32)))
+        h, ym, h2 = (mem_matrix(device, mem, *s) for s in ((tokens, hidden), (n, heads * d), (n, hidden)))
+        sizes = dict(requests=n, heads=heads, kv_heads=kv, head_dim=d, block_size=block, blocks=blocks,
+                     table_len=table_len)
+        ops = [paged.PagePlan(device, **b, requests=n, tokens=tokens, table_len=table_len, block_size=block,
+                              free_len=blocks),
+               fp8.AddNorm(device, x, h, 1e-5, gamma=mem.put(gamma[0]), x_type=kind),
+               fp8.Gemm(device, h, m["qkv"], rows, c_type=kind),
+               paged8.PagedStore8(device, q=rows, k=rows, v=rows, k_offset=heads * d, v_offset=(heads + kv) * d,
+                                  q_stride=width, k_stride=width, v_stride=width, slots=b["slots"],
+                                  positions=b["positions"], rope=mem.put(cs), rope_rows=64, rotated=d // 2, qr=qr,
+                                  **pool, tokens=tokens, heads=heads, kv_heads=kv, head_dim=d, block_size=block,
+                                  blocks=blocks, rows_type=kind, q_type=out_type),
+               paged8.PagedAttend8(device, q=qr, **pool, table=b["table"], lengths=b["lengths"], out=y,
+                                   workspace=mem.empty(paged8.attend8_workspace(**sizes)), scale=d ** -0.5,
+                                   q_type=out_type, starts=b["starts"], q_rows=tokens, **sizes),
+               fp8.Quantize(device, y, ym, x_type=out_type), fp8.Gemm(device, ym, m["o"], o, c_type=kind),
+               fp8.AddNorm(device, o, h2, 1e-5, gamma=mem.put(gamma[1]), x_type=kind),
+               fp8.Gemm(device, h2, m["up"], up)]
+        return b, x, ops, [rows, qr, y, o, up, h.codes, h.scales, h2.codes, h2.scales, *pool.values(), b["lengths"]]
+
+    (cb, cx, cops, cheld), (eb, ex, eops, eheld) = layer(), layer()
+    stream = device.new_stream()
+    device.sync()
+    with device.capture(stream) as captured:
+        for op in cops:
+            op.enqueue(stream)
+        cb["cached"].copy_from(cb["lengths"], 4 * n, stream=stream)
+        cb["head"].copy_from(cb["counts"], 4, src_offset=12, stream=stream)
+    for step in range(12):
+        fresh = np.ones(n, np.uint32)
+        fresh[step % n] = step % 4
+        xs = held(rng.standard_normal((tokens, hidden)) * 2.0 ** (step % 3), kind)[0]
+        for b, x in ((cb, cx), (eb, ex)):
+            b["fresh"].write(fresh)
+            x.write(xs)
+        device.sync()
+        captured[0].replay(stream)
+        for op in eops:
+            op.enqueue()
+        eb["cached"].copy_from(eb["lengths"], 4 * n)
+        eb["head"].copy_from(eb["counts"], 4, src_offset=12)
+        device.sync(stream)
+        device.sync()
+        for i, (p, q) in enumerate(zip(cheld, eheld)):
+            assert np.array_equal(p.read(np.uint8), q.read(np.uint8)), (step, i)
+        got = cheld[4].read(np.float32, n * wide)
+        assert np.isfinite(got).all() and got.any()
+    assert cheld[-1].read(np.uint32, n).max() > block
     captured[0].destroy()
 
 
