@@ -34,9 +34,11 @@ __global__ void __launch_bounds__(FK_FP8_THREADS) op_fp8_dequantize(fk_fp8_dequa
   fk::fp8_dequantize<T>(a);
 }
 
+// (two rows of 16 bits: registers for 8 wavefronts a SIMD, three threadgroups of ten)
 template <int T, uint32_t ROWS, uint32_t H>
-__global__ void __launch_bounds__(1024) op_fp8_add_norm(fk_fp8_add_norm_args a) {
-  fk::fp8_add_norm<T, ROWS, H>(a);
+__global__ void __launch_bounds__(1024, ROWS == 2 && T != FK_T_F32 ? 8 : 1)
+    op_fp8_add_norm(fk_fp8_add_norm_args a, double over_k) {
+  fk::fp8_add_norm<T, ROWS, H>(a, over_k);
 }
 
 template <uint32_t MB, uint32_t NB, uint32_t W, int T>
@@ -71,11 +73,11 @@ uint32_t block_groups(uint32_t rows, uint32_t k) {
 }
 
 // The norm's launch: rows a threadgroup, blocks a lane, and tiles of 16 rows by
-// 8, one an XCD.  Where the rows fill the card, rows of 17 to 64 blocks go by two,
-// with two blocks a lane (8192 x 4096 bf16 47.6 us, by one 51.1; of 16 blocks, f32,
-// 46 and 45); few rows, which wait on their own chain of steps, by one, with as few
-// blocks a lane as there are threads for (1 x 5000 4.1 us with one block, 4.9 with
-// two, 6.7 with four; by two rows 5.7).
+// 8, one an XCD.  Where the rows fill the card, rows of up to 64 blocks go by two,
+// with two blocks a lane (29631 x 533 f16 44 us, by one 75; 8191 x 5000 bf16 69 and
+// 110; 8192 x 2048 f32 47 both); few rows, which wait on their own chain of steps, by
+// one, with as few blocks a lane as there are threads for (1 x 5000 4.1 us with one
+// block, 4.9 with two, 6.7 with four; by two rows 5.7).
 constexpr uint32_t norm_most = 4 * 16 * FK_FP8_NORM_HELD * 128;
 struct NormLaunch {
   uint32_t rows, held, threads, groups;
@@ -83,7 +85,7 @@ struct NormLaunch {
 NormLaunch norm_launch(const fk_fp8_add_norm_args &a) {
   NormLaunch l;
   const uint32_t blocks = fk::fp8_blocks(a.k);
-  l.rows = a.rows >= 1024 && blocks > 16 && blocks <= 64 ? 2 : 1;
+  l.rows = a.rows >= 1024 && blocks <= 64 ? 2 : 1;
   const uint32_t each = (blocks * l.rows + 3) / 4;  // blocks for the wavefronts' 16 lanes
   l.held = l.rows == 2 ? 2 : (each <= 16 ? 1 : (each <= 32 ? 2 : FK_FP8_NORM_HELD));
   l.threads = 64 * ((each + l.held - 1) / l.held);
@@ -186,7 +188,7 @@ void queue_picked(uint32_t form, const fk_fp8_gemm_args &a, hipStream_t s, std::
 
 template <int T, uint32_t ROWS, uint32_t H>
 void queue_norm(const fk_fp8_add_norm_args &a, const NormLaunch &l, hipStream_t s) {
-  hipLaunchKernelGGL((op_fp8_add_norm<T, ROWS, H>), dim3(l.groups), dim3(l.threads), 0, s, a);
+  hipLaunchKernelGGL((op_fp8_add_norm<T, ROWS, H>), dim3(l.groups), dim3(l.threads), 0, s, a, 1.0 / a.k);
 }
 }  // namespace
 

@@ -148,7 +148,8 @@ __device__ __forceinline__ void fp8_dequantize(const fk_fp8_dequantize_args &a) 
   }
 }
 
-// The norm: s = x + residual, y = s / sqrt(mean(s^2) + eps) * gamma, as codes.
+// The norm: s = x + residual, y = s / sqrt(mean(s^2) + eps) * gamma, as codes:
+// the exact value's, so the squares are added and their root taken in binary64.
 // A row is held in registers from the first load to the codes, so that it is
 // read once: 16 lanes a block of 128, H blocks a lane, and a wavefront's four 16s
 // four blocks of one row or, with ROWS 2, two of two rows.  Bound by what it moves:
@@ -157,9 +158,9 @@ __device__ __forceinline__ void fp8_dequantize(const fk_fp8_dequantize_args &a) 
 // next, so that a row's codes leave as many short writes; two rows' pieces lie
 // together.  The 16 rows of a tile go to threadgroups on one XCD (a launch's go to
 // the 8 in turn), so that each line of codes is whole in one L2 before it leaves.
-//   8191 x 5000 bf16: 65 us, 4.4 TB/s (one row a threadgroup, 2 blocks a lane 67,
-//   1 or 4 blocks 74; four rows 92: too few of so large threadgroups fit a CU);
-//   8192 x 4096 47 us, 5.0 TB/s (one row 52, four 48); 8 x 2048 f32 3.5 us.
+//   8191 x 5000 bf16: 69 us, 4.2 TB/s (in binary32, where each 2 10^6th code is
+//   another, 65; by one row a threadgroup 110); 8192 x 4096 48 us, 4.9 TB/s;
+//   29631 x 533 f16 44 us; 8 x 2048 f32 3.6 us.
 template <uint32_t ROWS>
 __device__ __forceinline__ uint32_t fp8_norm_row(uint32_t group) {
   constexpr uint32_t each = 16 / ROWS;
@@ -167,22 +168,47 @@ __device__ __forceinline__ uint32_t fp8_norm_row(uint32_t group) {
   return (i / each * 8 + group % 8) * 16 + i % each * ROWS;
 }
 
+template <int CTRL>
+__device__ __forceinline__ double fp8_dpp(double x) {
+  const uint64_t b = __builtin_bit_cast(uint64_t, x);
+  const uint32_t lo = (uint32_t)dpp_i<CTRL>((int)(uint32_t)b), hi = (uint32_t)dpp_i<CTRL>((int)(uint32_t)(b >> 32));
+  return __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
+}
+
 // A row's sum over a threadgroup, the same in every lane of the row.
 template <uint32_t ROWS>
-__device__ __forceinline__ float fp8_norm_sum(float x, float (&slots)[16][4]) {
-  x = x + dpp_f<0xB1>(x);
-  x = x + dpp_f<0x4E>(x);
-  x = x + dpp_f<0x141>(x);
-  x = x + dpp_f<0x140>(x);
+__device__ __forceinline__ double fp8_norm_sum(double x, double (&slots)[16][4]) {
+  x = x + fp8_dpp<0xB1>(x);
+  x = x + fp8_dpp<0x4E>(x);
+  x = x + fp8_dpp<0x141>(x);
+  x = x + fp8_dpp<0x140>(x);
   const uint32_t lane = threadIdx.x % FK_WAVE, waves = blockDim.x / FK_WAVE;
   if (lane % 16 == 0) slots[threadIdx.x / FK_WAVE][lane / 16] = x;
   __syncthreads();
-  float sum = 0.0f;
+  double sum = 0.0;
   for (uint32_t w = 0; w < waves; w++) {
     if constexpr (ROWS == 2) sum += slots[w][lane / 32 * 2] + slots[w][lane / 32 * 2 + 1];
     else sum += (slots[w][0] + slots[w][1]) + (slots[w][2] + slots[w][3]);
   }
   return sum;
+}
+
+// 1 / sqrt(x) to about 2^-50: 0 of infinity.
+__device__ __forceinline__ double fp8_rsqrt(double x) {
+  double r = __builtin_amdgcn_rsq(x);
+#pragma unroll
+  for (int i = 0; i < 2; i++) r = r * __builtin_fma(-0.5 * x * r, r, 1.5);
+  return x == __builtin_inf() ? 0.0 : r;
+}
+
+// x rounded to the nearest binary32, but to the odd one of two that it lies
+// between: rounded once more, to fewer bits, it goes where x would.
+__device__ __forceinline__ float fp8_odd(double x) {
+  const float f = (float)x;
+  const uint32_t u = __float_as_uint(f);
+  const double off = x - (double)f;
+  const bool out = (off > 0.0) == (u >> 31 == 0);
+  return off != 0.0 && (u & 1u) == 0 ? __uint_as_float(out ? u + 1 : u - 1) : f;
 }
 
 // x rounded to T and widened again.
@@ -194,8 +220,8 @@ __device__ __forceinline__ float fp8_rounded(float x) {
 }
 
 template <int T, uint32_t ROWS, uint32_t H>
-__device__ __forceinline__ void fp8_add_norm(const fk_fp8_add_norm_args &a) {
-  __shared__ float slots[16][4];
+__device__ __forceinline__ void fp8_add_norm(const fk_fp8_add_norm_args &a, double over_k) {
+  __shared__ double slots[16][4];
   constexpr uint32_t B = mx4_bytes_of(T);
   const uint32_t blocks = fp8_blocks(a.k), quads = fp8_quads(a.k), waves = blockDim.x / FK_WAVE;
   const uint32_t lane = threadIdx.x % FK_WAVE, wave = threadIdx.x / FK_WAVE;
@@ -212,7 +238,7 @@ __device__ __forceinline__ void fp8_add_norm(const fk_fp8_add_norm_args &a) {
     fp8_load8<T, true>(a.x + row * a.x_stride * B, col, a.k, h[i]);
     if (a.residual) fp8_load8<T, true>(a.residual + row * a.residual_stride * B, col, a.k, r[i]);
   }
-  float squares = 0.0f;
+  double squares = 0.0;
 #pragma unroll
   for (uint32_t i = 0; i < H; i++) {
     const uint32_t col = there ? 128 * block_of(i) + within : a.k;
@@ -222,10 +248,10 @@ __device__ __forceinline__ void fp8_add_norm(const fk_fp8_add_norm_args &a) {
     }
     if (a.sum) fp8_store8<T>(a.sum + row * a.sum_stride * B, col, a.k, h[i]);
 #pragma unroll
-    for (int j = 0; j < 8; j++) squares += h[i][j] * h[i][j];
+    for (int j = 0; j < 8; j++) squares = __builtin_fma((double)h[i][j], (double)h[i][j], squares);
   }
-  const float mean = fp8_norm_sum<ROWS>(squares, slots) / (float)a.k;
-  const float scale = 1.0f / __builtin_sqrtf(mean + a.eps);
+  const double factor = fp8_rsqrt(fp8_norm_sum<ROWS>(squares, slots) * over_k + (double)a.eps);
+  const float scale = (float)factor;
 #pragma unroll
   for (uint32_t i = 0; i < H; i++) {
     const uint32_t block = block_of(i), col = 128 * block + within;
@@ -233,19 +259,41 @@ __device__ __forceinline__ void fp8_add_norm(const fk_fp8_add_norm_args &a) {
     float g[8];
     if (a.gamma) {
       fp8_load8<FK_T_F32, false>(a.gamma, col, a.k, g);
-#pragma unroll
-      for (int j = 0; j < 8; j++) h[i][j] = h[i][j] * scale * g[j];
     } else {
 #pragma unroll
-      for (int j = 0; j < 8; j++) h[i][j] = h[i][j] * scale;
+      for (int j = 0; j < 8; j++) g[j] = 1.0f;
+    }
+    // Off by less than 4 of its last places, y goes to another code than the exact
+    // value only beside a halfway case, or the largest of a scale: those have 19
+    // zeros at their end.  Few wavefronts hold one that near, and make theirs anew.
+    float y[8];
+    uint32_t near = ~0u;
+#pragma unroll
+    for (int j = 0; j < 8; j++) {
+      y[j] = h[i][j] * scale * g[j];
+      near = min(near, (__float_as_uint(y[j]) << 13) + (4u << 13));
+    }
+    if (col + 8 > a.k) {  // (the zeros behind a row are none)
+      near = ~0u;
+#pragma unroll
+      for (uint32_t j = 0; j < 7; j++)
+        if (col + j < a.k) near = min(near, (__float_as_uint(y[j]) << 13) + (4u << 13));
+    }
+    if (__builtin_amdgcn_ballot_w64(near < 8u << 13 && there)) {
+#pragma unroll
+      for (int j = 0; j < 8; j++) {
+        float again = h[i][j];
+        asm volatile("" : "+v"(again));  // (widened here: the squares' doubles, kept, halve the threadgroups of a CU)
+        y[j] = fp8_odd((double)again * factor * (double)g[j]);
+      }
     }
     if (!there || col + 8 > a.k) {
       // (what lies behind the rows and the row is 0 whatever the factor)
 #pragma unroll
-      for (uint32_t j = 0; j < 8; j++) h[i][j] = there && col + j < a.k ? h[i][j] : 0.0f;
+      for (uint32_t j = 0; j < 8; j++) y[j] = there && col + j < a.k ? y[j] : 0.0f;
     }
     uint32_t byte;
-    const u32x2 codes = fp8_encode(h[i], byte);
+    const u32x2 codes = fp8_encode(y, byte);
     *global_at<u32x2>(a.codes + fp8_code_at(row, col / 8, blocks)) = codes;
     // (the last block's lanes 1 to 3 write the scales of those that fill its four up)
     const uint32_t scaled = block + lane % 16;

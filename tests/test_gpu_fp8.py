@@ -222,6 +222,24 @@ def test_add_norm_of_zeros_large_and_small_rows(device, mem):
     hold_norm(device, mem, rng, 6, 300, "f16", residual=False, rows=rows * (np.abs(rows) < 100), eps=0.5)
 
 
+@pytest.mark.parametrize("kind,n,k,size,eps", [
+    ("bf16", 1100, 5000, 0, 1e-5), ("f16", 8000, 533, 0, 1e-5), ("f16", 1025, 1, 0, 1e-5), ("f32", 3000, 130, 0, 1e-5), ("f32", 1030, 4096, 0, 1e-5), ("f32", 1500, 2048, 0, 0.0),
+    ("bf16", 40, 30001, 0, 1e-5), ("f32", 300, 1000, 100, 0.0), ("f32", 300, 9000, -100, 0.0), ("f32", 64, 700, -60, 1e-30)])
+def test_add_norm_s_codes_are_the_exact_value_s(device, mem, kind, n, k, size, eps):
+    """Byte for byte: in binary32 a few in a million would be others.  `size`:
+    of the rows, a power of two, whose squares binary32 does not hold."""
+    rng = np.random.default_rng(n + k)
+    xb, x = held(rng.standard_normal((n, k)) * 2.0 ** size, kind)
+    rb, r = held(rng.standard_normal((n, k)) * 2.0 ** size, kind)
+    hb, h = add(x, r, kind)
+    g = (1 + 0.1 * rng.standard_normal(k)).astype(np.float32)
+    m = matrix(device, mem, n, k)
+    fp8.AddNorm(device, mem.put(xb), m, eps, gamma=mem.put(g), residual=mem.put(rb), x_type=kind).enqueue()
+    device.sync()
+    for got, want in zip((m.codes, m.scales), F.pack(*F.quantize(F.norm(h, g, np.float64(np.float32(eps)))))):
+        assert np.array_equal(got.read(np.uint8), want)
+
+
 def test_add_norm_of_rows_that_are_not_finite(device, mem):
     """A row with a NaN or an infinity is NaN where the formula is; the others are
     as ever."""
