@@ -14,10 +14,10 @@
 // The 8-bit operations add eight products of consecutive k of an operand as
 // whole numbers of 2^-14 of the largest one's power of two (measured: a product
 // below that is lost beside it, one of the next eight is not), so a sum is off
-// by up to 7 2^-14 of such a largest product: 1 to 5 10^-5 of C for normal
-// rows, with some columns 20 times as large.  C of 16 bits, rounded at 2^-9 or
-// 2^-12, takes that for twice the rate.  C of f32 does not: its operands are
-// widened to bf16, scales and all, which is exact from 2^-126 on, and go to
+// by up to 7 2^-14 of such a largest product: 1 to 6 10^-5 of C for normal
+// rows, with some columns 20 times as large.  CUT: C of 16 bits whose caller asked
+// for that, for up to twice the rate.  Otherwise the operands are widened to bf16,
+// scales and all, which is exact from 2^-126 on, and go to
 // v_mfma_f32_16x16x32_bf16 and 32x32x16, whose sums are binary32's.
 #pragma once
 
@@ -55,12 +55,12 @@ __device__ __forceinline__ fk_fp8_bf16x8 fp8_widen(fk_fp8_u32x8 x, uint32_t i, u
 }
 
 // acc[i][j] += A's block i times B's block j, over the 32 elements a lane holds
-// of each, for A's blocks I0 .. I1 - 1; T: C's type.
-template <int T, uint32_t I0, uint32_t I1, uint32_t M, uint32_t N, typename Acc>
+// of each, for A's blocks I0 .. I1 - 1.
+template <bool CUT, uint32_t I0, uint32_t I1, uint32_t M, uint32_t N, typename Acc>
 __device__ __forceinline__ void fp8_multiply(Acc (&acc)[M][N], const fk_fp8_u32x8 (&fb)[N], const uint32_t (&sb)[N],
                                              const fk_fp8_u32x8 (&fa)[M], const uint32_t (&sa)[M]) {
   constexpr bool WIDE = sizeof(Acc) == sizeof(fk_float16v);
-  if constexpr (T != FK_T_F32) {
+  if constexpr (CUT) {
 #pragma unroll
     for (uint32_t i = I0; i < I1; i++)
 #pragma unroll
@@ -95,7 +95,7 @@ __device__ __forceinline__ void fp8_multiply(Acc (&acc)[M][N], const fk_fp8_u32x
 // and so loads in flight, gained nothing.  So a block is as wide as leaves all CUs
 // one: 100 rows by 5000, k 8192, f32 in blocks of 4 x 2 31.6 µs, of 4 x 3, 210 of
 // them, 22.6; 8 rows in 313 of 1 x 1 12.0, in 157 of 1 x 2 10.6.
-template <uint32_t MB, uint32_t NB, uint32_t W, int T>
+template <uint32_t MB, uint32_t NB, uint32_t W, int T, bool CUT>
 __device__ __forceinline__ void fp8_gemm_few(const fk_fp8_gemm_args &a) {
   __shared__ fk_float4v sums[W][MB * NB][FK_WAVE];
   const uint32_t lane = threadIdx.x % FK_WAVE;
@@ -149,10 +149,12 @@ __device__ __forceinline__ void fp8_gemm_few(const fk_fp8_gemm_args &a) {
     }
     return x;
   };
-  auto multiply = [&](const Block &x) { fp8_multiply<T, 0, MB>(acc, x.b, x.bs, x.a, x.as); };
+  auto multiply = [&](const Block &x) { fp8_multiply<CUT, 0, MB>(acc, x.b, x.bs, x.a, x.as); };
   // (nothing moves past where loads have gone out)
 #define FK_FP8_OUT() __builtin_amdgcn_sched_barrier(0)
-  if (wave + W < blocks) {
+  if constexpr (!CUT && MB == 8) {  // (no registers for two blocks and what the widening holds)
+    for (uint32_t p = wave; p < blocks; p += W) multiply(load(p));
+  } else if (wave + W < blocks) {
     Block x = load(wave), y = load(wave + W);
     FK_FP8_OUT();
     uint32_t p = wave + 2 * W;
@@ -204,16 +206,16 @@ __device__ __forceinline__ void fp8_gemm_few(const fk_fp8_gemm_args &a) {
 //   threadgroups a CU, one's loads, reads and stores under another's matrix
 //   operations; or, where the tiles do not fill the CUs that often, as many as
 //   the LDS holds for one threadgroup, so that a step's loads have the time of
-//   seven others to land: 400 rows by 5000, k 8192 52 µs by three stages, 36 by
-//   eight; 200 rows 51, and 29 in tiles of 64 rows.  What bounds it there is
-//   what a CU takes in, about 60 KB a µs (as the few rows' form).
+//   seven others to land: 400 rows by 5000, k 8192, 62 µs by three stages, 58 by
+//   eight (cut 52 and 36); 200 rows 61, and 41 in tiles of 64 rows (51 and 29).
+//   The widening bounds it there, and with cut sums what a CU takes in.
 // - fp8_gemm_many: 256 × 256 tiles whose sums take half the register file, one
 //   threadgroup a CU, four stages, the next step's operands read and a later
 //   step's loaded between a step's matrix operations, and tile after tile with
-//   the next one's first loads under the stores.  8192 by 8192 to f16: k 2048 119
-//   to 124 µs (2.2 to 2.3 PFLOP/s), k 8192 411 (2.7); what bounds it is the clock
-//   that power leaves (3.0 to 3.4 PFLOP/s from registers alone, random data) and,
-//   8 µs a turn of tiles, C's stores.
+//   the next one's first loads under the stores.  8192 by 8192 to f16, k 2048: 205
+//   to 210 µs (1.3 PFLOP/s; the library's bf16 product 1.37), cut 119 to 124 (2.2 to
+//   2.3; from registers alone, random data, 3.0 to 3.4), of which C's stores take
+//   8 µs a turn of tiles.
 #define FK_FP8_STAGES 4
 constexpr uint32_t fp8_many_side = 16;  // row tiles of a tile's side
 constexpr uint32_t fp8_many_lds = FK_FP8_STAGES * 2 * fp8_many_side * 1024;
@@ -237,7 +239,7 @@ __device__ __forceinline__ Fp8Source fp8_source(uint64_t codes, uint64_t scales,
   return s;
 }
 
-template <uint32_t GM, uint32_t GN, uint32_t STAGES, int T>
+template <uint32_t GM, uint32_t GN, uint32_t STAGES, int T, bool CUT>
 __device__ __forceinline__ void fp8_gemm_mid(const fk_fp8_gemm_args &a) {
   static_assert(GN >= 2, "the stores' rows of a wavefront are of 128 bytes at least");
   extern __shared__ u32x4 fp8_lds[];
@@ -319,7 +321,7 @@ __device__ __forceinline__ void fp8_gemm_mid(const fk_fp8_gemm_args &a) {
       fa[i] = fp8_join(from[ra + 128 * i], from[ra + 128 * i + 32]);
       xa[i] = sa[i] >> (8 * byte) & 255u;
     }
-    fp8_multiply<T, 0, GM>(acc, fb, xb, fa, xa);
+    fp8_multiply<CUT, 0, GM>(acc, fb, xb, fa, xa);
     at = at == STAGES - 1 ? 0 : at + 1;
     to = to == STAGES - 1 ? 0 : to + 1;
   };
@@ -353,7 +355,7 @@ __device__ __forceinline__ void fp8_gemm_mid(const fk_fp8_gemm_args &a) {
                                    reinterpret_cast<char *>(fp8_lds) + wave * GN * 2048);
 }
 
-template <int T>
+template <int T, bool CUT>
 __device__ __forceinline__ void fp8_gemm_many(const fk_fp8_gemm_args &a) {
   extern __shared__ u32x4 fp8_lds[];
   constexpr uint32_t GB = fp8_many_side / 4;       // a wavefront's blocks of 32, each way
@@ -428,7 +430,7 @@ __device__ __forceinline__ void fp8_gemm_many(const fk_fp8_gemm_args &a) {
         __builtin_amdgcn_raw_ptr_buffer_load_lds(as.codes, d_ + q * 1024, 16, a_at[q], so_, 0, 0);            \
     _Pragma("unroll") for (uint32_t j = 0; j < GB; j++) NB[j] = fp8_join(s_[rb + 128 * j], s_[rb + 128 * j + 32]); \
     _Pragma("unroll") for (uint32_t i = 0; i < H; i++) NA[i] = fp8_join(s_[ra + 128 * i], s_[ra + 128 * i + 32]); \
-    fp8_multiply<T, 0, H>(acc, FB, sb0, FA, sa0);                                                             \
+    fp8_multiply<CUT, 0, H>(acc, FB, sb0, FA, sa0);                                                             \
     _Pragma("unroll") for (uint32_t g_ = 0; g_ < H * GB; g_++) {                                              \
       __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);                                                      \
       __builtin_amdgcn_sched_group_barrier(0x020, 2, 0);                                                      \
@@ -439,7 +441,7 @@ __device__ __forceinline__ void fp8_gemm_many(const fk_fp8_gemm_args &a) {
     _Pragma("unroll") for (uint32_t q = 0; q < Q; q++)                                                        \
         __builtin_amdgcn_raw_ptr_buffer_load_lds(bs.codes, d_ + SLAB + q * 1024, 16, b_at[q], so_, 0, 0);     \
     _Pragma("unroll") for (uint32_t i = H; i < GB; i++) NA[i] = fp8_join(s_[ra + 128 * i], s_[ra + 128 * i + 32]); \
-    fp8_multiply<T, H, GB>(acc, FB, sb0, FA, sa0);                                                            \
+    fp8_multiply<CUT, H, GB>(acc, FB, sb0, FA, sa0);                                                            \
     _Pragma("unroll") for (uint32_t g_ = 0; g_ < H * GB; g_++) {                                              \
       __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);                                                      \
       __builtin_amdgcn_sched_group_barrier(0x020, 1, 0);                                                      \

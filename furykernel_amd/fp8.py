@@ -129,26 +129,36 @@ class AddNorm(runtime.Operation):
         super().__init__(device, e, args, (x, residual, sum, gamma, to))
 
 
-def gemm_form(m: int, n: int, k: int, c_type: str = "f32") -> str:
+CUT_SUMS = 0x100   # FK_FP8_CUT_SUMS
+
+
+def _c_type(entry: str, c_type: str, cut_sums: bool) -> tuple[int, int]:
+    """C's type as the call has it, and its elements' bytes."""
+    wide = element(entry, c_type, ("f16", "bf16") if cut_sums else ("f32", "f16", "bf16"))
+    return TYPES[c_type] | (CUT_SUMS if cut_sums else 0), wide
+
+
+def gemm_form(m: int, n: int, k: int, c_type: str = "f32", cut_sums: bool = False) -> str:
     """The kernel that a Gemm of these sizes takes (fk_fp8_gemm_form)."""
     whole("fk_fp8_gemm", m=m, n=n, k=k)
-    element("fk_fp8_gemm", c_type)
-    return runtime.library().fk_fp8_gemm_form(m, n, k, TYPES[c_type]).decode()
+    return runtime.library().fk_fp8_gemm_form(m, n, k, _c_type("fk_fp8_gemm", c_type, cut_sums)[0]).decode()
 
 
 class Gemm(runtime.Operation):
     """C [m][n] = A Bᵀ of A [m, k] and B [n, k] (a weight, outputs first), in
-    rows of `c_type` `c_stride` elements apart (fk_fp8_gemm)."""
+    rows of `c_type` `c_stride` elements apart (fk_fp8_gemm).  Sums are
+    binary32's; with `cut_sums` those of C of f16 or bf16 are the matrix cores'
+    8-bit operations' own, off by up to 7 2^-14 of Σ |a b|, at up to twice the
+    rate (FK_FP8_CUT_SUMS)."""
 
     def __init__(self, device, a: Fp8Matrix, b: Fp8Matrix, c: runtime.Buffer, c_type: str = "f32",
-                 c_stride: int | None = None):
+                 c_stride: int | None = None, cut_sums: bool = False):
         e = "fk_fp8_gemm"
-        wide = element(e, c_type)
+        kind, wide = _c_type(e, c_type, cut_sums)
         if a.k != b.k:
             raise LaunchError(f"{e}: rows of {a.k} and of {b.k}")
         c_stride = row_stride(e, "c_stride", c_stride, b.rows)
         at = need(e, "c", c, ((a.rows - 1) * c_stride + b.rows) * wide, device)
-        args = GemmArgs(*a._held(e, "A", device), *b._held(e, "B", device), at, c_stride, a.rows, b.rows, a.k,
-                        TYPES[c_type])
+        args = GemmArgs(*a._held(e, "A", device), *b._held(e, "B", device), at, c_stride, a.rows, b.rows, a.k, kind)
         admit(e, args)
         super().__init__(device, e, args, (a, b, c))
