@@ -29,10 +29,10 @@ __global__ void __launch_bounds__(FK_LOAD8_THREADS)
   fk::paged_load8<T>(a, block, units);
 }
 
-template <uint32_t DP, uint32_t EIGHTS, bool FULL, bool BF16, uint32_t PARTS>
+template <uint32_t DP, uint32_t EIGHTS, bool FULL, bool BF16>
 __global__ void __launch_bounds__(64 * FK_PAGED_WAVES, DP == 256 ? 1 : 2)
     op_pages8_attend(fk_paged_attend_args a, uint64_t scales, fk::PagedPlan pl) {
-  fk::paged_attend8<DP, EIGHTS, FULL, BF16, PARTS>(a, scales, pl);
+  fk::paged_attend8<DP, EIGHTS, FULL, BF16>(a, scales, pl);
 }
 
 template <uint32_t W, bool BF16>
@@ -156,22 +156,22 @@ fk_paged_attend_args shared_args(const fk_paged_attend8_args &a) {
 
 // The keys of a group: a tile's where blocks are of whole tiles, 16, or 8 (and
 // heads that do not fill their tiles).
-template <uint32_t DP, bool BF16, uint32_t PARTS>
+template <uint32_t DP, bool BF16>
 void queue_attend(const fk_paged_attend_args &a, uint64_t scales, const AttendLaunch &l, hipStream_t s) {
   constexpr uint32_t tile = fk::attend8_keys(DP);
   auto queue = [&](auto kernel) {
     hipLaunchKernelGGL(kernel, dim3(l.groups), dim3(64 * FK_PAGED_WAVES), 0, s, a, scales, l.plan);
   };
-  if (a.head_dim != DP || a.block_size % 16) queue(op_pages8_attend<DP, 1, false, BF16, PARTS>);
-  else if (a.block_size % tile) queue(op_pages8_attend<DP, 2, true, BF16, PARTS>);
-  else queue(op_pages8_attend<DP, tile / 8, true, BF16, PARTS>);
+  if (a.head_dim != DP || a.block_size % 16) queue(op_pages8_attend<DP, 1, false, BF16>);
+  else if (a.block_size % tile) queue(op_pages8_attend<DP, 2, true, BF16>);
+  else queue(op_pages8_attend<DP, tile / 8, true, BF16>);
 }
 
-template <bool BF16, uint32_t PARTS>
+template <bool BF16>
 void queue_attend(const fk_paged_attend_args &a, uint64_t scales, const AttendLaunch &l, hipStream_t s) {
-  if (l.width == 256) queue_attend<256, BF16, PARTS>(a, scales, l, s);
-  else if (l.width == 128) queue_attend<128, BF16, PARTS>(a, scales, l, s);
-  else queue_attend<64, BF16, PARTS>(a, scales, l, s);
+  if (l.width == 256) queue_attend<256, BF16>(a, scales, l, s);
+  else if (l.width == 128) queue_attend<128, BF16>(a, scales, l, s);
+  else queue_attend<64, BF16>(a, scales, l, s);
 }
 
 template <uint32_t W>
@@ -336,8 +336,7 @@ extern "C" int fk_paged_attend8(fk_ctx *ctx, const fk_paged_attend8_args *a, fk_
   const AttendLaunch l = attend_launch(*a);
   const fk_paged_attend_args s = shared_args(*a);
   const hipStream_t on = stream_of(ctx, stream);
-  if (a->q_bf16) a->out_f32 ? queue_attend<true, 3>(s, a->scales, l, on) : queue_attend<true, 2>(s, a->scales, l, on);
-  else a->out_f32 ? queue_attend<false, 3>(s, a->scales, l, on) : queue_attend<false, 2>(s, a->scales, l, on);
+  a->q_bf16 ? queue_attend<true>(s, a->scales, l, on) : queue_attend<false>(s, a->scales, l, on);
   if (int st = launched(ctx, "fk_paged_attend8")) return st;
   if (l.plan.whole) return FK_OK;
   const uint32_t states = l.groups / l.joins;  // of a pair, about

@@ -27,13 +27,14 @@
 // The vector operations are what a tile costs beside its bytes, so the running
 // maximum is compared lane by lane and joined over the lanes only where one is
 // passed, which is rare behind the first tiles, and the sum is joined at the
-// end.  The probabilities go in as bf16 parts, each rounded to nearest: two,
-// which leave 2^-18 of a probability, where the result is rounded to 16 bits;
-// three, cut off, which hold all 24, where it is f32.
+// end.  The probabilities go in as three bf16 parts, cut off, which hold all
+// their 24 bits (by two, which leave 2^-18 of one, 41 requests of up to 700 keys
+// took 7.26 µs, by three 7.50; the longest and the largest 48.6 48.8 and 125.0
+// 125.6).
 //
 // Measured, f16 and bf16 out: one request of 131072 keys, 8 heads of 128 (268 MB)
 // 42.5 µs, 6.3 TB/s, and the join 4.6; 64 of up to 16384 (732 MB) 120 µs, 6.1 TB/s,
-// and 5; 41 of up to 700, 4 heads of 64, 7.2 µs, which the longest's round trips bound.
+// and 5; 41 of up to 700, 4 heads of 64, 7.5 µs, which the longest's round trips bound.
 #pragma once
 
 #include "fk_paged_attend.h"
@@ -60,30 +61,17 @@ __device__ __forceinline__ typename PagedOperand<BF16>::vec attend8_widen(uint32
   return __builtin_bit_cast(typename PagedOperand<BF16>::vec, w);
 }
 
-// The bf16 parts of two probabilities, a word each.
-template <uint32_t PARTS>
-__device__ __forceinline__ void attend8_cut(float p0, float p1, uint32_t (&to)[PARTS]) {
-  typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
-  if constexpr (PARTS == 3) {
-    PagedOperand<true>::cut(p0, p1, to);
-  } else {
-    to[0] = __builtin_bit_cast(uint32_t, bf16x2{(__bf16)p0, (__bf16)p1});
-    p0 -= __uint_as_float(to[0] << 16);
-    p1 -= __uint_as_float(to[0] & 0xFFFF0000u);
-    to[1] = __builtin_bit_cast(uint32_t, bf16x2{(__bf16)p0, (__bf16)p1});
-  }
-}
-
 constexpr uint32_t attend8_keys(uint32_t dp) { return dp == 64 ? 64 : 32; }  // a tile's
 
 // DP: the head's width in the tiles (64, 128 or 256; head_dim at most that);
 // EIGHTS: the keys of a group by eights (1, 2, or a tile's);
-// FULL: head_dim is DP; BF16: q's type; PARTS: of a probability.
-template <uint32_t DP, uint32_t EIGHTS, bool FULL, bool BF16, uint32_t PARTS>
+// FULL: head_dim is DP; BF16: q's type.
+template <uint32_t DP, uint32_t EIGHTS, bool FULL, bool BF16>
 __device__ __forceinline__ void paged_attend8(const fk_paged_attend_args &a, uint64_t scales, const PagedPlan &pl) {
   using Op = PagedOperand<BF16>;
   using PV = PagedOperand<true>;
   using vec = typename Op::vec;
+  constexpr uint32_t PARTS = PV::parts;
   constexpr uint32_t W = FK_PAGED_WAVES;
   constexpr uint32_t KT = attend8_keys(DP);
   constexpr uint32_t S = KT / 16, P = DP / 64;  // groups of 16 keys, pieces of K that a lane holds of one
@@ -334,7 +322,7 @@ __device__ __forceinline__ void paged_attend8(const fk_paged_attend_args &a, uin
               const float p1 = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[s][i + 1], kf[s], -mc));
               l += p0 + p1;
               uint32_t words[PARTS];
-              attend8_cut<PARTS>(p0, p1, words);
+              PV::cut(p0, p1, words);
 #pragma unroll
               for (uint32_t z = 0; z < PARTS; z++) parts[s / 2][z][s % 2 * 2 + i / 2] = words[z];
             }

@@ -87,10 +87,10 @@ int fk_paged_load8(fk_ctx *ctx, const fk_paged_load8_args *args, fk_stream *stre
  * hold, does not matter.
  *
  * Scores, the running maximum, the sums and the weighted values are binary32,
- * rounded once on the way out (probabilities go to the matrix cores as bf16
- * parts: two, off by up to 2^-18 of one, where out is of 16 bits; three, which
- * hold all their bits, where it is f32).  The same
- * lengths give the same bits, whatever else the pool holds. */
+ * rounded once on the way out (probabilities go to the matrix cores as three
+ * bf16 parts, which hold all their bits; of values below 2^-126 what bfloat16
+ * holds, or nothing).  The same lengths give the same bits, whatever else the pool
+ * holds. */
 typedef struct fk_paged_attend8_args {
   uint64_t q;         /* rows of [heads][head_dim], f16 or bf16: a request's each, or with starts q_rows */
   uint64_t kpool, vpool;
