@@ -245,9 +245,10 @@ int check(const fk_fp8_add_norm_args &a, Refusal &no) {
   if (a.sum)
     if (int st = check_rows(no, "sum", a.sum_stride, a.k, a.x_type)) return st;
   // (over x or the residual, element by element, the sum is no overlap: each is
-  // read by the thread that writes it, before)
-  const bool over_x = a.sum == a.x && a.sum_stride == a.x_stride;
-  const bool over_r = a.sum == a.residual && a.sum_stride == a.residual_stride;
+  // read by the thread that writes it, before; at their address but another stride
+  // it is one)
+  const bool over_x = a.sum == a.x && (a.rows == 1 || a.sum_stride == a.x_stride);
+  const bool over_r = a.sum == a.residual && (a.rows == 1 || a.sum_stride == a.residual_stride);
   const Span x = rows_of("x", a.x, a.rows, a.x_stride, a.k, a.x_type);
   const Span r = rows_of("residual", a.residual, a.residual ? a.rows : 0, a.residual_stride, a.k, a.x_type);
   const Span sum = rows_of("sum", a.sum, a.sum ? a.rows : 0, a.sum_stride, a.k, a.x_type);
@@ -258,13 +259,12 @@ int check(const fk_fp8_add_norm_args &a, Refusal &no) {
     const Span reads[] = {x, r, gamma}, writes[] = {codes, scales};
     if (int st = check_spans(no, reads, 3, writes, 2)) return st;
   }
-  Span reads[4] = {codes, scales, gamma};
+  Span reads[5] = {codes, scales, gamma};
   size_t n = 3;
-  if (!over_x && !(a.residual == a.x && over_r)) reads[n++] = x;
+  if (!over_x) reads[n++] = x;
+  if (!over_r) reads[n++] = r;
   const Span one[] = {sum};
-  if (int st = check_spans(no, reads, n, one, 1)) return st;
-  const Span other[] = {r};
-  return over_r || (a.residual == a.x && over_x) ? FK_OK : check_spans(no, other, 1, one, 1);
+  return check_spans(no, reads, n, one, 1);
 }
 
 int check(const fk_fp8_gemm_args &a, Refusal &no) {

@@ -4,7 +4,7 @@ import pytest
 
 from furykernel_amd import fp8, runtime
 from furykernel_amd.kernels import LaunchError
-from test_fp8 import FakeMatrix
+from test_fp8 import FakeMatrix, norm
 from test_serve import DEVICE, FakeBuffer
 
 
@@ -30,3 +30,24 @@ def test_cut_sums_are_of_products_to_16_bits():
             with pytest.raises(runtime.FkError):
                 runtime.serve_check("fk_fp8_gemm", args)
             assert form == b""
+
+
+def test_a_norm_s_sum_lies_over_rows_of_its_own_stride_only():
+    """x and the residual in one buffer at two strides: the sum's row 2 would be the
+    other's row 1, which another threadgroup reads."""
+    x = FakeBuffer(9 * 2000 * 4)
+    both = dict(x=x, residual=x, sum=x)
+    norm(**both)
+    norm(**both, x_stride=2000, residual_stride=2000, sum_stride=2000)
+    for over in (dict(residual_stride=2000), dict(x_stride=2000), dict(sum_stride=2000),
+                 dict(x_stride=2000, sum_stride=2000), dict(residual_stride=2000, sum_stride=2000),
+                 dict(x_stride=1001, residual_stride=2000, sum_stride=1001)):
+        with pytest.raises(LaunchError):
+            norm(**both, **over)
+    r = FakeBuffer(9 * 1000 * 4, ptr=x.ptr)
+    for over in (dict(sum=x, sum_stride=2000), dict(sum=r), dict(sum=r, residual_stride=1001)):
+        with pytest.raises(LaunchError):
+            norm(x=x, x_stride=2000, residual=r, **over)
+    norm(x=x, x_stride=2000, residual=r)               # read only
+    one = FakeBuffer(1000 * 4)                         # (a row has no stride)
+    norm(x=one, x_stride=2000, residual=one, sum=one, to=FakeMatrix(1, 1000))
