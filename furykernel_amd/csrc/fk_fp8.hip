@@ -236,8 +236,10 @@ int check(const fk_fp8_dequantize_args &a, Refusal &no) {
 int check(const fk_fp8_add_norm_args &a, Refusal &no) {
   if (!matrix(a.rows, a.k) || a.k > norm_most)
     return no(FK_ERR_RANGE, "no matrix of %u rows of %u (at most %u)", a.rows, a.k, norm_most);
-  if (fk::fp8_row_tiles(a.rows) >= 1u << 18)  // a launch of 2^32 threads
-    return no(FK_ERR_RANGE, "%u rows: 2^22 and more", a.rows);
+  if (fk::fp8_row_tiles(a.rows) >= 1u << 18) return no(FK_ERR_RANGE, "%u rows: 2^22 and more", a.rows);
+  const NormLaunch l = norm_launch(a);
+  if ((uint64_t)l.groups * l.threads >= 1ull << 32)
+    return no(FK_ERR_RANGE, "%u rows of %u: a launch of 2^32 threads", a.rows, a.k);
   if (!(a.eps >= 0.0f) || std::isinf(a.eps)) return no(FK_ERR_ARG, "eps = %g", (double)a.eps);
   if (int st = check_rows(no, "x", a.x_stride, a.k, a.x_type)) return st;
   if (a.residual)

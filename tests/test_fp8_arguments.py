@@ -51,3 +51,20 @@ def test_a_norm_s_sum_lies_over_rows_of_its_own_stride_only():
     norm(x=x, x_stride=2000, residual=r)               # read only
     one = FakeBuffer(1000 * 4)                         # (a row has no stride)
     norm(x=one, x_stride=2000, residual=one, sum=one, to=FakeMatrix(1, 1000))
+
+
+def test_a_norm_whose_launch_would_be_2_to_32_threads():
+    """Row tiles go by eights, one an XCD: their rounding up counts."""
+    def taken(rows, k):
+        args = fp8.AddNormArgs(x=1 << 45, codes=1 << 46, scales=1 << 47, x_stride=k, rows=rows, k=k, x_type=2, eps=1e-5)
+        try:
+            runtime.serve_check("fk_fp8_add_norm", args)
+        except runtime.FkError:
+            return False
+        return True
+
+    most = 16 * ((1 << 18) - 8)
+    for k in (16384, 15361, 32768, 30721):              # threadgroups of 1024 threads, a row each
+        assert taken(most, k) and not taken(most + 1, k) and not taken(most + 16 * 7, k)
+    for k in (15360, 8192, 2048, 1):                    # fewer threads
+        assert taken(most + 1, k) and taken(most + 16 * 7, k) and not taken(most + 16 * 7 + 1, k)
