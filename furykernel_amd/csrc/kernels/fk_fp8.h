@@ -202,13 +202,15 @@ __device__ __forceinline__ double fp8_rsqrt(double x) {
 }
 
 // x rounded to the nearest binary32, but to the odd one of two that it lies
-// between: rounded once more, to fewer bits, it goes where x would.
+// between: rounded once more, to fewer bits, it goes where x would.  Past
+// binary32's range, infinite or NaN: as the cast has it.
 __device__ __forceinline__ float fp8_odd(double x) {
   const float f = (float)x;
   const uint32_t u = __float_as_uint(f);
   const double off = x - (double)f;
   const bool out = (off > 0.0) == (u >> 31 == 0);
-  return off != 0.0 && (u & 1u) == 0 ? __uint_as_float(out ? u + 1 : u - 1) : f;
+  const bool between = off != 0.0 && (u & 0x7F800000u) != 0x7F800000u;
+  return between && (u & 1u) == 0 ? __uint_as_float(out ? u + 1 : u - 1) : f;
 }
 
 // x rounded to T and widened again.

@@ -71,8 +71,9 @@ int fk_fp8_dequantize(fk_ctx *ctx, const fk_fp8_dequantize_args *args, fk_stream
 
 /* h = x + residual, rounded to x_type, into sum; y = h / sqrt(mean of h^2 +
  * eps) times gamma to 8 bits: the codes and scales of y itself, but for what lies
- * within 2^-40 of where they change.  Without a residual h is x.  The sum
- * may be written over x or over the residual (the same address and stride). */
+ * within 2^-40 of where they change (a y past binary32's range is not finite).
+ * Without a residual h is x.  The sum may be written over x or over the residual
+ * (the same address and stride). */
 typedef struct fk_fp8_add_norm_args {
   uint64_t x;             /* [rows][k] of x_type */
   uint64_t residual;      /* likewise, or 0 */
