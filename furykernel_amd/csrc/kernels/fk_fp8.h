@@ -6,6 +6,8 @@
 // bits 11.6 us (4.3 TB/s), 8191 x 5000 back to bf16 20.5 us (6.0).
 #pragma once
 
+#include <cfloat>
+
 #include "fk_e4m3.h"
 #include "fk_mx4.h"
 
@@ -253,7 +255,8 @@ __device__ __forceinline__ void fp8_add_norm(const fk_fp8_add_norm_args &a, doub
     for (int j = 0; j < 8; j++) squares = __builtin_fma((double)h[i][j], (double)h[i][j], squares);
   }
   const double factor = fp8_rsqrt(fp8_norm_sum<ROWS>(squares, slots) * over_k + (double)a.eps);
-  const float scale = (float)factor;
+  // (past binary32's normal range NaN: each y is made anew)
+  const float scale = factor >= FLT_MIN && factor <= FLT_MAX ? (float)factor : __builtin_nanf("");
 #pragma unroll
   for (uint32_t i = 0; i < H; i++) {
     const uint32_t block = block_of(i), col = 128 * block + within;
@@ -267,21 +270,20 @@ __device__ __forceinline__ void fp8_add_norm(const fk_fp8_add_norm_args &a, doub
     }
     // Off by less than 4 of its last places, y goes to another code than the exact
     // value only beside a halfway case, or the largest of a scale: those have 19
-    // zeros at their end.  Few wavefronts hold one that near, and make theirs anew.
-    float y[8];
+    // zeros at their end.  Few wavefronts hold one that near, and make theirs anew;
+    // so do those of a y or a product on its way below binary32's normal range, which
+    // holds fewer bits.
+    float y[8], least = 1.0f;
     uint32_t near = ~0u;
+    auto ends = [](float x) { return (__float_as_uint(x) << 13) + (4u << 13); };
 #pragma unroll
     for (int j = 0; j < 8; j++) {
-      y[j] = h[i][j] * scale * g[j];
-      near = min(near, (__float_as_uint(y[j]) << 13) + (4u << 13));
+      const float t = h[i][j] * scale;
+      y[j] = t * g[j];
+      near = min(near, ends(y[j]));
+      least = __builtin_fminf(least, __builtin_fminf(__builtin_fabsf(t), __builtin_fabsf(y[j])));
     }
-    if (col + 8 > a.k) {  // (the zeros behind a row are none)
-      near = ~0u;
-#pragma unroll
-      for (uint32_t j = 0; j < 7; j++)
-        if (col + j < a.k) near = min(near, (__float_as_uint(y[j]) << 13) + (4u << 13));
-    }
-    if (__builtin_amdgcn_ballot_w64(near < 8u << 13 && there)) {
+    if (__builtin_amdgcn_ballot_w64(near < 8u << 13 || least < FLT_MIN)) {
 #pragma unroll
       for (int j = 0; j < 8; j++) {
         float again = h[i][j];

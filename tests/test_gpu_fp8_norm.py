@@ -90,3 +90,34 @@ def test_a_gamma_that_is_not_finite_and_values_past_the_range(device, mem, n):  
     x[5, 3:900:31], g = x[5, 3:900:31] * 20, np.full(1000, 1.5 * 2.0 ** 126, np.float32)
     hold(device, mem, x, x, g, "f32")
     hold(device, mem, x, x, -g, "f32")
+
+
+@pytest.mark.parametrize("n", [64, 1100])
+@pytest.mark.parametrize("gamma", [0, -120, -126, -130, -135])
+def test_values_below_the_normal_range(device, mem, n, gamma):  # noqa: F811
+    """Results, products on their way and rows below 2^-126, where a binary32 has
+    fewer bits than its largest ones."""
+    rng = np.random.default_rng(6 - gamma)
+    g = np.ldexp(1 + 0.2 * rng.standard_normal(1000), gamma).astype(np.float32)
+    for size, eps in ((0, 1e-5), (-126, 1e-5), (-130, 1e-5), (-136, 1e-5), (-140, 1e-5), (-140, 0.0)):
+        print(f"exact norm below the range {n} {gamma} {size} {eps}", flush=True)
+        xb, x = held(rng.standard_normal((n, 1000)) * 2.0 ** size, "f32")
+        hold(device, mem, xb, x, g, "f32", eps)
+    # some far below their row's others, a large gamma over them
+    x = (rng.standard_normal((n, 1000)) * np.exp2(rng.choice([0, -126, -130, -138], (n, 1000)))).astype(np.float32)
+    hold(device, mem, x, x, np.ldexp(g.astype(np.float64), 40 - 2 * gamma // 3).astype(np.float32), "f32")
+
+
+@pytest.mark.parametrize("n", [64, 1100])
+def test_rows_at_the_upper_end(device, mem, n):  # noqa: F811
+    """Rows whose root binary32 holds in part or not at all, large and small
+    elements among them."""
+    rng = np.random.default_rng(7)
+    for size in (120, 125, 126, 127):
+        x = np.ldexp(np.clip(rng.standard_normal((n, 1000)), -1.9, 1.9), size - rng.integers(0, 2, (n, 1000)) * 20)
+        xb, x = held(x, "f32")
+        for g in (0, 30, 100):
+            print(f"exact norm at the upper end {n} {size} {g}", flush=True)
+            hold(device, mem, xb, x, np.ldexp(1 + 0.2 * rng.standard_normal(1000), g).astype(np.float32), "f32")
+    xb, x = held(np.ldexp(rng.standard_normal((n, 1000)) * 0.5, 127), "bf16")
+    hold(device, mem, xb, x, None, "bf16")
