@@ -160,9 +160,9 @@ __device__ __forceinline__ void fp8_dequantize(const fk_fp8_dequantize_args &a) 
 // next, so that a row's codes leave as many short writes; two rows' pieces lie
 // together.  The 16 rows of a tile go to threadgroups on one XCD (a launch's go to
 // the 8 in turn), so that each line of codes is whole in one L2 before it leaves.
-//   8191 x 5000 bf16: 69 us, 4.2 TB/s (in binary32, where each 2 10^6th code is
-//   another, 65; by one row a threadgroup 110); 8192 x 4096 48 us, 4.9 TB/s;
-//   29631 x 533 f16 44 us; 8 x 2048 f32 3.6 us.
+//   8191 x 5000 bf16: 72 us, 4.0 TB/s (in binary32, where a code in 2 to 3 10^6 is
+//   another, 65; by one row a threadgroup 110); 8192 x 4096 49 us, 4.8 TB/s;
+//   29631 x 533 f16 46 us; 8 x 2048 f32 3.6 us.
 template <uint32_t ROWS>
 __device__ __forceinline__ uint32_t fp8_norm_row(uint32_t group) {
   constexpr uint32_t each = 16 / ROWS;
@@ -273,6 +273,9 @@ __device__ __forceinline__ void fp8_add_norm(const fk_fp8_add_norm_args &a, doub
     // zeros at their end.  Few wavefronts hold one that near, and make theirs anew;
     // so do those of a y or a product on its way below binary32's normal range, which
     // holds fewer bits.
+    // Zeros look like both, but are exact: a wavefront that holds some looks again
+    // without them (a block's turn of a bf16 residual sum holds some 4 times in 10: made
+    // anew for them too, 8191 x 5000 took 77 us, so 72 to 74).
     float y[8], least = 1.0f;
     uint32_t near = ~0u;
     auto ends = [](float x) { return (__float_as_uint(x) << 13) + (4u << 13); };
@@ -283,12 +286,24 @@ __device__ __forceinline__ void fp8_add_norm(const fk_fp8_add_norm_args &a, doub
       near = min(near, ends(y[j]));
       least = __builtin_fminf(least, __builtin_fminf(__builtin_fabsf(t), __builtin_fabsf(y[j])));
     }
-    if (__builtin_amdgcn_ballot_w64(near < 8u << 13 || least < FLT_MIN)) {
+    const bool small = there && least < FLT_MIN;
+    if (__builtin_amdgcn_ballot_w64((there && near < 8u << 13) || small)) {
+      bool anew = true;
+      if (__builtin_amdgcn_ballot_w64(small)) {
+        anew = scale != scale;
 #pragma unroll
-      for (int j = 0; j < 8; j++) {
-        float again = h[i][j];
-        asm volatile("" : "+v"(again));  // (widened here: the squares' doubles, kept, halve the threadgroups of a CU)
-        y[j] = fp8_odd((double)again * factor * (double)g[j]);
+        for (int j = 0; j < 8; j++) {
+          const float low = __builtin_fminf(__builtin_fabsf(h[i][j] * scale), __builtin_fabsf(y[j]));
+          anew = anew || ((ends(y[j]) < 8u << 13 || low < FLT_MIN) && h[i][j] != 0.0f && g[j] != 0.0f);
+        }
+      }
+      if (__builtin_amdgcn_ballot_w64(anew)) {
+#pragma unroll
+        for (int j = 0; j < 8; j++) {
+          float again = h[i][j];
+          asm volatile("" : "+v"(again));  // (widened here: the squares' doubles, kept, halve the threadgroups of a CU)
+          y[j] = fp8_odd((double)again * factor * (double)g[j]);
+        }
       }
     }
     if (!there || col + 8 > a.k) {
