@@ -57,7 +57,12 @@ class Fp8Matrix:
         if not all(sizes):
             raise LaunchError(f"Fp8Matrix: no matrix of {rows} rows of {k}")
         self.device, self.rows, self.k = device, rows, k
-        self.codes, self.scales = (device.alloc(n) for n in sizes)
+        self.codes = device.alloc(sizes[0])
+        try:
+            self.scales = device.alloc(sizes[1])
+        except runtime.FkError:
+            self.codes.free()
+            raise
 
     def free(self) -> None:
         self.codes.free()

@@ -2,7 +2,7 @@
 
 import pytest
 
-from furykernel_amd import fp8, runtime
+from furykernel_amd import fp8, mx4, runtime
 from furykernel_amd.kernels import LaunchError
 from test_fp8 import FakeMatrix, norm
 from test_serve import DEVICE, FakeBuffer
@@ -68,3 +68,22 @@ def test_a_norm_whose_launch_would_be_2_to_32_threads():
         assert taken(most, k) and not taken(most + 1, k) and not taken(most + 16 * 7, k)
     for k in (15360, 8192, 2048, 1):                    # fewer threads
         assert taken(most + 1, k) and taken(most + 16 * 7, k) and not taken(most + 16 * 7 + 1, k)
+
+
+@pytest.mark.parametrize("kind", [fp8.Fp8Matrix, mx4.Mx4Matrix])
+def test_a_matrix_whose_scales_find_no_memory_leaves_none_taken(kind):
+    class Device:
+        taken = 0
+
+        def alloc(self, nbytes):
+            if self.taken:
+                raise runtime.FkError(1, "no memory")
+            self.taken += 1
+            buf = FakeBuffer(nbytes, self)
+            buf.free = lambda: setattr(self, "taken", self.taken - 1)
+            return buf
+
+    device = Device()
+    with pytest.raises(runtime.FkError):
+        kind(device, 100, 1000)
+    assert device.taken == 0
