@@ -118,7 +118,8 @@ AttendLaunch attend_launch(const fk_paged_attend8_args &a) {
     l.joins = l.plan.by_pair ? (uint32_t)pairs : l.groups;
     // Few units a pair at most: a threadgroup takes pairs whole, which saves the
     // prefix sum and the join and costs each further unit's time, and a long
-    // pair's to the launch.  µs whole and split of requests of up to u units (256
+    // pair's to the launch.  µs (by two parts of a probability; three take 0.1 to 0.3
+    // more) whole and split of requests of up to u units (256
     // keys of 64, 128 of 128 and 256), evenly spread | of one unit but for one:
     //   pairs, width   u = 4                  6                      8                      12
     //     8 of 64    7.6  9.5              9.5  9.5             11.4  9.7             15.2  9.9

@@ -91,10 +91,11 @@ __device__ __forceinline__ void fp8_multiply(Acc (&acc)[M][N], const fk_fp8_u32x
 // every W-th block of k, the operands straight from memory, two blocks in
 // flight; the wavefronts' sums are added in their order in LDS.  Bound by the
 // weights' stream where there are many of them (8 rows by 16384, k 8192: 23 µs,
-// 5.8 TB/s), else by what a CU takes in, about 60 KB a µs: twice the wavefronts,
-// and so loads in flight, gained nothing.  So a block is as wide as leaves all CUs
-// one: 100 rows by 5000, k 8192, f32 in blocks of 4 x 2 31.6 µs, of 4 x 3, 210 of
-// them, 22.6; 8 rows in 313 of 1 x 1 12.0, in 157 of 1 x 2 10.6.
+// 5.8 TB/s), else by what each CU takes in (306 KB of 100 rows by 5000, k 3080, in a
+// kernel of 9.4 µs): twice the wavefronts, and so loads in flight, gained nothing.  So
+// a block is as wide as leaves all CUs one: 100 rows by 5000, k 8192, f32 in blocks of
+// 4 x 2 31.6 µs, of 4 x 3, 210 of them, 22.6; 8 rows in 313 of 1 x 1 12.0, in 157 of
+// 1 x 2 10.6.
 template <uint32_t MB, uint32_t NB, uint32_t W, int T, bool CUT>
 __device__ __forceinline__ void fp8_gemm_few(const fk_fp8_gemm_args &a) {
   __shared__ fk_float4v sums[W][MB * NB][FK_WAVE];

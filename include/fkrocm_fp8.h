@@ -97,7 +97,8 @@ int fk_fp8_add_norm(fk_ctx *ctx, const fk_fp8_add_norm_args *args, fk_stream *st
 /* C [m][n] = A Bᵀ of A [m, k] and B [n, k] (a weight, outputs first), rounded
  * once to c_type, c_stride elements from row to row.  Sums are binary32's (of
  * elements below 2^-126 what bfloat16 holds, or nothing), but for what
- * FK_FP8_CUT_SUMS allows. */
+ * FK_FP8_CUT_SUMS allows.  C of 2^31 tiles of 16 by 16 and more is refused, and what
+ * would be a launch of 2^32 threads (a few rows by 2^27, of k up to 128). */
 typedef struct fk_fp8_gemm_args {
   uint64_t a_codes, a_scales;
   uint64_t b_codes, b_scales;
