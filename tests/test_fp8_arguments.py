@@ -27,9 +27,9 @@ def test_cut_sums_are_of_products_to_16_bits():
             runtime.serve_check("fk_fp8_gemm", args)
             assert form
         else:
-            with pytest.raises(runtime.FkError):
+            with pytest.raises(runtime.FkError) as refusal:
                 runtime.serve_check("fk_fp8_gemm", args)
-            assert form == b""
+            assert form == b"" and refusal.value.status == -2   # FK_ERR_ARG
 
 
 def test_a_norm_s_sum_lies_over_rows_of_its_own_stride_only():
