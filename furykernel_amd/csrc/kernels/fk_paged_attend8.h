@@ -33,7 +33,7 @@
 // 125.6).
 //
 // Measured, f16 and bf16 out: one request of 131072 keys, 8 heads of 128 (268 MB)
-// 42.5 µs, 6.3 TB/s, and the join 4.6; 64 of up to 16384 (732 MB) 120 µs, 6.1 TB/s,
+// 43 µs, 6.2 TB/s, and the join 4.7; 64 of up to 16384 (732 MB) 120 to 124 µs, 6 TB/s,
 // and 5; 41 of up to 700, 4 heads of 64, 7.5 µs, which the longest's round trips bound.
 #pragma once
 
