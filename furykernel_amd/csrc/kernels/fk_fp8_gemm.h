@@ -214,7 +214,7 @@ __device__ __forceinline__ void fp8_gemm_few(const fk_fp8_gemm_args &a) {
 //   threadgroup a CU, four stages, the next step's operands read and a later
 //   step's loaded between a step's matrix operations, and tile after tile with
 //   the next one's first loads under the stores.  8192 by 8192 to f16, k 2048: 205
-//   to 210 µs (1.3 PFLOP/s; the library's bf16 product 1.37), cut 119 to 124 (2.2 to
+//   to 214 µs (1.3 PFLOP/s; the library's bf16 product 1.37), cut 119 to 124 (2.2 to
 //   2.3; from registers alone, random data, 3.0 to 3.4), of which C's stores take
 //   8 µs a turn of tiles.
 #define FK_FP8_STAGES 4
